@@ -21,8 +21,10 @@ LIB_DIR = os.path.join(HERE, "lib")
 HIP_SO = os.path.join(LIB_DIR, "libdsv4_hip.so")
 AMD_SO = os.path.join(LIB_DIR, "libdsv4_amd.so")
 
-# src/00_base/dsv4.h:86 plus this library's DSV4_WFP8_F32S
-DSV4_WF32, DSV4_WBF16, DSV4_WFP8, DSV4_WFP4, DSV4_WFP8_F32S = 0, 1, 2, 3, 4
+# src/00_base/dsv4.h:86 plus this library's DSV4_WFP8_F32S and DSV4_WI8
+DSV4_WF32, DSV4_WBF16, DSV4_WFP8, DSV4_WFP4, DSV4_WFP8_F32S, DSV4_WI8 = 0, 1, 2, 3, 4, 5
+# element types of activations
+DSV4_HIP_F32, DSV4_HIP_BF16, DSV4_HIP_F16 = 0, 1, 2
 
 # every symbol include/*.h declares
 EXPORTS = (
@@ -41,6 +43,9 @@ EXPORTS = (
     "dsv4_hip_moe_grouped_mx_mid_dev", "dsv4_hip_shared_fp8q_mid_dev",
     "dsv4_hip_route_dev", "dsv4_hip_moe_layer_dev", "dsv4_hip_moe_layer_n_dev",
     "dsv4_hip_alloc_count", "dsv4_hip_mmq_multi_dev",
+    "dsv4_hip_quant_i8_dev", "dsv4_hip_swiglu_quant_i8_dev", "dsv4_hip_gemm_i8_dev",
+    "dsv4_hip_gemm_i8_grouped_dev", "dsv4_hip_moe_permute_dev", "dsv4_hip_moe_permute_bwd_dev",
+    "dsv4_hip_moe_unpermute_dev", "dsv4_hip_moe_unpermute_bwd_dev",
 )
 # the reference-named C mirror (host/dsv4_compute_hip.c)
 MIRROR_EXPORTS = ("dsv4_mmq_n", "dsv4_mmq", "dsv4_expert_forward")
@@ -163,6 +168,17 @@ class Lib:
                                                       _F, _P]
         L.dsv4_hip_shared_fp8q_mid_dev.restype = _I
         L.dsv4_hip_shared_fp8q_mid_dev.argtypes = [_P, _P, _P, _I, _P, _I, _F, _P]
+        for n, args in (
+                ("dsv4_hip_quant_i8_dev", [_P, _P, _P, _I, C.c_int64, _I, _I, _P]),
+                ("dsv4_hip_swiglu_quant_i8_dev", [_P, _P, _P, _P, _I, C.c_int64, _I, _I, _F, _P]),
+                ("dsv4_hip_gemm_i8_dev", [_P, _I, _P, _P, _I, C.POINTER(QMat), _P]),
+                ("dsv4_hip_gemm_i8_grouped_dev", [_P, _I, _P, _P, _I, _P, _I, _P, _P, _I, _I, _I, _P]),
+                ("dsv4_hip_moe_permute_dev", [_P, _P, _P, _P, _P, _I, _P, _I, _I, _I, _I, _P]),
+                ("dsv4_hip_moe_permute_bwd_dev", [_P, _P, _I, _P, _I, _I, _I, _P]),
+                ("dsv4_hip_moe_unpermute_dev", [_P, _P, _I, _P, _P, _P, _I, _I, _I, _P]),
+                ("dsv4_hip_moe_unpermute_bwd_dev", [_P, _P, _P, _P, _I, _P, _P, _I, _I, _I, _P])):
+            getattr(L, n).restype = _I
+            getattr(L, n).argtypes = args
 
     # ------------------------------------------------------------ basics
     def alloc_count(self) -> int:
@@ -383,6 +399,45 @@ class Lib:
     def quant_act_mxfp8_dev(self, Q, S, a, n, k, stream=None):
         self.check(self.lib.dsv4_hip_quant_act_mxfp8_dev(Q, S, a, n, k, stream),
                    "quant_act_mxfp8_dev")
+
+    def quant_i8_dev(self, q_ptr, s_ptr, a_ptr, type_, ld, n, k, stream=None):
+        self.check(self.lib.dsv4_hip_quant_i8_dev(q_ptr, s_ptr, a_ptr, type_, ld, n, k, stream), "quant_i8_dev")
+
+    def swiglu_quant_i8_dev(self, q_ptr, s_ptr, g_ptr, u_ptr, type_, ld, n, k, limit, stream=None):
+        self.check(self.lib.dsv4_hip_swiglu_quant_i8_dev(q_ptr, s_ptr, g_ptr, u_ptr, type_, ld, n, k, limit, stream),
+                   "swiglu_quant_i8_dev")
+
+    def gemm_i8_dev(self, c_ptr, out_type, aq_ptr, sa_ptr, m, desc: QMat, stream=None):
+        self.check(self.lib.dsv4_hip_gemm_i8_dev(c_ptr, out_type, aq_ptr, sa_ptr, m, C.byref(desc), stream),
+                   "dsv4_hip_gemm_i8_dev")
+
+    def gemm_i8_grouped_dev(self, c_ptr, out_type, aq_ptr, sa_ptr, n_a, row_tok_ptr, n_rows, ex_off_ptr, table_ptr,
+                            n_experts, n, k, stream=None):
+        """table_ptr: a device array of n_experts QMat (DSV4_WI8, n x k)."""
+        self.check(self.lib.dsv4_hip_gemm_i8_grouped_dev(c_ptr, out_type, aq_ptr, sa_ptr, n_a, row_tok_ptr, n_rows,
+                                                         ex_off_ptr, table_ptr, n_experts, n, k, stream),
+                   "dsv4_hip_gemm_i8_grouped_dev")
+
+    def moe_permute_dev(self, rows_ptr, ex_off_ptr, row_tok_ptr, pos_ptr, x_ptr, type_, idx_ptr, n, topk, n_experts,
+                        hidden, stream=None):
+        self.check(self.lib.dsv4_hip_moe_permute_dev(rows_ptr, ex_off_ptr, row_tok_ptr, pos_ptr, x_ptr, type_, idx_ptr,
+                                                     n, topk, n_experts, hidden, stream),
+                   "dsv4_hip_moe_permute_dev")
+
+    def moe_permute_bwd_dev(self, dx_ptr, drows_ptr, type_, pos_ptr, n, topk, hidden, stream=None):
+        self.check(self.lib.dsv4_hip_moe_permute_bwd_dev(dx_ptr, drows_ptr, type_, pos_ptr, n, topk, hidden, stream),
+                   "dsv4_hip_moe_permute_bwd_dev")
+
+    def moe_unpermute_dev(self, out_ptr, rows_ptr, type_, pos_ptr, w_ptr, shared_ptr, n, topk, hidden, stream=None):
+        self.check(self.lib.dsv4_hip_moe_unpermute_dev(out_ptr, rows_ptr, type_, pos_ptr, w_ptr, shared_ptr, n, topk,
+                                                       hidden, stream),
+                   "dsv4_hip_moe_unpermute_dev")
+
+    def moe_unpermute_bwd_dev(self, drows_ptr, dw_ptr, dout_ptr, rows_ptr, type_, pos_ptr, w_ptr, n, topk, hidden,
+                              stream=None):
+        self.check(self.lib.dsv4_hip_moe_unpermute_bwd_dev(drows_ptr, dw_ptr, dout_ptr, rows_ptr, type_, pos_ptr,
+                                                           w_ptr, n, topk, hidden, stream),
+                   "dsv4_hip_moe_unpermute_bwd_dev")
 
     def synth_normal_dev(self, out_ptr, n, seed, sigma, round_bf16=False, stream=None):
         self.check(self.lib.dsv4_hip_synth_normal_dev(out_ptr, n, seed, float(sigma),

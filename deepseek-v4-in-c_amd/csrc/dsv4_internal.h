@@ -528,6 +528,73 @@ struct CombineArgs {
 };
 hipError_t moe_combine_launch(const CombineArgs &a, hipStream_t st);
 
+/* ------------------------------------------------ int8 products ------ */
+
+/* rows to int8 codes and a scale each: a (and with SwiGLU u, a being the
+ * gate) rows of k elements, `ld` elements apart, 16-byte aligned; Q [n][k]
+ * 8-byte aligned. hipErrorInvalidConfiguration: more rows than a launch takes. */
+struct QuantI8Args {
+    int8_t *Q;
+    float *S;
+    const void *a, *u;
+    long ld;
+    int n, k;
+    float limit;
+};
+hipError_t quant_i8_launch(const QuantI8Args &a, int type, bool swiglu, hipStream_t st);
+
+/* C [M][N]. One matrix: W [N][K], Sw [N], Aq [M][K], Sa [M]. Grouped (table
+ * set): row r of bucket e (ex_off[e] <= r < ex_off[e + 1]) from row row_tok[r]
+ * (or r) of Aq [n_a][K], n_a * K < 2^31. K a multiple of 16, Aq and W 16-byte
+ * aligned. hipErrorInvalidConfiguration: more tiles than a launch takes. */
+struct I8Args {
+    const uint8_t *Aq;
+    const float *Sa;
+    const uint8_t *W;
+    const float *Sw;
+    void *C;
+    int M, N, K;
+    const DSV4QMat *table;
+    const int *ex_off, *row_tok;
+    int n_experts, n_a;
+    unsigned *status;
+};
+hipError_t gemm_i8_launch(const I8Args &a, int out_type, hipStream_t st);
+
+/* ------------------------------------------------- expert order ------ */
+
+/* pairs up to which the sort and the copy are one launch */
+constexpr long PERMUTE_ONE_MAX = 32768;
+
+struct PermuteArgs {
+    void *rows;
+    int *ex_off, *row_tok, *pos;
+    const void *x;
+    const int *idx;
+    int n, topk, n_experts, hidden;
+    unsigned *status;
+};
+struct UnpermuteArgs {
+    void *out;
+    const void *rows;
+    const int *pos;
+    const float *w;           /* NULL: ones */
+    const void *shared;       /* or NULL    */
+    int n, topk, hidden;
+};
+struct UnpermuteBwdArgs {
+    void *drows;
+    float *dw;
+    const void *dout, *rows;
+    const int *pos;
+    const float *w;
+    int n, topk, hidden;
+};
+/* hipErrorInvalidConfiguration: more elements than a launch takes */
+hipError_t permute_launch(const PermuteArgs &a, int type, hipStream_t st);
+hipError_t unpermute_launch(const UnpermuteArgs &a, int type, hipStream_t st);
+hipError_t unpermute_bwd_launch(const UnpermuteBwdArgs &a, int type, hipStream_t st);
+
 } // namespace dsv4
 
 #endif /* DSV4_INTERNAL_H */

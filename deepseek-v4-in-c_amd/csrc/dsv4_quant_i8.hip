@@ -1,0 +1,280 @@
+/* SPDX-License-Identifier: Apache-2.0 */
+/* dsv4_quant_i8.hip - rows to 8-bit integers with one fp32 scale a row, the
+ * operands of the int8 products: tokens, weight rows, or the experts' SwiGLU
+ * output straight from the gate and up products.
+ *
+ * With amax = max_j |a_j|:  scale = amax / 127 (fp32, rounded once; 1 for a
+ * row of zeros) and code_j = the integer nearest to 127 a_j / amax, ties to
+ * even. A row with a value that is not finite has scale NaN and codes 0.
+ *
+ * EXACT CODES
+ *   fp32 gives 127 a_j / amax as a_j * (127 / amax), off by at most 2^-23 of
+ *   it (two roundings), so by 2^-16 absolutely: a code is certain unless the
+ *   product lies within 2^-15 of a half-integer. Only there (one element in
+ *   16,000) fp64 decides, where 127 a_j is exact and the quotient rounds to a
+ *   half-integer only if it is one: codes depend on no rounding on the way.
+ *   With SwiGLU the values are fp32 ones within 7 x 2^-24 (exp 1 ulp, 1 + e
+ *   half, reciprocal 1 ulp, two products): certain outside 2^-13 of a
+ *   half-integer. Inside it, and for the row's largest value, the SwiGLU is
+ *   taken in fp64: codes and scale are those of fp64 values. Rows whose largest value is below 2^-60 or beyond 2^120
+ *   compute everything in fp64.
+ */
+#include "dsv4_elem.h"
+#include "dsv4_internal.h"
+
+namespace dsv4 {
+
+namespace {
+
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+
+constexpr int QU = 8;                              /* elements of a lane's unit  */
+constexpr float ROUND_MAGIC = 12582912.0f;         /* 1.5 x 2^23: the low byte of v + this is rint(v) */
+
+__device__ __forceinline__ double swiglu64(float g, float u, float limit)
+{
+    if (limit > 0.0f) {
+        u = u > limit ? limit : u;
+        u = u < -limit ? -limit : u;
+        g = g > limit ? limit : g;
+    }
+    return (double)g / (1.0 + exp(-(double)g)) * (double)u;
+}
+
+__device__ __forceinline__ float swiglu32(float g, float u, float limit)
+{
+    if (limit > 0.0f) {
+        u = u > limit ? limit : u;
+        u = u < -limit ? -limit : u;
+        g = g > limit ? limit : g;
+    }
+    return __fmul_rn(__fmul_rn(g, __builtin_amdgcn_rcpf(__fadd_rn(1.0f, expf(-g)))), u);
+}
+
+/* the unit's 8 elements (a, or gate and up) at element offset j */
+template <int TYPE>
+__device__ __forceinline__ void load8(const void *row, int j, u32x4 (&r)[TYPE == DSV4_HIP_F32 ? 2 : 1])
+{
+    const uint8_t *p = (const uint8_t *)row + (size_t)j * elem_bytes<TYPE>();
+    r[0] = *gptr((const u32x4 *)p);
+    if constexpr (TYPE == DSV4_HIP_F32) r[1] = *gptr((const u32x4 *)(p + 16));
+}
+template <int TYPE>
+__device__ __forceinline__ void widen8(const u32x4 (&r)[TYPE == DSV4_HIP_F32 ? 2 : 1], float (&f)[QU])
+{
+    if constexpr (TYPE == DSV4_HIP_F32) {
+#pragma unroll
+        for (int i = 0; i < 8; i++) f[i] = __uint_as_float(r[i >> 2][i & 3]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            f[2 * i] = widen16<TYPE>(r[0][i] & 0xFFFFu);
+            f[2 * i + 1] = widen16<TYPE>(r[0][i] >> 16);
+        }
+    }
+}
+
+__device__ __forceinline__ uint32_t wave_max_u32(uint32_t v)
+{
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) v = max(v, (uint32_t)__shfl_xor((int)v, d, 64));
+    return v;
+}
+__device__ __forceinline__ double wave_max_f64(double v)
+{
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) v = fmax(v, __shfl_xor(v, d, 64));
+    return v;
+}
+
+/* the code in fp64: 127 a is exact for an fp32 a, and a quotient of such
+ * numbers that is not a tie is too far from one for fp64 to make it one */
+__device__ __forceinline__ uint32_t code64(double a, double amax) { return (uint32_t)(int)rint(a * 127.0 / amax); }
+
+} // namespace
+
+/* NW waves a row, NCH units of 8 elements a lane and pass; rows of more than
+ * NCH * NW * 512 elements are read again in the second pass (from L2). */
+template <int TYPE, bool SWIGLU, int NW, int NCH>
+__global__ __launch_bounds__(NW == 1 ? 256 : 64 * NW) void k_quant_i8(QuantI8Args a)
+{
+    constexpr int RPW = NW == 1 ? 4 : 1;           /* rows of a workgroup         */
+    constexpr int STEP = 64 * NW * QU;
+    constexpr int RW = TYPE == DSV4_HIP_F32 ? 2 : 1;
+    __shared__ uint32_t smax[NW];
+    __shared__ double smax64[NW];
+    const int lane = threadIdx.x & 63, wv = wave_in_group();
+    const long row = (long)blockIdx.x * RPW + (NW == 1 ? wv : 0);
+    if (row >= a.n) return;                        /* whole waves; one row a workgroup has no idle waves */
+    const size_t off = (size_t)row * (size_t)a.ld * elem_bytes<TYPE>();
+    const uint8_t *pa = (const uint8_t *)a.a + off, *pu = SWIGLU ? (const uint8_t *)a.u + off : nullptr;
+    const int j0 = ((NW == 1 ? 0 : wv * 64) + lane) * QU;
+    const bool once = a.k <= NCH * STEP;
+
+    u32x4 ra[NCH][RW], ru[SWIGLU ? NCH : 1][RW];
+    float f[NCH][QU];
+    auto fetch = [&](int base) {
+#pragma unroll
+        for (int c = 0; c < NCH; c++) {
+            const int j = base + j0 + c * STEP;
+            if (j < a.k) {
+                load8<TYPE>(pa, j, ra[c]);
+                if constexpr (SWIGLU) load8<TYPE>(pu, j, ru[c]);
+            }
+        }
+#pragma unroll
+        for (int c = 0; c < NCH; c++) {
+            const int j = base + j0 + c * STEP;
+            if (j < a.k) {
+                widen8<TYPE>(ra[c], f[c]);
+                if constexpr (SWIGLU) {
+                    float u[QU];
+                    widen8<TYPE>(ru[c], u);
+#pragma unroll
+                    for (int i = 0; i < QU; i++) f[c][i] = swiglu32(f[c][i], u[i], a.limit);
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < QU; i++) f[c][i] = 0.0f;
+            }
+        }
+    };
+    /* element i of the unit at j, exactly */
+    auto exact = [&](int j) -> double {
+        float g, u = 0.0f;
+        Elem<TYPE, 1> e;
+        float t[1];
+        e.load(pa + (size_t)j * elem_bytes<TYPE>());
+        e.get(t);
+        g = t[0];
+        if constexpr (SWIGLU) {
+            e.load(pu + (size_t)j * elem_bytes<TYPE>());
+            e.get(t);
+            u = t[0];
+            return swiglu64(g, u, a.limit);
+        }
+        return (double)g;
+    };
+
+    /* the largest magnitude, as the bits of |a|: NaN above inf above all else */
+    uint32_t m = 0;
+    for (int base = 0; base < a.k; base += NCH * STEP) {
+        fetch(base);
+#pragma unroll
+        for (int c = 0; c < NCH; c++)
+#pragma unroll
+            for (int i = 0; i < QU; i++) m = max(m, __float_as_uint(f[c][i]) & 0x7FFFFFFFu);
+    }
+    m = wave_max_u32(m);
+    if constexpr (NW > 1) {
+        if (lane == 0) smax[wv] = m;
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < NW; w++) m = max(m, smax[w]);
+    }
+    m = (uint32_t)__builtin_amdgcn_readfirstlane((int)m);
+    const float amax = __uint_as_float(m);
+    double amax64 = (double)amax;
+    /* SwiGLU's fp32 values serve rows of this range; others take fp64 ones */
+    const bool wide = SWIGLU && !(amax >= 0x1p-60f && amax <= 0x1p120f);
+    bool bad = !SWIGLU && m >= 0x7F800000u;
+    if constexpr (SWIGLU) {
+        double d = 0.0;
+        bool nan = false;
+        if (wide) {
+            for (int j = j0; j < a.k; j += STEP)
+                for (int i = 0; i < QU; i++) {
+                    const double v = fabs(exact(j + i));
+                    nan |= !(v <= 1.7976931348623157e308);
+                    d = fmax(d, v);
+                }
+        } else {
+            const float near = amax * (1.0f - 0x1p-18f);
+            for (int base = 0; base < a.k; base += NCH * STEP) {
+                if (!once) fetch(base);
+#pragma unroll
+                for (int c = 0; c < NCH; c++)
+#pragma unroll
+                    for (int i = 0; i < QU; i++)
+                        if (fabsf(f[c][i]) >= near) d = fmax(d, fabs(exact(base + j0 + c * STEP + i)));
+            }
+        }
+        d = wave_max_f64(d);
+        nan = __any(nan);
+        if constexpr (NW > 1) {
+            if (lane == 0) smax64[wv] = nan ? __builtin_nan("") : d;
+            __syncthreads();
+#pragma unroll
+            for (int w = 0; w < NW; w++) {
+                const double s = smax64[w];
+                nan |= s != s;
+                d = fmax(d, s);
+            }
+        }
+        amax64 = d;
+        bad = nan;
+    }
+    if (lane == 0 && (NW == 1 || wv == 0))
+        a.S[row] = bad ? __builtin_nanf("") : amax64 > 0.0 ? (SWIGLU ? (float)(amax64 / 127.0) : amax / 127.0f) : 1.0f;
+
+    /* tiny rows are multiplied by 2^64 first (exactly), so that 127 / amax
+     * stays finite and the values normal */
+    const bool tiny = !SWIGLU && amax < 0x1p-64f;
+    const float up = tiny ? 0x1p64f : 1.0f;
+    const float inv = bad || wide || !(amax > 0.0f) ? 0.0f
+                    : SWIGLU ? (float)(127.0 / amax64) : 127.0f / (amax * up);
+    constexpr float SURE = SWIGLU ? 0.5f - 0x1p-13f : 0.5f - 0x1p-15f;
+    int8_t *q = a.Q + (size_t)row * (size_t)a.k;
+    for (int base = 0; base < a.k; base += NCH * STEP) {
+        if (!once) fetch(base);
+#pragma unroll
+        for (int c = 0; c < NCH; c++) {
+            const int j = base + j0 + c * STEP;
+            if (j >= a.k) continue;
+            uint32_t t[QU];
+            float far = 0.0f;
+#pragma unroll
+            for (int i = 0; i < QU; i++) {
+                const float x = inv == 0.0f ? 0.0f : f[c][i];
+                const float v = __fmul_rn(__fmul_rn(x, up), inv);
+                const float s = __fadd_rn(v, ROUND_MAGIC);
+                t[i] = __float_as_uint(s);
+                far = fmaxf(far, fabsf(__fsub_rn(v, __fsub_rn(s, ROUND_MAGIC))));
+            }
+            if (wide && !bad && amax64 > 0.0) {
+                for (int i = 0; i < QU; i++) t[i] = code64(exact(j + i), amax64);
+            } else if (far > SURE) {
+                for (int i = 0; i < QU; i++) {
+                    const float v = __fmul_rn(__fmul_rn(f[c][i], up), inv);
+                    if (fabsf(__fsub_rn(v, rintf(v))) > SURE) t[i] = code64(exact(j + i), amax64);
+                }
+            }
+            u32x2 o;
+            o.x = (t[0] & 0xFFu) | (t[1] & 0xFFu) << 8 | (t[2] & 0xFFu) << 16 | t[3] << 24;
+            o.y = (t[4] & 0xFFu) | (t[5] & 0xFFu) << 8 | (t[6] & 0xFFu) << 16 | t[7] << 24;
+            *(DSV4_GLOBAL u32x2 *)(q + j) = o;
+        }
+    }
+}
+
+template <int TYPE, bool SWIGLU>
+static hipError_t quant_i8_t(const QuantI8Args &a, hipStream_t st)
+{
+    const dim3 one((unsigned)a.n);
+    hipLaunchKernelGGL((k_quant_i8<TYPE, SWIGLU, 8, 2>), one, dim3(512), 0, st, a);
+    return hipGetLastError();
+}
+
+hipError_t quant_i8_launch(const QuantI8Args &a, int type, bool swiglu, hipStream_t st)
+{
+    if (a.n <= 0 || a.k <= 0 || a.k % QU) return hipErrorInvalidValue;
+    if (a.n >= 1 << 23) return hipErrorInvalidConfiguration;       /* 2^32 threads */
+    switch (type) {
+    case DSV4_HIP_F32: return swiglu ? quant_i8_t<DSV4_HIP_F32, true>(a, st) : quant_i8_t<DSV4_HIP_F32, false>(a, st);
+    case DSV4_HIP_BF16: return swiglu ? quant_i8_t<DSV4_HIP_BF16, true>(a, st) : quant_i8_t<DSV4_HIP_BF16, false>(a, st);
+    case DSV4_HIP_F16: return swiglu ? quant_i8_t<DSV4_HIP_F16, true>(a, st) : quant_i8_t<DSV4_HIP_F16, false>(a, st);
+    default: return hipErrorInvalidValue;
+    }
+}
+
+} // namespace dsv4

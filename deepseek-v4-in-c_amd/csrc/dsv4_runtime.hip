@@ -41,6 +41,7 @@
 
 #include <rocprofiler-sdk-roctx/roctx.h>
 
+#include "dsv4_elem.h"
 #include "dsv4_internal.h"
 #include "../../include/dsv4_hip_aux.h"
 
@@ -2116,6 +2117,196 @@ int dsv4_hip_moe_route_dev(int *ex_off, int *ex_tok, int *ex_k, int *pos, const 
     return 0;
 }
 
+/* ------------------------------- int8 products, expert order ---------- */
+
+/* These calls run on the library's device whichever is current, and take only
+ * streams of that device. Workspaces they have none. */
+struct OnDevice {
+    int was = -1;
+    bool ok = true;
+    OnDevice()
+    {
+        int d = -1;
+        if (hipGetDevice(&d) != hipSuccess) ok = false;
+        else if (d != g.device) {
+            if (hipSetDevice(g.device) != hipSuccess) ok = false;
+            else was = d;
+        }
+    }
+    ~OnDevice() { if (was >= 0) (void)hipSetDevice(was); }
+};
+
+static int stream_check(const OnDevice &on, void *stream, const char *what)
+{
+    if (!on.ok) return fail("%s: device %d cannot be selected", what, g.device);
+    hipDevice_t d = g.device;
+    if (stream && (hipStreamGetDevice((hipStream_t)stream, &d) != hipSuccess || d != g.device)) {
+        (void)hipGetLastError();
+        return fail("%s: the stream is not one of device %d", what, g.device);
+    }
+    return 0;
+}
+
+/* hipErrorInvalidConfiguration is a launcher's answer to a call that is too
+ * large for one launch: nothing has been enqueued */
+#define LAUNCH(expr, what)                                                     \
+    do {                                                                       \
+        const hipError_t e_ = (expr);                                          \
+        if (e_ == hipErrorInvalidConfiguration) return fail("%s: too large for one launch", what); \
+        if (e_ != hipSuccess) return hip_fail(e_, what);                       \
+    } while (0)
+
+static bool elem_type_ok(int type) { return type == DSV4_HIP_F32 || type == DSV4_HIP_BF16 || type == DSV4_HIP_F16; }
+static bool elem_aligned(const void *p, int type) { return ((uintptr_t)p & (uintptr_t)(elem_bytes_of(type) - 1)) == 0; }
+
+constexpr int I8_KMAX = 131056;                    /* 128 * 128 * K < 2^31 */
+
+int dsv4_hip_gemm_i8_dev(void *C, int out_type, const int8_t *Aq, const float *Sa, int M, const DSV4QMat *W,
+                         void *stream)
+{
+    std::lock_guard<std::mutex> lk(g.mu);
+    Range rg("dsv4_hip_gemm_i8_dev");
+    if (!W || (M && (!C || !Aq || !Sa || !W->w || !W->s))) return fail("gemm_i8_dev: NULL pointer");
+    if (M < 0 || !elem_type_ok(out_type)) return fail("gemm_i8_dev: bad M %d or out_type %d", M, out_type);
+    if (W->wdt != DSV4_WI8 || W->rows < 1 || W->cols < 16 || W->cols % 16 || W->cols > I8_KMAX)
+        return fail("gemm_i8_dev: W must be DSV4_WI8 with cols a multiple of 16 up to %d (got wdt %d, %d x %d)",
+                    I8_KMAX, W->wdt, W->rows, W->cols);
+    if (!aligned16(Aq) || !aligned16(W->w) || ((uintptr_t)Sa & 3u) || ((uintptr_t)W->s & 3u) ||
+        !elem_aligned(C, out_type))
+        return fail("gemm_i8_dev: Aq and w must be 16-byte aligned, scales and C to their elements");
+    if (usable()) return -1;
+    if (M == 0) return 0;
+    OnDevice on;
+    if (stream_check(on, stream, "gemm_i8_dev")) return -1;
+    dev_call();
+    I8Args a;
+    memset(&a, 0, sizeof a);
+    a.Aq = (const uint8_t *)Aq; a.Sa = Sa; a.W = (const uint8_t *)W->w; a.Sw = (const float *)W->s; a.C = C;
+    a.M = M; a.N = W->rows; a.K = W->cols; a.status = g.st;
+    LAUNCH(gemm_i8_launch(a, out_type, (hipStream_t)stream), "gemm_i8_dev");
+    return 0;
+}
+
+int dsv4_hip_gemm_i8_grouped_dev(void *C, int out_type, const int8_t *Aq, const float *Sa, int n_a,
+                                 const int *row_tok, int n_rows, const int *ex_off, const DSV4QMat *table,
+                                 int n_experts, int N, int K, void *stream)
+{
+    std::lock_guard<std::mutex> lk(g.mu);
+    Range rg("dsv4_hip_gemm_i8_grouped_dev");
+    if (n_rows && (!C || !Aq || !Sa || !ex_off || !table)) return fail("gemm_i8_grouped_dev: NULL pointer");
+    if (n_rows < 0 || n_a < (n_rows > 0) || !elem_type_ok(out_type))
+        return fail("gemm_i8_grouped_dev: bad n_rows %d, n_a %d or out_type %d", n_rows, n_a, out_type);
+    if (n_experts < 1 || n_experts > 1024)
+        return fail("gemm_i8_grouped_dev: n_experts %d outside 1..1024", n_experts);
+    if (N < 1 || K < 16 || K % 16 || K > I8_KMAX)
+        return fail("gemm_i8_grouped_dev: need N > 0 and K a multiple of 16 up to %d (got %d, %d)", I8_KMAX, N, K);
+    if ((long)n_a * K > 0x7FFFFFFFL) return fail("gemm_i8_grouped_dev: n_a * K is 2^31 or more");
+    if (!aligned16(Aq) || ((uintptr_t)Sa & 3u) || ((uintptr_t)ex_off & 3u) || ((uintptr_t)row_tok & 3u) ||
+        ((uintptr_t)table & 7u) || !elem_aligned(C, out_type))
+        return fail("gemm_i8_grouped_dev: Aq must be 16-byte aligned, the others to their elements");
+    if (usable()) return -1;
+    if (n_rows == 0) return 0;
+    OnDevice on;
+    if (stream_check(on, stream, "gemm_i8_grouped_dev")) return -1;
+    dev_call();
+    I8Args a;
+    memset(&a, 0, sizeof a);
+    a.Aq = (const uint8_t *)Aq; a.Sa = Sa; a.C = C; a.M = n_rows; a.N = N; a.K = K;
+    a.table = table; a.ex_off = ex_off; a.row_tok = row_tok; a.n_experts = n_experts; a.n_a = n_a;
+    a.status = g.st;
+    LAUNCH(gemm_i8_launch(a, out_type, (hipStream_t)stream), "gemm_i8_grouped_dev");
+    return 0;
+}
+
+/* shared checks of the expert-order calls */
+static int order_checks(int type, int n, int topk, int hidden, std::initializer_list<const void *> elems,
+                        std::initializer_list<const void *> words, const char *what)
+{
+    if (!elem_type_ok(type)) return fail("%s: unknown element type %d", what, type);
+    if (n < 0 || topk < 1 || topk > 16 || (long)n * topk > (1L << 26) || hidden < 1)
+        return fail("%s: bad n %d, topk %d or hidden %d", what, n, topk, hidden);
+    for (const void *p : elems)
+        if ((!p && n) || !elem_aligned(p, type)) return fail("%s: NULL or misaligned rows", what);
+    for (const void *p : words)
+        if ((!p && n) || ((uintptr_t)p & 3u)) return fail("%s: NULL or misaligned index or weight array", what);
+    return 0;
+}
+
+int dsv4_hip_moe_permute_dev(void *rows, int *ex_off, int *row_tok, int *pos, const void *x, int type,
+                             const int *idx, int n, int topk, int n_experts, int hidden, void *stream)
+{
+    std::lock_guard<std::mutex> lk(g.mu);
+    Range rg("dsv4_hip_moe_permute_dev");
+    if (order_checks(type, n, topk, hidden, {rows, x}, {row_tok, pos, idx}, "moe_permute_dev")) return -1;
+    if (!ex_off || ((uintptr_t)ex_off & 3u)) return fail("moe_permute_dev: NULL or misaligned ex_off");
+    if (n_experts < 1 || n_experts > 1024)
+        return fail("moe_permute_dev: n_experts %d outside 1..1024", n_experts);
+    if (usable()) return -1;
+    OnDevice on;
+    if (stream_check(on, stream, "moe_permute_dev")) return -1;
+    dev_call();
+    PermuteArgs a;
+    a.rows = rows; a.ex_off = ex_off; a.row_tok = row_tok; a.pos = pos; a.x = x; a.idx = idx;
+    a.n = n; a.topk = topk; a.n_experts = n_experts; a.hidden = hidden; a.status = g.st;
+    LAUNCH(permute_launch(a, type, (hipStream_t)stream), "moe_permute_dev");
+    return 0;
+}
+
+int dsv4_hip_moe_permute_bwd_dev(void *dx, const void *drows, int type, const int *pos, int n, int topk,
+                                 int hidden, void *stream)
+{
+    std::lock_guard<std::mutex> lk(g.mu);
+    Range rg("dsv4_hip_moe_permute_bwd_dev");
+    if (order_checks(type, n, topk, hidden, {dx, drows}, {pos}, "moe_permute_bwd_dev")) return -1;
+    if (usable()) return -1;
+    if (n == 0) return 0;
+    OnDevice on;
+    if (stream_check(on, stream, "moe_permute_bwd_dev")) return -1;
+    dev_call();
+    UnpermuteArgs a;
+    a.out = dx; a.rows = drows; a.pos = pos; a.w = nullptr; a.shared = nullptr;
+    a.n = n; a.topk = topk; a.hidden = hidden;
+    LAUNCH(unpermute_launch(a, type, (hipStream_t)stream), "moe_permute_bwd_dev");
+    return 0;
+}
+
+int dsv4_hip_moe_unpermute_dev(void *out, const void *rows, int type, const int *pos, const float *w,
+                               const void *shared, int n, int topk, int hidden, void *stream)
+{
+    std::lock_guard<std::mutex> lk(g.mu);
+    Range rg("dsv4_hip_moe_unpermute_dev");
+    if (order_checks(type, n, topk, hidden, {out, rows}, {pos, w}, "moe_unpermute_dev")) return -1;
+    if (!elem_aligned(shared, type)) return fail("moe_unpermute_dev: misaligned shared");
+    if (usable()) return -1;
+    if (n == 0) return 0;
+    OnDevice on;
+    if (stream_check(on, stream, "moe_unpermute_dev")) return -1;
+    dev_call();
+    UnpermuteArgs a;
+    a.out = out; a.rows = rows; a.pos = pos; a.w = w; a.shared = shared;
+    a.n = n; a.topk = topk; a.hidden = hidden;
+    LAUNCH(unpermute_launch(a, type, (hipStream_t)stream), "moe_unpermute_dev");
+    return 0;
+}
+
+int dsv4_hip_moe_unpermute_bwd_dev(void *drows, float *dw, const void *dout, const void *rows, int type,
+                                   const int *pos, const float *w, int n, int topk, int hidden, void *stream)
+{
+    std::lock_guard<std::mutex> lk(g.mu);
+    Range rg("dsv4_hip_moe_unpermute_bwd_dev");
+    if (order_checks(type, n, topk, hidden, {drows, dout, rows}, {dw, pos, w}, "moe_unpermute_bwd_dev")) return -1;
+    if (usable()) return -1;
+    if (n == 0) return 0;
+    OnDevice on;
+    if (stream_check(on, stream, "moe_unpermute_bwd_dev")) return -1;
+    dev_call();
+    UnpermuteBwdArgs a;
+    a.drows = drows; a.dw = dw; a.dout = dout; a.rows = rows; a.pos = pos; a.w = w;
+    a.n = n; a.topk = topk; a.hidden = hidden;
+    LAUNCH(unpermute_bwd_launch(a, type, (hipStream_t)stream), "moe_unpermute_bwd_dev");
+    return 0;
+}
+
 int dsv4_hip_status(unsigned *bits)
 {
     std::lock_guard<std::mutex> lk(g.mu);
@@ -2190,6 +2381,41 @@ int dsv4_hip_quant_act_mxfp8_dev(uint8_t *Q, uint8_t *S, const float *a, int n,
     if (!aligned16(Q) || !aligned16(a)) return fail("quant_act_mxfp8_dev: Q and a must be 16-byte aligned");
     HIPCHK(quant_act_mxfp8_launch(Q, S, a, n, k, (hipStream_t)stream), "quant launch");
     return 0;
+}
+
+static int quant_i8(int8_t *Q, float *S, const void *x, const void *u, bool swiglu, int type, int64_t ld, int n,
+                    int k, float limit, void *stream, const char *what)
+{
+    if (n && (!Q || !S || !x || (swiglu && !u))) return fail("%s: NULL pointer", what);
+    if (!elem_type_ok(type)) return fail("%s: unknown element type %d", what, type);
+    if (n < 0 || k < 16 || k % 16 || ld < k || ld > (1LL << 40) || ld * elem_bytes_of(type) % 16)
+        return fail("%s: need n >= 0, k a multiple of 16 and ld >= k of whole 16-byte steps (got %d, %d, %lld)", what,
+                    n, k, (long long)ld);
+    if (!aligned16(x) || !aligned16(u) || ((uintptr_t)Q & 7u) || ((uintptr_t)S & 3u))
+        return fail("%s: need rows 16-, Q 8- and S 4-byte aligned", what);
+    if (usable()) return -1;
+    if (n == 0) return 0;
+    OnDevice on;
+    if (stream_check(on, stream, what)) return -1;
+    QuantI8Args a;
+    a.Q = Q; a.S = S; a.a = x; a.u = u; a.ld = (long)ld; a.n = n; a.k = k; a.limit = limit;
+    LAUNCH(quant_i8_launch(a, type, swiglu, (hipStream_t)stream), what);
+    return 0;
+}
+
+int dsv4_hip_quant_i8_dev(int8_t *Q, float *S, const void *a, int type, int64_t ld, int n, int k, void *stream)
+{
+    std::lock_guard<std::mutex> lk(g.mu);
+    Range rg("dsv4_hip_quant_i8_dev");
+    return quant_i8(Q, S, a, nullptr, false, type, ld, n, k, 0.0f, stream, "quant_i8_dev");
+}
+
+int dsv4_hip_swiglu_quant_i8_dev(int8_t *Q, float *S, const void *g_, const void *u, int type, int64_t ld, int n,
+                                 int k, float limit, void *stream)
+{
+    std::lock_guard<std::mutex> lk(g.mu);
+    Range rg("dsv4_hip_swiglu_quant_i8_dev");
+    return quant_i8(Q, S, g_, u, true, type, ld, n, k, limit, stream, "swiglu_quant_i8_dev");
 }
 
 int dsv4_hip_synth_normal_dev(float *out, size_t n, uint64_t seed, float sigma,

@@ -66,6 +66,15 @@ typedef struct {
  * element is e4m3(w) * scale, one fp32 multiply. */
 #define DSV4_WFP8_F32S 4
 
+/* New tag, no counterpart in the reference: 8-bit integer weights with one
+ * fp32 scale a row (blk_r 1, blk_c = cols; s holds `rows` floats). The value
+ * of an element is w * s[row]. Taken by the int8 products below only. */
+#define DSV4_WI8 5
+
+/* Element types of the activations that the int8 products and the expert
+ * order calls read and write. */
+enum { DSV4_HIP_F32 = 0, DSV4_HIP_BF16 = 1, DSV4_HIP_F16 = 2 };
+
 /* ---------------------------------------------------------- lifecycle ---- */
 
 /* Select and initialise `device`. 0 ok, -1 when no usable gfx950 GPU exists
@@ -353,6 +362,76 @@ int  dsv4_hip_gemm_mxfp8_dev(void *C, int out_bf16, const void *A, int a_bf16,
 int  dsv4_hip_gemm_mxfp8q_dev(void *C, int out_bf16, const uint8_t *Aq,
                               const uint8_t *As, int M, const DSV4QMat *W,
                               void *stream);
+
+/* ------------------------------------------------ int8 products -----------
+ * No counterpart in the reference: checkpoints quantized to 8-bit integers
+ * with a scale for each weight row, against tokens quantized row by row
+ * (dsv4_hip_quant_i8_dev, dsv4_hip_swiglu_quant_i8_dev).
+ *   C[m][n] = Sa[m] * s[n] * sum_k Aq[m][k] * w[n][k]
+ * Aq [M][cols] codes, Sa [M], W a HOST descriptor (DSV4_WI8) holding device
+ * pointers, C [M][W->rows] of out_type. The integer sum is exact; the result
+ * is ((float)sum * Sa) * s, rounded once more for a 16-bit out_type (values
+ * beyond fp16 become infinite). cols a multiple of 16 up to 131,056; M and
+ * W->rows any; Aq and w 16-byte aligned. A scale of NaN makes its row NaN.
+ * No workspace: calls on several streams, and captured graphs, do not meet.
+ * 0 enqueued (M = 0: nothing), -1 otherwise. */
+int  dsv4_hip_gemm_i8_dev(void *C, int out_type, const int8_t *Aq, const float *Sa, int M,
+                          const DSV4QMat *W, void *stream);
+
+/* The same for rows in expert order: row r of bucket e (ex_off[e] <= r <
+ * ex_off[e + 1], as dsv4_hip_moe_permute_dev or dsv4_hip_moe_route_dev order
+ * them) is multiplied by expert e's matrix:
+ *   C[r][j] = Sa[t] * s_e[j] * sum_k Aq[t][k] * w_e[j][k],  t = row_tok[r]
+ * so the tokens' codes Aq [n_a][K] need no copy in expert order; row_tok NULL:
+ * t = r. C [n_rows][N]; rows from ex_off[n_experts] on stay as they are.
+ * `table` is a DEVICE array of n_experts descriptors (DSV4_WI8, [N x K],
+ * device pointers, w 16-byte aligned); one of another kind raises status bit
+ * 1 and its rows become NaN. A row_tok outside [0, n_a) raises bit 0 and its
+ * row becomes NaN. n_experts <= 1024; n_a * K < 2^31; else as above. */
+int  dsv4_hip_gemm_i8_grouped_dev(void *C, int out_type, const int8_t *Aq, const float *Sa, int n_a,
+                                  const int *row_tok, int n_rows, const int *ex_off,
+                                  const DSV4QMat *table, int n_experts, int N, int K, void *stream);
+
+/* --------------------------------------- tokens in expert order -----------
+ * The steps of the reference's union path around its bucket products
+ * (src/80_prefill/dsv4_prefill_union.c:30-66, dsv4_prefill_experts.c:47-76,
+ * dsv4_prefill_union_run.c:109-121) as calls of their own, in three element
+ * types and with gradients, which the reference does not have.
+ *
+ * permute: the stable counting sort of the n * topk (token, k) pairs by
+ * expert and the tokens copied to their rows. idx [n][topk]; ex_off
+ * [n_experts + 1] the first row of each expert's bucket; row_tok [n * topk]
+ * the token of each row (rows of a bucket in token-major, k-minor order); pos
+ * [n][topk] the row of each pair; rows[pos[t][k]] = x[t]. An id of -1 is a
+ * pair without an expert here (held by another device, dropped): its pos is
+ * -1. Any other id outside [0, n_experts) is treated the same and raises
+ * status bit 0. Rows, and entries of row_tok, from ex_off[n_experts] on stay
+ * as they are. n = 0 gives empty buckets.
+ * x [n][hidden], rows [n * topk][hidden] of `type`; n_experts <= 1024, topk <=
+ * 16, n * topk <= 2^26, any hidden (rows of whole 16-byte vectors are the
+ * fast ones). Outputs must not overlap inputs. No workspace. */
+int  dsv4_hip_moe_permute_dev(void *rows, int *ex_off, int *row_tok, int *pos, const void *x, int type,
+                              const int *idx, int n, int topk, int n_experts, int hidden, void *stream);
+
+/* Gradient of permute: dx[t] = sum_k drows[pos[t][k]], fp32 in k order, one
+ * rounding. A pair whose pos is outside [0, n * topk) adds nothing; a token
+ * without pairs gets zeros. */
+int  dsv4_hip_moe_permute_bwd_dev(void *dx, const void *drows, int type, const int *pos, int n, int topk,
+                                  int hidden, void *stream);
+
+/* out[t] = sum_k w[t][k] * rows[pos[t][k]] + shared[t], fp32 in k order (the
+ * shared expert's output last and unweighted; NULL: none), one rounding to
+ * `type`. Pairs without a row as above. out may be `shared` itself. */
+int  dsv4_hip_moe_unpermute_dev(void *out, const void *rows, int type, const int *pos, const float *w,
+                                const void *shared, int n, int topk, int hidden, void *stream);
+
+/* Gradients of unpermute: drows[pos[t][k]] = w[t][k] * dout[t] (rows that no
+ * pair has stay as they are) and dw[t][k] = sum_j dout[t][j] *
+ * rows[pos[t][k]][j] in fp32 (0 for a pair without a row); the gradient of
+ * `shared` is dout itself. drows may be `rows` itself. */
+int  dsv4_hip_moe_unpermute_bwd_dev(void *drows, float *dw, const void *dout, const void *rows, int type,
+                                    const int *pos, const float *w, int n, int topk, int hidden,
+                                    void *stream);
 
 /* ------------------------------------- checkpoint experts (loader hook) --
  * The loader's upload-once path for the routed experts, which the reference

@@ -44,6 +44,23 @@ int dsv4_hip_quant_act_fp8_1x128_dev(uint8_t *Q, float *S, const float *a,
 int dsv4_hip_quant_act_mxfp8_dev(uint8_t *Q, uint8_t *S, const float *a,
                                  int n, int k, void *stream);
 
+/* n rows of k elements of `type` (DSV4_HIP_*), `ld` elements apart -> int8
+ * codes Q[n][k] and an fp32 scale S[n] a row: with amax the row's largest
+ * magnitude S = amax / 127 (1 for a row of zeros) and code = the integer
+ * nearest to 127 a / amax, ties to even, decided exactly. A row with a value
+ * that is not finite gets scale NaN and codes 0. Tokens for the int8 products,
+ * or weight rows (DSV4_WI8). k and the bytes of ld multiples of 16, a 16-byte,
+ * Q 8-byte and S 4-byte aligned; n = 0: nothing. No workspace. */
+int dsv4_hip_quant_i8_dev(int8_t *Q, float *S, const void *a, int type, int64_t ld, int n, int k,
+                          void *stream);
+
+/* The same for a = SwiGLU(g, u), the reference's element with its asymmetric
+ * clamp (src/10_compute/dsv4_ops.c:61-79; limit <= 0: none): g and u rows of
+ * gate and up outputs, both `ld` elements apart (two arrays, or the halves of
+ * one). Codes and scale are those of the exact SwiGLU values. */
+int dsv4_hip_swiglu_quant_i8_dev(int8_t *Q, float *S, const void *g, const void *u, int type, int64_t ld,
+                                 int n, int k, float limit, void *stream);
+
 /* The grouped MoE's permutation on its own (the first step of
  * dsv4_hip_moe_grouped_dev): the counting sort of the n * topk routing ids
  * idx[n][topk] by expert, as src/80_prefill/dsv4_prefill_union.c:30-51
