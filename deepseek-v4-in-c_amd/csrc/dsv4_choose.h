@@ -208,6 +208,65 @@ inline Bf16Form bf16_form(int rows, int cols, int nt)
  * 91.4), 60000 of 256 10.4 / 9.8. */
 constexpr int bf16_rows_depth(int rows, int cols) { return cols < 1024 && rows >= 65536 ? 4 : 8; }
 
+/* ------------------------------------------------------ int8 products ---- */
+
+/* Forms of the int8 product, named by their tiles (features x 16-row groups);
+ * the same bits in all. I8_PAIR: weights straight to registers, one matrix in
+ * workgroups of 8 weight rows x 8 tokens, experts in 32 x 16. I8_64x2_DEEP:
+ * two blocks of K a stage. */
+enum I8Form { I8_PAIR = 1, I8_64x2, I8_64x2_DEEP, I8_64x4, I8_128x4, I8_128x8, I8_256x8 };
+
+/* One matrix. Few rows of a matrix of few rows are latency: the pair form's
+ * workgroups wait out one load (us, pair / 64x2 deep / 64x2: 1 x 4096 x 4096
+ * 5.0 / 7.0 / 7.8, 8 x 4096 x 4096 6.2 / 7.2 / 7.9, 12 x 1024 x 4096 4.3 / 7.0 /
+ * 7.8; but 16 x 4096 x 4096 9.7 / 7.3 / 8.0, 1 x 32768 x 1024 14.1 / 7.7 / 7.5).
+ * Otherwise the form of least cost, in tenths of a us at K = 4096: `per` a full
+ * round of 256 workgroups, `base` a nearly empty one, `c0` once. They were
+ * fitted to (us, 64x2 / 64x4 / 128x4 / 128x8 / 256x8) 128 rows 4096 x 4096 8.4 /
+ * 10.2 / 12.3 / 16.2 / 26, 333 rows 16.3 / 14.1 / 12.9 / 16.2 / 26, 700 rows 29.1
+ * / 21.7 / 21.9 / 18.4 / 27.9, 1,024 rows 38 / 29 / 24 / 22 / 30, 2,048 rows 75 /
+ * 55 / 46 / 42 / 36; 1,000 rows 2048 x 2048 13.4 / 11.2 / 9.0 / 11.3 / 17.4. In
+ * one round 64x2 takes two blocks of K a stage (8.0 -> 7.2 at 16 rows; with
+ * three workgroups a CU its longer ring costs, 512 rows 21.4 -> 21.9). */
+constexpr long I8_PAIR_GROUPS = 768;
+inline I8Form i8_form(int M, int N, int K)
+{
+    if (ceil_div(M, 8) * ceil_div(N, 8) <= I8_PAIR_GROUPS) return I8_PAIR;
+    struct { I8Form form; int F, TR, c0, base, per; } const f[] = {
+        {I8_64x2, 64, 32, 5, 40, 45}, {I8_64x4, 64, 64, 0, 65, 65}, {I8_128x4, 128, 64, -5, 95, 110},
+        {I8_128x8, 128, 128, -20, 145, 205}, {I8_256x8, 256, 128, -20, 250, 345}};
+    I8Form best = I8_64x2;
+    long least = -1;
+    for (const auto &c : f) {
+        const long w = ceil_div(M, c.TR) * ceil_div(N, c.F), full = (w - 1) / CUS, last = w - full * CUS;
+        const long cost = 30 * 4096L + (c.c0 + full * c.per + c.base + (c.per - c.base) * last / CUS) * K;
+        if (least < 0 || cost < least) {
+            least = cost;
+            best = c.form;
+            if (c.form == I8_64x2 && w <= CUS && K >= 1024) best = I8_64x2_DEEP;
+        }
+    }
+    return best;
+}
+
+/* Buckets of ne experts, M rows in all. Up to 16 rows an expert the weights
+ * are streamed once whatever the form, and the pair form streams best (us,
+ * pair / 64x2 / 128x4, experts 2048 x 4096: 42 rows on 256 57 / 62 / 68, 384 rows
+ * Zipf 176 / 182 / 195, 1,536 rows 344 / 367 / 396, 2,400 rows 370 / 369),
+ * unless there is too little of it to fill the CUs (6 rows 15.4 / 12.3; 160 rows
+ * on 64 of 512 x 1024 8.7 / 6.7). Then 128x4 (6,144 rows Zipf 64x2 423, 128x4
+ * 419, 256x8 458; 12,288 rows 529 / 439 / 494), and the large tiles from 80 rows an
+ * expert (24,576 rows Zipf 746 / 580 / 547; 6,144 rows on 64 experts 191 / 141 /
+ * 141). */
+inline I8Form i8_grouped_form(int M, int N, int K, int ne)
+{
+    const long hit = M < ne ? M : ne;
+    if (hit * N * K < 1L << 26 && M <= 32 * hit) return I8_64x2;
+    if (M <= 10 * hit) return I8_PAIR;
+    if (M <= 20 * hit) return I8_64x2;
+    return M < 80 * hit ? I8_128x4 : I8_256x8;
+}
+
 } // namespace dsv4
 
 #endif /* DSV4_CHOOSE_H */

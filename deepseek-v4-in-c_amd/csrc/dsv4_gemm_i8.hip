@@ -113,108 +113,383 @@ __device__ __forceinline__ void i8_store(void *C, size_t i, float v)
 } // namespace
 
 /* ------------------------------------------------------- few rows -------
- * A workgroup of four waves takes 16 weight rows and up to 16 TT rows of
- * tokens; the waves share out K in blocks of 128 and add their sums in LDS.
- * Both operands go straight to registers. Bound: the weight stream. */
-template <int TT, bool GROUPED, int OUT>
-__global__ __launch_bounds__(256) void k_i8_stream(I8Args a)
+ * Weights as whole 128-byte lines: an instruction takes 128 codes of 8 weight
+ * rows, lane l (row l % 8) its 16 codes from 64 (l / 8 % 2) + 16 (l / 16).
+ * Rows 0 - 7 of the MFMA's A operand are then the 8 weight rows at the block's
+ * first 64 codes, rows 8 - 15 the same rows at its last 64; the B operand holds
+ * 8 tokens the same way, and of the 16 x 16 result the two quadrants that
+ * multiply equal codes count. A workgroup takes 8 RT weight rows by 8 TT
+ * tokens, its waves share out K in blocks of 128, B of them in flight, and add
+ * up in LDS. */
+template <int RT, int TT, int NW, int B, bool GROUPED, int OUT>
+__global__ __launch_bounds__(64 * NW) void k_i8_pair(I8Args a)
 {
-    constexpr int NW = 4, B = 2;                   /* waves along K, blocks of 128 in flight a wave */
-    __shared__ int sum[NW][TT][256];
+    constexpr int TR = 8 * TT, FR = 8 * RT;
+    __shared__ int sum[NW][2][TT * RT][64];
     const int lane = threadIdx.x & 63, wave = wave_in_group();
-    const int r = lane & 15, g = lane >> 4;
-    const int slabs = (a.N + 15) / 16, tile = blockIdx.x / slabs, n0 = (blockIdx.x - tile * slabs) * 16;
+    const int r8 = lane & 7, half = (lane >> 3) & 1, g = lane >> 4;
+    const int slabs = (a.N + FR - 1) / FR, tile = blockIdx.x / slabs, n0 = (blockIdx.x - tile * slabs) * FR;
     Tile t;
     if constexpr (GROUPED) {
-        t = bucket_tile<16 * TT>(a, tile, lane);
+        t = bucket_tile<TR>(a, tile, lane);
         if (t.rows <= 0) return;
     } else {
         t.w = a.W; t.s = a.Sw; t.bad = false;
-        t.r0 = tile * 16 * TT;
-        t.rows = min(16 * TT, a.M - t.r0);
+        t.r0 = tile * TR;
+        t.rows = min(TR, a.M - t.r0);
     }
+    const int nf = min(FR, a.N - n0);
     if (GROUPED && t.bad) {
         if (threadIdx.x == 0) atomicOr(a.status, ST_BAD_DESCRIPTOR);
-        for (int i = threadIdx.x; i < t.rows * 16; i += 256)
-            if (n0 + (i & 15) < a.N) i8_store<OUT>(a.C, (size_t)(t.r0 + i / 16) * a.N + n0 + (i & 15), __builtin_nanf(""));
+        for (int i = threadIdx.x; i < t.rows * nf; i += 64 * NW)
+            i8_store<OUT>(a.C, (size_t)(t.r0 + i / nf) * a.N + n0 + i % nf, __builtin_nanf(""));
         return;
     }
     const uint32_t K = (uint32_t)a.K;
-    const __amdgpu_buffer_rsrc_t rw = i8_rsrc(t.w + (size_t)n0 * K, (uint32_t)min(16, a.N - n0) * K);
+    const __amdgpu_buffer_rsrc_t rw = i8_rsrc(t.w + (size_t)n0 * K, (uint32_t)nf * K);
     const uint8_t *xb = GROUPED ? a.Aq : a.Aq + (size_t)t.r0 * K;
     const __amdgpu_buffer_rsrc_t rx = i8_rsrc(xb, GROUPED ? (uint32_t)a.n_a * K : (uint32_t)t.rows * K);
-    /* source row of product row i of the tile; -1 where there is none */
     auto src_of = [&](int i) -> int {
         if (i >= t.rows) return -1;
         if (!GROUPED) return i;
         const int s = a.row_tok ? a.row_tok[t.r0 + i] : t.r0 + i;
         return (unsigned)s < (unsigned)a.n_a ? s : -1;
     };
-    uint32_t xo[TT];
+    const uint32_t kc = 64u * half + 16u * g;
+    uint32_t xo[TT], wo[RT];
 #pragma unroll
     for (int u = 0; u < TT; u++) {
-        const int s = src_of(16 * u + r);
-        xo[u] = s < 0 ? I8_OOB : (uint32_t)s * K + 16u * g;
+        const int s = src_of(8 * u + r8);
+        xo[u] = s < 0 ? I8_OOB : (uint32_t)s * K + kc;
     }
-    const uint32_t wo = (uint32_t)r * K + 16u * g;
+#pragma unroll
+    for (int i = 0; i < RT; i++) wo[i] = (uint32_t)(8 * i + r8) * K + kc;
     const int nblk = (a.K + 127) / 128;
-    v4i acc[TT];
+    v4i acc[RT][TT];
 #pragma unroll
-    for (int u = 0; u < TT; u++) acc[u] = v4i{0, 0, 0, 0};
-    /* codes past K: the tokens' read as zeros, whatever the weights' are */
+    for (int i = 0; i < RT; i++)
+#pragma unroll
+        for (int u = 0; u < TT; u++) acc[i][u] = v4i{0, 0, 0, 0};
     for (int b0 = wave; b0 < nblk; b0 += NW * B) {
-        v4i w[B][2], x[B][2][TT];
+        v4i w[B][RT], x[B][TT];
+#pragma unroll
+        for (int b = 0; b < B; b++) {
+            const uint32_t c = (uint32_t)(b0 + NW * b) * 128u;
+            const bool in = c + kc < K;
+#pragma unroll
+            for (int i = 0; i < RT; i++) w[b][i] = i8_ld16<2>(rw, in ? wo[i] + c : I8_OOB);
+#pragma unroll
+            for (int u = 0; u < TT; u++) x[b][u] = i8_ld16<0>(rx, in && xo[u] != I8_OOB ? xo[u] + c : I8_OOB);
+        }
 #pragma unroll
         for (int b = 0; b < B; b++)
 #pragma unroll
-            for (int h = 0; h < 2; h++) {
-                const int c = (b0 + NW * b) * 128 + 64 * h;
-                const bool in = c + 16 * g < a.K;
-                w[b][h] = i8_ld16<2>(rw, in ? wo + (uint32_t)c : I8_OOB);
-#pragma unroll
-                for (int u = 0; u < TT; u++) x[b][h][u] = i8_ld16<0>(rx, in && xo[u] != I8_OOB ? xo[u] + (uint32_t)c : I8_OOB);
-            }
-#pragma unroll
-        for (int b = 0; b < B; b++)
-#pragma unroll
-            for (int h = 0; h < 2; h++)
+            for (int i = 0; i < RT; i++)
 #pragma unroll
                 for (int u = 0; u < TT; u++)
-                    acc[u] = __builtin_amdgcn_mfma_i32_16x16x64_i8(w[b][h], x[b][h][u], acc[u], 0, 0, 0);
+                    acc[i][u] = __builtin_amdgcn_mfma_i32_16x16x64_i8(w[b][i], x[b][u], acc[i][u], 0, 0, 0);
     }
+    /* element e of lane l: weight row 4 (g % 2) + e at half g / 2, token l % 8
+     * at half l / 8 % 2 */
+    if (half == g >> 1) {
 #pragma unroll
-    for (int u = 0; u < TT; u++)
+        for (int i = 0; i < RT; i++)
 #pragma unroll
-        for (int e = 0; e < 4; e++) sum[wave][u][(4 * g + e) * 16 + r] = acc[u][e];
+            for (int u = 0; u < TT; u++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) sum[wave][half][i * TT + u][r8 * 8 + 4 * (g & 1) + e] = acc[i][u][e];
+    }
     __syncthreads();
-    /* thread: weight row threadIdx % 16 of the workgroup's, row threadIdx / 16 */
-    const int n = threadIdx.x & 15, m16 = threadIdx.x >> 4;
-    if (n0 + n >= a.N) return;
-    const float sw = t.s[n0 + n];
-#pragma unroll
-    for (int u = 0; u < TT; u++) {
-        const int i = 16 * u + m16;
-        if (i >= t.rows) continue;
+    for (int o = threadIdx.x; o < TR * FR; o += 64 * NW) {
+        const int n = o % FR, i = o / FR;
+        if (i >= t.rows || n >= nf) continue;
         int v = 0;
 #pragma unroll
-        for (int w = 0; w < NW; w++) v += sum[w][u][n * 16 + m16];
+        for (int w = 0; w < NW; w++)
+#pragma unroll
+            for (int h = 0; h < 2; h++) v += sum[w][h][(n / 8) * TT + i / 8][(i & 7) * 8 + (n & 7)];
         const int s = src_of(i);
         float f = __builtin_nanf("");
-        if (s >= 0) f = (float)v * (GROUPED ? a.Sa[s] : a.Sa[t.r0 + s]) * sw;
+        if (s >= 0) f = (float)v * (GROUPED ? a.Sa[s] : a.Sa[t.r0 + s]) * t.s[n0 + n];
         else if (n == 0) atomicOr(a.status, ST_BAD_EXPERT_ID);
         i8_store<OUT>(a.C, (size_t)(t.r0 + i) * a.N + n0 + n, f);
     }
 }
 
-template <bool GROUPED, int OUT>
-static hipError_t i8_stream(const I8Args &a, hipStream_t st)
+template <int RT, int TT, int NW, int B, bool GROUPED, int OUT>
+static hipError_t i8_pair(const I8Args &a, hipStream_t st)
 {
-    constexpr int TT = 4, TR = 16 * TT;
+    constexpr int TR = 8 * TT, FR = 8 * RT;
     const long tiles = GROUPED ? a.M / TR + (a.n_experts < a.M ? a.n_experts : a.M) : (a.M + TR - 1) / TR;
-    const long groups = tiles * ((a.N + 15) / 16);
-    if (groups >= 1L << 24) return hipErrorInvalidConfiguration;   /* 2^32 threads */
-    hipLaunchKernelGGL((k_i8_stream<TT, GROUPED, OUT>), dim3((unsigned)groups), dim3(256), 0, st, a);
+    const long groups = tiles * ((a.N + FR - 1) / FR);
+    if (groups * NW >= 1L << 26) return hipErrorInvalidConfiguration;         /* 2^32 threads */
+    hipLaunchKernelGGL((k_i8_pair<RT, TT, NW, B, GROUPED, OUT>), dim3((unsigned)groups), dim3(64 * NW), 0, st, a);
     return hipGetLastError();
+}
+
+/* ------------------------------------------------------ many rows -------
+ * A workgroup takes F features by 16 T rows, wave (wr, wt) F / 4 features by
+ * 16 T / WT rows. K goes in blocks of 128 codes, one staged row a 128-byte
+ * line: both operands by loads straight to LDS into a ring of NST blocks (16-
+ * byte pieces XOR-swizzled by row), a wave reading the operands of the next 64
+ * codes while it multiplies these. One barrier a block: after it every wave's
+ * loads of the next block have landed and no wave still reads this one, so
+ * the block NST ahead takes its place. Loads past K read nothing and multiply
+ * as zeros. The tile leaves through LDS as whole 16-byte pieces of rows. */
+template <int F, int T, int KB, int NST_> struct I8Tile {
+    static constexpr int WT = T >= 4 ? 2 : 1, NWAVE = 4 * WT, U = T / WT, WI = F / 64;
+    static constexpr int OFF_X = F * 128, SUB = OFF_X + 16 * T * 128, STAGE = KB * SUB;
+    static constexpr int NST = NST_;
+    static constexpr int LW = F / 8 / NWAVE, LX = 2 * T / NWAVE, VM = KB * (LW + LX);
+    static constexpr int RING = NST * STAGE;
+    static constexpr int out_ld(int eb) { return F * eb + 16; }
+    static constexpr int lds(int eb) { return RING > 16 * T * out_ld(eb) ? RING : 16 * T * out_ld(eb); }
+    static_assert(LX * NWAVE == 2 * T && LW * NWAVE * 8 == F && (NST - 1) * VM < 64 && lds(4) <= 160 * 1024, "ring");
+};
+
+typedef __attribute__((address_space(3))) void i8_lds;
+
+__device__ __forceinline__ void i8_dma16(__amdgpu_buffer_rsrc_t r, uint32_t voff, int soff, uint8_t *dst)
+{
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (i8_lds *)dst, 16, (int)voff, soff, 0, 0);
+}
+template <int N>
+__device__ __forceinline__ void i8_wait_vm()
+{
+    __builtin_amdgcn_s_waitcnt(0x0F70 | (N & 15) | ((N >> 4) << 14));
+}
+
+template <int F, int T, int KB, int NST, bool GROUPED, int OUT>
+__global__ __launch_bounds__((64 * I8Tile<F, T, KB, NST>::NWAVE)) void k_i8_tile(I8Args a)
+{
+    using C = I8Tile<F, T, KB, NST>;
+    constexpr int U = C::U, WI = C::WI, TR = 16 * T, EB = elem_bytes<OUT>();
+    extern __shared__ __align__(16) uint8_t lds[];
+    const int lane = threadIdx.x & 63, wave = wave_in_group();
+    const int rr = lane & 15, gq = lane >> 4, wr = wave & 3, wt = wave >> 2;
+    const int nt = (a.N + F - 1) / F, nblk = (a.K + 127) / 128, nst = (nblk + KB - 1) / KB;
+    Tile t;
+    int n0;
+    if constexpr (GROUPED) {
+        /* workgroups go round the eight XCDs: with a multiple of eight feature
+         * tiles each XCD's L2 keeps its features of an expert over its rows */
+        const int tile = blockIdx.x / nt;
+        n0 = (blockIdx.x - tile * nt) * F;
+        t = bucket_tile<TR>(a, tile, lane);
+        if (t.rows <= 0) return;
+    } else {
+        /* each XCD a contiguous run of tiles, eight row tiles by their feature
+         * tiles at a time */
+        const int mt = (a.M + TR - 1) / TR, total = mt * nt;
+        const int per = total / 8, rest = total % 8, x = blockIdx.x % 8, y = blockIdx.x / 8;
+        const int id = x * per + min(x, rest) + y;
+        const int grp = id / (8 * nt), gm = min(8, mt - 8 * grp), in = id - grp * 8 * nt;
+        t.w = a.W; t.s = a.Sw; t.bad = false;
+        t.r0 = (8 * grp + in % gm) * TR;
+        t.rows = min(TR, a.M - t.r0);
+        n0 = in / gm * F;
+    }
+    const int nf = min(F, a.N - n0);
+    if (GROUPED && t.bad) {
+        if (threadIdx.x == 0) atomicOr(a.status, ST_BAD_DESCRIPTOR);
+        for (int i = threadIdx.x; i < t.rows * nf; i += 64 * C::NWAVE)
+            i8_store<OUT>(a.C, (size_t)(t.r0 + i / nf) * a.N + n0 + i % nf, __builtin_nanf(""));
+        return;
+    }
+    const uint32_t K = (uint32_t)a.K;
+    const __amdgpu_buffer_rsrc_t rw = i8_rsrc(t.w + (size_t)n0 * K, (uint32_t)nf * K);
+    const uint8_t *xb = GROUPED ? a.Aq : a.Aq + (size_t)t.r0 * K;
+    const __amdgpu_buffer_rsrc_t rx = i8_rsrc(xb, GROUPED ? (uint32_t)a.n_a * K : (uint32_t)t.rows * K);
+    auto src_of = [&](int i) -> int {              /* row of Aq from xb on; -1: none */
+        if (i >= t.rows) return -1;
+        if (!GROUPED) return i;
+        const int s = a.row_tok ? a.row_tok[t.r0 + i] : t.r0 + i;
+        return (unsigned)s < (unsigned)a.n_a ? s : -1;
+    };
+    auto swz = [](int r, int c) { return c ^ ((r >> 1) & 7); };
+    uint32_t wo[C::LW], xo[C::LX], xl[C::LX];      /* xl: of the last block, pieces past K out of range */
+#pragma unroll
+    for (int i = 0; i < C::LW; i++) {
+        const int r = 8 * (C::LW * wave + i) + lane / 8;
+        wo[i] = (uint32_t)r * K + 16u * (uint32_t)swz(r, lane & 7);
+    }
+#pragma unroll
+    for (int i = 0; i < C::LX; i++) {
+        const int r = 8 * (C::LX * wave + i) + lane / 8, c = swz(r, lane & 7), s = src_of(r);
+        xo[i] = s < 0 ? I8_OOB : (uint32_t)s * K + 16u * (uint32_t)c;
+        xl[i] = (nblk - 1) * 128 + 16 * c < a.K ? xo[i] : I8_OOB;
+    }
+    /* load i of a wave's share of stage st; past the end zeros, no traffic */
+    auto issue = [&](int st, int slot, int i) {
+        constexpr int LB = C::LW + C::LX;
+        const int blk = st * KB + i / LB, k = i % LB;
+        const uint32_t oob = blk < nblk ? 0u : I8_OOB;
+        const int so = min(blk, nblk - 1) * 128;
+        uint8_t *buf = lds + slot * C::STAGE + i / LB * C::SUB;
+        if (k < C::LW) i8_dma16(rw, wo[min(k, C::LW - 1)] | oob, so, buf + 1024 * (C::LW * wave + k));
+        else {
+            const int j = max(0, min(k - C::LW, C::LX - 1));
+            i8_dma16(rx, (blk < nblk - 1 ? xo[j] : xl[j]) | oob, so, buf + C::OFF_X + 1024 * (C::LX * wave + j));
+        }
+    };
+#pragma unroll
+    for (int s = 0; s < C::NST; s++)
+#pragma unroll
+        for (int i = 0; i < C::VM; i++) issue(s, s, i);
+
+    struct Op { v4i w[WI], x[U]; };
+    auto read_w = [&](Op &o, const uint8_t *buf, int i, int h) {
+        const int r = 16 * (WI * wr + i) + rr;
+        o.w[i] = *(const v4i *)(buf + r * 128 + 16 * swz(r, gq + 4 * h));
+    };
+    auto read_x = [&](Op &o, const uint8_t *buf, int u, int h) {
+        const int r = 16 * (U * wt + u) + rr;
+        o.x[u] = *(const v4i *)(buf + C::OFF_X + r * 128 + 16 * swz(r, gq + 4 * h));
+    };
+    v4i acc[WI][U];
+#pragma unroll
+    for (int i = 0; i < WI; i++)
+#pragma unroll
+        for (int u = 0; u < U; u++) acc[i][u] = v4i{0, 0, 0, 0};
+    int slot = 0;
+    /* the products of `cur`, the reads of `nxt` (half h of the block in buf)
+     * and, with LOAD, block st's loads into slot `to`, spread among them */
+    auto half = [&](const Op &cur, Op &nxt, const uint8_t *buf, int h, bool load, int st, int to) {
+#pragma unroll
+        for (int q = 0; q < WI * U; q++) {
+            constexpr int N = WI * U, R = WI + U;
+            acc[q % WI][q / WI] = __builtin_amdgcn_mfma_i32_16x16x64_i8(cur.w[q % WI], cur.x[q / WI], acc[q % WI][q / WI], 0, 0, 0);
+#pragma unroll
+            for (int j = 0; j < R; j++)
+                if (j * N / (R + 1) == q) {
+                    if (j < WI) read_w(nxt, buf, j, h);
+                    else read_x(nxt, buf, j - WI, h);
+                }
+            if (load) {
+#pragma unroll
+                for (int l = 0; l < C::VM; l++)
+                    if (l * N / C::VM == q) issue(st, to, l);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    };
+    i8_wait_vm<(C::NST - 1) * C::VM>();
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    Op o0, o1;
+#pragma unroll
+    for (int i = 0; i < WI; i++) read_w(o0, lds, i, 0);
+#pragma unroll
+    for (int u = 0; u < U; u++) read_x(o0, lds, u, 0);
+    for (int st = 0; st < nst; st++) {
+        const uint8_t *buf = lds + slot * C::STAGE;
+#pragma unroll
+        for (int j = 0; j + 2 < 2 * KB; j += 2) {
+            half(o0, o1, buf + j / 2 * C::SUB, 1, false, 0, 0);
+            half(o1, o0, buf + (j / 2 + 1) * C::SUB, 0, false, 0, 0);
+        }
+        half(o0, o1, buf + (KB - 1) * C::SUB, 1, false, 0, 0);
+        __builtin_amdgcn_s_waitcnt(0xC07F);        /* this stage's operands are in registers */
+        i8_wait_vm<(C::NST - 2) * C::VM>();        /* the wave's loads of the next have landed */
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+        const int free = slot;
+        slot = slot + 1 == C::NST ? 0 : slot + 1;
+        half(o1, o0, lds + slot * C::STAGE, 0, true, st + C::NST, free);
+    }
+    /* the loads past the end, then the ring becomes the output tile */
+    __builtin_amdgcn_s_waitcnt(0xC07F);
+    i8_wait_vm<0>();
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    constexpr int LD = C::out_ld(EB);
+    float sw[WI][4];
+#pragma unroll
+    for (int i = 0; i < WI; i++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            const int n = 16 * (WI * wr + i) + 4 * gq + e;
+            sw[i][e] = n < nf ? gptr(t.s)[n0 + n] : 0.0f;
+        }
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+        const int m = 16 * (U * wt + u) + rr, s = src_of(m);
+        const float sa = s >= 0 ? gptr(a.Sa)[GROUPED ? s : t.r0 + s] : __builtin_nanf("");
+        if (GROUPED && s < 0 && m < t.rows && wr == 0 && gq == 0) atomicOr(a.status, ST_BAD_EXPERT_ID);
+#pragma unroll
+        for (int i = 0; i < WI; i++) {
+            uint8_t *o = lds + m * LD + (16 * (WI * wr + i) + 4 * gq) * EB;
+            float v[4];
+#pragma unroll
+            for (int e = 0; e < 4; e++) v[e] = (float)acc[i][u][e] * sa * sw[i][e];
+            if constexpr (OUT == DSV4_HIP_F32) {
+                *(f32x4 *)o = f32x4{v[0], v[1], v[2], v[3]};
+            } else {
+                uint2 p;
+                p.x = narrow16<OUT>(v[0]) | (narrow16<OUT>(v[1]) << 16);
+                p.y = narrow16<OUT>(v[2]) | (narrow16<OUT>(v[3]) << 16);
+                *(uint2 *)o = p;
+            }
+        }
+    }
+    __syncthreads();
+    uint8_t *out = (uint8_t *)a.C + ((size_t)t.r0 * a.N + n0) * EB;
+    const size_t ld = (size_t)a.N * EB;
+    if ((((uintptr_t)a.C | ld) & 15u) == 0) {      /* whole pieces: n0 and nf are multiples of one too */
+        const int pieces = nf * EB / 16;
+        constexpr int PMAX = F * EB / 16;
+        for (int i = threadIdx.x; i < t.rows * PMAX; i += 64 * C::NWAVE) {
+            const int m = i / PMAX, p = i % PMAX;
+            if (p < pieces)
+                __builtin_nontemporal_store(*(const u32x4 *)(lds + m * LD + 16 * p), (DSV4_GLOBAL u32x4 *)(out + m * ld + 16 * p));
+        }
+    } else {
+        for (int i = threadIdx.x; i < t.rows * F; i += 64 * C::NWAVE) {
+            const int m = i / F, n = i % F;
+            if (n >= nf) continue;
+            if constexpr (EB == 4) *(float *)(out + m * ld + 4 * n) = *(const float *)(lds + m * LD + 4 * n);
+            else *(uint16_t *)(out + m * ld + 2 * n) = *(const uint16_t *)(lds + m * LD + 2 * n);
+        }
+    }
+}
+
+template <int F, int T, int KB, int NST, bool GROUPED, int OUT>
+static hipError_t i8_tile(const I8Args &a, hipStream_t st)
+{
+    using C = I8Tile<F, T, KB, NST>;
+    constexpr int TR = 16 * T;
+    constexpr int lds = C::lds(elem_bytes<OUT>());
+    static bool attr_done = false;
+    if (!attr_done) {
+        const hipError_t e = hipFuncSetAttribute((const void *)k_i8_tile<F, T, KB, NST, GROUPED, OUT>,
+                                                 hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+        if (e != hipSuccess) return e;
+        attr_done = true;
+    }
+    const long tiles = GROUPED ? a.M / TR + (a.n_experts < a.M ? a.n_experts : a.M) : (a.M + TR - 1) / TR;
+    const long groups = tiles * ((a.N + F - 1) / F);
+    if (groups * C::NWAVE >= 1L << 26) return hipErrorInvalidConfiguration;   /* 2^32 threads */
+    hipLaunchKernelGGL((k_i8_tile<F, T, KB, NST, GROUPED, OUT>), dim3((unsigned)groups), dim3(64 * C::NWAVE), lds, st, a);
+    return hipGetLastError();
+}
+
+template <bool GROUPED, int OUT>
+static hipError_t i8_launch(const I8Args &a, hipStream_t st)
+{
+    const int form = GROUPED ? i8_grouped_form(a.M, a.N, a.K, a.n_experts) : i8_form(a.M, a.N, a.K);
+    if constexpr (GROUPED) {
+        if (form == I8_PAIR) return i8_pair<4, 2, 4, 2, GROUPED, OUT>(a, st);
+    } else {
+        if (form == I8_PAIR) return i8_pair<1, 1, 8, 4, GROUPED, OUT>(a, st);
+        if (form == I8_64x2_DEEP) return i8_tile<64, 2, 2, 3, GROUPED, OUT>(a, st);
+        if (form == I8_64x4) return i8_tile<64, 4, 1, 3, GROUPED, OUT>(a, st);
+        if (form == I8_128x8) return i8_tile<128, 8, 1, 4, GROUPED, OUT>(a, st);
+    }
+    switch (form) {
+    case I8_64x2: return i8_tile<64, 2, 1, 4, GROUPED, OUT>(a, st);
+    case I8_128x4: return i8_tile<128, 4, 1, 3, GROUPED, OUT>(a, st);
+    default: return i8_tile<256, 8, 1, 3, GROUPED, OUT>(a, st);
+    }
 }
 
 hipError_t gemm_i8_launch(const I8Args &a, int out_type, hipStream_t st)
@@ -222,9 +497,9 @@ hipError_t gemm_i8_launch(const I8Args &a, int out_type, hipStream_t st)
     if (a.M <= 0 || a.N <= 0 || a.K <= 0 || a.K % 16) return hipErrorInvalidValue;
     const bool grouped = a.table != nullptr;
     switch (out_type) {
-    case DSV4_HIP_F32: return grouped ? i8_stream<true, DSV4_HIP_F32>(a, st) : i8_stream<false, DSV4_HIP_F32>(a, st);
-    case DSV4_HIP_BF16: return grouped ? i8_stream<true, DSV4_HIP_BF16>(a, st) : i8_stream<false, DSV4_HIP_BF16>(a, st);
-    case DSV4_HIP_F16: return grouped ? i8_stream<true, DSV4_HIP_F16>(a, st) : i8_stream<false, DSV4_HIP_F16>(a, st);
+    case DSV4_HIP_F32: return grouped ? i8_launch<true, DSV4_HIP_F32>(a, st) : i8_launch<false, DSV4_HIP_F32>(a, st);
+    case DSV4_HIP_BF16: return grouped ? i8_launch<true, DSV4_HIP_BF16>(a, st) : i8_launch<false, DSV4_HIP_BF16>(a, st);
+    case DSV4_HIP_F16: return grouped ? i8_launch<true, DSV4_HIP_F16>(a, st) : i8_launch<false, DSV4_HIP_F16>(a, st);
     default: return hipErrorInvalidValue;
     }
 }

@@ -212,7 +212,8 @@ SHAPES = [(1, 4096, 4096), (1, 1, 16), (1, 17, 48), (2, 255, 1040), (5, 300, 512
           (9, 64, 128), (15, 33, 4096), (16, 16, 64), (17, 257, 80), (31, 1024, 144), (33, 515, 1024), (63, 48, 272),
           (64, 64, 4096), (65, 129, 96), (100, 1000, 512), (129, 128, 128), (130, 384, 1136), (257, 260, 2048),
           (300, 1024, 4096), (333, 777, 4112), (512, 513, 640), (1000, 1023, 208), (2048, 256, 1024),
-          (701, 2048, 4096), (1300, 1536, 16), (3, 5, 16384), (2, 40000, 256), (4097, 100, 192), (2051, 4099, 528)]
+          (701, 2048, 4096), (1300, 1536, 16), (3, 5, 16384), (2, 40000, 256), (4097, 100, 192), (2051, 4099, 528),
+          (1000, 4096, 528), (1025, 4080, 272), (2048, 4096, 4096), (2050, 4100, 1040), (40, 32768, 1024), (14, 700, 8208)]
 
 
 @pytest.mark.parametrize("M,N,K", SHAPES)
@@ -327,7 +328,9 @@ def buckets(counts):
 GROUPS = [([0, 0, 1, 0], 40, 64), ([3, 0, 17, 5, 64, 1], 130, 272), ([65, 0, 128, 129], 257, 512), ([300], 100, 1040),
           ([0] * 70 + [2] + [0] * 60 + [1, 1, 40], 48, 128), ([1] * 256, 64, 4096), ([2, 1] * 500, 33, 48),
           ([700, 3, 0, 0, 40, 1], 515, 2048), ([0, 0], 16, 16), ([16, 15, 17, 33, 31, 32], 512, 144),
-          ([100, 90, 110, 95] * 4, 1024, 640)]
+          ([100, 90, 110, 95] * 4, 1024, 640), ([1, 0, 3, 16, 2, 9, 40, 1] * 8, 1030, 1040),
+          ([0, 7, 20, 1] * 16, 1024, 2064),
+          ([40, 0, 30, 50, 65], 300, 272)]
 
 
 @pytest.mark.parametrize("case", range(len(GROUPS)))

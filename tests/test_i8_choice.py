@@ -1,0 +1,54 @@
+# SPDX-License-Identifier: Apache-2.0
+"""The rules that pick an int8 product's form by its sizes (csrc/dsv4_choose.h),
+compiled for the host: the forms that were measured to be the faster ones, and
+that the GPU tests of the products reach every form."""
+import ctypes as C
+import os
+import subprocess
+
+import pytest
+
+import test_gpu_i8
+from conftest import PKG_DIR
+
+SHIM = """
+#include "dsv4_choose.h"
+using namespace dsv4;
+extern "C" {
+int c_form(int M, int N, int K) { return i8_form(M, N, K); }
+int c_grouped(int M, int N, int K, int ne) { return i8_grouped_form(M, N, K, ne); }
+}
+"""
+PAIR, T64x2, T64x2_DEEP, T64x4, T128x4, T128x8, T256x8 = range(1, 8)
+
+
+@pytest.fixture(scope="module")
+def rules(tmp_path_factory):
+    d = tmp_path_factory.mktemp("i8")
+    src, so = d / "shim.cpp", d / "shim.so"
+    src.write_text(SHIM)
+    subprocess.run(["g++", "-O1", "-std=c++17", "-Wall", "-Werror", "-shared", "-fPIC", "-I",
+                    os.path.join(PKG_DIR, "csrc"), str(src), "-o", str(so)], check=True)
+    return C.CDLL(str(so))
+
+
+@pytest.mark.parametrize("M,N,K,form", [
+    (1, 4096, 4096, PAIR), (8, 4096, 4096, PAIR), (12, 1024, 4096, PAIR), (16, 4096, 4096, T64x2_DEEP),
+    (128, 4096, 4096, T64x2_DEEP), (333, 1024, 4096, T64x2_DEEP), (5, 32768, 1024, T64x2), (333, 4096, 4096, T128x4),
+    (1000, 2048, 2048, T128x4), (1024, 4096, 4096, T128x8), (2048, 4096, 4096, T256x8), (1000, 32768, 1024, T256x8)])
+def test_product_form(rules, M, N, K, form):
+    assert rules.c_form(M, N, K) == form
+
+
+@pytest.mark.parametrize("M,N,K,ne,form", [
+    (6, 2048, 4096, 256, T64x2), (42, 2048, 4096, 256, PAIR), (1536, 2048, 4096, 256, PAIR),
+    (160, 512, 1024, 64, T64x2), (12288, 2048, 4096, 256, T128x4), (24576, 2048, 4096, 256, T256x8),
+    (6144, 2048, 4096, 64, T256x8)])
+def test_experts_form(rules, M, N, K, ne, form):
+    assert rules.c_grouped(M, N, K, ne) == form
+
+
+def test_gpu_tests_reach_every_form(rules):
+    assert {rules.c_form(*s) for s in test_gpu_i8.SHAPES} == set(range(1, 8))
+    groups = {rules.c_grouped(sum(c) + 5, N, K, len(c)) for c, N, K in test_gpu_i8.GROUPS}
+    assert groups == {PAIR, T64x2, T128x4, T256x8}
