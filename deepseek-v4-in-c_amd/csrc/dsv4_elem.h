@@ -53,6 +53,17 @@ struct Elem {
         else if constexpr (TYPE == DSV4_HIP_F32) *(DSV4_GLOBAL uint32_t *)p = raw.x;
         else *(DSV4_GLOBAL uint16_t *)p = (uint16_t)raw.x;
     }
+    /* bytes that the call touches once */
+    __device__ __forceinline__ void load_stream(const void *p)
+    {
+        if constexpr (V > 1) raw = __builtin_nontemporal_load(gptr((const u32x4 *)p));
+        else load(p);
+    }
+    __device__ __forceinline__ void store_stream(void *p) const
+    {
+        if constexpr (V > 1) __builtin_nontemporal_store(raw, (DSV4_GLOBAL u32x4 *)p);
+        else store(p);
+    }
     __device__ __forceinline__ void get(float (&f)[V]) const
     {
         if constexpr (TYPE == DSV4_HIP_F32) {

@@ -14,6 +14,7 @@
  * topk)) adds nothing, receives nothing and has dw 0. All of them stream
  * memory and are bound by it; none uses a workspace.
  */
+#include <algorithm>
 #include <initializer_list>
 
 #include "dsv4_elem.h"
@@ -24,7 +25,7 @@ namespace dsv4 {
 namespace {
 
 constexpr int MAX_E = 1024, MAX_TOPK = 16;
-constexpr size_t MAX_THREADS = 0xFFFFFF00u;        /* of one launch               */
+constexpr long MAX_WAVES = (1L << 26) - 4;         /* of one launch: 2^32 threads */
 
 /* Lanes of the wave that hold the same expert id; ids outside [0, E) share
  * one of their own. One ballot a bit of id + 1. */
@@ -70,10 +71,10 @@ __device__ __forceinline__ int scan_wave(int *off, const int *cnt, int E, int la
     return __shfl(incl, 63, 64);
 }
 
-/* pairs of each expert among [lo, hi) to cnt and, of those below `own`, to
- * bef: a wave takes 64 pairs, one LDS add an expert and wave. Returns whether
- * this thread met an id that is neither an expert nor -1. */
-__device__ __forceinline__ bool count_pairs(int *cnt, int *bef, const int *idx, int lo, int hi, int own, int E)
+/* Pairs of each expert among [lo, hi) to cnt: a wave takes 64 pairs, one LDS
+ * add an expert and wave. Returns whether this thread met an id that is neither
+ * an expert nor -1. */
+__device__ __forceinline__ bool count_pairs(int *cnt, const int *idx, int lo, int hi, int E)
 {
     const int lane = threadIdx.x & 63, bits = id_bits(E);
     bool bad = false;
@@ -82,13 +83,7 @@ __device__ __forceinline__ bool count_pairs(int *cnt, int *bef, const int *idx, 
         const int e = p < hi ? idx[p] : -1;
         bad |= e != -1 && (unsigned)e >= (unsigned)E;
         const uint64_t peers = lanes_of_id(e, E, bits);
-        if ((unsigned)e < (unsigned)E && (peers & lanes_below(lane)) == 0) {
-            atomicAdd(&cnt[e], __popcll(peers));
-            if (bef && p0 < own) {
-                const int n = __popcll(own - p0 >= 64 ? peers : peers & lanes_below(own - p0));
-                if (n) atomicAdd(&bef[e], n);
-            }
-        }
+        if ((unsigned)e < (unsigned)E && (peers & lanes_below(lane)) == 0) atomicAdd(&cnt[e], __popcll(peers));
     }
     return bad;
 }
@@ -97,57 +92,125 @@ __device__ __forceinline__ bool count_pairs(int *cnt, int *bef, const int *idx, 
 
 /* ---------------------------------------------------------------- sort --- */
 
-/* Sort and copy in one launch: workgroup b owns `tpb` tokens (at most 128
+/* Sort and copy in one launch: workgroup b owns `tpb` tokens (at most 256
  * pairs), counts every pair by itself (at most 32,768: 128 KB of ids from L2),
- * places its own and copies their rows. No workgroup waits for another. */
+ * places its own and copies their rows. No workgroup waits for another. Its
+ * tokens' first PF vectors a thread are in flight while it counts. A counter
+ * word holds the expert's pairs in the low half and those before the
+ * workgroup's own in the high half. Lanes that share the first lane's id add
+ * once for all of them, so an expert that takes most pairs does not serialise
+ * the adds. Eight ids a thread are asked for together. */
 template <int TYPE, int V>
-__global__ __launch_bounds__(512) void k_permute_one(PermuteArgs a, int tpb)
+__global__ __launch_bounds__(1024) void k_permute_one(PermuteArgs a, int tpb)
 {
-    __shared__ int cnt[MAX_E], bef[MAX_E], off[MAX_E];
-    __shared__ int own_id[128], own_row[128];
+    constexpr int NT = 1024, PF = 8, IDS = 8, EB = elem_bytes<TYPE>();
+    static_assert(PERMUTE_ONE_MAX < 65536, "two counts in a word");
+    __shared__ uint32_t cnt[MAX_E];
+    __shared__ int off[MAX_E];
+    __shared__ int own_row[256];
     const int tid = threadIdx.x, lane = tid & 63, E = a.n_experts;
     const int npairs = a.n * a.topk;
     const int t0 = blockIdx.x * tpb, nt = min(tpb, a.n - t0);
-    const int p0 = t0 * a.topk, np = nt * a.topk;  /* nt may be 0 in a call without tokens */
-    for (int e = tid; e < E; e += 512) {
-        cnt[e] = 0;
-        bef[e] = 0;
-    }
-    if (tid < np) own_id[tid] = a.idx[p0 + tid];
-    __syncthreads();
-    const bool bad = count_pairs(cnt, bef, a.idx, 0, npairs, p0, E);
-    if (bad && blockIdx.x == 0) atomicOr(a.status, ST_BAD_EXPERT_ID);
-    __syncthreads();
-    if (tid < 64) {
-        const int total = scan_wave(off, cnt, E, lane);
-        if (blockIdx.x == 0 && lane == 0) a.ex_off[E] = total;
-    }
-    __syncthreads();
-    if (blockIdx.x == 0)
-        for (int e = tid; e < E; e += 512) a.ex_off[e] = off[e];
-    if (tid < np) {
-        const int e = own_id[tid];
-        int r = -1;
-        if ((unsigned)e < (unsigned)E) {
-            r = off[e] + bef[e];
-            for (int i = 0; i < tid; i++) r += own_id[i] == e;
-            a.row_tok[r] = t0 + tid / a.topk;
-        }
-        a.pos[p0 + tid] = r;
-        own_row[tid] = r;
-    }
-    __syncthreads();
-    constexpr int EB = elem_bytes<TYPE>();
+    const int p0 = t0 * a.topk, np = nt * a.topk;  /* nt is 0 in a call without tokens */
     const int nv = a.hidden / V;
     const size_t rowb = (size_t)a.hidden * EB;
-    for (int t = 0; t < nt; t++) {
-        const uint8_t *src = (const uint8_t *)a.x + (size_t)(t0 + t) * rowb;
-        for (int i = tid; i < nv; i += 512) {
-            Elem<TYPE, V> v;
-            v.load(src + (size_t)i * V * EB);
+    const long items = (long)nt * nv;              /* vectors of the workgroup's tokens, one after another */
+    const uint8_t *src = (const uint8_t *)a.x + (size_t)t0 * rowb;
+    Elem<TYPE, V> v[PF];
+    auto fetch = [&](long base) {
+#pragma unroll
+        for (int j = 0; j < PF; j++) {
+            const long it = base + j * NT + tid;
+            if (it < items) v[j].load(src + (size_t)it * V * EB);
+        }
+    };
+    if (tid < E) cnt[tid] = 0;
+    fetch(0);
+    __syncthreads();
+    bool bad = false;
+    for (int b0 = 0; b0 < npairs; b0 += IDS * NT) {
+        int id[IDS];
+#pragma unroll
+        for (int i = 0; i < IDS; i++) {
+            const int q = b0 + i * NT + tid;
+            id[i] = q < npairs ? a.idx[q] : -1;
+        }
+#pragma unroll
+        for (int i = 0; i < IDS; i++) {
+            const int q0 = b0 + i * NT + (tid & ~63), e = id[i];
+            if (q0 >= npairs) break;               /* the wave's */
+            const bool ok = (unsigned)e < (unsigned)E;
+            bad |= !ok && e != -1;
+            const int e0 = __builtin_amdgcn_readfirstlane(e);
+            const uint64_t same = __ballot(e == e0);
+            if (e != e0) {
+                if (ok) atomicAdd(&cnt[e], q0 + lane < p0 ? 0x10001u : 1u);
+            } else if (ok && lane == 0) {
+                const int before = min(max(p0 - q0, 0), 64);
+                const uint64_t m = before == 64 ? same : same & lanes_below(before);
+                atomicAdd(&cnt[e], (uint32_t)__popcll(same) + ((uint32_t)__popcll(m) << 16));
+            }
+        }
+    }
+    if (bad && blockIdx.x == 0) atomicOr(a.status, ST_BAD_EXPERT_ID);
+    __syncthreads();
+    if (tid < 64) {                                /* first rows: exclusive scan of the counts */
+        const int per = (E + 63) / 64;
+        int sum = 0;
+        for (int i = 0; i < per; i++) {
+            const int e = lane * per + i;
+            sum += e < E ? (int)(cnt[e] & 0xFFFFu) : 0;
+        }
+        int incl = sum;
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) {
+            const int u = __shfl_up(incl, d, 64);
+            if (lane >= d) incl += u;
+        }
+        int run = incl - sum;
+        for (int i = 0; i < per; i++) {
+            const int e = lane * per + i;
+            if (e < E) {
+                off[e] = run;
+                run += (int)(cnt[e] & 0xFFFFu);
+            }
+        }
+        if (blockIdx.x == 0 && lane == 63) a.ex_off[E] = incl;
+    }
+    __syncthreads();
+    if (blockIdx.x == 0 && tid < E) a.ex_off[tid] = off[tid];
+    /* own pairs, a wave of them after the other: the high halves run on */
+    const int bits = id_bits(E);
+    for (int w = 0; w < (np + 63) / 64; w++) {
+        if ((tid >> 6) == w) {
+            const int e = tid < np ? a.idx[p0 + tid] : -1;
+            const bool ok = (unsigned)e < (unsigned)E;
+            const uint64_t peers = lanes_of_id(e, E, bits);
+            const int rank = __popcll(peers & lanes_below(lane));
+            int r = -1;
+            if (ok) {
+                r = off[e] + (int)(cnt[e] >> 16) + rank;
+                a.row_tok[r] = t0 + tid / a.topk;
+            }
+            if (ok && rank == 0) cnt[e] += (uint32_t)__popcll(peers) << 16;
+            if (tid < np) {
+                a.pos[p0 + tid] = r;
+                own_row[tid] = r;
+            }
+        }
+        __syncthreads();
+    }
+    for (long base = 0; base < items; base += PF * NT) {
+        if (base) fetch(base);
+#pragma unroll
+        for (int j = 0; j < PF; j++) {
+            const long it = base + j * NT + tid;
+            if (it >= items) break;
+            const int t = (int)((uint32_t)it / (uint32_t)nv), i = (int)it - t * nv;
+            uint8_t *dst = (uint8_t *)a.rows + (size_t)i * V * EB;
             for (int k = 0; k < a.topk; k++) {
                 const int r = own_row[t * a.topk + k];
-                if (r >= 0) v.store((uint8_t *)a.rows + (size_t)r * rowb + (size_t)i * V * EB);
+                if (r >= 0) v[j].store_stream(dst + (size_t)r * rowb);
             }
         }
     }
@@ -165,7 +228,7 @@ __global__ __launch_bounds__(1024) void k_permute_count(PermuteArgs a, int nch)
     const int tid = threadIdx.x, c = blockIdx.x;
     cnt[tid] = 0;
     __syncthreads();
-    const bool bad = count_pairs(cnt, nullptr, a.idx, c * 1024, chunk_end(c, nch, a.n * a.topk), 0, a.n_experts);
+    const bool bad = count_pairs(cnt, a.idx, c * 1024, chunk_end(c, nch, a.n * a.topk), a.n_experts);
     if (bad) atomicOr(a.status, ST_BAD_EXPERT_ID);
     __syncthreads();
     if (tid < a.n_experts) a.pos[c * 1024 + tid] = cnt[tid];
@@ -224,64 +287,97 @@ __global__ __launch_bounds__(1024) void k_permute_place(PermuteArgs a, int nch)
     }
 }
 
-/* a thread copies one vector of a token to its topk rows */
+/* Wave w of a launch takes 128 vectors of a token, so that the token's rows
+ * and weights are scalar loads and the branches on them uniform. */
+constexpr int WAVE_VECS = 128;
+struct WaveItem {
+    int t, j;                                      /* token, the lane's first vector (the second is 64 on) */
+};
+__device__ __forceinline__ WaveItem wave_item(int nv)
+{
+    const int cpt = (nv + WAVE_VECS - 1) / WAVE_VECS, w = wave_id();
+    const int t = __builtin_amdgcn_readfirstlane((int)((uint32_t)w / (uint32_t)cpt));
+    return WaveItem{t, (w - t * cpt) * WAVE_VECS + (int)(threadIdx.x & 63)};
+}
+
+/* a token's vectors to its topk rows */
 template <int TYPE, int V>
 __global__ __launch_bounds__(256) void k_permute_copy(PermuteArgs a)
 {
     constexpr int EB = elem_bytes<TYPE>();
     const int nv = a.hidden / V;
-    const size_t i = (size_t)blockIdx.x * 256 + threadIdx.x;
-    if (i >= (size_t)a.n * nv) return;
-    const int t = (int)(i / nv), j = (int)(i - (size_t)t * nv);
-    const size_t rowb = (size_t)a.hidden * EB, o = (size_t)j * V * EB;
-    Elem<TYPE, V> v;
-    v.load((const uint8_t *)a.x + t * rowb + o);
+    const WaveItem it = wave_item(nv);
+    if (it.t >= a.n) return;
+    const size_t rowb = (size_t)a.hidden * EB;
+    Elem<TYPE, V> v[2];
+#pragma unroll
+    for (int h = 0; h < 2; h++)
+        if (it.j + 64 * h < nv) v[h].load((const uint8_t *)a.x + it.t * rowb + (size_t)(it.j + 64 * h) * V * EB);
     for (int k = 0; k < a.topk; k++) {
-        const int r = a.pos[(size_t)t * a.topk + k];
-        if (r >= 0) v.store((uint8_t *)a.rows + r * rowb + o);
+        const int r = ld_uniform(a.pos, it.t * a.topk + k);
+        if (r < 0) continue;
+#pragma unroll
+        for (int h = 0; h < 2; h++)
+            if (it.j + 64 * h < nv) v[h].store_stream((uint8_t *)a.rows + r * rowb + (size_t)(it.j + 64 * h) * V * EB);
     }
 }
 
 /* ------------------------------------------------------------ way back --- */
 
-/* A thread sums one vector over the token's topk rows, every row's load
- * issued before the first is used. W: weights (else 1). */
+/* A lane sums two vectors over the token's topk rows, every row's load issued
+ * before the first is used. W: weights (else 1). */
 template <int TYPE, int V, int KMAX, bool W>
 __global__ __launch_bounds__(256) void k_unpermute(UnpermuteArgs a)
 {
     constexpr int EB = elem_bytes<TYPE>();
     const int nv = a.hidden / V;
-    const size_t i = (size_t)blockIdx.x * 256 + threadIdx.x;
-    if (i >= (size_t)a.n * nv) return;
-    const int t = (int)(i / nv), j = (int)(i - (size_t)t * nv);
-    const size_t rowb = (size_t)a.hidden * EB, o = (size_t)j * V * EB;
+    const WaveItem it = wave_item(nv);
+    if (it.t >= a.n) return;
+    const size_t rowb = (size_t)a.hidden * EB;
     const int nrows = a.n * a.topk;
     int p[KMAX];
 #pragma unroll
-    for (int k = 0; k < KMAX; k++) p[k] = k < a.topk ? a.pos[(size_t)t * a.topk + k] : -1;
-    Elem<TYPE, V> v[KMAX], s;
-#pragma unroll
-    for (int k = 0; k < KMAX; k++)
-        if ((unsigned)p[k] < (unsigned)nrows) v[k].load((const uint8_t *)a.rows + p[k] * rowb + o);
-    if (a.shared) s.load((const uint8_t *)a.shared + t * rowb + o);
-    float acc[V], f[V];
-#pragma unroll
-    for (int q = 0; q < V; q++) acc[q] = 0.0f;
+    for (int k = 0; k < KMAX; k++) p[k] = k < a.topk ? ld_uniform(a.pos, it.t * a.topk + k) : -1;
+    const bool two = it.j + 64 < nv;
+    if (it.j >= nv) return;
+    const size_t o0 = (size_t)it.j * V * EB, o1 = two ? o0 + (size_t)64 * V * EB : o0;
+    Elem<TYPE, V> v[KMAX][2], s[2];
 #pragma unroll
     for (int k = 0; k < KMAX; k++)
         if ((unsigned)p[k] < (unsigned)nrows) {
-            const float w = W ? a.w[(size_t)t * a.topk + k] : 1.0f;
-            v[k].get(f);
-#pragma unroll
-            for (int q = 0; q < V; q++) acc[q] = W ? fmaf(w, f[q], acc[q]) : acc[q] + f[q];
+            v[k][0].load_stream((const uint8_t *)a.rows + p[k] * rowb + o0);
+            v[k][1].load_stream((const uint8_t *)a.rows + p[k] * rowb + o1);
         }
     if (a.shared) {
-        s.get(f);
-#pragma unroll
-        for (int q = 0; q < V; q++) acc[q] += f[q];
+        s[0].load((const uint8_t *)a.shared + it.t * rowb + o0);
+        s[1].load((const uint8_t *)a.shared + it.t * rowb + o1);
     }
-    s.set(acc);
-    s.store((uint8_t *)a.out + t * rowb + o);
+    float acc[2][V], f[V];
+#pragma unroll
+    for (int q = 0; q < V; q++) acc[0][q] = acc[1][q] = 0.0f;
+#pragma unroll
+    for (int k = 0; k < KMAX; k++)
+        if ((unsigned)p[k] < (unsigned)nrows) {
+            const float w = W ? ld_uniform(a.w, it.t * a.topk + k) : 1.0f;
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                v[k][h].get(f);
+#pragma unroll
+                for (int q = 0; q < V; q++) acc[h][q] = W ? fmaf(w, f[q], acc[h][q]) : acc[h][q] + f[q];
+            }
+        }
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+        if (a.shared) {
+            s[h].get(f);
+#pragma unroll
+            for (int q = 0; q < V; q++) acc[h][q] += f[q];
+        }
+        if (h == 0 || two) {
+            s[h].set(acc[h]);
+            s[h].store((uint8_t *)a.out + it.t * rowb + (h ? o1 : o0));
+        }
+    }
 }
 
 /* A workgroup takes a token: dout once, its rows once, drows written and the
@@ -337,32 +433,35 @@ __global__ __launch_bounds__(256) void k_unpermute_bwd(UnpermuteBwdArgs a)
 
 namespace {
 
+long wave_items(long n, long nv) { return n * ((nv + WAVE_VECS - 1) / WAVE_VECS); }
+
 template <int TYPE, int V>
 hipError_t permute_t(const PermuteArgs &a, hipStream_t st)
 {
     const long pairs = (long)a.n * a.topk;
     if (pairs <= PERMUTE_ONE_MAX) {
-        int tpb = 8;                               /* 128 pairs at the largest topk */
+        /* a workgroup a CU (each counts every pair), of at most 16 tokens */
+        const int tpb = std::min(16, (a.n + 255) / 256 + (a.n == 0));
         const int blocks = a.n > 0 ? (a.n + tpb - 1) / tpb : 1;
-        hipLaunchKernelGGL((k_permute_one<TYPE, V>), dim3(blocks), dim3(512), 0, st, a, tpb);
+        hipLaunchKernelGGL((k_permute_one<TYPE, V>), dim3(blocks), dim3(1024), 0, st, a, tpb);
         return hipGetLastError();
     }
     const int nch = (int)(pairs / 1024);
-    const size_t vecs = (size_t)a.n * (a.hidden / V);
-    if (vecs > MAX_THREADS) return hipErrorInvalidConfiguration;
+    const long waves = wave_items(a.n, a.hidden / V);
+    if (waves > MAX_WAVES) return hipErrorInvalidConfiguration;
     hipLaunchKernelGGL(k_permute_count, dim3(nch), dim3(1024), 0, st, a, nch);
     hipLaunchKernelGGL(k_permute_scan, dim3(1), dim3(1024), 0, st, a, nch);
     hipLaunchKernelGGL(k_permute_place, dim3(nch), dim3(1024), 0, st, a, nch);
-    hipLaunchKernelGGL((k_permute_copy<TYPE, V>), dim3((unsigned)((vecs + 255) / 256)), dim3(256), 0, st, a);
+    hipLaunchKernelGGL((k_permute_copy<TYPE, V>), dim3((unsigned)((waves + 3) / 4)), dim3(256), 0, st, a);
     return hipGetLastError();
 }
 
 template <int TYPE, int V, bool W>
 hipError_t unpermute_t(const UnpermuteArgs &a, hipStream_t st)
 {
-    const size_t vecs = (size_t)a.n * (a.hidden / V);
-    if (vecs > MAX_THREADS) return hipErrorInvalidConfiguration;
-    const dim3 grid((unsigned)((vecs + 255) / 256)), block(256);
+    const long waves = wave_items(a.n, a.hidden / V);
+    if (waves > MAX_WAVES) return hipErrorInvalidConfiguration;
+    const dim3 grid((unsigned)((waves + 3) / 4)), block(256);
     if (a.topk <= 8) hipLaunchKernelGGL((k_unpermute<TYPE, V, 8, W>), grid, block, 0, st, a);
     else hipLaunchKernelGGL((k_unpermute<TYPE, V, MAX_TOPK, W>), grid, block, 0, st, a);
     return hipGetLastError();
@@ -371,7 +470,7 @@ hipError_t unpermute_t(const UnpermuteArgs &a, hipStream_t st)
 template <int TYPE, int V>
 hipError_t unpermute_bwd_t(const UnpermuteBwdArgs &a, hipStream_t st)
 {
-    if ((size_t)a.n * 256 > MAX_THREADS) return hipErrorInvalidConfiguration;
+    if ((long)a.n * 4 > MAX_WAVES) return hipErrorInvalidConfiguration;
     if (a.topk <= 8) hipLaunchKernelGGL((k_unpermute_bwd<TYPE, V, 8>), dim3(a.n), dim3(256), 0, st, a);
     else hipLaunchKernelGGL((k_unpermute_bwd<TYPE, V, MAX_TOPK>), dim3(a.n), dim3(256), 0, st, a);
     return hipGetLastError();

@@ -13,8 +13,8 @@
  *   product lies within 2^-15 of a half-integer. Only there (one element in
  *   16,000) fp64 decides, where 127 a_j is exact and the quotient rounds to a
  *   half-integer only if it is one: codes depend on no rounding on the way.
- *   With SwiGLU the values are fp32 ones within 7 x 2^-24 (exp 1 ulp, 1 + e
- *   half, reciprocal 1 ulp, two products): certain outside 2^-13 of a
+ *   With SwiGLU the values are fp32 ones within 8 x 2^-24 (exp 1 ulp and
+ *   its correction half, 1 + e half, reciprocal 1 ulp, two products): certain outside 2^-13 of a
  *   half-integer. Inside it, and for the row's largest value, the SwiGLU is
  *   taken in fp64: codes and scale are those of fp64 values. Rows whose largest value is below 2^-60 or beyond 2^120
  *   compute everything in fp64.
@@ -48,7 +48,13 @@ __device__ __forceinline__ float swiglu32(float g, float u, float limit)
         u = u < -limit ? -limit : u;
         g = g > limit ? limit : g;
     }
-    return __fmul_rn(__fmul_rn(g, __builtin_amdgcn_rcpf(__fadd_rn(1.0f, expf(-g)))), u);
+    /* exp(-g) = 2^t (1 + ln 2 * r): t the rounded product with log2 e, r what
+     * the rounding and log2 e's own last bits left. Infinite and NaN gates give
+     * NaN here and are decided in fp64. */
+    const float t = __fmul_rn(-g, 0x1.715476p+0f);
+    const float r = fmaf(-g, 0x1.4ae0cp-26f, fmaf(-g, 0x1.715476p+0f, -t));
+    const float e = __builtin_amdgcn_exp2f(t);
+    return __fmul_rn(__fmul_rn(g, __builtin_amdgcn_rcpf(__fadd_rn(1.0f, fmaf(__fmul_rn(e, 0x1.62e43p-1f), r, e)))), u);
 }
 
 /* the unit's 8 elements (a, or gate and up) at element offset j */
@@ -74,17 +80,18 @@ __device__ __forceinline__ void widen8(const u32x4 (&r)[TYPE == DSV4_HIP_F32 ? 2
     }
 }
 
+/* largest of the wave's values, to every lane */
 __device__ __forceinline__ uint32_t wave_max_u32(uint32_t v)
 {
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) v = max(v, (uint32_t)__shfl_xor((int)v, d, 64));
-    return v;
-}
-__device__ __forceinline__ double wave_max_f64(double v)
-{
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) v = fmax(v, __shfl_xor(v, d, 64));
-    return v;
+#define QMAX(CTRL, ROWS) v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, (CTRL), (ROWS), 0xF, false))
+    QMAX(DPP_QUAD_1032, 0xF);
+    QMAX(DPP_QUAD_2301, 0xF);
+    QMAX(DPP_ROW_HALF_MIRROR, 0xF);
+    QMAX(DPP_ROW_MIRROR, 0xF);
+    QMAX(DPP_ROW_BCAST15, 0xA);
+    QMAX(DPP_ROW_BCAST31, 0xC);
+#undef QMAX
+    return (uint32_t)__builtin_amdgcn_readlane((int)v, 63);
 }
 
 /* the code in fp64: 127 a is exact for an fp32 a, and a quotient of such
@@ -102,10 +109,14 @@ __global__ __launch_bounds__(NW == 1 ? 256 : 64 * NW) void k_quant_i8(QuantI8Arg
     constexpr int STEP = 64 * NW * QU;
     constexpr int RW = TYPE == DSV4_HIP_F32 ? 2 : 1;
     __shared__ uint32_t smax[NW];
-    __shared__ double smax64[NW];
+    __shared__ unsigned long long smax64[RPW];     /* SwiGLU: the fp64 maximum's bits */
     const int lane = threadIdx.x & 63, wv = wave_in_group();
     const long row = (long)blockIdx.x * RPW + (NW == 1 ? wv : 0);
     if (row >= a.n) return;                        /* whole waves; one row a workgroup has no idle waves */
+    unsigned long long *m64 = &smax64[NW == 1 ? wv : 0];
+    if constexpr (SWIGLU) {
+        if (lane == 0 && (NW == 1 || wv == 0)) *m64 = 0;       /* seen by all after the first barrier */
+    }
     const size_t off = (size_t)row * (size_t)a.ld * elem_bytes<TYPE>();
     const uint8_t *pa = (const uint8_t *)a.a + off, *pu = SWIGLU ? (const uint8_t *)a.u + off : nullptr;
     const int j0 = ((NW == 1 ? 0 : wv * 64) + lane) * QU;
@@ -179,40 +190,39 @@ __global__ __launch_bounds__(NW == 1 ? 256 : 64 * NW) void k_quant_i8(QuantI8Arg
     const bool wide = SWIGLU && !(amax >= 0x1p-60f && amax <= 0x1p120f);
     bool bad = !SWIGLU && m >= 0x7F800000u;
     if constexpr (SWIGLU) {
-        double d = 0.0;
-        bool nan = false;
+        /* magnitudes order as their bits do, NaN above all: one LDS maximum of
+         * the few candidates */
+        auto take = [&](double v) {
+            v = fabs(v);
+            atomicMax(m64, (unsigned long long)__double_as_longlong(v == v ? v : __builtin_inf()));
+        };
         if (wide) {
             for (int j = j0; j < a.k; j += STEP)
-                for (int i = 0; i < QU; i++) {
-                    const double v = fabs(exact(j + i));
-                    nan |= !(v <= 1.7976931348623157e308);
-                    d = fmax(d, v);
-                }
+                for (int i = 0; i < QU; i++) take(exact(j + i));
         } else {
             const float near = amax * (1.0f - 0x1p-18f);
             for (int base = 0; base < a.k; base += NCH * STEP) {
                 if (!once) fetch(base);
 #pragma unroll
-                for (int c = 0; c < NCH; c++)
+                for (int c = 0; c < NCH; c++) {
+                    float top = 0.0f;
 #pragma unroll
-                    for (int i = 0; i < QU; i++)
-                        if (fabsf(f[c][i]) >= near) d = fmax(d, fabs(exact(base + j0 + c * STEP + i)));
+                    for (int i = 0; i < QU; i++) top = fmaxf(top, fabsf(f[c][i]));
+                    if (top >= near)
+                        for (int i = 0; i < QU; i++) {
+                            const int j = base + j0 + c * STEP + i;
+                            float t = 0.0f;
+#pragma unroll
+                            for (int q = 0; q < QU; q++) t = i == q ? f[c][q] : t;
+                            if (fabsf(t) >= near) take(exact(j));
+                        }
+                }
             }
         }
-        d = wave_max_f64(d);
-        nan = __any(nan);
-        if constexpr (NW > 1) {
-            if (lane == 0) smax64[wv] = nan ? __builtin_nan("") : d;
-            __syncthreads();
-#pragma unroll
-            for (int w = 0; w < NW; w++) {
-                const double s = smax64[w];
-                nan |= s != s;
-                d = fmax(d, s);
-            }
-        }
-        amax64 = d;
-        bad = nan;
+        if constexpr (NW > 1) __syncthreads();
+        else __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");
+        amax64 = __longlong_as_double((long long)*(volatile unsigned long long *)m64);
+        bad = !(amax64 <= 1.7976931348623157e308);
     }
     if (lane == 0 && (NW == 1 || wv == 0))
         a.S[row] = bad ? __builtin_nanf("") : amax64 > 0.0 ? (SWIGLU ? (float)(amax64 / 127.0) : amax / 127.0f) : 1.0f;
@@ -257,18 +267,37 @@ __global__ __launch_bounds__(NW == 1 ? 256 : 64 * NW) void k_quant_i8(QuantI8Arg
     }
 }
 
+/* Two units a lane: the smallest number of waves that holds the row, so that
+ * it is read once and many rows are in flight. us, waves x units: 4,206 rows
+ * of 2,048, SwiGLU, 1 x 4 15.4, 2 x 2 14.1, 4 x 1 14.0, 8 x 1 20.4; 2,048 of
+ * 4,096 bf16 2 x 4 11.7, 4 x 2 9.0, 8 x 1 8.4; 8,192 of them 23.2, 19.6, 22.3;
+ * 4,096 of 8,192 fp32 4 x 4 28.8, 8 x 2 28.3, 16 x 1 31.0; 5,000 of 14,336,
+ * SwiGLU, 8 x 2 (each row read three times) 156, 16 x 2 111; 24,576 of 512,
+ * SwiGLU, 1 x 1 20.6, 1 x 2 22.3, 2 x 1 27. */
+template <int TYPE, bool SWIGLU, int NW, int NCH>
+static hipError_t quant_i8_n(const QuantI8Args &a, hipStream_t st)
+{
+    constexpr int RPW = NW == 1 ? 4 : 1;
+    hipLaunchKernelGGL((k_quant_i8<TYPE, SWIGLU, NW, NCH>), dim3((unsigned)((a.n + RPW - 1) / RPW)),
+                       dim3(NW == 1 ? 256 : 64 * NW), 0, st, a);
+    return hipGetLastError();
+}
+
 template <int TYPE, bool SWIGLU>
 static hipError_t quant_i8_t(const QuantI8Args &a, hipStream_t st)
 {
-    const dim3 one((unsigned)a.n);
-    hipLaunchKernelGGL((k_quant_i8<TYPE, SWIGLU, 8, 2>), one, dim3(512), 0, st, a);
-    return hipGetLastError();
+    if (a.k <= 512) return quant_i8_n<TYPE, SWIGLU, 1, 1>(a, st);
+    if (a.k <= 1024) return quant_i8_n<TYPE, SWIGLU, 1, 2>(a, st);
+    if (a.k <= 2048) return quant_i8_n<TYPE, SWIGLU, 2, 2>(a, st);
+    if (a.k <= 4096) return quant_i8_n<TYPE, SWIGLU, 4, 2>(a, st);
+    if (a.k <= 8192) return quant_i8_n<TYPE, SWIGLU, 8, 2>(a, st);
+    return quant_i8_n<TYPE, SWIGLU, 16, 2>(a, st);
 }
 
 hipError_t quant_i8_launch(const QuantI8Args &a, int type, bool swiglu, hipStream_t st)
 {
     if (a.n <= 0 || a.k <= 0 || a.k % QU) return hipErrorInvalidValue;
-    if (a.n >= 1 << 23) return hipErrorInvalidConfiguration;       /* 2^32 threads */
+    if (a.n >= 1 << 22) return hipErrorInvalidConfiguration;       /* 2^32 threads */
     switch (type) {
     case DSV4_HIP_F32: return swiglu ? quant_i8_t<DSV4_HIP_F32, true>(a, st) : quant_i8_t<DSV4_HIP_F32, false>(a, st);
     case DSV4_HIP_BF16: return swiglu ? quant_i8_t<DSV4_HIP_BF16, true>(a, st) : quant_i8_t<DSV4_HIP_BF16, false>(a, st);

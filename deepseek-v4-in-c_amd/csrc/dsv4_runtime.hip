@@ -2223,7 +2223,7 @@ static int order_checks(int type, int n, int topk, int hidden, std::initializer_
                         std::initializer_list<const void *> words, const char *what)
 {
     if (!elem_type_ok(type)) return fail("%s: unknown element type %d", what, type);
-    if (n < 0 || topk < 1 || topk > 16 || (long)n * topk > (1L << 26) || hidden < 1)
+    if (n < 0 || topk < 1 || topk > 16 || (long)n * topk > (1L << 26) || hidden < 1 || hidden > 1 << 24)
         return fail("%s: bad n %d, topk %d or hidden %d", what, n, topk, hidden);
     for (const void *p : elems)
         if ((!p && n) || !elem_aligned(p, type)) return fail("%s: NULL or misaligned rows", what);

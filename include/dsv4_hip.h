@@ -408,7 +408,7 @@ int  dsv4_hip_gemm_i8_grouped_dev(void *C, int out_type, const int8_t *Aq, const
  * status bit 0. Rows, and entries of row_tok, from ex_off[n_experts] on stay
  * as they are. n = 0 gives empty buckets.
  * x [n][hidden], rows [n * topk][hidden] of `type`; n_experts <= 1024, topk <=
- * 16, n * topk <= 2^26, any hidden (rows of whole 16-byte vectors are the
+ * 16, n * topk <= 2^26, hidden up to 2^24 (rows of whole 16-byte vectors are the
  * fast ones). Outputs must not overlap inputs. No workspace. */
 int  dsv4_hip_moe_permute_dev(void *rows, int *ex_off, int *row_tok, int *pos, const void *x, int type,
                               const int *idx, int n, int topk, int n_experts, int hidden, void *stream);
