@@ -41,9 +41,12 @@ template <int TYPE, int V>
 struct Elem {
     static_assert(V == 1 || V * elem_bytes<TYPE>() == 16, "one element or a whole vector");
     u32x4 raw;
+    /* ONCE: bytes that the call reads once and that no cache should keep */
+    template <bool ONCE = false>
     __device__ __forceinline__ void load(const void *p)
     {
-        if constexpr (V > 1) raw = *gptr((const u32x4 *)p);
+        if constexpr (V > 1 && ONCE) raw = __builtin_nontemporal_load(gptr((const u32x4 *)p));
+        else if constexpr (V > 1) raw = *gptr((const u32x4 *)p);
         else if constexpr (TYPE == DSV4_HIP_F32) raw.x = *gptr((const uint32_t *)p);
         else raw.x = *gptr((const uint16_t *)p);
     }
@@ -52,17 +55,6 @@ struct Elem {
         if constexpr (V > 1) *(DSV4_GLOBAL u32x4 *)p = raw;
         else if constexpr (TYPE == DSV4_HIP_F32) *(DSV4_GLOBAL uint32_t *)p = raw.x;
         else *(DSV4_GLOBAL uint16_t *)p = (uint16_t)raw.x;
-    }
-    /* bytes that the call touches once */
-    __device__ __forceinline__ void load_stream(const void *p)
-    {
-        if constexpr (V > 1) raw = __builtin_nontemporal_load(gptr((const u32x4 *)p));
-        else load(p);
-    }
-    __device__ __forceinline__ void store_stream(void *p) const
-    {
-        if constexpr (V > 1) __builtin_nontemporal_store(raw, (DSV4_GLOBAL u32x4 *)p);
-        else store(p);
     }
     __device__ __forceinline__ void get(float (&f)[V]) const
     {

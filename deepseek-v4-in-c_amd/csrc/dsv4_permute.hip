@@ -210,7 +210,7 @@ __global__ __launch_bounds__(1024) void k_permute_one(PermuteArgs a, int tpb)
             uint8_t *dst = (uint8_t *)a.rows + (size_t)i * V * EB;
             for (int k = 0; k < a.topk; k++) {
                 const int r = own_row[t * a.topk + k];
-                if (r >= 0) v[j].store_stream(dst + (size_t)r * rowb);
+                if (r >= 0) v[j].store(dst + (size_t)r * rowb);
             }
         }
     }
@@ -318,7 +318,7 @@ __global__ __launch_bounds__(256) void k_permute_copy(PermuteArgs a)
         if (r < 0) continue;
 #pragma unroll
         for (int h = 0; h < 2; h++)
-            if (it.j + 64 * h < nv) v[h].store_stream((uint8_t *)a.rows + r * rowb + (size_t)(it.j + 64 * h) * V * EB);
+            if (it.j + 64 * h < nv) v[h].store((uint8_t *)a.rows + r * rowb + (size_t)(it.j + 64 * h) * V * EB);
     }
 }
 
@@ -326,7 +326,7 @@ __global__ __launch_bounds__(256) void k_permute_copy(PermuteArgs a)
 
 /* A lane sums two vectors over the token's topk rows, every row's load issued
  * before the first is used. W: weights (else 1). */
-template <int TYPE, int V, int KMAX, bool W>
+template <int TYPE, int V, int KMAX, bool W, bool ONCE>
 __global__ __launch_bounds__(256) void k_unpermute(UnpermuteArgs a)
 {
     constexpr int EB = elem_bytes<TYPE>();
@@ -345,8 +345,8 @@ __global__ __launch_bounds__(256) void k_unpermute(UnpermuteArgs a)
 #pragma unroll
     for (int k = 0; k < KMAX; k++)
         if ((unsigned)p[k] < (unsigned)nrows) {
-            v[k][0].load_stream((const uint8_t *)a.rows + p[k] * rowb + o0);
-            v[k][1].load_stream((const uint8_t *)a.rows + p[k] * rowb + o1);
+            v[k][0].template load<ONCE>((const uint8_t *)a.rows + p[k] * rowb + o0);
+            v[k][1].template load<ONCE>((const uint8_t *)a.rows + p[k] * rowb + o1);
         }
     if (a.shared) {
         s[0].load((const uint8_t *)a.shared + it.t * rowb + o0);
@@ -382,7 +382,7 @@ __global__ __launch_bounds__(256) void k_unpermute(UnpermuteArgs a)
 
 /* A workgroup takes a token: dout once, its rows once, drows written and the
  * topk dot products kept in registers until the end. */
-template <int TYPE, int V, int KMAX>
+template <int TYPE, int V, int KMAX, bool ONCE>
 __global__ __launch_bounds__(256) void k_unpermute_bwd(UnpermuteBwdArgs a)
 {
     constexpr int EB = elem_bytes<TYPE>();
@@ -402,10 +402,10 @@ __global__ __launch_bounds__(256) void k_unpermute_bwd(UnpermuteBwdArgs a)
     for (int i = tid; i < nv; i += 256) {
         const size_t o = (size_t)i * V * EB;
         Elem<TYPE, V> d, y[KMAX];
-        d.load((const uint8_t *)a.dout + t * rowb + o);
+        d.template load<ONCE>((const uint8_t *)a.dout + t * rowb + o);
 #pragma unroll
         for (int k = 0; k < KMAX; k++)
-            if (p[k] >= 0) y[k].load((const uint8_t *)a.rows + p[k] * rowb + o);
+            if (p[k] >= 0) y[k].template load<ONCE>((const uint8_t *)a.rows + p[k] * rowb + o);
         float fd[V], f[V];
         d.get(fd);
 #pragma unroll
@@ -432,6 +432,13 @@ __global__ __launch_bounds__(256) void k_unpermute_bwd(UnpermuteBwdArgs a)
 /* ----------------------------------------------------------- launchers --- */
 
 namespace {
+
+/* Rows beyond what the caches keep are read past them: 24,576 rows of 8 KB 66
+ * -> 43 us, and their gradients' 16,818 of which half are there 29 -> 30 after a
+ * forward pass that left 18 rather than 24. A batch's rows, just written by the
+ * products, are better found there (384 rows of 16 KB 3.9 -> 3.3). */
+template <int TYPE>
+bool reads_once(long n, long topk, long hidden) { return n * topk * hidden * elem_bytes<TYPE>() > 64L << 20; }
 
 long wave_items(long n, long nv) { return n * ((nv + WAVE_VECS - 1) / WAVE_VECS); }
 
@@ -462,8 +469,12 @@ hipError_t unpermute_t(const UnpermuteArgs &a, hipStream_t st)
     const long waves = wave_items(a.n, a.hidden / V);
     if (waves > MAX_WAVES) return hipErrorInvalidConfiguration;
     const dim3 grid((unsigned)((waves + 3) / 4)), block(256);
-    if (a.topk <= 8) hipLaunchKernelGGL((k_unpermute<TYPE, V, 8, W>), grid, block, 0, st, a);
-    else hipLaunchKernelGGL((k_unpermute<TYPE, V, MAX_TOPK, W>), grid, block, 0, st, a);
+    const bool once = reads_once<TYPE>(a.n, a.topk, a.hidden);
+#define GO(KMAX)                                                                                           \
+    if (once) hipLaunchKernelGGL((k_unpermute<TYPE, V, KMAX, W, true>), grid, block, 0, st, a);            \
+    else hipLaunchKernelGGL((k_unpermute<TYPE, V, KMAX, W, false>), grid, block, 0, st, a)
+    if (a.topk <= 8) { GO(8); } else { GO(MAX_TOPK); }
+#undef GO
     return hipGetLastError();
 }
 
@@ -471,8 +482,13 @@ template <int TYPE, int V>
 hipError_t unpermute_bwd_t(const UnpermuteBwdArgs &a, hipStream_t st)
 {
     if ((long)a.n * 4 > MAX_WAVES) return hipErrorInvalidConfiguration;
-    if (a.topk <= 8) hipLaunchKernelGGL((k_unpermute_bwd<TYPE, V, 8>), dim3(a.n), dim3(256), 0, st, a);
-    else hipLaunchKernelGGL((k_unpermute_bwd<TYPE, V, MAX_TOPK>), dim3(a.n), dim3(256), 0, st, a);
+    const dim3 grid(a.n), block(256);
+    const bool once = reads_once<TYPE>(a.n, a.topk, a.hidden);
+#define GO(KMAX)                                                                                           \
+    if (once) hipLaunchKernelGGL((k_unpermute_bwd<TYPE, V, KMAX, true>), grid, block, 0, st, a);           \
+    else hipLaunchKernelGGL((k_unpermute_bwd<TYPE, V, KMAX, false>), grid, block, 0, st, a)
+    if (a.topk <= 8) { GO(8); } else { GO(MAX_TOPK); }
+#undef GO
     return hipGetLastError();
 }
 
