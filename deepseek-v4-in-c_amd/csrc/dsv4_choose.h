@@ -249,22 +249,20 @@ inline I8Form i8_form(int M, int N, int K)
     return best;
 }
 
-/* Buckets of ne experts, M rows in all. Up to 16 rows an expert the weights
- * are streamed once whatever the form, and the pair form streams best (us,
- * pair / 64x2 / 128x4, experts 2048 x 4096: 42 rows on 256 57 / 62 / 68, 384 rows
- * Zipf 176 / 182 / 195, 1,536 rows 344 / 367 / 396, 2,400 rows 370 / 369),
- * unless there is too little of it to fill the CUs (6 rows 15.4 / 12.3; 160 rows
- * on 64 of 512 x 1024 8.7 / 6.7). Then 128x4 (6,144 rows Zipf 64x2 423, 128x4
- * 419, 256x8 458; 12,288 rows 529 / 439 / 494), and the large tiles from 80 rows an
- * expert (24,576 rows Zipf 746 / 580 / 547; 6,144 rows on 64 experts 191 / 141 /
- * 141). */
+/* Buckets of ne experts, M rows in all; the mean bucket decides. us, pair /
+ * 64x2 / 128x4 / 256x8, experts 2048 x 4096 on 256: 384 rows Zipf 178 / 176 /
+ * 176 / 192, 768 rows 322 / 350 / 359 / 370, 2,400 rows 370 / 377 / 384 / 379,
+ * 3,072 rows 414 / 380 / 389 / 382, 6,144 rows Zipf 740 / 415 / 398 / 423, 12,288
+ * rows Zipf - / 522 / 446 / 455, even 530 / 414 / 403 (64x2 on), 24,576 rows Zipf
+ * 745 / 565 / 522. Too little weight to fill the CUs: 6 rows 15.1 / 12.4 / 14.8,
+ * 160 rows on 64 of 512 x 1024 8.5 / 7.0 / 8.1, but 1,600 of them - / 9.3 / 8.7. */
 inline I8Form i8_grouped_form(int M, int N, int K, int ne)
 {
     const long hit = M < ne ? M : ne;
-    if (hit * N * K < 1L << 26 && M <= 32 * hit) return I8_64x2;
+    if (hit * N * K < 1L << 26 && M <= 16 * hit) return I8_64x2;
     if (M <= 10 * hit) return I8_PAIR;
     if (M <= 20 * hit) return I8_64x2;
-    return M < 80 * hit ? I8_128x4 : I8_256x8;
+    return M < 60 * hit ? I8_128x4 : I8_256x8;
 }
 
 } // namespace dsv4

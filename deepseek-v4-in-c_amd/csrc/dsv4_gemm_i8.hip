@@ -45,6 +45,7 @@ struct Tile {
     const uint8_t *w;
     const float *s;
     int r0, rows;
+    int e;                                         /* its expert */
     bool bad;                                      /* the table's entry is not an int8 N x K matrix */
 };
 
@@ -74,7 +75,7 @@ __device__ __forceinline__ Tile bucket_tile(const I8Args &a, int t, int lane)
         if (lane >= d) incl += v;
     }
     Tile o;
-    o.w = nullptr; o.s = nullptr; o.r0 = 0; o.rows = 0; o.bad = false;
+    o.w = nullptr; o.s = nullptr; o.r0 = 0; o.rows = 0; o.e = 0; o.bad = false;
     const uint64_t past = __ballot(incl > t);
     if (!past) return o;
     const int L = __builtin_ctzll(past);
@@ -92,7 +93,8 @@ __device__ __forceinline__ Tile bucket_tile(const I8Args &a, int t, int lane)
         left -= tiles;
         lo = hi;
     }
-    const DSV4QMat m = ld_uniform(a.table, __builtin_amdgcn_readfirstlane(e));
+    o.e = __builtin_amdgcn_readfirstlane(e);
+    const DSV4QMat m = ld_uniform(a.table, o.e);
     o.w = (const uint8_t *)m.w;
     o.s = (const float *)m.s;
     o.bad = m.wdt != DSV4_WI8 || m.rows != a.N || m.cols != a.K || !m.w || !m.s || ((uintptr_t)m.w & 15u) ||
@@ -134,7 +136,7 @@ __global__ __launch_bounds__(64 * NW) void k_i8_pair(I8Args a)
         t = bucket_tile<TR>(a, tile, lane);
         if (t.rows <= 0) return;
     } else {
-        t.w = a.W; t.s = a.Sw; t.bad = false;
+        t.w = a.W; t.s = a.Sw; t.e = 0; t.bad = false;
         t.r0 = tile * TR;
         t.rows = min(TR, a.M - t.r0);
     }
@@ -227,6 +229,69 @@ static hipError_t i8_pair(const I8Args &a, hipStream_t st)
     return hipGetLastError();
 }
 
+/* bytes between rows of a tile of F features on its way out through LDS: 16
+ * more than the row, so that the 16 rows of a store spread over the banks */
+constexpr int i8_out_ld(int F, int eb) { return F * eb + 16; }
+
+/* A workgroup's sums, acc[i][u] the wave's 16 features from f0 + 16 i by 16 rows
+ * from m0 + 16 u, scaled, rounded, put together in LDS (free by now) and
+ * written as whole 16-byte pieces of rows where C's rows consist of such. */
+template <int F, bool GROUPED, int OUT, int NTHREADS, int WI, int U, class SRC>
+__device__ __forceinline__ void i8_leave(const I8Args &a, const Tile &t, int n0, int nf, uint8_t *lds,
+                                         const v4i (&acc)[WI][U], int f0, int m0, SRC src_of)
+{
+    constexpr int EB = elem_bytes<OUT>(), LD = i8_out_ld(F, EB);
+    const int lane = threadIdx.x & 63, rr = lane & 15, gq = lane >> 4;
+    float sw[WI][4];
+#pragma unroll
+    for (int i = 0; i < WI; i++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            const int n = f0 + 16 * i + 4 * gq + e;
+            sw[i][e] = n < nf ? gptr(t.s)[n0 + n] : 0.0f;
+        }
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+        const int m = m0 + 16 * u + rr, s = src_of(m);
+        const float sa = s >= 0 ? gptr(a.Sa)[GROUPED ? s : t.r0 + s] : __builtin_nanf("");
+        if (GROUPED && s < 0 && m < t.rows && f0 == 0 && gq == 0) atomicOr(a.status, ST_BAD_EXPERT_ID);
+#pragma unroll
+        for (int i = 0; i < WI; i++) {
+            uint8_t *o = lds + m * LD + (f0 + 16 * i + 4 * gq) * EB;
+            float v[4];
+#pragma unroll
+            for (int e = 0; e < 4; e++) v[e] = (float)acc[i][u][e] * sa * sw[i][e];
+            if constexpr (OUT == DSV4_HIP_F32) {
+                *(f32x4 *)o = f32x4{v[0], v[1], v[2], v[3]};
+            } else {
+                uint2 p;
+                p.x = narrow16<OUT>(v[0]) | (narrow16<OUT>(v[1]) << 16);
+                p.y = narrow16<OUT>(v[2]) | (narrow16<OUT>(v[3]) << 16);
+                *(uint2 *)o = p;
+            }
+        }
+    }
+    __syncthreads();
+    uint8_t *out = (uint8_t *)a.C + ((size_t)t.r0 * a.N + n0) * EB;
+    const size_t ld = (size_t)a.N * EB;
+    if ((((uintptr_t)a.C | ld) & 15u) == 0) {      /* n0 and nf are whole pieces then too */
+        const int pieces = nf * EB / 16;
+        constexpr int PMAX = F * EB / 16;
+        for (int i = threadIdx.x; i < t.rows * PMAX; i += NTHREADS) {
+            const int m = i / PMAX, p = i % PMAX;
+            if (p < pieces)
+                __builtin_nontemporal_store(*(const u32x4 *)(lds + m * LD + 16 * p), (DSV4_GLOBAL u32x4 *)(out + m * ld + 16 * p));
+        }
+    } else {
+        for (int i = threadIdx.x; i < t.rows * F; i += NTHREADS) {
+            const int m = i / F, n = i % F;
+            if (n >= nf) continue;
+            if constexpr (EB == 4) *(float *)(out + m * ld + 4 * n) = *(const float *)(lds + m * LD + 4 * n);
+            else *(uint16_t *)(out + m * ld + 2 * n) = *(const uint16_t *)(lds + m * LD + 2 * n);
+        }
+    }
+}
+
 /* ------------------------------------------------------ many rows -------
  * A workgroup takes F features by 16 T rows, wave (wr, wt) F / 4 features by
  * 16 T / WT rows. K goes in blocks of 128 codes, one staged row a 128-byte
@@ -242,8 +307,8 @@ template <int F, int T, int KB, int NST_> struct I8Tile {
     static constexpr int NST = NST_;
     static constexpr int LW = F / 8 / NWAVE, LX = 2 * T / NWAVE, VM = KB * (LW + LX);
     static constexpr int RING = NST * STAGE;
-    static constexpr int out_ld(int eb) { return F * eb + 16; }
-    static constexpr int lds(int eb) { return RING > 16 * T * out_ld(eb) ? RING : 16 * T * out_ld(eb); }
+    static constexpr int OUTB(int eb) { return 16 * T * i8_out_ld(F, eb); }
+    static constexpr int lds(int eb) { return RING > OUTB(eb) ? RING : OUTB(eb); }
     static_assert(LX * NWAVE == 2 * T && LW * NWAVE * 8 == F && (NST - 1) * VM < 64 && lds(4) <= 160 * 1024, "ring");
 };
 
@@ -263,7 +328,7 @@ template <int F, int T, int KB, int NST, bool GROUPED, int OUT>
 __global__ __launch_bounds__((64 * I8Tile<F, T, KB, NST>::NWAVE)) void k_i8_tile(I8Args a)
 {
     using C = I8Tile<F, T, KB, NST>;
-    constexpr int U = C::U, WI = C::WI, TR = 16 * T, EB = elem_bytes<OUT>();
+    constexpr int U = C::U, WI = C::WI, TR = 16 * T;
     extern __shared__ __align__(16) uint8_t lds[];
     const int lane = threadIdx.x & 63, wave = wave_in_group();
     const int rr = lane & 15, gq = lane >> 4, wr = wave & 3, wt = wave >> 2;
@@ -284,7 +349,7 @@ __global__ __launch_bounds__((64 * I8Tile<F, T, KB, NST>::NWAVE)) void k_i8_tile
         const int per = total / 8, rest = total % 8, x = blockIdx.x % 8, y = blockIdx.x / 8;
         const int id = x * per + min(x, rest) + y;
         const int grp = id / (8 * nt), gm = min(8, mt - 8 * grp), in = id - grp * 8 * nt;
-        t.w = a.W; t.s = a.Sw; t.bad = false;
+        t.w = a.W; t.s = a.Sw; t.e = 0; t.bad = false;
         t.r0 = (8 * grp + in % gm) * TR;
         t.rows = min(TR, a.M - t.r0);
         n0 = in / gm * F;
@@ -319,17 +384,24 @@ __global__ __launch_bounds__((64 * I8Tile<F, T, KB, NST>::NWAVE)) void k_i8_tile
         xo[i] = s < 0 ? I8_OOB : (uint32_t)s * K + 16u * (uint32_t)c;
         xl[i] = (nblk - 1) * 128 + 16 * c < a.K ? xo[i] : I8_OOB;
     }
+    /* The block this workgroup begins with. Rows of 4 KB put the lines of one
+     * block into a few memory channels, and workgroups that run through K side
+     * by side into the same ones; begun at different places they spread (sums
+     * are exact in any order). Those that share weights keep step. us: 24,576
+     * rows of 256 experts 525 -> 451, with Zipf 546 -> 522, 6,144 rows 477 ->
+     * 390, 1,536 rows in these tiles 462 -> 374. One matrix gains nothing. */
+    const int rot = GROUPED ? (n0 / F * 4 + t.e) % nblk : 0;
     /* load i of a wave's share of stage st; past the end zeros, no traffic */
     auto issue = [&](int st, int slot, int i) {
         constexpr int LB = C::LW + C::LX;
-        const int blk = st * KB + i / LB, k = i % LB;
-        const uint32_t oob = blk < nblk ? 0u : I8_OOB;
-        const int so = min(blk, nblk - 1) * 128;
+        const int in = st * KB + i / LB, k = i % LB, blk = in + rot < nblk ? in + rot : in + rot - nblk;
+        const uint32_t oob = in < nblk ? 0u : I8_OOB;
+        const int so = in < nblk ? blk * 128 : 0;
         uint8_t *buf = lds + slot * C::STAGE + i / LB * C::SUB;
         if (k < C::LW) i8_dma16(rw, wo[min(k, C::LW - 1)] | oob, so, buf + 1024 * (C::LW * wave + k));
         else {
             const int j = max(0, min(k - C::LW, C::LX - 1));
-            i8_dma16(rx, (blk < nblk - 1 ? xo[j] : xl[j]) | oob, so, buf + C::OFF_X + 1024 * (C::LX * wave + j));
+            i8_dma16(rx, (blk != nblk - 1 ? xo[j] : xl[j]) | oob, so, buf + C::OFF_X + 1024 * (C::LX * wave + j));
         }
     };
 #pragma unroll
@@ -359,6 +431,9 @@ __global__ __launch_bounds__((64 * I8Tile<F, T, KB, NST>::NWAVE)) void k_i8_tile
         for (int q = 0; q < WI * U; q++) {
             constexpr int N = WI * U, R = WI + U;
             acc[q % WI][q / WI] = __builtin_amdgcn_mfma_i32_16x16x64_i8(cur.w[q % WI], cur.x[q / WI], acc[q % WI][q / WI], 0, 0, 0);
+            /* the wait for `cur` is not one for the reads below; with few products
+             * to wait behind, the reads had better go first */
+            if (WI * U >= 8 && q == 0) __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
             for (int j = 0; j < R; j++)
                 if (j * N / (R + 1) == q) {
@@ -402,55 +477,7 @@ __global__ __launch_bounds__((64 * I8Tile<F, T, KB, NST>::NWAVE)) void k_i8_tile
     i8_wait_vm<0>();
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
-    constexpr int LD = C::out_ld(EB);
-    float sw[WI][4];
-#pragma unroll
-    for (int i = 0; i < WI; i++)
-#pragma unroll
-        for (int e = 0; e < 4; e++) {
-            const int n = 16 * (WI * wr + i) + 4 * gq + e;
-            sw[i][e] = n < nf ? gptr(t.s)[n0 + n] : 0.0f;
-        }
-#pragma unroll
-    for (int u = 0; u < U; u++) {
-        const int m = 16 * (U * wt + u) + rr, s = src_of(m);
-        const float sa = s >= 0 ? gptr(a.Sa)[GROUPED ? s : t.r0 + s] : __builtin_nanf("");
-        if (GROUPED && s < 0 && m < t.rows && wr == 0 && gq == 0) atomicOr(a.status, ST_BAD_EXPERT_ID);
-#pragma unroll
-        for (int i = 0; i < WI; i++) {
-            uint8_t *o = lds + m * LD + (16 * (WI * wr + i) + 4 * gq) * EB;
-            float v[4];
-#pragma unroll
-            for (int e = 0; e < 4; e++) v[e] = (float)acc[i][u][e] * sa * sw[i][e];
-            if constexpr (OUT == DSV4_HIP_F32) {
-                *(f32x4 *)o = f32x4{v[0], v[1], v[2], v[3]};
-            } else {
-                uint2 p;
-                p.x = narrow16<OUT>(v[0]) | (narrow16<OUT>(v[1]) << 16);
-                p.y = narrow16<OUT>(v[2]) | (narrow16<OUT>(v[3]) << 16);
-                *(uint2 *)o = p;
-            }
-        }
-    }
-    __syncthreads();
-    uint8_t *out = (uint8_t *)a.C + ((size_t)t.r0 * a.N + n0) * EB;
-    const size_t ld = (size_t)a.N * EB;
-    if ((((uintptr_t)a.C | ld) & 15u) == 0) {      /* whole pieces: n0 and nf are multiples of one too */
-        const int pieces = nf * EB / 16;
-        constexpr int PMAX = F * EB / 16;
-        for (int i = threadIdx.x; i < t.rows * PMAX; i += 64 * C::NWAVE) {
-            const int m = i / PMAX, p = i % PMAX;
-            if (p < pieces)
-                __builtin_nontemporal_store(*(const u32x4 *)(lds + m * LD + 16 * p), (DSV4_GLOBAL u32x4 *)(out + m * ld + 16 * p));
-        }
-    } else {
-        for (int i = threadIdx.x; i < t.rows * F; i += 64 * C::NWAVE) {
-            const int m = i / F, n = i % F;
-            if (n >= nf) continue;
-            if constexpr (EB == 4) *(float *)(out + m * ld + 4 * n) = *(const float *)(lds + m * LD + 4 * n);
-            else *(uint16_t *)(out + m * ld + 2 * n) = *(const uint16_t *)(lds + m * LD + 2 * n);
-        }
-    }
+    i8_leave<F, GROUPED, OUT, 64 * C::NWAVE>(a, t, n0, nf, lds, acc, 16 * WI * wr, 16 * U * wt, src_of);
 }
 
 template <int F, int T, int KB, int NST, bool GROUPED, int OUT>
