@@ -235,6 +235,7 @@ inline I8Form i8_form(int M, int N, int K)
     struct { I8Form form; int F, TR, c0, base, per; } const f[] = {
         {I8_64x2, 64, 32, 5, 40, 45}, {I8_64x4, 64, 64, 0, 65, 65}, {I8_128x4, 128, 64, -5, 95, 110},
         {I8_128x8, 128, 128, -20, 145, 205}, {I8_256x8, 256, 128, -20, 250, 345}};
+    if (ceil_div(M, 128) * ceil_div(N, 256) >= 1L << 20) return I8_256x8;     /* costs beyond 64 bits */
     I8Form best = I8_64x2;
     long least = -1;
     for (const auto &c : f) {
@@ -263,6 +264,18 @@ inline I8Form i8_grouped_form(int M, int N, int K, int ne)
     if (M <= 10 * hit) return I8_PAIR;
     if (M <= 20 * hit) return I8_64x2;
     return M < 60 * hit ? I8_128x4 : I8_256x8;
+}
+
+/* Waves of the launch that multiplies M rows by N features in a form: tiles
+ * of its features and rows, and with ne experts one more row tile for each that
+ * may end inside one. A launch takes 2^32 threads. */
+constexpr long I8_MAX_WAVES = (1L << 26) - 1;
+inline long i8_waves(I8Form form, long M, long N, long ne)
+{
+    const long F = form == I8_PAIR ? (ne ? 32 : 8) : form <= I8_64x4 ? 64 : form == I8_256x8 ? 256 : 128;
+    const long TR = form == I8_PAIR ? (ne ? 16 : 8) : form <= I8_64x2_DEEP ? 32 : form <= I8_128x4 ? 64 : 128;
+    const long waves = form == I8_PAIR ? (ne ? 4 : 8) : form <= I8_64x2_DEEP ? 4 : 8;
+    return (ne ? M / TR + (M < ne ? M : ne) : ceil_div(M, TR)) * ceil_div(N, F) * waves;
 }
 
 } // namespace dsv4

@@ -122,7 +122,10 @@ __device__ __forceinline__ void i8_store(void *C, size_t i, float v)
  * 8 tokens the same way, and of the 16 x 16 result the two quadrants that
  * multiply equal codes count. A workgroup takes 8 RT weight rows by 8 TT
  * tokens, its waves share out K in blocks of 128, B of them in flight, and add
- * up in LDS. */
+ * up in LDS. Bound: the weight stream, and below some 20 MB its latency: one
+ * token of 4096 x 4096 5.2 us (3.2 TB/s), 247 experts of 2048 x 4096 with three
+ * rows each 321 us (6.5 TB/s). Whole lines matter: 16 rows x 64 bytes an
+ * instruction took 5.9 and 594 us. */
 template <int RT, int TT, int NW, int B, bool GROUPED, int OUT>
 __global__ __launch_bounds__(64 * NW) void k_i8_pair(I8Args a)
 {
@@ -221,10 +224,7 @@ __global__ __launch_bounds__(64 * NW) void k_i8_pair(I8Args a)
 template <int RT, int TT, int NW, int B, bool GROUPED, int OUT>
 static hipError_t i8_pair(const I8Args &a, hipStream_t st)
 {
-    constexpr int TR = 8 * TT, FR = 8 * RT;
-    const long tiles = GROUPED ? a.M / TR + (a.n_experts < a.M ? a.n_experts : a.M) : (a.M + TR - 1) / TR;
-    const long groups = tiles * ((a.N + FR - 1) / FR);
-    if (groups * NW >= 1L << 26) return hipErrorInvalidConfiguration;         /* 2^32 threads */
+    const long groups = i8_waves(I8_PAIR, a.M, a.N, GROUPED ? a.n_experts : 0) / NW;
     hipLaunchKernelGGL((k_i8_pair<RT, TT, NW, B, GROUPED, OUT>), dim3((unsigned)groups), dim3(64 * NW), 0, st, a);
     return hipGetLastError();
 }
@@ -297,10 +297,18 @@ __device__ __forceinline__ void i8_leave(const I8Args &a, const Tile &t, int n0,
  * 16 T / WT rows. K goes in blocks of 128 codes, one staged row a 128-byte
  * line: both operands by loads straight to LDS into a ring of NST blocks (16-
  * byte pieces XOR-swizzled by row), a wave reading the operands of the next 64
- * codes while it multiplies these. One barrier a block: after it every wave's
- * loads of the next block have landed and no wave still reads this one, so
- * the block NST ahead takes its place. Loads past K read nothing and multiply
- * as zeros. The tile leaves through LDS as whole 16-byte pieces of rows. */
+ * codes while it multiplies these. One barrier a stage of KB blocks: after it
+ * every wave's loads of the next stage have landed and no wave still reads this
+ * one, so the stage NST ahead takes its place. Loads past K read nothing and
+ * multiply as zeros. The tile leaves through LDS as whole 16-byte pieces of rows,
+ * written past the caches (16 MB of bf16 36.7 -> 35.6 us of the call).
+ * Bound: 256 x 128 tiles issue an MFMA in half of their cycles (2,048 x 4096 x
+ * 4096 34 us, 2.0 of 4.3 POP/s that registers alone reach; the library's int8
+ * product takes 41.7), the rest are barriers and LDS; experts' buckets the HBM
+ * stream beside that (24,576 rows of 256 experts, Zipf, 522 us, 359 with every
+ * table entry the same matrix, 316 for the weights alone); few rows the chain of
+ * stages (16 to 128 rows of 4096 x 4096 7 to 8 us; K split over teams of waves
+ * gained nothing, weights straight to registers lost 10 to 20 %). */
 template <int F, int T, int KB, int NST_> struct I8Tile {
     static constexpr int WT = T >= 4 ? 2 : 1, NWAVE = 4 * WT, U = T / WT, WI = F / 64;
     static constexpr int OFF_X = F * 128, SUB = OFF_X + 16 * T * 128, STAGE = KB * SUB;
@@ -480,22 +488,26 @@ __global__ __launch_bounds__((64 * I8Tile<F, T, KB, NST>::NWAVE)) void k_i8_tile
     i8_leave<F, GROUPED, OUT, 64 * C::NWAVE>(a, t, n0, nf, lds, acc, 16 * WI * wr, 16 * U * wt, src_of);
 }
 
+/* more than 64 KB of LDS has to be asked for, once on each device */
+static hipError_t allow_lds(const void *kernel, int bytes, uint64_t &done)
+{
+    int d = 0;
+    hipError_t e = hipGetDevice(&d);
+    if (e != hipSuccess || (d < 64 && (done >> d & 1))) return e;
+    e = hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e == hipSuccess && d < 64) done |= 1ull << d;
+    return e;
+}
+
 template <int F, int T, int KB, int NST, bool GROUPED, int OUT>
-static hipError_t i8_tile(const I8Args &a, hipStream_t st)
+static hipError_t i8_tile(const I8Args &a, I8Form form, hipStream_t st)
 {
     using C = I8Tile<F, T, KB, NST>;
-    constexpr int TR = 16 * T;
     constexpr int lds = C::lds(elem_bytes<OUT>());
-    static bool attr_done = false;
-    if (!attr_done) {
-        const hipError_t e = hipFuncSetAttribute((const void *)k_i8_tile<F, T, KB, NST, GROUPED, OUT>,
-                                                 hipFuncAttributeMaxDynamicSharedMemorySize, lds);
-        if (e != hipSuccess) return e;
-        attr_done = true;
-    }
-    const long tiles = GROUPED ? a.M / TR + (a.n_experts < a.M ? a.n_experts : a.M) : (a.M + TR - 1) / TR;
-    const long groups = tiles * ((a.N + F - 1) / F);
-    if (groups * C::NWAVE >= 1L << 26) return hipErrorInvalidConfiguration;   /* 2^32 threads */
+    static uint64_t done = 0;
+    const hipError_t e = allow_lds((const void *)k_i8_tile<F, T, KB, NST, GROUPED, OUT>, lds, done);
+    if (e != hipSuccess) return e;
+    const long groups = i8_waves(form, a.M, a.N, GROUPED ? a.n_experts : 0) / C::NWAVE;
     hipLaunchKernelGGL((k_i8_tile<F, T, KB, NST, GROUPED, OUT>), dim3((unsigned)groups), dim3(64 * C::NWAVE), lds, st, a);
     return hipGetLastError();
 }
@@ -503,19 +515,20 @@ static hipError_t i8_tile(const I8Args &a, hipStream_t st)
 template <bool GROUPED, int OUT>
 static hipError_t i8_launch(const I8Args &a, hipStream_t st)
 {
-    const int form = GROUPED ? i8_grouped_form(a.M, a.N, a.K, a.n_experts) : i8_form(a.M, a.N, a.K);
+    const I8Form form = GROUPED ? i8_grouped_form(a.M, a.N, a.K, a.n_experts) : i8_form(a.M, a.N, a.K);
+    if (i8_waves(form, a.M, a.N, GROUPED ? a.n_experts : 0) > I8_MAX_WAVES) return hipErrorInvalidConfiguration;
     if constexpr (GROUPED) {
         if (form == I8_PAIR) return i8_pair<4, 2, 4, 2, GROUPED, OUT>(a, st);
     } else {
         if (form == I8_PAIR) return i8_pair<1, 1, 8, 4, GROUPED, OUT>(a, st);
-        if (form == I8_64x2_DEEP) return i8_tile<64, 2, 2, 3, GROUPED, OUT>(a, st);
-        if (form == I8_64x4) return i8_tile<64, 4, 1, 3, GROUPED, OUT>(a, st);
-        if (form == I8_128x8) return i8_tile<128, 8, 1, 4, GROUPED, OUT>(a, st);
+        if (form == I8_64x2_DEEP) return i8_tile<64, 2, 2, 3, GROUPED, OUT>(a, form, st);
+        if (form == I8_64x4) return i8_tile<64, 4, 1, 3, GROUPED, OUT>(a, form, st);
+        if (form == I8_128x8) return i8_tile<128, 8, 1, 4, GROUPED, OUT>(a, form, st);
     }
     switch (form) {
-    case I8_64x2: return i8_tile<64, 2, 1, 4, GROUPED, OUT>(a, st);
-    case I8_128x4: return i8_tile<128, 4, 1, 3, GROUPED, OUT>(a, st);
-    default: return i8_tile<256, 8, 1, 3, GROUPED, OUT>(a, st);
+    case I8_64x2: return i8_tile<64, 2, 1, 4, GROUPED, OUT>(a, form, st);
+    case I8_128x4: return i8_tile<128, 4, 1, 3, GROUPED, OUT>(a, form, st);
+    default: return i8_tile<256, 8, 1, 3, GROUPED, OUT>(a, form, st);
     }
 }
 

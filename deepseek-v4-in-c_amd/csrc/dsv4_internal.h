@@ -532,7 +532,7 @@ hipError_t moe_combine_launch(const CombineArgs &a, hipStream_t st);
 
 /* rows to int8 codes and a scale each: a (and with SwiGLU u, a being the
  * gate) rows of k elements, `ld` elements apart, 16-byte aligned; Q [n][k]
- * 8-byte aligned. hipErrorInvalidConfiguration: more rows than a launch takes. */
+ * 8-byte aligned, n < 2^22. */
 struct QuantI8Args {
     int8_t *Q;
     float *S;
@@ -546,7 +546,7 @@ hipError_t quant_i8_launch(const QuantI8Args &a, int type, bool swiglu, hipStrea
 /* C [M][N]. One matrix: W [N][K], Sw [N], Aq [M][K], Sa [M]. Grouped (table
  * set): row r of bucket e (ex_off[e] <= r < ex_off[e + 1]) from row row_tok[r]
  * (or r) of Aq [n_a][K], n_a * K < 2^31. K a multiple of 16, Aq and W 16-byte
- * aligned. hipErrorInvalidConfiguration: more tiles than a launch takes. */
+ * aligned, i8_waves() at most I8_MAX_WAVES. */
 struct I8Args {
     const uint8_t *Aq;
     const float *Sa;

@@ -2171,6 +2171,8 @@ int dsv4_hip_gemm_i8_dev(void *C, int out_type, const int8_t *Aq, const float *S
     if (W->wdt != DSV4_WI8 || W->rows < 1 || W->cols < 16 || W->cols % 16 || W->cols > I8_KMAX)
         return fail("gemm_i8_dev: W must be DSV4_WI8 with cols a multiple of 16 up to %d (got wdt %d, %d x %d)",
                     I8_KMAX, W->wdt, W->rows, W->cols);
+    if (M && i8_waves(i8_form(M, W->rows, W->cols), M, W->rows, 0) > I8_MAX_WAVES)
+        return fail("gemm_i8_dev: %d x %d results are too many for one launch", M, W->rows);
     if (!aligned16(Aq) || !aligned16(W->w) || ((uintptr_t)Sa & 3u) || ((uintptr_t)W->s & 3u) ||
         !elem_aligned(C, out_type))
         return fail("gemm_i8_dev: Aq and w must be 16-byte aligned, scales and C to their elements");
@@ -2201,6 +2203,8 @@ int dsv4_hip_gemm_i8_grouped_dev(void *C, int out_type, const int8_t *Aq, const 
     if (N < 1 || K < 16 || K % 16 || K > I8_KMAX)
         return fail("gemm_i8_grouped_dev: need N > 0 and K a multiple of 16 up to %d (got %d, %d)", I8_KMAX, N, K);
     if ((long)n_a * K > 0x7FFFFFFFL) return fail("gemm_i8_grouped_dev: n_a * K is 2^31 or more");
+    if (n_rows && i8_waves(i8_grouped_form(n_rows, N, K, n_experts), n_rows, N, n_experts) > I8_MAX_WAVES)
+        return fail("gemm_i8_grouped_dev: %d x %d results are too many for one launch", n_rows, N);
     if (!aligned16(Aq) || ((uintptr_t)Sa & 3u) || ((uintptr_t)ex_off & 3u) || ((uintptr_t)row_tok & 3u) ||
         ((uintptr_t)table & 7u) || !elem_aligned(C, out_type))
         return fail("gemm_i8_grouped_dev: Aq must be 16-byte aligned, the others to their elements");
@@ -2388,6 +2392,7 @@ static int quant_i8(int8_t *Q, float *S, const void *x, const void *u, bool swig
 {
     if (n && (!Q || !S || !x || (swiglu && !u))) return fail("%s: NULL pointer", what);
     if (!elem_type_ok(type)) return fail("%s: unknown element type %d", what, type);
+    if (n >= 1 << 22) return fail("%s: %d rows are too many for one launch", what, n);
     if (n < 0 || k < 16 || k % 16 || ld < k || ld > (1LL << 40) || ld * elem_bytes_of(type) % 16)
         return fail("%s: need n >= 0, k a multiple of 16 and ld >= k of whole 16-byte steps (got %d, %d, %lld)", what,
                     n, k, (long long)ld);

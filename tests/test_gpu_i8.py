@@ -393,3 +393,66 @@ def test_experts_product_stays_in_bounds_with_bad_offsets(lib, pkg):
     for off in ([0, 10, 5, 1 << 30, 20, 25], [-50, -1, 3, 3, 2, 900], [30, 30, 30, 30, 30, 30]):
         run_grouped(lib, pkg, a, sa, torch.tensor(off, dtype=torch.int32, device=DEV), None, R, w, sw, torch.float32)
     lib.status()
+
+
+# ------------------------------------------------------------- large sizes ----
+
+def test_product_beyond_4_gib(lib, pkg):
+    """Results, then tokens, of more than 2^32 bytes: the last rows are right."""
+    M, N, K = 300001, 8192, 64
+    a, sa, w, sw = operands(M, N, K, 1)
+    C = torch.empty(M, N, dtype=torch.bfloat16, device=DEV)
+    run_gemm(lib, pkg, a, sa, w, sw, torch.bfloat16, C=C)
+    for r in (slice(0, 40), slice(262100, 262200), slice(M - 70, M)):
+        close(C[r], a[r], sa[r], w, sw)
+    del C
+    M, N, K = 1100003, 24, 4096
+    a, sa, w, sw = operands(M, N, K, 2)
+    C = run_gemm(lib, pkg, a, sa, w, sw, torch.float32)
+    for r in (slice(0, 40), slice(1048500, 1048700), slice(M - 70, M)):
+        close(C[r], a[r], sa[r], w, sw)
+
+
+def test_experts_product_beyond_4_gib(lib, pkg):
+    R, N, K = 300001, 8192, 64
+    a, sa, w, sw = operands(1000, 2 * N, K, 3)
+    w, sw = w.view(2, N, K), sw.view(2, N)
+    off = buckets([270000, R - 270000]).to(DEV)
+    tok = torch.randint(0, 1000, (R,), dtype=torch.int32, device=DEV, generator=gen(4))
+    C = run_grouped(lib, pkg, a, sa, off, tok, R, w, sw, torch.bfloat16)
+    for e, r in ((0, slice(0, 40)), (0, slice(269900, 270000)), (1, slice(270000, 270100)), (1, slice(R - 70, R))):
+        i = tok[r].long()
+        close(C[r], a[i], sa[i], w[e], sw[e])
+
+
+def test_rows_beyond_4_gib(lib):
+    n, k = 300001, 8192
+    x = torch.empty(n, k, dtype=torch.bfloat16, device=DEV).normal_(generator=gen(5))
+    q, s = quant(lib, x)
+    for r in (slice(0, 8), slice(262140, 262150), slice(n - 8, n)):
+        check_rows(q[r], s[r], x[r].double())
+
+
+def test_too_large_for_a_launch_is_refused(lib, pkg):
+    """and leaves the library alive"""
+    a, sa, w, sw = operands(2, 3, 16, 6)
+    c = torch.empty(2, 3, device=DEV)
+    d = pkg.qmat(pkg.DSV4_WI8, w.data_ptr(), sw.data_ptr(), 1 << 20, 16, 1, 16)
+    for m in ((1 << 31) - 1, 1 << 28):
+        with pytest.raises(pkg.Dsv4Error, match="too many"):
+            lib.gemm_i8_dev(c.data_ptr(), 0, a.data_ptr(), sa.data_ptr(), m, d)
+    with pytest.raises(pkg.Dsv4Error, match="too many"):
+        lib.quant_i8_dev(a.data_ptr(), sa.data_ptr(), w.data_ptr(), 0, 16, 1 << 30, 16)
+    close(run_gemm(lib, pkg, a, sa, w, sw, torch.float32), a, sa, w, sw)
+
+
+def test_other_calls_refuse_int8_weights(lib, pkg):
+    """fp32 tokens have no exact product with them: the drop-in matmul and the
+    dequantizer know only the packed formats."""
+    _, _, w, sw = operands(1, 128, 128, 7)
+    x, y = torch.zeros(128, device=DEV), torch.zeros(128 * 128, device=DEV)
+    d = pkg.qmat(pkg.DSV4_WI8, w.data_ptr(), sw.data_ptr(), 128, 128, 1, 128)
+    for call in (lambda: lib.mmq_n_dev(y.data_ptr(), x.data_ptr(), d, 1), lambda: lib.dequant_dev(y.data_ptr(), d),
+                 lambda: lib.gemm_fp8_dev(y.data_ptr(), False, x.data_ptr(), False, 1, d)):
+        with pytest.raises(pkg.Dsv4Error):
+            call()

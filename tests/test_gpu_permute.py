@@ -302,6 +302,48 @@ def test_on_streams_and_in_a_graph(lib):
             close(out, want, x.double().abs() * (1 + w.double().sum(1, keepdim=True)), (topk + 1) * U)
 
 
+def test_rows_beyond_4_gib(lib):
+    n, topk, E, h = 70001, 8, 256, 4096
+    ids = routing(n, topk, E, 1)
+    idx = torch.from_numpy(ids).to(DEV)
+    x = torch.empty(n, h, dtype=torch.bfloat16, device=DEV).normal_(generator=gen(1))
+    o = room(x, idx, E)
+    permute_into(lib, o, x, idx, E)
+    off, tok, pos = want_order(ids, E)
+    assert torch.equal(o["pos"][1:-1].cpu(), torch.from_numpy(pos).int())
+    assert torch.equal(o["off"][1:-1].cpu(), torch.from_numpy(off).int())
+    rows, p32 = o["rows"][1:-1], o["pos"][1:-1].contiguous()
+    for r in (slice(0, 50), slice(524280, 524300), slice(n * topk - 50, n * topk)):
+        assert torch.equal(rows[r], x[torch.from_numpy(tok[r]).to(DEV)])
+    w = torch.rand(n, topk, device=DEV, generator=gen(2))
+    out = torch.empty_like(x)
+    lib.moe_unpermute_dev(out.data_ptr(), rows.data_ptr(), 1, p32.data_ptr(), w.data_ptr(), None, n, topk, h)
+    drows, dw = torch.empty_like(o["rows"]), torch.empty_like(w)
+    lib.moe_unpermute_bwd_dev(drows[1:].data_ptr(), dw.data_ptr(), x.data_ptr(), rows.data_ptr(), 1, p32.data_ptr(),
+                              w.data_ptr(), n, topk, h)
+    for t in (0, 65530, n - 1):
+        want = x[t].double() * w[t].double().sum()
+        close(out[t], want, want.abs(), (topk + 1) * U)
+        sq = (x[t].double() ** 2).sum()
+        assert ((dw[t].double() - sq).abs() <= h * U * sq).all()
+        for k in range(topk):
+            d = w[t, k].double() * x[t].double()
+            close(drows[1 + int(pos[t * topk + k])], d, d.abs(), U)
+
+
+def test_route_dev_orders_the_rows_of_these_calls(lib):
+    """The framework's own permutation gives the same order, so its arrays serve
+    the way back and the experts' products as well."""
+    n, topk, E, h = 321, 6, 40, 64
+    ids = routing(n, topk, E, 3)
+    idx = torch.from_numpy(ids).to(DEV)
+    x = torch.randn(n, h, device=DEV, generator=gen(1))
+    o = permute(lib, x, idx, E)
+    off, tok, k, pos = (torch.empty(s, dtype=torch.int32, device=DEV) for s in (E + 1, n * topk, n * topk, n * topk))
+    lib.moe_route_dev(off.data_ptr(), tok.data_ptr(), k.data_ptr(), pos.data_ptr(), idx.data_ptr(), n, topk, E)
+    assert torch.equal(off, o["off"][1:-1]) and torch.equal(tok, o["tok"][1:-1]) and torch.equal(pos, o["pos"][1:-1])
+
+
 # ------------------------------------------------------- an expert layer ----
 
 @pytest.mark.parametrize("n,dropped", [(1, 0.0), (7, 0.0), (77, 0.3), (300, 0.0)])

@@ -17,6 +17,7 @@ using namespace dsv4;
 extern "C" {
 int c_form(int M, int N, int K) { return i8_form(M, N, K); }
 int c_grouped(int M, int N, int K, int ne) { return i8_grouped_form(M, N, K, ne); }
+long c_waves(int form, long M, long N, long ne) { return i8_waves((I8Form)form, M, N, ne); }
 }
 """
 PAIR, T64x2, T64x2_DEEP, T64x4, T128x4, T128x8, T256x8 = range(1, 8)
@@ -29,7 +30,9 @@ def rules(tmp_path_factory):
     src.write_text(SHIM)
     subprocess.run(["g++", "-O1", "-std=c++17", "-Wall", "-Werror", "-shared", "-fPIC", "-I",
                     os.path.join(PKG_DIR, "csrc"), str(src), "-o", str(so)], check=True)
-    return C.CDLL(str(so))
+    lib = C.CDLL(str(so))
+    lib.c_waves.argtypes, lib.c_waves.restype = [C.c_int, C.c_long, C.c_long, C.c_long], C.c_long
+    return lib
 
 
 @pytest.mark.parametrize("M,N,K,form", [
@@ -52,3 +55,21 @@ def test_gpu_tests_reach_every_form(rules):
     assert {rules.c_form(*s) for s in test_gpu_i8.SHAPES} == set(range(1, 8))
     groups = {rules.c_grouped(sum(c) + 5, N, K, len(c)) for c, N, K in test_gpu_i8.GROUPS}
     assert groups == {PAIR, T64x2, T128x4, T256x8}
+
+
+@pytest.mark.parametrize("form,F,TR,waves", [(PAIR, 8, 8, 8), (T64x2, 64, 32, 4), (T64x2_DEEP, 64, 32, 4),
+                                             (T64x4, 64, 64, 8), (T128x4, 128, 64, 8), (T128x8, 128, 128, 8),
+                                             (T256x8, 256, 128, 8)])
+def test_waves_of_a_launch(rules, form, F, TR, waves):
+    """A tile for every F features and TR rows; rows and features of 2^31 - 1 do
+    not wrap."""
+    for M, N in ((1, 1), (TR, F), (TR + 1, F + 1), (1000, 777), ((1 << 31) - 1, (1 << 31) - 1)):
+        assert rules.c_waves(form, M, N, 0) == -(-M // TR) * -(-N // F) * waves
+
+
+@pytest.mark.parametrize("form,F,TR,waves", [(PAIR, 32, 16, 4), (T64x2, 64, 32, 4), (T128x4, 128, 64, 8),
+                                             (T256x8, 256, 128, 8)])
+@pytest.mark.parametrize("counts", [[0, 0, 5], [1] * 300, [127, 129, 0, 31, 33], [2000]])
+def test_waves_hold_every_bucket(rules, form, F, TR, waves, counts):
+    tiles = sum(-(-c // TR) for c in counts)
+    assert rules.c_waves(form, sum(counts), 100, len(counts)) >= tiles * -(-100 // F) * waves

@@ -94,6 +94,23 @@ def test_bad_argument_is_refused(calls, name, arg, value):
     assert rc == -1 and why and "init" not in why
 
 
+@pytest.mark.parametrize("m,n", [((1 << 31) - 1, 1 << 20), (1 << 28, 1 << 20), ((1 << 31) - 1, 64), (1, (1 << 31) - 1),
+                                 (1 << 24, 1 << 16), ((1 << 31) - 100, 3)])
+def test_more_than_a_launch_takes_is_refused(calls, m, n):
+    run, w = calls
+    rc, why = run("gemm", M=m, W=w(rows=n))
+    assert rc == -1 and "too many" in why
+    rc, why = run("grouped", n_rows=m, N=n)
+    assert rc == -1 and "too many" in why
+
+
+@pytest.mark.parametrize("n", [1 << 22, (1 << 31) - 1])
+def test_more_rows_than_a_launch_takes_are_refused(calls, n):
+    for name in ("quant", "swiglu"):
+        rc, why = calls[0](name, n=n)
+        assert rc == -1 and "too many" in why
+
+
 @pytest.mark.parametrize("field,value", [("wdt", 2), ("rows", 0), ("cols", 0), ("cols", 40), ("cols", 131072),
                                          ("w", None), ("s", None), ("w", P + 8), ("s", P + 2)])
 def test_bad_matrix_is_refused(calls, field, value):
