@@ -402,14 +402,16 @@ __global__ __launch_bounds__((64 * I8Tile<F, T, KB, NST>::NWAVE)) void k_i8_tile
     /* load i of a wave's share of stage st; past the end zeros, no traffic */
     auto issue = [&](int st, int slot, int i) {
         constexpr int LB = C::LW + C::LX;
-        const int in = st * KB + i / LB, k = i % LB, blk = in + rot < nblk ? in + rot : in + rot - nblk;
+        const int in = st * KB + i / LB, k = i % LB;
         const uint32_t oob = in < nblk ? 0u : I8_OOB;
-        const int so = in < nblk ? blk * 128 : 0;
+        int blk = min(in, nblk - 1);
+        if (GROUPED) blk = blk + rot < nblk ? blk + rot : blk + rot - nblk;
+        const int so = blk * 128;
         uint8_t *buf = lds + slot * C::STAGE + i / LB * C::SUB;
         if (k < C::LW) i8_dma16(rw, wo[min(k, C::LW - 1)] | oob, so, buf + 1024 * (C::LW * wave + k));
         else {
             const int j = max(0, min(k - C::LW, C::LX - 1));
-            i8_dma16(rx, (blk != nblk - 1 ? xo[j] : xl[j]) | oob, so, buf + C::OFF_X + 1024 * (C::LX * wave + j));
+            i8_dma16(rx, (blk < nblk - 1 ? xo[j] : xl[j]) | oob, so, buf + C::OFF_X + 1024 * (C::LX * wave + j));
         }
     };
 #pragma unroll
