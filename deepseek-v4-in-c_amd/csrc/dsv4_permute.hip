@@ -11,9 +11,12 @@
  * Sums run in fp32 in k order (dw: over a thread's elements, then over
  * threads in a fixed tree) and are rounded once to the element type, so the
  * same call gives the same bits. A pair without a row (pos outside [0, n *
- * topk)) adds nothing, receives nothing and has dw 0. All of them stream
- * memory and are bound by it; none uses a workspace.
- */
+ * topk)) adds nothing, receives nothing and has dw 0. None uses a workspace.
+ *
+ * Bound: memory. us at 4,096 tokens of 4,096 bf16, six rows each (235 MB, 46 at
+ * the rate of a plain copy): sort and copy 48.5, the gradient 43; 2,803 tokens of
+ * which half the pairs are here: way back 18.2 (5.1 TB/s), both gradients 29.9
+ * (5.4 TB/s). 64 tokens 5.2, the sort's chain of loads, counts and barriers. */
 #include <algorithm>
 #include <initializer_list>
 

@@ -14,10 +14,15 @@
  *   16,000) fp64 decides, where 127 a_j is exact and the quotient rounds to a
  *   half-integer only if it is one: codes depend on no rounding on the way.
  *   With SwiGLU the values are fp32 ones within 8 x 2^-24 (exp 1 ulp and
- *   its correction half, 1 + e half, reciprocal 1 ulp, two products): certain outside 2^-13 of a
- *   half-integer. Inside it, and for the row's largest value, the SwiGLU is
+ *   its correction half, 1 + e half, reciprocal 1 ulp, two products): with the product by 127 /
+ *   amax 10 x 2^-24 of at most 127: certain outside 1.37 x 2^-14 of a half-integer. Inside it, and for the row's largest value, the SwiGLU is
  *   taken in fp64: codes and scale are those of fp64 values. Rows whose largest value is below 2^-60 or beyond 2^120
  *   compute everything in fp64.
+ *
+ * Bound: HBM for plain rows (8,192 of 4,096 bf16 19.6 us, 5.1 TB/s), the vector
+ * unit for SwiGLU (some 40 instructions an element, 10 of the 14 us of 4,206
+ * rows of 2,048 whose bytes take 8.5; 24,576 rows 59 to 64, 4 TB/s), latency for
+ * a few rows (one of 4,096 2.6 us, less than the launch costs its caller).
  */
 #include "dsv4_elem.h"
 #include "dsv4_internal.h"
@@ -168,13 +173,20 @@ __global__ __launch_bounds__(NW == 1 ? 256 : 64 * NW) void k_quant_i8(QuantI8Arg
     };
 
     /* the largest magnitude, as the bits of |a|: NaN above inf above all else */
-    uint32_t m = 0;
+    uint32_t m = 0, top[NCH];                      /* of the row, of each unit */
+    auto tops = [&]() {
+#pragma unroll
+        for (int c = 0; c < NCH; c++) {
+            top[c] = 0;
+#pragma unroll
+            for (int i = 0; i < QU; i++) top[c] = max(top[c], __float_as_uint(f[c][i]) & 0x7FFFFFFFu);
+        }
+    };
     for (int base = 0; base < a.k; base += NCH * STEP) {
         fetch(base);
+        tops();
 #pragma unroll
-        for (int c = 0; c < NCH; c++)
-#pragma unroll
-            for (int i = 0; i < QU; i++) m = max(m, __float_as_uint(f[c][i]) & 0x7FFFFFFFu);
+        for (int c = 0; c < NCH; c++) m = max(m, top[c]);
     }
     m = wave_max_u32(m);
     if constexpr (NW > 1) {
@@ -202,13 +214,13 @@ __global__ __launch_bounds__(NW == 1 ? 256 : 64 * NW) void k_quant_i8(QuantI8Arg
         } else {
             const float near = amax * (1.0f - 0x1p-18f);
             for (int base = 0; base < a.k; base += NCH * STEP) {
-                if (!once) fetch(base);
+                if (!once) {
+                    fetch(base);
+                    tops();
+                }
 #pragma unroll
                 for (int c = 0; c < NCH; c++) {
-                    float top = 0.0f;
-#pragma unroll
-                    for (int i = 0; i < QU; i++) top = fmaxf(top, fabsf(f[c][i]));
-                    if (top >= near)
+                    if (__uint_as_float(top[c]) >= near)
                         for (int i = 0; i < QU; i++) {
                             const int j = base + j0 + c * STEP + i;
                             float t = 0.0f;
@@ -230,10 +242,9 @@ __global__ __launch_bounds__(NW == 1 ? 256 : 64 * NW) void k_quant_i8(QuantI8Arg
     /* tiny rows are multiplied by 2^64 first (exactly), so that 127 / amax
      * stays finite and the values normal */
     const bool tiny = !SWIGLU && amax < 0x1p-64f;
-    const float up = tiny ? 0x1p64f : 1.0f;
-    const float inv = bad || wide || !(amax > 0.0f) ? 0.0f
-                    : SWIGLU ? (float)(127.0 / amax64) : 127.0f / (amax * up);
-    constexpr float SURE = SWIGLU ? 0.5f - 0x1p-13f : 0.5f - 0x1p-15f;
+    const bool sure = !bad && !wide && amax > 0.0f;    /* the codes of fp32 products */
+    const float inv = !sure ? 0.0f : SWIGLU ? (float)(127.0 / amax64) : 127.0f / (tiny ? amax * 0x1p64f : amax);
+    constexpr float SURE = SWIGLU ? 0.5f - 0x1.6p-14f : 0.5f - 0x1p-15f;
     int8_t *q = a.Q + (size_t)row * (size_t)a.k;
     for (int base = 0; base < a.k; base += NCH * STEP) {
         if (!once) fetch(base);
@@ -243,10 +254,13 @@ __global__ __launch_bounds__(NW == 1 ? 256 : 64 * NW) void k_quant_i8(QuantI8Arg
             if (j >= a.k) continue;
             uint32_t t[QU];
             float far = 0.0f;
+            if (!sure || tiny) {
+#pragma unroll
+                for (int i = 0; i < QU; i++) f[c][i] = sure ? __fmul_rn(f[c][i], 0x1p64f) : 0.0f;
+            }
 #pragma unroll
             for (int i = 0; i < QU; i++) {
-                const float x = inv == 0.0f ? 0.0f : f[c][i];
-                const float v = __fmul_rn(__fmul_rn(x, up), inv);
+                const float v = __fmul_rn(f[c][i], inv);
                 const float s = __fadd_rn(v, ROUND_MAGIC);
                 t[i] = __float_as_uint(s);
                 far = fmaxf(far, fabsf(__fsub_rn(v, __fsub_rn(s, ROUND_MAGIC))));
@@ -255,13 +269,15 @@ __global__ __launch_bounds__(NW == 1 ? 256 : 64 * NW) void k_quant_i8(QuantI8Arg
                 for (int i = 0; i < QU; i++) t[i] = code64(exact(j + i), amax64);
             } else if (far > SURE) {
                 for (int i = 0; i < QU; i++) {
-                    const float v = __fmul_rn(__fmul_rn(f[c][i], up), inv);
+                    const float v = __fmul_rn(f[c][i], inv);
                     if (fabsf(__fsub_rn(v, rintf(v))) > SURE) t[i] = code64(exact(j + i), amax64);
                 }
             }
-            u32x2 o;
-            o.x = (t[0] & 0xFFu) | (t[1] & 0xFFu) << 8 | (t[2] & 0xFFu) << 16 | t[3] << 24;
-            o.y = (t[4] & 0xFFu) | (t[5] & 0xFFu) << 8 | (t[6] & 0xFFu) << 16 | t[7] << 24;
+            u32x2 o;                               /* the low bytes, in order */
+#pragma unroll
+            for (int h = 0; h < 2; h++)
+                o[h] = __builtin_amdgcn_perm(__builtin_amdgcn_perm(t[4 * h + 3], t[4 * h + 2], 0x0C0C0400u),
+                                             __builtin_amdgcn_perm(t[4 * h + 1], t[4 * h], 0x0C0C0400u), 0x05040100u);
             *(DSV4_GLOBAL u32x2 *)(q + j) = o;
         }
     }
