@@ -216,35 +216,47 @@ constexpr int bf16_rows_depth(int rows, int cols) { return cols < 1024 && rows >
  * two blocks of K a stage. */
 enum I8Form { I8_PAIR = 1, I8_64x2, I8_64x2_DEEP, I8_64x4, I8_128x4, I8_128x8, I8_256x8 };
 
+/* Cost of a tiled form with `tiles` row tiles, in hundredths of a us: c0 once,
+ * and for a round of 256 workgroups `fix` (first loads, the tile's way out) and
+ * `slope` at K = 4096; the last round costs the share `r` of one and the rest by
+ * how full it is. Fitted to (us, 64x2 / 64x4 / 128x4 / 128x8 / 256x8) K = 4096: 128
+ * rows 4096 x 4096 8.4 / 10.2 / 12.3 / 16.2 / 26, 333 rows 16.3 / 14.1 / 12.9 / 16.2
+ * / 26, 700 rows 29.1 / 21.7 / 21.9 / 18.4 / 27.9, 1,024 rows 38 / 29 / 24 / 22 / 30,
+ * 2,048 rows 75 / 55 / 46 / 42 / 36; 1,000 rows 2048 x 2048 13.4 / 11.2 / 9.0 / 11.3
+ * / 17.4; and short rows, where a round is all start and end: 1,630 rows 10288 x
+ * 208 34 / 24 / 23 / 29 / 29, 10288 x 1040 65 / 47 / 44 / 49 / 48; 260 rows 24952 x
+ * 384 19 / 14.8 / 12.8 / 18.8 / 19.4. */
+struct I8Cost { I8Form form; int F, TR, c0, fix, slope, r; };
+constexpr I8Cost I8_COSTS[] = {
+    {I8_64x2, 64, 32, 50, 85, 365, 89},   {I8_64x4, 64, 64, 0, 110, 540, 100}, {I8_128x4, 128, 64, -50, 200, 900, 86},
+    {I8_128x8, 128, 128, -200, 470, 1580, 71}, {I8_256x8, 256, 128, -200, 790, 2660, 72}};
+inline long i8_cost(const I8Cost &c, long tiles, long N, long K, long more = 0)
+{
+    const long w = tiles * ceil_div(N, c.F), full = (w - 1) / CUS, last = w - full * CUS;
+    const long round = c.fix + more + c.slope * K / 4096;
+    return c.c0 * K / 4096 + round * full + round * (c.r + (100 - c.r) * last / CUS) / 100;
+}
+
 /* One matrix. Few rows of a matrix of few rows are latency: the pair form's
  * workgroups wait out one load (us, pair / 64x2 deep / 64x2: 1 x 4096 x 4096
  * 5.0 / 7.0 / 7.8, 8 x 4096 x 4096 6.2 / 7.2 / 7.9, 12 x 1024 x 4096 4.3 / 7.0 /
  * 7.8; but 16 x 4096 x 4096 9.7 / 7.3 / 8.0, 1 x 32768 x 1024 14.1 / 7.7 / 7.5).
- * Otherwise the form of least cost, in tenths of a us at K = 4096: `per` a full
- * round of 256 workgroups, `base` a nearly empty one, `c0` once. They were
- * fitted to (us, 64x2 / 64x4 / 128x4 / 128x8 / 256x8) 128 rows 4096 x 4096 8.4 /
- * 10.2 / 12.3 / 16.2 / 26, 333 rows 16.3 / 14.1 / 12.9 / 16.2 / 26, 700 rows 29.1
- * / 21.7 / 21.9 / 18.4 / 27.9, 1,024 rows 38 / 29 / 24 / 22 / 30, 2,048 rows 75 /
- * 55 / 46 / 42 / 36; 1,000 rows 2048 x 2048 13.4 / 11.2 / 9.0 / 11.3 / 17.4. In
- * one round 64x2 takes two blocks of K a stage (8.0 -> 7.2 at 16 rows; with
- * three workgroups a CU its longer ring costs, 512 rows 21.4 -> 21.9). */
+ * Otherwise the form of least cost. In one round 64x2 takes two blocks of K a
+ * stage (8.0 -> 7.2 at 16 rows; with three workgroups a CU its longer ring
+ * costs, 512 rows 21.4 -> 21.9). */
 constexpr long I8_PAIR_GROUPS = 768;
 inline I8Form i8_form(int M, int N, int K)
 {
     if (ceil_div(M, 8) * ceil_div(N, 8) <= I8_PAIR_GROUPS) return I8_PAIR;
-    struct { I8Form form; int F, TR, c0, base, per; } const f[] = {
-        {I8_64x2, 64, 32, 5, 40, 45}, {I8_64x4, 64, 64, 0, 65, 65}, {I8_128x4, 128, 64, -5, 95, 110},
-        {I8_128x8, 128, 128, -20, 145, 205}, {I8_256x8, 256, 128, -20, 250, 345}};
     if (ceil_div(M, 128) * ceil_div(N, 256) >= 1L << 20) return I8_256x8;     /* costs beyond 64 bits */
-    I8Form best = I8_64x2;
+    I8Form best = I8_256x8;
     long least = -1;
-    for (const auto &c : f) {
-        const long w = ceil_div(M, c.TR) * ceil_div(N, c.F), full = (w - 1) / CUS, last = w - full * CUS;
-        const long cost = 30 * 4096L + (c.c0 + full * c.per + c.base + (c.per - c.base) * last / CUS) * K;
+    for (const I8Cost &c : I8_COSTS) {
+        const long cost = i8_cost(c, ceil_div(M, c.TR), N, K);
         if (least < 0 || cost < least) {
             least = cost;
             best = c.form;
-            if (c.form == I8_64x2 && w <= CUS && K >= 1024) best = I8_64x2_DEEP;
+            if (c.form == I8_64x2 && ceil_div(M, c.TR) * ceil_div(N, c.F) <= CUS && K >= 1024) best = I8_64x2_DEEP;
         }
     }
     return best;
@@ -253,14 +265,32 @@ inline I8Form i8_form(int M, int N, int K)
 /* Buckets of ne experts, M rows in all; the mean bucket decides. us, pair /
  * 64x2 / 128x4 / 256x8, experts 2048 x 4096 on 256: 384 rows Zipf 178 / 176 /
  * 176 / 192, 768 rows 322 / 350 / 359 / 370, 2,400 rows 370 / 377 / 384 / 379,
- * 3,072 rows 414 / 380 / 389 / 382, 6,144 rows Zipf 740 / 415 / 398 / 423, 12,288
+ * 6,144 rows Zipf 740 / 415 / 398 / 423, 12,288
  * rows Zipf - / 522 / 446 / 455, even 530 / 414 / 403 (64x2 on), 24,576 rows Zipf
  * 745 / 565 / 522. Too little weight to fill the CUs: 6 rows 15.1 / 12.4 / 14.8,
- * 160 rows on 64 of 512 x 1024 8.5 / 7.0 / 8.1, but 1,600 of them - / 9.3 / 8.7. */
+ * 160 rows on 64 of 512 x 1024 8.5 / 7.0 / 8.1, but 1,600 of them - / 9.2 / 8.9 /
+ * 14.8; from there the form of least cost, a round of buckets 1.5 us more than
+ * one matrix's: 8,000 of them - / 23.2 / 21.8 / 18.8, 1,200 rows on 16 of 1024 x
+ * 2048 - / 12.9 / 11.8 / 20.3, 1,400 rows on 36 of 128 x 608 - / 5.5 / 6.7 / 11.5. */
+constexpr int I8_BUCKET_COST = 150;
 inline I8Form i8_grouped_form(int M, int N, int K, int ne)
 {
     const long hit = M < ne ? M : ne;
-    if (hit * N * K < 1L << 26 && M <= 16 * hit) return I8_64x2;
+    if (hit * N * K < 1L << 26) {                  /* no stream to feed: by cost, as one matrix */
+        if (M <= 16 * hit) return I8_64x2;
+        if (ceil_div(M, 128) * ceil_div(N, 256) >= 1L << 20) return I8_256x8;
+        I8Form best = I8_256x8;
+        long least = -1;
+        for (const I8Cost &c : I8_COSTS) {
+            if (c.form == I8_64x4 || c.form == I8_128x8) continue;             /* not built for buckets */
+            const long cost = i8_cost(c, M / c.TR + ceil_div(hit, 2), N, K, I8_BUCKET_COST);
+            if (least < 0 || cost < least) {
+                least = cost;
+                best = c.form;
+            }
+        }
+        return best;
+    }
     if (M <= 10 * hit) return I8_PAIR;
     if (M <= 20 * hit) return I8_64x2;
     return M < 60 * hit ? I8_128x4 : I8_256x8;

@@ -213,7 +213,8 @@ SHAPES = [(1, 4096, 4096), (1, 1, 16), (1, 17, 48), (2, 255, 1040), (5, 300, 512
           (64, 64, 4096), (65, 129, 96), (100, 1000, 512), (129, 128, 128), (130, 384, 1136), (257, 260, 2048),
           (300, 1024, 4096), (333, 777, 4112), (512, 513, 640), (1000, 1023, 208), (2048, 256, 1024),
           (701, 2048, 4096), (1300, 1536, 16), (3, 5, 16384), (2, 40000, 256), (4097, 100, 192), (2051, 4099, 528),
-          (1000, 4096, 528), (1025, 4080, 272), (2048, 4096, 4096), (2050, 4100, 1040), (40, 32768, 1024), (14, 700, 8208)]
+          (1000, 4096, 528), (1025, 4080, 272), (2048, 4096, 4096), (2050, 4100, 1040), (40, 32768, 1024), (14, 700, 8208),
+          (1000, 4095, 4096)]
 
 
 @pytest.mark.parametrize("M,N,K", SHAPES)
@@ -330,7 +331,7 @@ GROUPS = [([0, 0, 1, 0], 40, 64), ([3, 0, 17, 5, 64, 1], 130, 272), ([65, 0, 128
           ([700, 3, 0, 0, 40, 1], 515, 2048), ([0, 0], 16, 16), ([16, 15, 17, 33, 31, 32], 512, 144),
           ([100, 90, 110, 95] * 4, 1024, 640), ([1, 0, 3, 16, 2, 9, 40, 1] * 8, 1030, 1040),
           ([0, 7, 20, 1] * 16, 1024, 2064),
-          ([40, 0, 30, 50, 65], 300, 272)]
+          ([40, 0, 30, 50, 65], 300, 272), ([100, 64, 140, 90], 4100, 4112), ([120, 128, 0, 131] * 16, 510, 1024)]
 
 
 @pytest.mark.parametrize("case", range(len(GROUPS)))
