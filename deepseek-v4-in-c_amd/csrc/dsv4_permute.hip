@@ -108,6 +108,7 @@ __global__ __launch_bounds__(1024) void k_permute_one(PermuteArgs a, int tpb)
 {
     constexpr int NT = 1024, PF = 8, IDS = 8, EB = elem_bytes<TYPE>();
     static_assert(PERMUTE_ONE_MAX < 65536, "two counts in a word");
+    static_assert(PERMUTE_ONE_MAX / 256 + MAX_TOPK <= 256, "own pairs");
     __shared__ uint32_t cnt[MAX_E];
     __shared__ int off[MAX_E];
     __shared__ int own_row[256];
@@ -454,9 +455,16 @@ template <int TYPE, int V>
 hipError_t permute_t(const PermuteArgs &a, hipStream_t st)
 {
     const long pairs = (long)a.n * a.topk;
-    if (pairs <= PERMUTE_ONE_MAX) {
-        /* a workgroup a CU (each counts every pair), of at most 16 tokens */
-        const int tpb = std::min(16, (a.n + 255) / 256 + (a.n == 0));
+    /* One launch with a workgroup a CU, since each counts every pair (us, at most
+     * 16 tokens a workgroup / this / four launches: 32,000 x 1 of 128 bf16 69.4 /
+     * 16.0 / 19.4, 16,000 x 2 of 256 39.7 / 17.5 / 19.5, 8,000 x 2 of 1024 18.0 /
+     * 15.4 / 20.6). Four launches for more pairs (39,456 of 1024 36.2 in one, 28.5
+     * in four) and where the copy of long rows outweighs the launches (32,000 x 1
+     * of 2048 86.7 / 59.3 / 51.8, 16,000 x 2 of 4096 93.9 / 97.0 / 90.7; 4,096 x 6
+     * of 4096 45.0 / 45.0 / 46.4, 8,000 x 1 of 2048 15.6 / 14.7 / 23.5). */
+    const int tpb = a.n ? (int)(((long)a.n + 255) / 256) : 1;
+    const bool long_copy = tpb > 16 && (long)a.n * a.hidden * elem_bytes<TYPE>() > 64L << 20;
+    if (pairs <= PERMUTE_ONE_MAX && !long_copy) {
         const int blocks = a.n > 0 ? (a.n + tpb - 1) / tpb : 1;
         hipLaunchKernelGGL((k_permute_one<TYPE, V>), dim3(blocks), dim3(1024), 0, st, a, tpb);
         return hipGetLastError();

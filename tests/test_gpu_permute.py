@@ -98,7 +98,8 @@ def test_order(lib, n, topk, E, h, kind):
 
 
 @pytest.mark.parametrize("n,topk,E,h", [(32769, 1, 256, 16), (5500, 6, 256, 64), (4100, 8, 1024, 24), (2200, 16, 1, 9),
-                                        (20000, 6, 100, 8), (33000, 2, 1024, 4)])
+                                        (20000, 6, 100, 8), (33000, 2, 1024, 4), (32768, 1, 64, 24), (16383, 2, 1000, 40),
+                                        (8000, 4, 7, 72), (5461, 6, 128, 100), (4100, 7, 40, 33), (4097, 2, 16, 8208)])
 @pytest.mark.parametrize("kind", ["all", "dropped", "skew"])
 def test_order_of_many_pairs(lib, n, topk, E, h, kind):
     dtype = TYPES[n % 3]
