@@ -497,7 +497,7 @@ hipError_t unpermute_t(const UnpermuteArgs &a, hipStream_t st)
 template <int TYPE, int V>
 hipError_t unpermute_bwd_t(const UnpermuteBwdArgs &a, hipStream_t st)
 {
-    if ((long)a.n * 16 > MAX_WAVES) return hipErrorInvalidConfiguration;
+    if ((long)a.n * 4 > MAX_WAVES) return hipErrorInvalidConfiguration;
     const bool once = reads_once<TYPE>(a.n, a.topk, a.hidden);
     /* fewer tokens than CUs: more threads each (7 tokens of 7,216 bf16, the
      * forward pass included, 13.9 -> 10.2 us) */

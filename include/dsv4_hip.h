@@ -409,7 +409,9 @@ int  dsv4_hip_gemm_i8_grouped_dev(void *C, int out_type, const int8_t *Aq, const
  * as they are. n = 0 gives empty buckets.
  * x [n][hidden], rows [n * topk][hidden] of `type`; n_experts <= 1024, topk <=
  * 16, n * topk <= 2^26, hidden up to 2^24 (rows of whole 16-byte vectors are the
- * fast ones). Outputs must not overlap inputs. No workspace. */
+ * fast ones). A call that needs more than 2^32 threads (a wave for 128 vectors
+ * of a token) is refused, nothing enqueued. Outputs must not overlap inputs. No
+ * workspace. */
 int  dsv4_hip_moe_permute_dev(void *rows, int *ex_off, int *row_tok, int *pos, const void *x, int type,
                               const int *idx, int n, int topk, int n_experts, int hidden, void *stream);
 
@@ -428,7 +430,9 @@ int  dsv4_hip_moe_unpermute_dev(void *out, const void *rows, int type, const int
 /* Gradients of unpermute: drows[pos[t][k]] = w[t][k] * dout[t] (rows that no
  * pair has stay as they are) and dw[t][k] = sum_j dout[t][j] *
  * rows[pos[t][k]][j] in fp32 (0 for a pair without a row); the gradient of
- * `shared` is dout itself. drows may be `rows` itself. */
+ * `shared` is dout itself. drows may be `rows` itself. A row belongs to at most
+ * one pair, as permute gives them: of a row that several pairs name, drows
+ * holds any one's gradient. At most 2^24 - 1 tokens. */
 int  dsv4_hip_moe_unpermute_bwd_dev(void *drows, float *dw, const void *dout, const void *rows, int type,
                                     const int *pos, const float *w, int n, int topk, int hidden,
                                     void *stream);

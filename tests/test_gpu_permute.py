@@ -192,6 +192,22 @@ def test_way_back(lib, n, topk, h, shift, dtype):
     assert torch.equal(dw2, dw) and torch.equal(rows2[used], drows[used])
 
 
+def test_way_back_of_millions_of_tokens(lib):
+    """a workgroup a token: as many as one launch takes threads for"""
+    n, h = 4_300_001, 8
+    rows = torch.randn(n, h, device=DEV, generator=gen(5)).to(torch.bfloat16)
+    dout = torch.randn(n, h, device=DEV, generator=gen(6)).to(torch.bfloat16)
+    w = torch.rand(n, 1, device=DEV, generator=gen(7))
+    pos = torch.arange(n - 1, -1, -1, dtype=torch.int32, device=DEV)[:, None].contiguous()
+    drows, dw = torch.empty_like(rows), torch.empty_like(w)
+    lib.moe_unpermute_bwd_dev(drows.data_ptr(), dw.data_ptr(), dout.data_ptr(), rows.data_ptr(), 1, pos.data_ptr(),
+                              w.data_ptr(), n, 1, h)
+    want = w.double() * dout.double()
+    close(drows.flip(0), want, want.abs(), U)
+    dots = dout.double() * rows.flip(0).double()
+    assert ((dw.double() - dots.sum(-1, keepdim=True)).abs() <= h * U * dots.abs().sum(-1, keepdim=True)).all()
+
+
 def test_way_back_ignores_rows_out_of_range(lib):
     n, topk, h = 6, 4, 64
     rows = torch.randn(n * topk, h, device=DEV, generator=gen(1))
