@@ -532,7 +532,7 @@ hipError_t moe_combine_launch(const CombineArgs &a, hipStream_t st);
 
 /* rows to int8 codes and a scale each: a (and with SwiGLU u, a being the
  * gate) rows of k elements, `ld` elements apart, 16-byte aligned; Q [n][k]
- * 8-byte aligned, n < 2^22. */
+ * 8-byte aligned, n < 2^22, k <= 2^24. */
 struct QuantI8Args {
     int8_t *Q;
     float *S;

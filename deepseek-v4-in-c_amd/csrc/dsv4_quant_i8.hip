@@ -312,7 +312,7 @@ static hipError_t quant_i8_t(const QuantI8Args &a, hipStream_t st)
 
 hipError_t quant_i8_launch(const QuantI8Args &a, int type, bool swiglu, hipStream_t st)
 {
-    if (a.n <= 0 || a.n >= 1 << 22 || a.k <= 0 || a.k % QU) return hipErrorInvalidValue;
+    if (a.n <= 0 || a.n >= 1 << 22 || a.k <= 0 || a.k > 1 << 24 || a.k % QU) return hipErrorInvalidValue;
     switch (type) {
     case DSV4_HIP_F32: return swiglu ? quant_i8_t<DSV4_HIP_F32, true>(a, st) : quant_i8_t<DSV4_HIP_F32, false>(a, st);
     case DSV4_HIP_BF16: return swiglu ? quant_i8_t<DSV4_HIP_BF16, true>(a, st) : quant_i8_t<DSV4_HIP_BF16, false>(a, st);

@@ -2393,8 +2393,8 @@ static int quant_i8(int8_t *Q, float *S, const void *x, const void *u, bool swig
     if (n && (!Q || !S || !x || (swiglu && !u))) return fail("%s: NULL pointer", what);
     if (!elem_type_ok(type)) return fail("%s: unknown element type %d", what, type);
     if (n >= 1 << 22) return fail("%s: %d rows are too many for one launch", what, n);
-    if (n < 0 || k < 16 || k % 16 || ld < k || ld > (1LL << 40) || ld * elem_bytes_of(type) % 16)
-        return fail("%s: need n >= 0, k a multiple of 16 and ld >= k of whole 16-byte steps (got %d, %d, %lld)", what,
+    if (n < 0 || k < 16 || k % 16 || k > 1 << 24 || ld < k || ld > (1LL << 40) || ld * elem_bytes_of(type) % 16)
+        return fail("%s: need n >= 0, k a multiple of 16 up to 2^24 and ld >= k of whole 16-byte steps (got %d, %d, %lld)", what,
                     n, k, (long long)ld);
     if (!aligned16(x) || !aligned16(u) || ((uintptr_t)Q & 7u) || ((uintptr_t)S & 3u))
         return fail("%s: need rows 16-, Q 8- and S 4-byte aligned", what);

@@ -49,8 +49,9 @@ int dsv4_hip_quant_act_mxfp8_dev(uint8_t *Q, uint8_t *S, const float *a,
  * magnitude S = amax / 127 (1 for a row of zeros) and code = the integer
  * nearest to 127 a / amax, ties to even, decided exactly. A row with a value
  * that is not finite gets scale NaN and codes 0. Tokens for the int8 products,
- * or weight rows (DSV4_WI8). k and the bytes of ld multiples of 16, a 16-byte,
- * Q 8-byte and S 4-byte aligned; n < 2^22, n = 0: nothing. No workspace. */
+ * or weight rows (DSV4_WI8). k (up to 2^24) and the bytes of ld multiples of 16,
+ * a 16-byte, Q 8-byte and S 4-byte aligned; n < 2^22, n = 0: nothing. No
+ * workspace. */
 int dsv4_hip_quant_i8_dev(int8_t *Q, float *S, const void *a, int type, int64_t ld, int n, int k,
                           void *stream);
 

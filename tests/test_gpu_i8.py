@@ -71,6 +71,11 @@ def test_rows(lib, dtype, n, k):
     check_rows(*quant(lib, x), x.double())
 
 
+def test_widest_row(lib):
+    x = torch.randn(1, 1 << 24, device=DEV, generator=gen(24)).to(torch.bfloat16)
+    check_rows(*quant(lib, x), x.double())
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("k", [64, 4096, 8208])
 def test_rows_of_borders(lib, dtype, k):

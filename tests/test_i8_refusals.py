@@ -111,6 +111,15 @@ def test_more_rows_than_a_launch_takes_are_refused(calls, n):
         assert rc == -1 and "too many" in why
 
 
+@pytest.mark.parametrize("k", [(1 << 24) + 16, (1 << 31) - 16])
+def test_rows_whose_elements_an_index_does_not_hold_are_refused(calls, k):
+    for name in ("quant", "swiglu"):
+        rc, why = calls[0](name, k=k, ld=k)
+        assert rc == -1 and "2^24" in why
+        rc, why = calls[0](name, k=1 << 24, ld=k)
+        assert rc == -1 and "init" in why
+
+
 @pytest.mark.parametrize("field,value", [("wdt", 2), ("rows", 0), ("cols", 0), ("cols", 40), ("cols", 131072),
                                          ("w", None), ("s", None), ("w", P + 8), ("s", P + 2)])
 def test_bad_matrix_is_refused(calls, field, value):
