@@ -2139,6 +2139,8 @@ struct OnDevice {
 static int stream_check(const OnDevice &on, void *stream, const char *what)
 {
     if (!on.ok) return fail("%s: device %d cannot be selected", what, g.device);
+    /* a process that hands this handle to the runtime ends in a segmentation fault */
+    if (stream == (void *)hipStreamLegacy) return fail("%s: pass NULL for the default stream", what);
     hipDevice_t d = g.device;
     if (stream && (hipStreamGetDevice((hipStream_t)stream, &d) != hipSuccess || d != g.device)) {
         (void)hipGetLastError();

@@ -374,6 +374,8 @@ int  dsv4_hip_gemm_mxfp8q_dev(void *C, int out_bf16, const uint8_t *Aq,
  * beyond fp16 become infinite). cols a multiple of 16 up to 131,056; M and
  * W->rows any; Aq and w 16-byte aligned. A scale of NaN makes its row NaN.
  * No workspace: calls on several streams, and captured graphs, do not meet.
+ * Stream: one of the library's device, or NULL (hipStreamLegacy is refused);
+ * so for all the calls from here to the expert order.
  * 0 enqueued (M = 0: nothing), -1 otherwise. */
 int  dsv4_hip_gemm_i8_dev(void *C, int out_type, const int8_t *Aq, const float *Sa, int M,
                           const DSV4QMat *W, void *stream);

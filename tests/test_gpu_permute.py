@@ -121,6 +121,26 @@ def test_order_with_nothing_to_do(lib, n):
         assert lib.status() == bits
 
 
+def test_special_stream_handles(lib):
+    """the calling thread's own stream works, the default stream is NULL only"""
+    n, topk, E, h = 40, 3, 8, 64
+    ids = routing(n, topk, E, 3, 0.2, False)
+    idx, x = torch.from_numpy(ids).to(DEV), torch.randn(n, h, device=DEV, generator=gen(3))
+    off, tok, pos = (torch.zeros(k, dtype=torch.int32, device=DEV) for k in (E + 1, n * topk, n * topk))
+    rows = torch.zeros(n * topk, h, device=DEV)
+    torch.cuda.synchronize()
+    args = (rows.data_ptr(), off.data_ptr(), tok.data_ptr(), pos.data_ptr(), x.data_ptr(), 0, idx.data_ptr(), n, topk, E, h)
+    with pytest.raises(Exception, match="NULL for the default stream"):
+        lib.moe_permute_dev(*args, 1)
+    torch.cuda.synchronize()
+    assert (off == 0).all()
+    lib.moe_permute_dev(*args, 2)
+    torch.cuda.synchronize()
+    assert off[-1] == (ids >= 0).sum()
+    used = pos >= 0
+    assert torch.equal(rows[pos[used].long()], x.repeat_interleave(topk, 0)[used])
+
+
 def test_order_of_no_tokens(lib):
     off = torch.full((9,), 5, dtype=torch.int32, device=DEV)
     lib.moe_permute_dev(None, off.data_ptr(), None, None, None, 0, None, 0, 6, 8, 64)
