@@ -13,11 +13,13 @@
  *   product lies within 2^-15 of a half-integer. Only there (one element in
  *   16,000) fp64 decides, where 127 a_j is exact and the quotient rounds to a
  *   half-integer only if it is one: codes depend on no rounding on the way.
- *   With SwiGLU the values are fp32 ones within 8 x 2^-24 (exp 1 ulp and
- *   its correction half, 1 + e half, reciprocal 1 ulp, two products): with the product by 127 /
- *   amax 10 x 2^-24 of at most 127: certain outside 1.37 x 2^-14 of a half-integer. Inside it, and for the row's largest value, the SwiGLU is
- *   taken in fp64: codes and scale are those of fp64 values. Rows whose largest value is below 2^-60 or beyond 2^120
- *   compute everything in fp64.
+ *   With SwiGLU the values are fp32 ones within 8 x 2^-24 (exp 1 ulp and its
+ *   correction half, 1 + e half, reciprocal 1 ulp, two products), the product by
+ *   127 / amax within 10 x 2^-24 of at most 127: a code is certain outside 1.24 x
+ *   2^-14 (1.375 are taken) of a half-integer. Inside, and for the row's largest
+ *   value, the SwiGLU is taken in fp64: codes and scale are those of fp64 values.
+ *   Rows whose largest value is below 2^-60 or beyond 2^120 compute everything in
+ *   fp64.
  *
  * Bound: HBM for plain rows (8,192 of 4,096 bf16 19.6 us, 5.1 TB/s), the vector
  * unit for SwiGLU (some 40 instructions an element, 10 of the 14 us of 4,206
