@@ -263,15 +263,18 @@ inline I8Form i8_form(int M, int N, int K)
 }
 
 /* Buckets of ne experts, M rows in all; the mean bucket decides. us, pair /
- * 64x2 / 128x4 / 256x8, experts 2048 x 4096 on 256: 384 rows Zipf 178 / 176 /
- * 176 / 192, 768 rows 322 / 350 / 359 / 370, 2,400 rows 370 / 377 / 384 / 379,
- * 6,144 rows Zipf 740 / 415 / 398 / 423, 12,288
- * rows Zipf - / 522 / 446 / 455, even 530 / 414 / 403 (64x2 on), 24,576 rows Zipf
- * 745 / 565 / 522. Too little weight to fill the CUs: 6 rows 15.1 / 12.4 / 14.8,
- * 160 rows on 64 of 512 x 1024 8.5 / 7.0 / 8.1, but 1,600 of them - / 9.2 / 8.9 /
- * 14.8; from there the form of least cost, a round of buckets 1.5 us more than
- * one matrix's: 8,000 of them - / 23.2 / 21.8 / 18.8, 1,200 rows on 16 of 1024 x
- * 2048 - / 12.9 / 11.8 / 20.3, 1,400 rows on 36 of 128 x 608 - / 5.5 / 6.7 / 11.5. */
+ * 64x2 / 128x4 / 256x8, experts 2048 x 4096 on 256: 384 rows Zipf 187 / 188 /
+ * 184 / 198, 768 rows Zipf 260 / 259 / 259 / 264, 2,400 rows 372 / 376 / 386 / 374,
+ * 6,144 rows Zipf 724 / 409 / 392 / 390, 12,288 rows Zipf - / 510 / 439 / 426, even
+ * 527 / 413 / 391 (64x2 on), 24,576 rows Zipf 729 / 552 / 482. Where short rows or
+ * fewer experts make a stream of fewer rounds 128x4 holds out longer (128x4 /
+ * 256x8, mean 30 and 48: 256 of 4096 x 2048 409 / 430 and 439 / 450, Zipf 442 /
+ * 449 and 498 / 470; 64 of 4096 x 4096 207 / 215 and 214 / 218, Zipf 205 / 221 and
+ * 225 / 218). Too little weight to fill the CUs: 6 rows 15.1 / 12.4 / 14.8,
+ * 160 rows on 64 of 512 x 1024 8.5 / 7.0 / 8.1, but 1,600 of them - / 9.3 / 9.0 /
+ * 13.6; from there the form of least cost, a round of buckets 1.5 us more than
+ * one matrix's: 8,000 of them - / 23.8 / 22.0 / 17.4, 1,200 rows on 16 of 1024 x
+ * 2048 - / 13.1 / 11.5 / 20.2, 1,400 rows on 36 of 128 x 608 - / 5.4 / 6.6 / 11.0. */
 constexpr int I8_BUCKET_COST = 150;
 inline I8Form i8_grouped_form(int M, int N, int K, int ne)
 {
@@ -293,7 +296,7 @@ inline I8Form i8_grouped_form(int M, int N, int K, int ne)
     }
     if (M <= 10 * hit) return I8_PAIR;
     if (M <= 20 * hit) return I8_64x2;
-    return M < 60 * hit ? I8_128x4 : I8_256x8;
+    return M < 45 * hit ? I8_128x4 : I8_256x8;
 }
 
 /* Waves of the launch that multiplies M rows by N features in a form: tiles

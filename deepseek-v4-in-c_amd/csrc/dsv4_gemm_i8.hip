@@ -49,12 +49,22 @@ struct Tile {
     bool bad;                                      /* the table's entry is not an int8 N x K matrix */
 };
 
-/* Tile `t` of the buckets ex_off[0 .. E], each cut into tiles of TR rows;
- * rows == 0 past the last tile. Every wave finds it by itself: a lane counts
- * the tiles of E / 64 experts, a scan over the lanes finds the one that holds
- * t. Offsets are clamped to [0, R], so no table makes a row out of range. */
+/* Row tile `t` of the buckets ex_off[0 .. E], each cut into tiles of TR rows;
+ * rows == 0 past the last one. Every wave finds it by itself: a lane counts the
+ * tiles of E / 64 experts, a scan over the lanes finds the one that holds t.
+ * Offsets are clamped to [0, M], so no table makes a row out of range.
+ *
+ * With nt, `t` is the workgroup of a launch over nt feature tiles, *f the one it
+ * takes: workgroups go round the eight XCDs, and each XCD gets a contiguous
+ * eighth of the (row, feature) tiles, an expert's in groups of eight row tiles by
+ * its feature tiles. So an XCD's L2 fetches an expert's tokens once for all
+ * features and a popular expert's weights once for eight row tiles. us in 256 x
+ * 128 tiles, against feature tiles dealt out to the XCDs: 24,576 rows of 256
+ * experts 2048 x 4096 453 -> 429, with Zipf 520 -> 484, 6,144 rows of 64 of them
+ * 116 -> 106; groups of all row tiles by one feature tile after the other 485 and
+ * no groups 345 rather than 327 at 24,576 rows of 64 experts 4096 x 2048, Zipf. */
 template <int TR>
-__device__ __forceinline__ Tile bucket_tile(const I8Args &a, int t, int lane)
+__device__ __forceinline__ Tile bucket_tile(const I8Args &a, int t, int lane, int nt = 0, int *f = nullptr)
 {
     const int E = a.n_experts, per = (E + 63) / 64;
     auto clampr = [&](int v) { return min(max(v, 0), a.M); };
@@ -76,6 +86,16 @@ __device__ __forceinline__ Tile bucket_tile(const I8Args &a, int t, int lane)
     }
     Tile o;
     o.w = nullptr; o.s = nullptr; o.r0 = 0; o.rows = 0; o.e = 0; o.bad = false;
+    int in = 0;
+    if (nt) {
+        /* a sum that wraps comes from falling offsets: never more tiles than there are */
+        const uint32_t tiles = min((uint32_t)__builtin_amdgcn_readlane(incl, 63), gridDim.x / (uint32_t)nt);
+        const int total = (int)tiles * nt, x = t % 8, y = t / 8;
+        if (t >= total) return o;
+        const int id = x * (total / 8) + min(x, total % 8) + y;
+        t = id / nt;
+        in = id - t * nt;
+    }
     const uint64_t past = __ballot(incl > t);
     if (!past) return o;
     const int L = __builtin_ctzll(past);
@@ -86,6 +106,14 @@ __device__ __forceinline__ Tile bucket_tile(const I8Args &a, int t, int lane)
         const int hi = clampr(a.ex_off[e + 1]);
         const int n = max(hi - lo, 0), tiles = (n + TR - 1) / TR;
         if (left < tiles || e + 1 >= E) {
+            if (nt) {
+                constexpr int GROUP = 8;
+                in += left * nt;                   /* among the expert's tiles */
+                const int g0 = in / (GROUP * nt) * GROUP, rows = min(GROUP, tiles - g0);
+                in -= g0 * nt;
+                left = g0 + in % rows;
+                *f = __builtin_amdgcn_readfirstlane(in / rows);
+            }
             o.r0 = lo + left * TR;
             o.rows = min(TR, n - left * TR);
             break;
@@ -317,8 +345,8 @@ __device__ __forceinline__ void i8_leave(const I8Args &a, const Tile &t, int n0,
  * Bound: 256 x 128 tiles issue an MFMA in half of their cycles (2,048 x 4096 x
  * 4096 34 us, 2.0 of 4.3 POP/s that registers alone reach; the library's int8
  * product takes 41.7), the rest are barriers and LDS; experts' buckets the HBM
- * stream beside that (24,576 rows of 256 experts, Zipf, 522 us, 359 with every
- * table entry the same matrix, 316 for the weights alone); few rows the chain of
+ * stream beside that (24,576 rows of 256 experts, Zipf, 483 us, even 430; 359
+ * with every table entry the same matrix, 316 for the weights alone); few rows the chain of
  * stages (16 to 128 rows of 4096 x 4096 7 to 8 us; K split over teams of waves
  * gained nothing, weights straight to registers lost 10 to 20 %). */
 template <int F, int T, int KB, int NST_> struct I8Tile {
@@ -349,6 +377,11 @@ __global__ __launch_bounds__((64 * I8Tile<F, T, KB, NST>::NWAVE)) void k_i8_tile
 {
     using C = I8Tile<F, T, KB, NST>;
     constexpr int U = C::U, WI = C::WI, TR = 16 * T;
+    /* buckets of many rows: an XCD's workgroups share an expert (bucket_tile).
+     * Smaller tiles, dealt out / shared, us: 9,216 rows of 256 experts 2048 x 4096 in
+     * 128 x 64 411 / 425, 3,582 of 256 4096 x 2048 in 64 x 32 397 / 408, 1,200 of 16
+     * 1024 x 2048 in 128 x 64 11.4 / 11.7. */
+    constexpr bool SHARED = GROUPED && F == 256;
     extern __shared__ __align__(16) uint8_t lds[];
     const int lane = threadIdx.x & 63, wave = wave_in_group();
     const int rr = lane & 15, gq = lane >> 4, wr = wave & 3, wt = wave >> 2;
@@ -356,11 +389,10 @@ __global__ __launch_bounds__((64 * I8Tile<F, T, KB, NST>::NWAVE)) void k_i8_tile
     Tile t;
     int n0;
     if constexpr (GROUPED) {
-        /* workgroups go round the eight XCDs: with a multiple of eight feature
-         * tiles each XCD's L2 keeps its features of an expert over its rows */
-        const int tile = blockIdx.x / nt;
-        n0 = (blockIdx.x - tile * nt) * F;
-        t = bucket_tile<TR>(a, tile, lane);
+        int f = blockIdx.x % nt;
+        if constexpr (SHARED) t = bucket_tile<TR>(a, blockIdx.x, lane, nt, &f);
+        else t = bucket_tile<TR>(a, blockIdx.x / nt, lane);
+        n0 = f * F;
         if (t.rows <= 0) return;
     } else {
         /* each XCD a contiguous run of tiles, eight row tiles by their feature
@@ -405,12 +437,13 @@ __global__ __launch_bounds__((64 * I8Tile<F, T, KB, NST>::NWAVE)) void k_i8_tile
         xl[i] = (nblk - 1) * 128 + 16 * c < a.K ? xo[i] : I8_OOB;
     }
     /* The block this workgroup begins with. Rows of 4 KB put the lines of one
-     * block into a few memory channels, and workgroups that run through K side
-     * by side into the same ones; begun at different places they spread (sums
-     * are exact in any order). Those that share weights keep step. us: 24,576
-     * rows of 256 experts 525 -> 451, with Zipf 546 -> 522, 6,144 rows 477 ->
-     * 390, 1,536 rows in these tiles 462 -> 374. One matrix gains nothing. */
-    const int rot = GROUPED ? (n0 / F * 4 + t.e) % nblk : 0;
+     * block into a few memory channels, and experts that run through K side by
+     * side into the same ones; begun at different places they spread (sums are
+     * exact in any order). Workgroups that share weights, or in SHARED an expert's
+     * weights and tokens, keep step. us, 24,576 rows of 256 experts: all from block
+     * 0 525, by expert and feature tile 445, by expert 430; 1,536 rows in
+     * smaller tiles 462 and 374. One matrix gains nothing. */
+    const int rot = SHARED ? (t.e * 8 + t.e / 4) % nblk : GROUPED ? (n0 / F * 4 + t.e) % nblk : 0;
     /* load i of a wave's share of stage st; past the end zeros, no traffic */
     auto issue = [&](int st, int slot, int i) {
         constexpr int LB = C::LW + C::LX;
@@ -474,11 +507,25 @@ __global__ __launch_bounds__((64 * I8Tile<F, T, KB, NST>::NWAVE)) void k_i8_tile
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
     Op o0, o1;
+    int st = 0;
+    /* waves whose rows are all behind the bucket's last only load (24,576 rows,
+     * Zipf, 492 -> 483 us) */
+    if (GROUPED && C::WT > 1 && 16 * U * wt >= t.rows) {
+        for (; st < nst; st++) {
+            i8_wait_vm<(C::NST - 2) * C::VM>();
+            __builtin_amdgcn_s_barrier();
+            asm volatile("" ::: "memory");
 #pragma unroll
-    for (int i = 0; i < WI; i++) read_w(o0, lds, i, 0);
+            for (int l = 0; l < C::VM; l++) issue(st + C::NST, slot, l);
+            slot = slot + 1 == C::NST ? 0 : slot + 1;
+        }
+    } else {
 #pragma unroll
-    for (int u = 0; u < U; u++) read_x(o0, lds, u, 0);
-    for (int st = 0; st < nst; st++) {
+        for (int i = 0; i < WI; i++) read_w(o0, lds, i, 0);
+#pragma unroll
+        for (int u = 0; u < U; u++) read_x(o0, lds, u, 0);
+    }
+    for (; st < nst; st++) {
         const uint8_t *buf = lds + slot * C::STAGE;
 #pragma unroll
         for (int j = 0; j + 2 < 2 * KB; j += 2) {

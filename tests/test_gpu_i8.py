@@ -336,7 +336,8 @@ GROUPS = [([0, 0, 1, 0], 40, 64), ([3, 0, 17, 5, 64, 1], 130, 272), ([65, 0, 128
           ([700, 3, 0, 0, 40, 1], 515, 2048), ([0, 0], 16, 16), ([16, 15, 17, 33, 31, 32], 512, 144),
           ([100, 90, 110, 95] * 4, 1024, 640), ([1, 0, 3, 16, 2, 9, 40, 1] * 8, 1030, 1040),
           ([0, 7, 20, 1] * 16, 1024, 2064),
-          ([40, 0, 30, 50, 65], 300, 272), ([100, 64, 140, 90], 4100, 4112), ([120, 128, 0, 131] * 16, 510, 1024)]
+          ([40, 0, 30, 50, 65], 300, 272), ([100, 64, 140, 90], 4100, 4112), ([120, 128, 0, 131] * 16, 510, 1024), ([2500, 3, 0, 300], 2100, 8208),
+          ([1, 0, 1200, 0, 60, 200, 1100] * 3, 781, 4112)]
 
 
 @pytest.mark.parametrize("case", range(len(GROUPS)))
@@ -397,6 +398,17 @@ def test_experts_product_stays_in_bounds_with_bad_offsets(lib, pkg):
     _, _, w, sw = operands(1, E * N, K, 2)
     w, sw = w.view(E, N, K), sw.view(E, N)
     for off in ([0, 10, 5, 1 << 30, 20, 25], [-50, -1, 3, 3, 2, 900], [30, 30, 30, 30, 30, 30]):
+        run_grouped(lib, pkg, a, sa, torch.tensor(off, dtype=torch.int32, device=DEV), None, R, w, sw, torch.float32)
+    lib.status()
+
+
+def test_large_experts_product_stays_in_bounds_with_bad_offsets(lib, pkg):
+    E, N, K, R = 5, 1701, 8208, 2900
+    a, sa, _, _ = operands(R, 1, K, 1)
+    _, _, w, sw = operands(1, E * N, K, 2)
+    w, sw = w.view(E, N, K), sw.view(E, N)
+    for off in ([0, 1000, 500, 1 << 30, 2000, 2500], [-50, -1, 300, 300, 200, 90000], [R, 0, R, 0, R, 0],
+                [0, R, 0, R, 0, R], [-(1 << 31), (1 << 31) - 1, -(1 << 31), (1 << 31) - 1, 0, R]):
         run_grouped(lib, pkg, a, sa, torch.tensor(off, dtype=torch.int32, device=DEV), None, R, w, sw, torch.float32)
     lib.status()
 

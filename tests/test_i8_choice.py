@@ -45,7 +45,7 @@ def test_product_form(rules, M, N, K, form):
 
 @pytest.mark.parametrize("M,N,K,ne,form", [
     (6, 2048, 4096, 256, T64x2), (42, 2048, 4096, 256, PAIR), (1536, 2048, 4096, 256, PAIR),
-    (160, 512, 1024, 64, T64x2), (12288, 2048, 4096, 256, T128x4), (24576, 2048, 4096, 256, T256x8),
+    (160, 512, 1024, 64, T64x2), (7680, 2048, 4096, 256, T128x4), (12288, 2048, 4096, 256, T256x8), (24576, 2048, 4096, 256, T256x8),
     (6144, 2048, 4096, 64, T256x8)])
 def test_experts_form(rules, M, N, K, ne, form):
     assert rules.c_grouped(M, N, K, ne) == form
@@ -55,6 +55,9 @@ def test_gpu_tests_reach_every_form(rules):
     assert {rules.c_form(*s) for s in test_gpu_i8.SHAPES} == set(range(1, 8))
     groups = {rules.c_grouped(sum(c) + 5, N, K, len(c)) for c, N, K in test_gpu_i8.GROUPS}
     assert groups == {PAIR, T64x2, T128x4, T256x8}
+    for c in ([2500, 3, 0, 300], 2100, 8208), ([1, 0, 1200, 0, 60, 200, 1100] * 3, 781, 4112):
+        assert c in test_gpu_i8.GROUPS and rules.c_grouped(sum(c[0]) + 5, c[1], c[2], len(c[0])) == T256x8
+    assert rules.c_grouped(2900, 1701, 8208, 5) == T256x8        # the large product with bad offsets
 
 
 @pytest.mark.parametrize("form,F,TR,waves", [(PAIR, 8, 8, 8), (T64x2, 64, 32, 4), (T64x2_DEEP, 64, 32, 4),
