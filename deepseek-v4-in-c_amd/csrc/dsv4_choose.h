@@ -266,7 +266,10 @@ inline I8Form i8_form(int M, int N, int K)
  * 64x2 / 128x4 / 256x8, experts 2048 x 4096 on 256: 384 rows Zipf 187 / 188 /
  * 184 / 198, 768 rows Zipf 260 / 259 / 259 / 264, 2,400 rows 372 / 376 / 386 / 374,
  * 6,144 rows Zipf 724 / 409 / 392 / 390, 12,288 rows Zipf - / 510 / 439 / 426, even
- * 527 / 413 / 391 (64x2 on), 24,576 rows Zipf 729 / 552 / 482. Where short rows or
+ * 527 / 413 / 391 (64x2 on), 24,576 rows Zipf 729 / 552 / 482. The pair form's
+ * workgroups are too short where rows are (pair / 64x2: 384 rows on 256 of 2048 x
+ * 2048 131 / 148, but 512 rows on 512 of 2048 x 1024 221 / 178, 800 on 1000 of
+ * 1024 x 1024 264 / 179, of 512 x 512 123 / 73). Where short rows or
  * fewer experts make a stream of fewer rounds 128x4 holds out longer (128x4 /
  * 256x8, mean 30 and 48: 256 of 4096 x 2048 409 / 430 and 439 / 450, Zipf 442 /
  * 449 and 498 / 470; 64 of 4096 x 4096 207 / 215 and 214 / 218, Zipf 205 / 221 and
@@ -294,7 +297,7 @@ inline I8Form i8_grouped_form(int M, int N, int K, int ne)
         }
         return best;
     }
-    if (M <= 10 * hit) return I8_PAIR;
+    if (M <= 10 * hit && K >= 2048) return I8_PAIR;
     if (M <= 20 * hit) return I8_64x2;
     return M < 45 * hit ? I8_128x4 : I8_256x8;
 }

@@ -51,8 +51,9 @@ struct Tile {
 
 /* Row tile `t` of the buckets ex_off[0 .. E], each cut into tiles of TR rows;
  * rows == 0 past the last one. Every wave finds it by itself: a lane counts the
- * tiles of E / 64 experts, a scan over the lanes finds the one that holds t.
- * Offsets are clamped to [0, M], so no table makes a row out of range.
+ * tiles of E / 64 experts, a scan over the lanes finds the one that holds t, a
+ * scan of its experts' tiles the expert. Offsets are clamped to [0, M], so no
+ * table makes a row out of range.
  *
  * With nt, `t` is the workgroup of a launch over nt feature tiles, *f the one it
  * takes: workgroups go round the eight XCDs, and each XCD gets a contiguous
@@ -69,13 +70,17 @@ __device__ __forceinline__ Tile bucket_tile(const I8Args &a, int t, int lane, in
     const int E = a.n_experts, per = (E + 63) / 64;
     auto clampr = [&](int v) { return min(max(v, 0), a.M); };
     int mine = 0;
-    int lo = lane * per < E ? clampr(a.ex_off[lane * per]) : 0;
-    for (int i = 0; i < per; i++) {
-        const int e = lane * per + i;
-        if (e < E) {
-            const int hi = clampr(a.ex_off[e + 1]);
-            mine += (max(hi - lo, 0) + TR - 1) / TR;
-            lo = hi;
+    const auto off = gptr(a.ex_off);
+    int lo = clampr(off[min(lane * per, E)]);
+    for (int i = 0; i < per; i += 4) {             /* four loads in flight */
+        int hi[4];
+#pragma unroll
+        for (int j = 0; j < 4; j++) hi[j] = off[min(lane * per + min(i + j + 1, per), E)];
+#pragma unroll
+        for (int j = 0; j < 4; j++) {              /* past the lane's experts: empty buckets */
+            hi[j] = clampr(hi[j]);
+            mine += (max(hi[j] - lo, 0) + TR - 1) / TR;
+            lo = hi[j];
         }
     }
     int incl = mine;
@@ -100,35 +105,35 @@ __device__ __forceinline__ Tile bucket_tile(const I8Args &a, int t, int lane, in
     if (!past) return o;
     const int L = __builtin_ctzll(past);
     int left = t - __builtin_amdgcn_readlane(incl - mine, L);
-    int e = L * per;
-    lo = clampr(a.ex_off[e]);
-    for (;; e++) {                                 /* ends within the lane's experts: they hold tile t */
-        const int hi = clampr(a.ex_off[e + 1]);
-        const int n = max(hi - lo, 0), tiles = (n + TR - 1) / TR;
-        if (left < tiles || e + 1 >= E) {
-            if (nt) {
-                constexpr int GROUP = 8;
-                in += left * nt;                   /* among the expert's tiles */
-                const int g0 = in / (GROUP * nt) * GROUP, rows = min(GROUP, tiles - g0);
-                in -= g0 * nt;
-                left = g0 + in % rows;
-                *f = __builtin_amdgcn_readfirstlane(in / rows);
-            }
-            o.r0 = lo + left * TR;
-            o.rows = min(TR, n - left * TR);
-            break;
-        }
-        left -= tiles;
-        lo = hi;
+    /* its experts, one a lane */
+    const int mylo = clampr(off[min(L * per + min(lane, per), E)]);
+    const int n = max(__shfl_down(mylo, 1, 64) - mylo, 0), tiles = lane < per ? (n + TR - 1) / TR : 0;
+    int upto = tiles;
+#pragma unroll
+    for (int d = 1; d < 16; d <<= 1) {             /* per <= 16 */
+        const int v = __shfl_up(upto, d, 64);
+        if (lane >= d) upto += v;
     }
-    o.e = __builtin_amdgcn_readfirstlane(e);
+    const uint64_t holds = __ballot(lane < per && upto > left);
+    if (!holds) return o;
+    const int i = __builtin_ctzll(holds), mine_i = __builtin_amdgcn_readlane(tiles, i);
+    left -= __builtin_amdgcn_readlane(upto, i) - mine_i;
+    if (nt) {
+        constexpr int GROUP = 8;
+        in += left * nt;                           /* among the expert's tiles */
+        const int g0 = in / (GROUP * nt) * GROUP, rows = min(GROUP, mine_i - g0);
+        in -= g0 * nt;
+        left = g0 + in % rows;
+        *f = in / rows;
+    }
+    o.r0 = __builtin_amdgcn_readlane(mylo, i) + left * TR;
+    o.rows = min(TR, __builtin_amdgcn_readlane(n, i) - left * TR);
+    o.e = L * per + i;
     const DSV4QMat m = ld_uniform(a.table, o.e);
     o.w = (const uint8_t *)m.w;
     o.s = (const float *)m.s;
     o.bad = m.wdt != DSV4_WI8 || m.rows != a.N || m.cols != a.K || !m.w || !m.s || ((uintptr_t)m.w & 15u) ||
             ((uintptr_t)m.s & 3u);
-    o.r0 = __builtin_amdgcn_readfirstlane(o.r0);
-    o.rows = __builtin_amdgcn_readfirstlane(o.rows);
     return o;
 }
 
@@ -407,12 +412,6 @@ __global__ __launch_bounds__((64 * I8Tile<F, T, KB, NST>::NWAVE)) void k_i8_tile
         n0 = in / gm * F;
     }
     const int nf = min(F, a.N - n0);
-    if (GROUPED && t.bad) {
-        if (threadIdx.x == 0) atomicOr(a.status, ST_BAD_DESCRIPTOR);
-        for (int i = threadIdx.x; i < t.rows * nf; i += 64 * C::NWAVE)
-            i8_store<OUT>(a.C, (size_t)(t.r0 + i / nf) * a.N + n0 + i % nf, __builtin_nanf(""));
-        return;
-    }
     const uint32_t K = (uint32_t)a.K;
     const __amdgpu_buffer_rsrc_t rw = i8_rsrc(t.w + (size_t)n0 * K, (uint32_t)nf * K);
     const uint8_t *xb = GROUPED ? a.Aq : a.Aq + (size_t)t.r0 * K;
@@ -435,6 +434,12 @@ __global__ __launch_bounds__((64 * I8Tile<F, T, KB, NST>::NWAVE)) void k_i8_tile
         const int r = 8 * (C::LX * wave + i) + lane / 8, c = swz(r, lane & 7), s = src_of(r);
         xo[i] = s < 0 ? I8_OOB : (uint32_t)s * K + 16u * (uint32_t)c;
         xl[i] = (nblk - 1) * 128 + 16 * c < a.K ? xo[i] : I8_OOB;
+    }
+    if (GROUPED && t.bad) {
+        if (threadIdx.x == 0) atomicOr(a.status, ST_BAD_DESCRIPTOR);
+        for (int i = threadIdx.x; i < t.rows * nf; i += 64 * C::NWAVE)
+            i8_store<OUT>(a.C, (size_t)(t.r0 + i / nf) * a.N + n0 + i % nf, __builtin_nanf(""));
+        return;
     }
     /* The block this workgroup begins with. Rows of 4 KB put the lines of one
      * block into a few memory channels, and experts that run through K side by

@@ -337,7 +337,8 @@ GROUPS = [([0, 0, 1, 0], 40, 64), ([3, 0, 17, 5, 64, 1], 130, 272), ([65, 0, 128
           ([100, 90, 110, 95] * 4, 1024, 640), ([1, 0, 3, 16, 2, 9, 40, 1] * 8, 1030, 1040),
           ([0, 7, 20, 1] * 16, 1024, 2064),
           ([40, 0, 30, 50, 65], 300, 272), ([100, 64, 140, 90], 4100, 4112), ([120, 128, 0, 131] * 16, 510, 1024), ([2500, 3, 0, 300], 2100, 8208),
-          ([1, 0, 1200, 0, 60, 200, 1100] * 3, 781, 4112)]
+          ([1, 0, 1200, 0, 60, 200, 1100] * 3, 781, 4112), ([1, 0, 2] * 341 + [4], 40, 2064),
+          ([0] * 1023 + [70], 48, 512), ([5] + [0] * 64, 100, 528), ([0, 3] * 32, 513, 2064), ([40] * 1024, 300, 272)]
 
 
 @pytest.mark.parametrize("case", range(len(GROUPS)))

@@ -45,7 +45,8 @@ def test_product_form(rules, M, N, K, form):
 
 @pytest.mark.parametrize("M,N,K,ne,form", [
     (6, 2048, 4096, 256, T64x2), (42, 2048, 4096, 256, PAIR), (1536, 2048, 4096, 256, PAIR),
-    (160, 512, 1024, 64, T64x2), (7680, 2048, 4096, 256, T128x4), (12288, 2048, 4096, 256, T256x8), (24576, 2048, 4096, 256, T256x8),
+    (160, 512, 1024, 64, T64x2), (7680, 2048, 4096, 256, T128x4), (12288, 2048, 4096, 256, T256x8),
+    (24576, 2048, 4096, 256, T256x8), (800, 512, 512, 1000, T64x2), (384, 2048, 2048, 256, PAIR),
     (6144, 2048, 4096, 64, T256x8)])
 def test_experts_form(rules, M, N, K, ne, form):
     assert rules.c_grouped(M, N, K, ne) == form
