@@ -13,13 +13,12 @@
  *   product lies within 2^-15 of a half-integer. Only there (one element in
  *   16,000) fp64 decides, where 127 a_j is exact and the quotient rounds to a
  *   half-integer only if it is one: codes depend on no rounding on the way.
- *   With SwiGLU the values are fp32 ones within 8 x 2^-24 (exp 1 ulp and its
- *   correction half, 1 + e half, reciprocal 1 ulp, two products), the product by
- *   127 / amax within 10 x 2^-24 of at most 127: a code is certain outside 1.24 x
- *   2^-14 (1.375 are taken) of a half-integer. Inside, and for the row's largest
- *   value, the SwiGLU is taken in fp64: codes and scale are those of fp64 values.
- *   Rows whose largest value is below 2^-60 or beyond 2^120 compute everything in
- *   fp64.
+ *   With SwiGLU the values are fp32 ones within 8 x 2^-24 (dsv4_swiglu_math.h), the
+ *   product by 127 / amax within 10 x 2^-24 of at most 127: a code is certain
+ *   outside 1.24 x 2^-14 (1.375 are taken) of a half-integer. Inside, and for the
+ *   row's largest value, the SwiGLU is taken in fp64: codes and scale are those of
+ *   fp64 values. Rows whose largest value is below 2^-60 or beyond 2^120, or that
+ *   hold a value which fp32 lost, compute everything in fp64.
  *
  * Bound: HBM for plain rows (8,192 of 4,096 bf16 19.6 us, 5.1 TB/s), the vector
  * unit for SwiGLU (some 40 instructions an element, 10 of the 14 us of 4,206
@@ -28,6 +27,7 @@
  */
 #include "dsv4_elem.h"
 #include "dsv4_internal.h"
+#include "dsv4_swiglu_math.h"
 
 namespace dsv4 {
 
@@ -37,32 +37,6 @@ typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 
 constexpr int QU = 8;                              /* elements of a lane's unit  */
 constexpr float ROUND_MAGIC = 12582912.0f;         /* 1.5 x 2^23: the low byte of v + this is rint(v) */
-
-__device__ __forceinline__ double swiglu64(float g, float u, float limit)
-{
-    if (limit > 0.0f) {
-        u = u > limit ? limit : u;
-        u = u < -limit ? -limit : u;
-        g = g > limit ? limit : g;
-    }
-    return (double)g / (1.0 + exp(-(double)g)) * (double)u;
-}
-
-__device__ __forceinline__ float swiglu32(float g, float u, float limit)
-{
-    if (limit > 0.0f) {
-        u = u > limit ? limit : u;
-        u = u < -limit ? -limit : u;
-        g = g > limit ? limit : g;
-    }
-    /* exp(-g) = 2^t (1 + ln 2 * r): t the rounded product with log2 e, r what
-     * the rounding and log2 e's own last bits left. Infinite and NaN gates give
-     * NaN here and are decided in fp64. */
-    const float t = __fmul_rn(-g, 0x1.715476p+0f);
-    const float r = fmaf(-g, 0x1.4ae0cp-26f, fmaf(-g, 0x1.715476p+0f, -t));
-    const float e = __builtin_amdgcn_exp2f(t);
-    return __fmul_rn(__fmul_rn(g, __builtin_amdgcn_rcpf(__fadd_rn(1.0f, fmaf(__fmul_rn(e, 0x1.62e43p-1f), r, e)))), u);
-}
 
 /* the unit's 8 elements (a, or gate and up) at element offset j */
 template <int TYPE>
@@ -128,6 +102,7 @@ __global__ __launch_bounds__(NW == 1 ? 256 : 64 * NW) void k_quant_i8(QuantI8Arg
     const uint8_t *pa = (const uint8_t *)a.a + off, *pu = SWIGLU ? (const uint8_t *)a.u + off : nullptr;
     const int j0 = ((NW == 1 ? 0 : wv * 64) + lane) * QU;
     const bool once = a.k <= NCH * STEP;
+    const bool unbounded = SWIGLU && dsv4_swiglu::unbounded(a.limit);
 
     u32x4 ra[NCH][RW], ru[SWIGLU ? NCH : 1][RW];
     float f[NCH][QU];
@@ -146,10 +121,17 @@ __global__ __launch_bounds__(NW == 1 ? 256 : 64 * NW) void k_quant_i8(QuantI8Arg
             if (j < a.k) {
                 widen8<TYPE>(ra[c], f[c]);
                 if constexpr (SWIGLU) {
-                    float u[QU];
+                    float u[QU], v[QU];
                     widen8<TYPE>(ru[c], u);
 #pragma unroll
-                    for (int i = 0; i < QU; i++) f[c][i] = swiglu32(f[c][i], u[i], a.limit);
+                    for (int i = 0; i < QU; i++) v[i] = dsv4_swiglu::value32(f[c][i], u[i], a.limit);
+                    if (unbounded) {
+#pragma unroll
+                        for (int i = 0; i < QU; i++)
+                            if (dsv4_swiglu::lost(f[c][i], u[i], v[i])) v[i] = __builtin_nanf("");
+                    }
+#pragma unroll
+                    for (int i = 0; i < QU; i++) f[c][i] = v[i];
                 }
             } else {
 #pragma unroll
@@ -169,7 +151,7 @@ __global__ __launch_bounds__(NW == 1 ? 256 : 64 * NW) void k_quant_i8(QuantI8Arg
             e.load(pu + (size_t)j * elem_bytes<TYPE>());
             e.get(t);
             u = t[0];
-            return swiglu64(g, u, a.limit);
+            return dsv4_swiglu::value64(g, u, a.limit);
         }
         return (double)g;
     };
@@ -200,7 +182,8 @@ __global__ __launch_bounds__(NW == 1 ? 256 : 64 * NW) void k_quant_i8(QuantI8Arg
     m = (uint32_t)__builtin_amdgcn_readfirstlane((int)m);
     const float amax = __uint_as_float(m);
     double amax64 = (double)amax;
-    /* SwiGLU's fp32 values serve rows of this range; others take fp64 ones */
+    /* SwiGLU's fp32 values serve rows of this range; others, and those with a
+     * lost value's NaN, take fp64 ones */
     const bool wide = SWIGLU && !(amax >= 0x1p-60f && amax <= 0x1p120f);
     bool bad = !SWIGLU && m >= 0x7F800000u;
     if constexpr (SWIGLU) {
