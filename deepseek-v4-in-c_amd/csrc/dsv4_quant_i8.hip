@@ -17,8 +17,9 @@
  *   product by 127 / amax within 10 x 2^-24 of at most 127: a code is certain
  *   outside 1.24 x 2^-14 (1.375 are taken) of a half-integer. Inside, and for the
  *   row's largest value, the SwiGLU is taken in fp64: codes and scale are those of
- *   fp64 values. Rows whose largest value is below 2^-60 or beyond 2^120, or that
- *   hold a value which fp32 lost, compute everything in fp64.
+ *   fp64 values. Rows whose largest value is below 2^-60, beyond 2^120 or 2^98
+ *   times below the largest up value, where fp32 may have lost some, compute
+ *   everything in fp64.
  *
  * Bound: HBM for plain rows (8,192 of 4,096 bf16 19.6 us, 5.1 TB/s), the vector
  * unit for SwiGLU (some 40 instructions an element, 10 of the 14 us of 4,206
@@ -90,6 +91,7 @@ __global__ __launch_bounds__(NW == 1 ? 256 : 64 * NW) void k_quant_i8(QuantI8Arg
     constexpr int STEP = 64 * NW * QU;
     constexpr int RW = TYPE == DSV4_HIP_F32 ? 2 : 1;
     __shared__ uint32_t smax[NW];
+    __shared__ float sumax[SWIGLU ? NW : 1];
     __shared__ unsigned long long smax64[RPW];     /* SwiGLU: the fp64 maximum's bits */
     const int lane = threadIdx.x & 63, wv = wave_in_group();
     const long row = (long)blockIdx.x * RPW + (NW == 1 ? wv : 0);
@@ -103,6 +105,7 @@ __global__ __launch_bounds__(NW == 1 ? 256 : 64 * NW) void k_quant_i8(QuantI8Arg
     const int j0 = ((NW == 1 ? 0 : wv * 64) + lane) * QU;
     const bool once = a.k <= NCH * STEP;
     const bool unbounded = SWIGLU && dsv4_swiglu::unbounded(a.limit);
+    float umax = 0.0f;                             /* unbounded: the largest |u|  */
 
     u32x4 ra[NCH][RW], ru[SWIGLU ? NCH : 1][RW];
     float f[NCH][QU];
@@ -115,23 +118,26 @@ __global__ __launch_bounds__(NW == 1 ? 256 : 64 * NW) void k_quant_i8(QuantI8Arg
                 if constexpr (SWIGLU) load8<TYPE>(pu, j, ru[c]);
             }
         }
+        if (unbounded) {
+#pragma unroll
+            for (int c = 0; c < NCH; c++) {
+                if (base + j0 + c * STEP >= a.k) continue;
+                float u[QU];
+                widen8<TYPE>(ru[c], u);
+#pragma unroll
+                for (int i = 0; i < QU; i++) umax = fmaxf(umax, fabsf(u[i]));
+            }
+        }
 #pragma unroll
         for (int c = 0; c < NCH; c++) {
             const int j = base + j0 + c * STEP;
             if (j < a.k) {
                 widen8<TYPE>(ra[c], f[c]);
                 if constexpr (SWIGLU) {
-                    float u[QU], v[QU];
+                    float u[QU];
                     widen8<TYPE>(ru[c], u);
 #pragma unroll
-                    for (int i = 0; i < QU; i++) v[i] = dsv4_swiglu::value32(f[c][i], u[i], a.limit);
-                    if (unbounded) {
-#pragma unroll
-                        for (int i = 0; i < QU; i++)
-                            if (dsv4_swiglu::lost(f[c][i], u[i], v[i])) v[i] = __builtin_nanf("");
-                    }
-#pragma unroll
-                    for (int i = 0; i < QU; i++) f[c][i] = v[i];
+                    for (int i = 0; i < QU; i++) f[c][i] = dsv4_swiglu::value32(f[c][i], u[i], a.limit);
                 }
             } else {
 #pragma unroll
@@ -173,18 +179,25 @@ __global__ __launch_bounds__(NW == 1 ? 256 : 64 * NW) void k_quant_i8(QuantI8Arg
         for (int c = 0; c < NCH; c++) m = max(m, top[c]);
     }
     m = wave_max_u32(m);
+    if (unbounded) umax = __uint_as_float(wave_max_u32(__float_as_uint(umax)));
     if constexpr (NW > 1) {
-        if (lane == 0) smax[wv] = m;
+        if (lane == 0) {
+            smax[wv] = m;
+            if (unbounded) sumax[wv] = umax;
+        }
         __syncthreads();
 #pragma unroll
         for (int w = 0; w < NW; w++) m = max(m, smax[w]);
+        if (unbounded) {
+#pragma unroll
+            for (int w = 0; w < NW; w++) umax = fmaxf(umax, sumax[w]);
+        }
     }
     m = (uint32_t)__builtin_amdgcn_readfirstlane((int)m);
     const float amax = __uint_as_float(m);
     double amax64 = (double)amax;
-    /* SwiGLU's fp32 values serve rows of this range; others, and those with a
-     * lost value's NaN, take fp64 ones */
-    const bool wide = SWIGLU && !(amax >= 0x1p-60f && amax <= 0x1p120f);
+    /* SwiGLU: a row that takes fp64 values */
+    const bool wide = SWIGLU && !dsv4_swiglu::fp32_serves(amax, a.limit > 0.0f ? fminf(umax, a.limit) : umax);
     bool bad = !SWIGLU && m >= 0x7F800000u;
     if constexpr (SWIGLU) {
         /* magnitudes order as their bits do, NaN above all: one LDS maximum of

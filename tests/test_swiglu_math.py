@@ -1,12 +1,11 @@
 # SPDX-License-Identifier: Apache-2.0
 """The fp32 SwiGLU of the int8 quantizer (csrc/dsv4_swiglu_math.h), built for
-the host, against fp64: a value is within its bound or NaN, over every exponent
-of gate and up value.
+the host, against fp64, over every exponent of gate and up value.
 
-The bound. A row is served by fp32 values only where its largest is 2^-60 or
-more, and a code or scale follows from values within 2^-21 of the largest: so a
-value may be off by 2^-21 of itself (8 x 2^-24, the header's sum of steps) plus
-2^-81. Beyond fp32's range a value is infinite and its row goes to fp64."""
+The bound. A code and a scale follow from values within 2^-21 of the row's
+largest. A value may so be off by 2^-21 of itself (8 x 2^-24, the header's sum of
+steps) plus 2^-21 of the least largest value with which its row would still be
+served by fp32. A value that is NaN sends its row to fp64, one beyond 2^120 too."""
 import ctypes as C
 import os
 import subprocess
@@ -21,12 +20,17 @@ SHIM = """
 using namespace dsv4_swiglu;
 extern "C" void values(const float *g, const float *u, float limit, float *v, long n)
 {
-    const bool un = unbounded(limit);
+    for (long i = 0; i < n; i++) v[i] = value32(g[i], u[i], limit);
+}
+/* the least power of two that a row's largest value may be with up values of size u */
+extern "C" void least(const float *u, float limit, float *a, long n)
+{
     for (long i = 0; i < n; i++) {
-        v[i] = value32(g[i], u[i], limit);
-        if (un && lost(g[i], u[i], v[i])) v[i] = NAN;
+        const float um = !unbounded(limit) ? 0.0f : limit > 0 ? fminf(fabsf(u[i]), limit) : fabsf(u[i]);
+        for (a[i] = 0x1p-149f; !fp32_serves(a[i], um); a[i] *= 2) ;
     }
 }
+extern "C" int serves(float amax, float umax) { return fp32_serves(amax, umax); }
 """
 
 
@@ -40,11 +44,16 @@ def values(tmp_path_factory):
     lib = C.CDLL(str(so))
     P = np.ctypeslib.ndpointer(np.float32, flags="C_CONTIGUOUS")
     lib.values.argtypes, lib.values.restype = [P, P, C.c_float, P, C.c_long], None
+    lib.least.argtypes, lib.least.restype = [P, C.c_float, P, C.c_long], None
+    lib.serves.argtypes, lib.serves.restype = [C.c_float, C.c_float], C.c_int
 
     def run(g, u, limit):
-        v = np.empty_like(g)
+        """values, and the least largest value of a row that fp32 serves"""
+        v, a = np.empty_like(g), np.empty_like(g)
         lib.values(g, u, limit, v, g.size)
-        return v
+        lib.least(u, limit, a, u.size)
+        return v, a.astype(np.float64)
+    run.serves = lib.serves
     return run
 
 
@@ -67,30 +76,33 @@ def exact(g, u, limit):
         return g / (1 + np.exp(-g)) * u
 
 
-def in_bound(v, want):
-    big = np.abs(want) >= np.finfo(np.float32).max * (1 - 2.0 ** -20)
+def in_bound(v, want, least):
     with np.errstate(over="ignore", invalid="ignore"):
-        ok = np.abs(v.astype(np.float64) - want) <= 2.0 ** -21 * np.abs(want) + 2.0 ** -81
-    return ok | (big & (np.abs(v) >= 3.4e38))
+        ok = np.abs(v.astype(np.float64) - want) <= 2.0 ** -21 * (np.abs(want) + least)
+    return ok | ((np.abs(want) > 2.0 ** 120) & (np.abs(v) > 2.0 ** 120))
 
 
 @pytest.mark.parametrize("limit", [0.0, -1.0, 10.0, 2.0 ** 32, 2.0 ** 33, 1e20, 3e38])
 def test_values_hold_their_bound_or_are_nan(values, limit):
     g, u = grid()
-    v, want = values(g, u, limit), exact(g, u, limit)
-    assert (np.isnan(v) | in_bound(v, want)).all()
+    v, least = values(g, u, limit)
+    assert (np.isnan(v) | in_bound(v, exact(g, u, limit), least)).all()
 
 
-@pytest.mark.parametrize("g,u", [(-89.0, 1e37), (-87.5, 1e37), (-90.0, 1e37), (-95.0, 1e37), (-100.0, 2.0 ** 110),
-                                 (4.2e-45, 1e38), (3 * 2.0 ** -149, 2.0 ** 100)])
-def test_a_lost_value_is_nan(values, g, u):
-    """Gates whose silu leaves fp32's normal range under up values that make it count."""
-    assert np.isnan(values(np.float32([g]), np.float32([u]), 0.0)).all()
+@pytest.mark.parametrize("g,u", [(-89.0, 1e37), (-87.5, 1e37), (-90.0, 1e37), (-100.0, 2.0 ** 110), (4.2e-45, 1e38),
+                                 (3 * 2.0 ** -149, 2.0 ** 100)])
+def test_a_value_that_is_lost_has_its_row_decided_in_fp64(values, g, u):
+    """Be it the row's largest value or one that is 64 times smaller."""
+    size = abs(exact(np.float32([g]), np.float32([u]), 0.0)[0])
+    for largest in (size, 64 * size):
+        assert not values.serves(largest, u)
 
 
-def test_ordinary_gates_keep_large_up_values(values):
-    """Only a lost value becomes NaN, not every product with a large up value."""
-    g = np.float32([-80, -20, -1, -1e-30, 0, 1e-30, 1, 50] * 2)
-    u = np.float32([1e12] * 8 + [-1e30] * 8)
-    v = values(g, u, 0.0)
-    assert in_bound(v, exact(g, u, 0.0)).all()
+def test_large_up_values_under_ordinary_gates_are_served(values):
+    for u in (1.0, 1e12, 1e30):
+        assert values.serves(0.5 * u, u) and values.serves(1e-25 * u + 1e-15, u)
+
+
+@pytest.mark.parametrize("amax", [0.0, 1e-19, 2e36, float("inf"), float("nan")])
+def test_rows_beyond_fp32s_reach_are_not(values, amax):
+    assert not values.serves(amax, 0.0)
