@@ -65,12 +65,15 @@ DSV4_SWIGLU_HD float value32(float g, float u, float limit)
 {
     clamp(g, u, limit);
     /* exp(-g) = 2^t (1 + ln 2 * r): t the rounded product with log2 e, r what
-     * the rounding and log2 e's own last bits left. Infinite and NaN gates give
-     * NaN. */
+     * the rounding and log2 e's own last bits left. The correction is a factor
+     * next to 1, so that where e passes fp32's range (a gate below -88.7) the sum
+     * is infinite and the value 0: a term e * ln 2 * r beside e would be infinite
+     * of either sign, and the NaN of their sum would cost the row fp64 values.
+     * Infinite and NaN gates give NaN. */
     const float t = -g * 0x1.715476p+0f;
     const float r = fmaf(-g, 0x1.4ae0cp-26f, fmaf(-g, 0x1.715476p+0f, -t));
     const float e = DSV4_EXP2(t);
-    return g * DSV4_RCP(1.0f + fmaf(e * 0x1.62e43p-1f, r, e)) * u;
+    return g * DSV4_RCP(fmaf(e, fmaf(r, 0x1.62e43p-1f, 1.0f), 1.0f)) * u;
 }
 
 } // namespace dsv4_swiglu

@@ -4,7 +4,7 @@
 import pytest
 import torch
 
-from test_gpu_i8 import DEV, check_rows, gen, swiglu64, swiglu_quant
+from test_gpu_i8 import DEV, TYPES, check_rows, gen, swiglu64, swiglu_quant
 
 pytestmark = pytest.mark.gpu
 
@@ -45,4 +45,15 @@ def test_a_clamp_bounds_what_fp32_loses(lib, limit):
             g, u = rows_around(dtype, 4, 528, (odd[0], 1.0), 1.0, 9)
             g[:, 5:9], u[:, 5:9] = odd[0], odd[1]
             u[:, 20] = 1.0 / 128                   # beside the clamped values, ordinary ones
+            check_rows(*swiglu_quant(lib, g, u, limit), swiglu64(g, u, limit))
+
+
+@pytest.mark.parametrize("limit", [0.0, 10.0])
+@pytest.mark.parametrize("gate", [-88.5, -90.5, -92.5, -95.0, -1000.0, -65504.0])
+def test_a_very_negative_gate_among_ordinary_ones(lib, gate, limit):
+    """Its value is 0 beside the others', which keep their codes."""
+    for dtype in TYPES:
+        for n, k in ((5, 64), (300, 2048), (2, 8208)):
+            g, u = (torch.randn(n, k, device=DEV, generator=gen(n + i)).to(dtype) for i in range(2))
+            g[torch.arange(n), torch.arange(n, device=DEV) * 37 % k] = gate
             check_rows(*swiglu_quant(lib, g, u, limit), swiglu64(g, u, limit))

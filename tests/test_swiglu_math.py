@@ -106,3 +106,21 @@ def test_large_up_values_under_ordinary_gates_are_served(values):
 @pytest.mark.parametrize("amax", [0.0, 1e-19, 2e36, float("inf"), float("nan")])
 def test_rows_beyond_fp32s_reach_are_not(values, amax):
     assert not values.serves(amax, 0.0)
+
+
+@pytest.mark.parametrize("limit", [0.0, 10.0, 2.0 ** 32])
+def test_no_finite_gate_sends_its_row_to_fp64(values, limit):
+    """With up values of a model a value is finite however negative its gate: one
+    that is not costs all of its row two fp64 values an element."""
+    r = np.random.default_rng(2).random(2000)
+    g = np.concatenate([-np.linspace(60, 130, 7001), -np.ldexp(1 + r, 7 + np.arange(2000) % 120)]).astype(np.float32)
+    for u in (1.0, -0.03, 700.0):
+        u = np.full_like(g, u)
+        v, least = values(g, u, limit)
+        assert np.isfinite(v).all() and in_bound(v, exact(g, u, limit), least).all()
+
+
+@pytest.mark.parametrize("limit", [0.0, 10.0])
+def test_infinite_and_nan_gates_do(values, limit):
+    g = np.float32([-np.inf, np.nan] + ([np.inf] if limit == 0 else []))
+    assert np.isnan(values(g, np.ones_like(g), limit)[0]).all()
