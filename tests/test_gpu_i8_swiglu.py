@@ -57,3 +57,21 @@ def test_a_very_negative_gate_among_ordinary_ones(lib, gate, limit):
             g, u = (torch.randn(n, k, device=DEV, generator=gen(n + i)).to(dtype) for i in range(2))
             g[torch.arange(n), torch.arange(n, device=DEV) * 37 % k] = gate
             check_rows(*swiglu_quant(lib, g, u, limit), swiglu64(g, u, limit))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("limit", [0.0, 10.0])
+@pytest.mark.parametrize("k", [16400, 20000, 33024])
+def test_rows_that_are_read_again(lib, dtype, limit, k):
+    """Rows that no workgroup holds at once: the largest value in any pass, rows
+    in fp64, rows of zeros and with a value that is not finite."""
+    g, u = (torch.randn(9, k, device=DEV, generator=gen(k + i)).to(dtype) for i in range(2))
+    for r, at in ((1, 3), (2, 16390), (3, k - 1)):
+        g[r, at], u[r, at] = 9.0, -9.5             # the row's largest
+    u[4] = u[4].double().mul(1e-30).to(dtype)      # below what fp32 serves
+    g[5], u[6] = 0.0, 0.0
+    g[7, k - 5] = float("nan")
+    g[8, 16384::7] = -95.0
+    q, s = swiglu_quant(lib, g, u, limit)
+    check_rows(q, s, swiglu64(g, u, limit))
+    assert torch.isnan(s[7]) and (q[7] == 0).all()
