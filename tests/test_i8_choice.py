@@ -9,6 +9,7 @@ import subprocess
 import pytest
 
 import test_gpu_i8
+import test_gpu_i8_forms
 from conftest import PKG_DIR
 
 SHIM = """
@@ -77,3 +78,30 @@ def test_waves_of_a_launch(rules, form, F, TR, waves):
 def test_waves_hold_every_bucket(rules, form, F, TR, waves, counts):
     tiles = sum(-(-c // TR) for c in counts)
     assert rules.c_waves(form, sum(counts), 100, len(counts)) >= tiles * -(-100 // F) * waves
+
+
+FORMS = {"pair": PAIR, "64x2": T64x2, "64x2 deep": T64x2_DEEP, "64x4": T64x4, "128x4": T128x4, "128x8": T128x8,
+         "256x8": T256x8}
+TILES = {"pair": (8, 8), "64x2": (64, 32), "64x2 deep": (64, 32), "64x4": (64, 64), "128x4": (128, 64),
+         "128x8": (128, 128), "256x8": (256, 128)}                 # features, rows
+
+
+def test_gpu_tests_reach_the_forms_that_they_name(rules):
+    """and each with rows, features and K that end inside a tile"""
+    for cases in (test_gpu_i8_forms.ONE, test_gpu_i8_forms.WIDE, test_gpu_i8_forms.SLICES, test_gpu_i8_forms.EVEN):
+        assert set(cases) == set(FORMS)
+    for form, (F, TR) in TILES.items():
+        for M, N, K in test_gpu_i8_forms.ONE[form]:
+            assert rules.c_form(M, N, K) == FORMS[form] and M % TR and N % F and K % 128
+        assert rules.c_form(*test_gpu_i8_forms.WIDE[form], test_gpu_i8_forms.KMAX) == FORMS[form]
+        assert rules.c_form(test_gpu_i8_forms.SLICES[form], test_gpu_i8_forms.SLICES_N,
+                            test_gpu_i8_forms.SLICES_K) == FORMS[form]
+        M, N, K = test_gpu_i8_forms.EVEN[form]
+        assert rules.c_form(M, N, K) == FORMS[form] and N % 8 == 0
+
+
+def test_gpu_tests_reach_the_forms_of_the_experts_product(rules):
+    for cases in (test_gpu_i8_forms.GROUPED, test_gpu_i8_forms.GROUPED_WIDE):
+        for form in ("pair", "64x2", "128x4", "256x8"):
+            counts, N, K = cases[form]
+            assert rules.c_grouped(sum(counts), N, K, len(counts)) == FORMS[form]
