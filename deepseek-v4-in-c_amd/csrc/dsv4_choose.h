@@ -241,6 +241,12 @@ inline long i8_cost(const I8Cost &c, long tiles, long N, long K, long more = 0)
  * workgroups wait out one load (us, pair / 64x2 deep / 64x2: 1 x 4096 x 4096
  * 5.0 / 7.0 / 7.8, 8 x 4096 x 4096 6.2 / 7.2 / 7.9, 12 x 1024 x 4096 4.3 / 7.0 /
  * 7.8; but 16 x 4096 x 4096 9.7 / 7.3 / 8.0, 1 x 32768 x 1024 14.1 / 7.7 / 7.5).
+ * Where it stops pays depends on where the weights are, which no call tells, and
+ * the limit lies between. Pair / 64x2 deep with weights in HBM: 1 x 7168 x 2048
+ * 5.9 / 6.6, 1 x 7168 x 4096 7.4 / 10.4, 8 of these 9.7 / 10.6, 1 x 6152 x 7168 10.7 /
+ * 15.6, 8 of these 14.7 / 16.1, 1 x 14336 x 7168 18.1 / 19.9, 8 of these 25.6 / 19.9;
+ * with weights in the memory-side cache 5.8 / 5.0, 7.1 / 7.0, 9.5 / 7.0, 10.4 / 10.5,
+ * 14.4 / 10.8, 17.7 / 16.6, 25.3 / 17.1.
  * Otherwise the form of least cost. In one round 64x2 takes two blocks of K a
  * stage (8.0 -> 7.2 at 16 rows; with three workgroups a CU its longer ring
  * costs, 512 rows 21.4 -> 21.9). */

@@ -347,10 +347,11 @@ __device__ __forceinline__ void i8_leave(const I8Args &a, const Tile &t, int n0,
  * one, so the stage NST ahead takes its place. Loads past K read nothing and
  * multiply as zeros. The tile leaves through LDS as whole 16-byte pieces of rows,
  * written past the caches (16 MB of bf16 36.7 -> 35.6 us of the call).
- * Bound: 256 x 128 tiles issue an MFMA in half of their cycles (2,048 x 4096 x
- * 4096 34 us, 2.0 of 4.3 POP/s that registers alone reach; the library's int8
- * product takes 41.7), the rest are barriers and LDS; experts' buckets the HBM
- * stream beside that (24,576 rows of 256 experts, Zipf, 483 us, even 430; 359
+ * Bound: 256 x 128 tiles keep the MFMA units busy in 37 % of the cycles (2,048 x
+ * 4096 x 4096 34 us, 2.0 POP/s, of 5 nominal and 4.3 that products of registers
+ * alone reach; the library's int8 product takes 41.7), the rest are barriers and
+ * LDS; its XCDs fetch 8.4 MB each, eight row tiles by four feature tiles' operands,
+ * 67 MB for 25. Experts' buckets the HBM stream beside that (24,576 rows of 256 experts, Zipf, 483 us, even 430; 359
  * with every table entry the same matrix, 316 for the weights alone); few rows the chain of
  * stages (16 to 128 rows of 4096 x 4096 7 to 8 us; K split over teams of waves
  * gained nothing, weights straight to registers lost 10 to 20 %). */

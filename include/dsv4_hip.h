@@ -372,7 +372,9 @@ int  dsv4_hip_gemm_mxfp8q_dev(void *C, int out_bf16, const uint8_t *Aq,
  * pointers, C [M][W->rows] of out_type. The integer sum is exact; the result
  * is ((float)sum * Sa) * s, rounded once more for a 16-bit out_type (values
  * beyond fp16 become infinite). cols a multiple of 16 up to 131,056; M and
- * W->rows any; Aq and w 16-byte aligned. A scale of NaN makes its row NaN.
+ * W->rows any that cover less than 2^23 tiles of 128 x 256 results (2^30 rows of up
+ * to 256, 2^26 of 4096; more is refused, nothing enqueued); Aq and w 16-byte
+ * aligned. A scale of NaN makes its row NaN.
  * No workspace: calls on several streams, and captured graphs, do not meet.
  * Stream: one of the library's device, or NULL (hipStreamLegacy is refused);
  * so for all the calls from here to the expert order.
@@ -389,7 +391,8 @@ int  dsv4_hip_gemm_i8_dev(void *C, int out_type, const int8_t *Aq, const float *
  * `table` is a DEVICE array of n_experts descriptors (DSV4_WI8, [N x K],
  * device pointers, w 16-byte aligned); one of another kind raises status bit
  * 1 and its rows become NaN. A row_tok outside [0, n_a) raises bit 0 and its
- * row becomes NaN. n_experts <= 1024; n_a * K < 2^31; else as above. */
+ * row becomes NaN. n_experts <= 1024; n_a * K < 2^31; else as above, with up to one
+ * more row of tiles for each expert. */
 int  dsv4_hip_gemm_i8_grouped_dev(void *C, int out_type, const int8_t *Aq, const float *Sa, int n_a,
                                   const int *row_tok, int n_rows, const int *ex_off,
                                   const DSV4QMat *table, int n_experts, int N, int K, void *stream);

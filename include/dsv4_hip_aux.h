@@ -58,7 +58,8 @@ int dsv4_hip_quant_i8_dev(int8_t *Q, float *S, const void *a, int type, int64_t 
 /* The same for a = SwiGLU(g, u), the reference's element with its asymmetric
  * clamp (src/10_compute/dsv4_ops.c:61-79; limit <= 0: none): g and u rows of
  * gate and up outputs, both `ld` elements apart (two arrays, or the halves of
- * one). Codes and scale are those of the exact SwiGLU values. */
+ * one). Codes and scale are those of the exact SwiGLU values (taken in fp64; a
+ * scale beyond fp32 is infinite). */
 int dsv4_hip_swiglu_quant_i8_dev(int8_t *Q, float *S, const void *g, const void *u, int type, int64_t ld,
                                  int n, int k, float limit, void *stream);
 

@@ -105,3 +105,13 @@ def test_gpu_tests_reach_the_forms_of_the_experts_product(rules):
         for form in ("pair", "64x2", "128x4", "256x8"):
             counts, N, K = cases[form]
             assert rules.c_grouped(sum(counts), N, K, len(counts)) == FORMS[form]
+
+
+@pytest.mark.parametrize("M,N,K", [(1 << 30, 256, 16), ((1 << 30) - 128, 256, 4096), (1 << 30, 1, 16),
+                                   ((1 << 30) - 127, 1, 131056), (1 << 26, 4096, 64), ((1 << 26) - 128, 4096, 64),
+                                   (1 << 18, 1 << 20, 16), ((1 << 18) - 128, 1 << 20, 16), ((1 << 31) - 1, 1, 16),
+                                   ((1 << 27) - 5, 256, 16), ((1 << 27) + 5, 200, 16), ((1 << 22) - 300, 8000, 16)])
+def test_the_limit_of_a_launch(rules, M, N, K):
+    """less than 2^23 tiles of 128 x 256 results, whatever form a size takes"""
+    fits = -(-M // 128) * -(-N // 256) < 1 << 23
+    assert (rules.c_waves(rules.c_form(M, N, K), M, N, 0) < 1 << 26) == fits
