@@ -351,10 +351,11 @@ __device__ __forceinline__ void i8_leave(const I8Args &a, const Tile &t, int n0,
  * 4096 x 4096 34 us, 2.0 POP/s, of 5 nominal and 4.3 that products of registers
  * alone reach; the library's int8 product takes 41.7), the rest are barriers and
  * LDS; its XCDs fetch 8.4 MB each, eight row tiles by four feature tiles' operands,
- * 67 MB for 25. Experts' buckets the HBM stream beside that (24,576 rows of 256 experts, Zipf, 483 us, even 430; 359
- * with every table entry the same matrix, 316 for the weights alone); few rows the chain of
- * stages (16 to 128 rows of 4096 x 4096 7 to 8 us; K split over teams of waves
- * gained nothing, weights straight to registers lost 10 to 20 %). */
+ * 67 MB for 25. Experts' buckets the HBM stream beside that (24,576 rows of 256
+ * experts, Zipf, 483 us, even 430; 359 with every table entry the same matrix, 316
+ * for the weights alone); few rows the chain of stages (16 to 128 rows of 4096 x
+ * 4096 7 to 8 us; K split over teams of waves gained nothing, weights straight to
+ * registers lost 10 to 20 %). */
 template <int F, int T, int KB, int NST_> struct I8Tile {
     static constexpr int WT = T >= 4 ? 2 : 1, NWAVE = 4 * WT, U = T / WT, WI = F / 64;
     static constexpr int OFF_X = F * 128, SUB = OFF_X + 16 * T * 128, STAGE = KB * SUB;

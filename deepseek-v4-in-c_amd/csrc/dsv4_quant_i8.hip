@@ -23,8 +23,9 @@
  *
  * Bound: HBM for plain rows (8,192 of 4,096 bf16 19.6 us, 5.1 TB/s), the vector
  * unit for SwiGLU (38 instructions an element, 10 of the 13.3 us of 4,206 rows of
- * 2,048 whose bytes take 8.5; 24,576 rows 57, 4.4 TB/s; rows in fp64 190 rather than
- * 13), latency for a few rows (one of 4,096 2.6 us, less than the launch costs its caller).
+ * 2,048 whose bytes take 8.5; 24,576 rows 57, 4.4 TB/s; rows in fp64 190 rather
+ * than 13.3), latency for a few rows (one of 4,096 2.6 us, less than the launch
+ * costs its caller).
  */
 #include "dsv4_elem.h"
 #include "dsv4_internal.h"
