@@ -15,6 +15,7 @@
  * operand. Any order of k works as long as both operands use the same one, so
  * the four lane groups may take their 16 codes from wherever loads like best.
  */
+#include "dsv4_bucket.h"
 #include "dsv4_elem.h"
 #include "dsv4_internal.h"
 
@@ -22,119 +23,15 @@ namespace dsv4 {
 
 namespace {
 
-typedef int v4i __attribute__((ext_vector_type(4)));
+using I8Bucket = Bucket<float>;
 
-constexpr uint32_t I8_OOB = 0x80000000u;           /* beyond every buffer: reads zeros */
-
-__device__ __forceinline__ __amdgpu_buffer_rsrc_t i8_rsrc(const void *p, uint32_t bytes)
+/* whether a table's entry is an int8 N x K matrix */
+__device__ __forceinline__ auto i8_matrix(const I8Args &a)
 {
-    return __builtin_amdgcn_make_buffer_rsrc(const_cast<void *>(p), (short)0, (int)bytes, 0x00020000);
-}
-/* The whole offset goes into the per-lane part: the range check subtracts the
- * scalar part from the buffer's size, which wraps for a buffer shorter than
- * that (a single row). */
-template <int CPOL>
-__device__ __forceinline__ v4i i8_ld16(__amdgpu_buffer_rsrc_t r, uint32_t voff)
-{
-    return __builtin_bit_cast(v4i, __builtin_amdgcn_raw_buffer_load_b128(r, (int)voff, 0, CPOL));
-}
-
-/* what one workgroup multiplies: rows r0 .. r0 + rows of the product against
- * matrix w (scales s) */
-struct Tile {
-    const uint8_t *w;
-    const float *s;
-    int r0, rows;
-    int e;                                         /* its expert */
-    bool bad;                                      /* the table's entry is not an int8 N x K matrix */
-};
-
-/* Row tile `t` of the buckets ex_off[0 .. E], each cut into tiles of TR rows;
- * rows == 0 past the last one. Every wave finds it by itself: a lane counts the
- * tiles of E / 64 experts, a scan over the lanes finds the one that holds t, a
- * scan of its experts' tiles the expert. Offsets are clamped to [0, M], so no
- * table makes a row out of range.
- *
- * With nt, `t` is the workgroup of a launch over nt feature tiles, *f the one it
- * takes: workgroups go round the eight XCDs, and each XCD gets a contiguous
- * eighth of the (row, feature) tiles, an expert's in groups of eight row tiles by
- * its feature tiles. So an XCD's L2 fetches an expert's tokens once for all
- * features and a popular expert's weights once for eight row tiles. us in 256 x
- * 128 tiles, against feature tiles dealt out to the XCDs: 24,576 rows of 256
- * experts 2048 x 4096 453 -> 429, with Zipf 520 -> 484, 6,144 rows of 64 of them
- * 116 -> 106; groups of all row tiles by one feature tile after the other 485 and
- * no groups 345 rather than 327 at 24,576 rows of 64 experts 4096 x 2048, Zipf. */
-template <int TR>
-__device__ __forceinline__ Tile bucket_tile(const I8Args &a, int t, int lane, int nt = 0, int *f = nullptr)
-{
-    const int E = a.n_experts, per = (E + 63) / 64;
-    auto clampr = [&](int v) { return min(max(v, 0), a.M); };
-    int mine = 0;
-    const auto off = gptr(a.ex_off);
-    int lo = clampr(off[min(lane * per, E)]);
-    for (int i = 0; i < per; i += 4) {             /* four loads in flight */
-        int hi[4];
-#pragma unroll
-        for (int j = 0; j < 4; j++) hi[j] = off[min(lane * per + min(i + j + 1, per), E)];
-#pragma unroll
-        for (int j = 0; j < 4; j++) {              /* past the lane's experts: empty buckets */
-            hi[j] = clampr(hi[j]);
-            mine += (max(hi[j] - lo, 0) + TR - 1) / TR;
-            lo = hi[j];
-        }
-    }
-    int incl = mine;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        const int v = __shfl_up(incl, d, 64);
-        if (lane >= d) incl += v;
-    }
-    Tile o;
-    o.w = nullptr; o.s = nullptr; o.r0 = 0; o.rows = 0; o.e = 0; o.bad = false;
-    int in = 0;
-    if (nt) {
-        /* a sum that wraps comes from falling offsets: never more tiles than there are */
-        const uint32_t tiles = min((uint32_t)__builtin_amdgcn_readlane(incl, 63), gridDim.x / (uint32_t)nt);
-        const int total = (int)tiles * nt, x = t % 8, y = t / 8;
-        if (t >= total) return o;
-        const int id = x * (total / 8) + min(x, total % 8) + y;
-        t = id / nt;
-        in = id - t * nt;
-    }
-    const uint64_t past = __ballot(incl > t);
-    if (!past) return o;
-    const int L = __builtin_ctzll(past);
-    int left = t - __builtin_amdgcn_readlane(incl - mine, L);
-    /* its experts, one a lane */
-    const int mylo = clampr(off[min(L * per + min(lane, per), E)]);
-    const int n = max(__shfl_down(mylo, 1, 64) - mylo, 0), tiles = lane < per ? (n + TR - 1) / TR : 0;
-    int upto = tiles;
-#pragma unroll
-    for (int d = 1; d < 16; d <<= 1) {             /* per <= 16 */
-        const int v = __shfl_up(upto, d, 64);
-        if (lane >= d) upto += v;
-    }
-    const uint64_t holds = __ballot(lane < per && upto > left);
-    if (!holds) return o;
-    const int i = __builtin_ctzll(holds), mine_i = __builtin_amdgcn_readlane(tiles, i);
-    left -= __builtin_amdgcn_readlane(upto, i) - mine_i;
-    if (nt) {
-        constexpr int GROUP = 8;
-        in += left * nt;                           /* among the expert's tiles */
-        const int g0 = in / (GROUP * nt) * GROUP, rows = min(GROUP, mine_i - g0);
-        in -= g0 * nt;
-        left = g0 + in % rows;
-        *f = in / rows;
-    }
-    o.r0 = __builtin_amdgcn_readlane(mylo, i) + left * TR;
-    o.rows = min(TR, __builtin_amdgcn_readlane(n, i) - left * TR);
-    o.e = L * per + i;
-    const DSV4QMat m = ld_uniform(a.table, o.e);
-    o.w = (const uint8_t *)m.w;
-    o.s = (const float *)m.s;
-    o.bad = m.wdt != DSV4_WI8 || m.rows != a.N || m.cols != a.K || !m.w || !m.s || ((uintptr_t)m.w & 15u) ||
-            ((uintptr_t)m.s & 3u);
-    return o;
+    return [&a](const DSV4QMat &m) {
+        return m.wdt == DSV4_WI8 && m.rows == a.N && m.cols == a.K && m.w && m.s && !((uintptr_t)m.w & 15u) &&
+               !((uintptr_t)m.s & 3u);
+    };
 }
 
 /* one result: element n of row r */
@@ -167,9 +64,9 @@ __global__ __launch_bounds__(64 * NW) void k_i8_pair(I8Args a)
     const int lane = threadIdx.x & 63, wave = wave_in_group();
     const int r8 = lane & 7, half = (lane >> 3) & 1, g = lane >> 4;
     const int slabs = (a.N + FR - 1) / FR, tile = blockIdx.x / slabs, n0 = (blockIdx.x - tile * slabs) * FR;
-    Tile t;
+    I8Bucket t;
     if constexpr (GROUPED) {
-        t = bucket_tile<TR>(a, tile, lane);
+        t = bucket_tile<TR, float>(a, tile, lane, i8_matrix(a));
         if (t.rows <= 0) return;
     } else {
         t.w = a.W; t.s = a.Sw; t.e = 0; t.bad = false;
@@ -184,9 +81,9 @@ __global__ __launch_bounds__(64 * NW) void k_i8_pair(I8Args a)
         return;
     }
     const uint32_t K = (uint32_t)a.K;
-    const __amdgpu_buffer_rsrc_t rw = i8_rsrc(t.w + (size_t)n0 * K, (uint32_t)nf * K);
+    const __amdgpu_buffer_rsrc_t rw = buf_rsrc(t.w + (size_t)n0 * K, (uint32_t)nf * K);
     const uint8_t *xb = GROUPED ? a.Aq : a.Aq + (size_t)t.r0 * K;
-    const __amdgpu_buffer_rsrc_t rx = i8_rsrc(xb, GROUPED ? (uint32_t)a.n_a * K : (uint32_t)t.rows * K);
+    const __amdgpu_buffer_rsrc_t rx = buf_rsrc(xb, GROUPED ? (uint32_t)a.n_a * K : (uint32_t)t.rows * K);
     auto src_of = [&](int i) -> int {
         if (i >= t.rows) return -1;
         if (!GROUPED) return i;
@@ -198,7 +95,7 @@ __global__ __launch_bounds__(64 * NW) void k_i8_pair(I8Args a)
 #pragma unroll
     for (int u = 0; u < TT; u++) {
         const int s = src_of(8 * u + r8);
-        xo[u] = s < 0 ? I8_OOB : (uint32_t)s * K + kc;
+        xo[u] = s < 0 ? BUF_OOB : (uint32_t)s * K + kc;
     }
 #pragma unroll
     for (int i = 0; i < RT; i++) wo[i] = (uint32_t)(8 * i + r8) * K + kc;
@@ -215,9 +112,9 @@ __global__ __launch_bounds__(64 * NW) void k_i8_pair(I8Args a)
             const uint32_t c = (uint32_t)(b0 + NW * b) * 128u;
             const bool in = c + kc < K;
 #pragma unroll
-            for (int i = 0; i < RT; i++) w[b][i] = i8_ld16<2>(rw, in ? wo[i] + c : I8_OOB);
+            for (int i = 0; i < RT; i++) w[b][i] = buf_ld16<2>(rw, in ? wo[i] + c : BUF_OOB);
 #pragma unroll
-            for (int u = 0; u < TT; u++) x[b][u] = i8_ld16<0>(rx, in && xo[u] != I8_OOB ? xo[u] + c : I8_OOB);
+            for (int u = 0; u < TT; u++) x[b][u] = buf_ld16<0>(rx, in && xo[u] != BUF_OOB ? xo[u] + c : BUF_OOB);
         }
 #pragma unroll
         for (int b = 0; b < B; b++)
@@ -274,7 +171,7 @@ constexpr int i8_out_ld(int F, int eb) { return F * eb + 16; }
  * bf16 14.3 -> 11.9, 2,787 rows 2691 x 128 fp32 12.3 -> 10.9; aligned 10.0 and
  * 10.7 at 20544 and 2688). */
 template <int F, bool GROUPED, int OUT, int NTHREADS, int WI, int U, class SRC>
-__device__ __forceinline__ void i8_leave(const I8Args &a, const Tile &t, int n0, int nf, uint8_t *lds,
+__device__ __forceinline__ void i8_leave(const I8Args &a, const I8Bucket &t, int n0, int nf, uint8_t *lds,
                                          const v4i (&acc)[WI][U], int f0, int m0, SRC src_of)
 {
     constexpr int EB = elem_bytes<OUT>(), LD = i8_out_ld(F, EB);
@@ -367,18 +264,6 @@ template <int F, int T, int KB, int NST_> struct I8Tile {
     static_assert(LX * NWAVE == 2 * T && LW * NWAVE * 8 == F && (NST - 1) * VM < 64 && lds(4) <= 160 * 1024, "ring");
 };
 
-typedef __attribute__((address_space(3))) void i8_lds;
-
-__device__ __forceinline__ void i8_dma16(__amdgpu_buffer_rsrc_t r, uint32_t voff, int soff, uint8_t *dst)
-{
-    __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (i8_lds *)dst, 16, (int)voff, soff, 0, 0);
-}
-template <int N>
-__device__ __forceinline__ void i8_wait_vm()
-{
-    __builtin_amdgcn_s_waitcnt(0x0F70 | (N & 15) | ((N >> 4) << 14));
-}
-
 template <int F, int T, int KB, int NST, bool GROUPED, int OUT>
 __global__ __launch_bounds__((64 * I8Tile<F, T, KB, NST>::NWAVE)) void k_i8_tile(I8Args a)
 {
@@ -393,12 +278,12 @@ __global__ __launch_bounds__((64 * I8Tile<F, T, KB, NST>::NWAVE)) void k_i8_tile
     const int lane = threadIdx.x & 63, wave = wave_in_group();
     const int rr = lane & 15, gq = lane >> 4, wr = wave & 3, wt = wave >> 2;
     const int nt = (a.N + F - 1) / F, nblk = (a.K + 127) / 128, nst = (nblk + KB - 1) / KB;
-    Tile t;
+    I8Bucket t;
     int n0;
     if constexpr (GROUPED) {
         int f = blockIdx.x % nt;
-        if constexpr (SHARED) t = bucket_tile<TR>(a, blockIdx.x, lane, nt, &f);
-        else t = bucket_tile<TR>(a, blockIdx.x / nt, lane);
+        if constexpr (SHARED) t = bucket_tile<TR, float>(a, blockIdx.x, lane, i8_matrix(a), nt, &f);
+        else t = bucket_tile<TR, float>(a, blockIdx.x / nt, lane, i8_matrix(a));
         n0 = f * F;
         if (t.rows <= 0) return;
     } else {
@@ -415,9 +300,9 @@ __global__ __launch_bounds__((64 * I8Tile<F, T, KB, NST>::NWAVE)) void k_i8_tile
     }
     const int nf = min(F, a.N - n0);
     const uint32_t K = (uint32_t)a.K;
-    const __amdgpu_buffer_rsrc_t rw = i8_rsrc(t.w + (size_t)n0 * K, (uint32_t)nf * K);
+    const __amdgpu_buffer_rsrc_t rw = buf_rsrc(t.w + (size_t)n0 * K, (uint32_t)nf * K);
     const uint8_t *xb = GROUPED ? a.Aq : a.Aq + (size_t)t.r0 * K;
-    const __amdgpu_buffer_rsrc_t rx = i8_rsrc(xb, GROUPED ? (uint32_t)a.n_a * K : (uint32_t)t.rows * K);
+    const __amdgpu_buffer_rsrc_t rx = buf_rsrc(xb, GROUPED ? (uint32_t)a.n_a * K : (uint32_t)t.rows * K);
     auto src_of = [&](int i) -> int {              /* row of Aq from xb on; -1: none */
         if (i >= t.rows) return -1;
         if (!GROUPED) return i;
@@ -434,8 +319,8 @@ __global__ __launch_bounds__((64 * I8Tile<F, T, KB, NST>::NWAVE)) void k_i8_tile
 #pragma unroll
     for (int i = 0; i < C::LX; i++) {
         const int r = 8 * (C::LX * wave + i) + lane / 8, c = swz(r, lane & 7), s = src_of(r);
-        xo[i] = s < 0 ? I8_OOB : (uint32_t)s * K + 16u * (uint32_t)c;
-        xl[i] = (nblk - 1) * 128 + 16 * c < a.K ? xo[i] : I8_OOB;
+        xo[i] = s < 0 ? BUF_OOB : (uint32_t)s * K + 16u * (uint32_t)c;
+        xl[i] = (nblk - 1) * 128 + 16 * c < a.K ? xo[i] : BUF_OOB;
     }
     if (GROUPED && t.bad) {
         if (threadIdx.x == 0) atomicOr(a.status, ST_BAD_DESCRIPTOR);
@@ -455,15 +340,15 @@ __global__ __launch_bounds__((64 * I8Tile<F, T, KB, NST>::NWAVE)) void k_i8_tile
     auto issue = [&](int st, int slot, int i) {
         constexpr int LB = C::LW + C::LX;
         const int in = st * KB + i / LB, k = i % LB;
-        const uint32_t oob = in < nblk ? 0u : I8_OOB;
+        const uint32_t oob = in < nblk ? 0u : BUF_OOB;
         int blk = min(in, nblk - 1);
         if (GROUPED) blk = blk + rot < nblk ? blk + rot : blk + rot - nblk;
         const int so = blk * 128;
         uint8_t *buf = lds + slot * C::STAGE + i / LB * C::SUB;
-        if (k < C::LW) i8_dma16(rw, wo[min(k, C::LW - 1)] | oob, so, buf + 1024 * (C::LW * wave + k));
+        if (k < C::LW) buf_dma16(rw, wo[min(k, C::LW - 1)] | oob, so, buf + 1024 * (C::LW * wave + k));
         else {
             const int j = max(0, min(k - C::LW, C::LX - 1));
-            i8_dma16(rx, (blk < nblk - 1 ? xo[j] : xl[j]) | oob, so, buf + C::OFF_X + 1024 * (C::LX * wave + j));
+            buf_dma16(rx, (blk < nblk - 1 ? xo[j] : xl[j]) | oob, so, buf + C::OFF_X + 1024 * (C::LX * wave + j));
         }
     };
 #pragma unroll
@@ -510,7 +395,7 @@ __global__ __launch_bounds__((64 * I8Tile<F, T, KB, NST>::NWAVE)) void k_i8_tile
             __builtin_amdgcn_sched_barrier(0);
         }
     };
-    i8_wait_vm<(C::NST - 1) * C::VM>();
+    wait_vm<(C::NST - 1) * C::VM>();
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
     Op o0, o1;
@@ -519,7 +404,7 @@ __global__ __launch_bounds__((64 * I8Tile<F, T, KB, NST>::NWAVE)) void k_i8_tile
      * Zipf, 492 -> 483 us) */
     if (GROUPED && C::WT > 1 && 16 * U * wt >= t.rows) {
         for (; st < nst; st++) {
-            i8_wait_vm<(C::NST - 2) * C::VM>();
+            wait_vm<(C::NST - 2) * C::VM>();
             __builtin_amdgcn_s_barrier();
             asm volatile("" ::: "memory");
 #pragma unroll
@@ -541,7 +426,7 @@ __global__ __launch_bounds__((64 * I8Tile<F, T, KB, NST>::NWAVE)) void k_i8_tile
         }
         half(o0, o1, buf + (KB - 1) * C::SUB, 1, false, 0, 0);
         __builtin_amdgcn_s_waitcnt(0xC07F);        /* this stage's operands are in registers */
-        i8_wait_vm<(C::NST - 2) * C::VM>();        /* the wave's loads of the next have landed */
+        wait_vm<(C::NST - 2) * C::VM>();        /* the wave's loads of the next have landed */
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
         const int free = slot;
@@ -550,21 +435,10 @@ __global__ __launch_bounds__((64 * I8Tile<F, T, KB, NST>::NWAVE)) void k_i8_tile
     }
     /* the loads past the end, then the ring becomes the output tile */
     __builtin_amdgcn_s_waitcnt(0xC07F);
-    i8_wait_vm<0>();
+    wait_vm<0>();
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
     i8_leave<F, GROUPED, OUT, 64 * C::NWAVE>(a, t, n0, nf, lds, acc, 16 * WI * wr, 16 * U * wt, src_of);
-}
-
-/* more than 64 KB of LDS has to be asked for, once on each device */
-static hipError_t allow_lds(const void *kernel, int bytes, uint64_t &done)
-{
-    int d = 0;
-    hipError_t e = hipGetDevice(&d);
-    if (e != hipSuccess || (d < 64 && (done >> d & 1))) return e;
-    e = hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
-    if (e == hipSuccess && d < 64) done |= 1ull << d;
-    return e;
 }
 
 template <int F, int T, int KB, int NST, bool GROUPED, int OUT>
