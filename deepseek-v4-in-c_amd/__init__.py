@@ -25,6 +25,8 @@ AMD_SO = os.path.join(LIB_DIR, "libdsv4_amd.so")
 DSV4_WF32, DSV4_WBF16, DSV4_WFP8, DSV4_WFP4, DSV4_WFP8_F32S, DSV4_WI8 = 0, 1, 2, 3, 4, 5
 # element types of activations
 DSV4_HIP_F32, DSV4_HIP_BF16, DSV4_HIP_F16 = 0, 1, 2
+# scores of the router with groups
+DSV4_HIP_SQRT_SOFTPLUS, DSV4_HIP_SOFTMAX, DSV4_HIP_SIGMOID = 0, 1, 2
 
 # every symbol include/*.h declares
 EXPORTS = (
@@ -46,6 +48,9 @@ EXPORTS = (
     "dsv4_hip_quant_i8_dev", "dsv4_hip_swiglu_quant_i8_dev", "dsv4_hip_gemm_i8_dev",
     "dsv4_hip_gemm_i8_grouped_dev", "dsv4_hip_moe_permute_dev", "dsv4_hip_moe_permute_bwd_dev",
     "dsv4_hip_moe_unpermute_dev", "dsv4_hip_moe_unpermute_bwd_dev",
+    "dsv4_hip_quant_mxfp4_dev", "dsv4_hip_swiglu_quant_mxfp4_dev", "dsv4_hip_quant_mxfp4_t_dev",
+    "dsv4_hip_gemm_mxfp4q_dev", "dsv4_hip_gemm_mxfp4q_grouped_dev", "dsv4_hip_route_groups_dev",
+    "dsv4_hip_route_groups_bwd_dev",
 )
 # the reference-named C mirror (host/dsv4_compute_hip.c)
 MIRROR_EXPORTS = ("dsv4_mmq_n", "dsv4_mmq", "dsv4_expert_forward")
@@ -66,6 +71,12 @@ class HipJob(C.Structure):
 class ExpertW(C.Structure):
     """DSV4ExpertW (src/00_base/dsv4_weights.h:103-106)."""
     _fields_ = [("w1", QMat), ("w3", QMat), ("w2", QMat)]
+
+
+class Router(C.Structure):
+    """DSV4HipRouter."""
+    _fields_ = [("score", C.c_int), ("n_experts", C.c_int), ("topk", C.c_int), ("n_group", C.c_int),
+                ("topk_group", C.c_int), ("group_top", C.c_int), ("renorm", C.c_int), ("scale", C.c_float)]
 
 
 _P, _I, _F = C.c_void_p, C.c_int, C.c_float
@@ -173,6 +184,13 @@ class Lib:
                 ("dsv4_hip_swiglu_quant_i8_dev", [_P, _P, _P, _P, _I, C.c_int64, _I, _I, _F, _P]),
                 ("dsv4_hip_gemm_i8_dev", [_P, _I, _P, _P, _I, C.POINTER(QMat), _P]),
                 ("dsv4_hip_gemm_i8_grouped_dev", [_P, _I, _P, _P, _I, _P, _I, _P, _P, _I, _I, _I, _P]),
+                ("dsv4_hip_quant_mxfp4_dev", [_P, _P, _P, _I, C.c_int64, _I, _I, _P]),
+                ("dsv4_hip_swiglu_quant_mxfp4_dev", [_P, _P, _P, _P, _I, C.c_int64, _I, _I, _F, _P]),
+                ("dsv4_hip_quant_mxfp4_t_dev", [_P, _P, _P, _I, C.c_int64, _I, _I, _P]),
+                ("dsv4_hip_gemm_mxfp4q_dev", [_P, _I, _P, _P, _I, C.POINTER(QMat), _P]),
+                ("dsv4_hip_gemm_mxfp4q_grouped_dev", [_P, _I, _P, _P, _I, _P, _I, _P, _P, _I, _I, _I, _P]),
+                ("dsv4_hip_route_groups_dev", [_P, _P, _P, _P, _I, _I, _P, C.POINTER(Router), _P]),
+                ("dsv4_hip_route_groups_bwd_dev", [_P, _P, _P, _P, _I, _P, _I, C.POINTER(Router), _P]),
                 ("dsv4_hip_moe_permute_dev", [_P, _P, _P, _P, _P, _I, _P, _I, _I, _I, _I, _P]),
                 ("dsv4_hip_moe_permute_bwd_dev", [_P, _P, _I, _P, _I, _I, _I, _P]),
                 ("dsv4_hip_moe_unpermute_dev", [_P, _P, _I, _P, _P, _P, _I, _I, _I, _P]),
@@ -417,6 +435,39 @@ class Lib:
         self.check(self.lib.dsv4_hip_gemm_i8_grouped_dev(c_ptr, out_type, aq_ptr, sa_ptr, n_a, row_tok_ptr, n_rows,
                                                          ex_off_ptr, table_ptr, n_experts, n, k, stream),
                    "dsv4_hip_gemm_i8_grouped_dev")
+
+    def quant_mxfp4_dev(self, q_ptr, s_ptr, a_ptr, type_, ld, n, k, stream=None):
+        self.check(self.lib.dsv4_hip_quant_mxfp4_dev(q_ptr, s_ptr, a_ptr, type_, ld, n, k, stream), "quant_mxfp4_dev")
+
+    def swiglu_quant_mxfp4_dev(self, q_ptr, s_ptr, g_ptr, u_ptr, type_, ld, n, k, limit, stream=None):
+        self.check(self.lib.dsv4_hip_swiglu_quant_mxfp4_dev(q_ptr, s_ptr, g_ptr, u_ptr, type_, ld, n, k, limit, stream),
+                   "swiglu_quant_mxfp4_dev")
+
+    def quant_mxfp4_t_dev(self, q_ptr, s_ptr, a_ptr, type_, ld, n, k, stream=None):
+        """The columns of a: q_ptr [k][ceil32(n) / 2], s_ptr [k][ceil32(n) / 32]."""
+        self.check(self.lib.dsv4_hip_quant_mxfp4_t_dev(q_ptr, s_ptr, a_ptr, type_, ld, n, k, stream), "quant_mxfp4_t_dev")
+
+    def gemm_mxfp4q_dev(self, c_ptr, out_type, aq_ptr, as_ptr, m, desc: QMat, stream=None):
+        self.check(self.lib.dsv4_hip_gemm_mxfp4q_dev(c_ptr, out_type, aq_ptr, as_ptr, m, C.byref(desc), stream),
+                   "dsv4_hip_gemm_mxfp4q_dev")
+
+    def gemm_mxfp4q_grouped_dev(self, c_ptr, out_type, aq_ptr, as_ptr, n_a, row_tok_ptr, n_rows, ex_off_ptr, table_ptr,
+                                n_experts, n, k, stream=None):
+        """table_ptr: a device array of n_experts QMat (DSV4_WFP4, n x k, 1 x 32 blocks)."""
+        self.check(self.lib.dsv4_hip_gemm_mxfp4q_grouped_dev(c_ptr, out_type, aq_ptr, as_ptr, n_a, row_tok_ptr, n_rows,
+                                                             ex_off_ptr, table_ptr, n_experts, n, k, stream),
+                   "dsv4_hip_gemm_mxfp4q_grouped_dev")
+
+    def route_groups_dev(self, idx_ptr, w_ptr, scores_ptr, logits_ptr, type_, n, bias_ptr, router: Router, stream=None):
+        self.check(self.lib.dsv4_hip_route_groups_dev(idx_ptr, w_ptr, scores_ptr, logits_ptr, type_, n, bias_ptr,
+                                                      C.byref(router), stream),
+                   "dsv4_hip_route_groups_dev")
+
+    def route_groups_bwd_dev(self, dlogits_ptr, dw_ptr, dscores_ptr, logits_ptr, type_, idx_ptr, n, router: Router,
+                             stream=None):
+        self.check(self.lib.dsv4_hip_route_groups_bwd_dev(dlogits_ptr, dw_ptr, dscores_ptr, logits_ptr, type_, idx_ptr, n,
+                                                          C.byref(router), stream),
+                   "dsv4_hip_route_groups_bwd_dev")
 
     def moe_permute_dev(self, rows_ptr, ex_off_ptr, row_tok_ptr, pos_ptr, x_ptr, type_, idx_ptr, n, topk, n_experts,
                         hidden, stream=None):

@@ -320,6 +320,58 @@ inline long i8_waves(I8Form form, long M, long N, long ne)
     return (ne ? M / TR + (M < ne ? M : ne) : ceil_div(M, TR)) * ceil_div(N, F) * waves;
 }
 
+/* ------------------------------------------------ 4-bit products -------- */
+
+/* Forms of the product of 4-bit rows. FP4_PAIR: weights as whole lines straight
+ * to registers, one matrix in workgroups of 8 weight rows x 8 tokens, experts in
+ * 32 x 16. FP4_SPLIT: 32 x 32 results a workgroup, K over its waves. The others
+ * by their tiles, features x rows, through a ring in LDS. */
+enum Fp4Form { FP4_PAIR = 1, FP4_SPLIT, FP4_64x64, FP4_128x128, FP4_256x128, FP4_256x256 };
+struct Fp4Shape { int F, TR, waves; };
+inline Fp4Shape fp4_shape(Fp4Form form, bool grouped)
+{
+    switch (form) {
+    case FP4_PAIR: return grouped ? Fp4Shape{32, 16, 4} : Fp4Shape{8, 8, 8};
+    case FP4_SPLIT: return {32, 32, 8};
+    case FP4_64x64: return {64, 64, 4};
+    case FP4_128x128: return {128, 128, 4};
+    case FP4_256x128: return {256, 128, 8};
+    default: return {256, 256, 8};
+    }
+}
+
+inline Fp4Form fp4_form(int M, int N, int K)
+{
+    (void)K;
+    if (M <= 8 && N <= 1 << 20) return FP4_PAIR;
+    if (ceil_div(M, 64) * ceil_div(N, 64) < CUS) return FP4_SPLIT;
+    if (ceil_div(M, 128) * ceil_div(N, 128) < CUS) return FP4_64x64;
+    if (ceil_div(M, 256) * ceil_div(N, 128) < CUS) return FP4_128x128;
+    if (ceil_div(M, 256) * ceil_div(N, 256) < CUS) return FP4_256x128;
+    return FP4_256x256;
+}
+
+/* Buckets of ne experts, M rows in all; the mean bucket decides. */
+inline Fp4Form fp4_grouped_form(int M, int N, int K, int ne)
+{
+    (void)N; (void)K;
+    const long hit = M < ne ? M : ne;
+    if (M <= 10 * hit) return FP4_PAIR;
+    if (M <= 24 * hit) return FP4_SPLIT;
+    if (M <= 48 * hit) return FP4_64x64;
+    return M <= 96 * hit ? FP4_128x128 : FP4_256x128;
+}
+
+/* Waves of the launch that multiplies M rows by N features in a form: tiles
+ * of its features and rows, and with ne experts one more row tile for each that
+ * may end inside one. A launch takes 2^32 threads. */
+constexpr long FP4_MAX_WAVES = (1L << 26) - 1;
+inline long fp4_waves(Fp4Form form, long M, long N, long ne)
+{
+    const Fp4Shape s = fp4_shape(form, ne != 0);
+    return (ne ? M / s.TR + (M < ne ? M : ne) : ceil_div(M, s.TR)) * ceil_div(N, s.F) * s.waves;
+}
+
 } // namespace dsv4
 
 #endif /* DSV4_CHOOSE_H */

@@ -1,0 +1,642 @@
+/* SPDX-License-Identifier: Apache-2.0 */
+/* dsv4_gemm_fp4.hip - products of 4-bit rows, both operands e2m1 codes with one
+ * E8M0 scale for 32 values along the sum:
+ *   C[m][n] = sum_b 2^(sa[m][b] - 127) 2^(sw[n][b] - 127) sum_{k in b} a[m][k] w[n][k]
+ * and the same for every expert's bucket of rows (its own matrix, rows taken
+ * from the tokens through row_tok).
+ *
+ * The matrix instructions take codes and scale bytes as they are stored: no
+ * value is decoded, the sum stays in their fp32 accumulators, each result is
+ * rounded once more for a 16-bit output. A scale byte of 255 is NaN, and so is
+ * every result that it meets. Products of codes are multiples of 1/4 up to 36,
+ * so within a block, and over blocks of like scales, sums are exact; the whole
+ * is nearer to the exact sum than fp32 additions one after the other (4,096
+ * values, scales over 18 powers of two: relative L2 1.3e-7 against 4.9e-7).
+ *
+ * v_mfma_scale_f32_16x16x128_f8f6f4: lane l holds the 32 codes (16 bytes, low
+ * nibble first) of row l % 16, block l / 16, and their scale in the byte of a
+ * register that the instruction names; element e of lane l of the result is row
+ * 4 (l / 16) + e of A, row l % 16 of B. v_mfma_scale_f32_32x32x64_f8f6f4: row l %
+ * 32, block l / 32; element e is row 8 (e / 4) + 4 (l / 32) + e % 4 of A, row l %
+ * 32 of B. Weight rows are the A operand, tokens the B operand. Registers alone
+ * reach 5.3 PFLOP/s with the first and 6.8 with the second (10 nominal).
+ *
+ * Codes past a row's end (K no multiple of a load's) come as zeros for the
+ * tokens, and scales there as finite ones, so whatever the weights' side reads
+ * adds nothing.
+ */
+#include "dsv4_bucket.h"
+#include "dsv4_elem.h"
+
+namespace dsv4 {
+
+namespace {
+
+typedef int v8i __attribute__((ext_vector_type(8)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef u32x4 u32x4_any __attribute__((aligned(1)));
+template <int N> struct IC { static constexpr int value = N; };
+
+using Fp4Bucket = Bucket<uint8_t>;
+
+/* whether a table's entry is an FP4 N x K matrix */
+__device__ __forceinline__ auto fp4_matrix(const Fp4Args &a)
+{
+    return [&a](const DSV4QMat &m) {
+        return m.wdt == DSV4_WFP4 && m.rows == a.N && m.cols == a.K && m.blk_r == 1 && m.blk_c == 32 && m.w && m.s &&
+               !((uintptr_t)m.w & 15u);
+    };
+}
+
+/* 16 scale bytes of a row from block b on (nb blocks a row); blocks past the
+ * row's end 0. Rows of scales have any alignment. */
+__device__ __forceinline__ u32x4 fp4_scales(const uint8_t *row, int b, int nb)
+{
+    if (b + 16 <= nb) return *(const DSV4_GLOBAL u32x4_any *)(row + b);
+    u32x4 v = {0, 0, 0, 0};
+    for (int i = 0; i < nb - b; i++) {
+        const uint32_t s = gptr(row)[b + i] << (8 * (i & 3));
+#pragma unroll
+        for (int j = 0; j < 4; j++) v[j] |= i / 4 == j ? s : 0u;
+    }
+    return v;
+}
+
+__device__ __forceinline__ v8i fp4_operand(const v4i &v)
+{
+    return __builtin_shufflevector(v, v, 0, 1, 2, 3, -1, -1, -1, -1);
+}
+/* B: which byte of the scale registers */
+template <int B>
+__device__ __forceinline__ f32x4 fp4_mfma16(const v4i &w, const v4i &x, f32x4 c, uint32_t sw, uint32_t sx)
+{
+    return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(fp4_operand(w), fp4_operand(x), c, 4, 4, B, (int)sw, B, (int)sx);
+}
+template <int B>
+__device__ __forceinline__ f32x16 fp4_mfma32(const v4i &w, const v4i &x, f32x16 c, uint32_t sw, uint32_t sx)
+{
+    return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(fp4_operand(w), fp4_operand(x), c, 4, 4, B, (int)sw, B, (int)sx);
+}
+
+/* one result: element i of C */
+template <int OUT>
+__device__ __forceinline__ void fp4_store(void *C, size_t i, float v)
+{
+    if constexpr (OUT == DSV4_HIP_F32) ((float *)C)[i] = v;
+    else ((uint16_t *)C)[i] = (uint16_t)narrow16<OUT>(v);
+}
+
+/* rows of an expert whose table entry is no matrix of the product */
+template <int OUT>
+__device__ __forceinline__ void fp4_bad(const Fp4Args &a, const Fp4Bucket &t, int n0, int nf, int threads)
+{
+    if (threadIdx.x == 0) atomicOr(a.status, ST_BAD_DESCRIPTOR);
+    for (int i = threadIdx.x; i < t.rows * nf; i += threads)
+        fp4_store<OUT>(a.C, (size_t)(t.r0 + i / nf) * a.N + n0 + i % nf, __builtin_nanf(""));
+}
+
+/* the row of Aq that row i of the tile multiplies (from the tile's first on for
+ * one matrix); -1: none */
+template <bool GROUPED>
+__device__ __forceinline__ int fp4_source(const Fp4Args &a, const Fp4Bucket &t, int i)
+{
+    if (i >= t.rows) return -1;
+    if (!GROUPED) return i;
+    const int s = a.row_tok ? a.row_tok[t.r0 + i] : t.r0 + i;
+    return (unsigned)s < (unsigned)a.n_a ? s : -1;
+}
+
+} // namespace
+
+/* ------------------------------------------------------- few rows -------
+ * Weights as whole 128-byte lines: an instruction takes 256 codes of 8 weight
+ * rows, lane l (row l % 8) block 4 (l / 8 % 2) + l / 16 of the line's eight. Rows
+ * 0 - 7 of the MFMA's A operand are then the 8 weight rows at the line's first
+ * four blocks, rows 8 - 15 the same rows at its last four; the B operand holds 8
+ * tokens the same way, and of the 16 x 16 result the two quadrants that multiply
+ * equal blocks count. A workgroup takes 8 RT weight rows by 8 TT tokens, its
+ * waves share out K in lines, B of them in flight, and add up in LDS, in wave
+ * order. */
+template <int RT, int TT, int NW, int B, bool GROUPED, int OUT>
+__global__ __launch_bounds__(64 * NW) void k_fp4_pair(Fp4Args a)
+{
+    constexpr int TR = 8 * TT, FR = 8 * RT;
+    __shared__ float sum[NW][2][TT * RT][64];
+    const int lane = threadIdx.x & 63, wave = wave_in_group();
+    const int r8 = lane & 7, half = (lane >> 3) & 1, g = lane >> 4;
+    const int slabs = (a.N + FR - 1) / FR, tile = blockIdx.x / slabs, n0 = (blockIdx.x - tile * slabs) * FR;
+    Fp4Bucket t;
+    if constexpr (GROUPED) {
+        t = bucket_tile<TR, uint8_t>(a, tile, lane, fp4_matrix(a));
+        if (t.rows <= 0) return;
+    } else {
+        t.w = a.W; t.s = a.Sw; t.e = 0; t.bad = false;
+        t.r0 = tile * TR;
+        t.rows = min(TR, a.M - t.r0);
+    }
+    const int nf = min(FR, a.N - n0);
+    if (GROUPED && t.bad) {
+        fp4_bad<OUT>(a, t, n0, nf, 64 * NW);
+        return;
+    }
+    const uint32_t KB = (uint32_t)a.K / 2, nb = (uint32_t)a.K / 32;   /* a row's bytes, its scales */
+    const __amdgpu_buffer_rsrc_t rw = buf_rsrc(t.w + (size_t)n0 * KB, (uint32_t)nf * KB);
+    const __amdgpu_buffer_rsrc_t rsw = buf_rsrc(t.s + (size_t)n0 * nb, (uint32_t)nf * nb);
+    const size_t x0 = GROUPED ? 0 : (size_t)t.r0;
+    const uint32_t xr = GROUPED ? (uint32_t)a.n_a : (uint32_t)t.rows;
+    const __amdgpu_buffer_rsrc_t rx = buf_rsrc(a.Aq + x0 * KB, xr * KB), rsx = buf_rsrc(a.As + x0 * nb, xr * nb);
+    const uint32_t blk = 4u * half + g;
+    uint32_t xo[TT], xs[TT], wo[RT], ws[RT];
+#pragma unroll
+    for (int u = 0; u < TT; u++) {
+        const int s = fp4_source<GROUPED>(a, t, 8 * u + r8);
+        xo[u] = s < 0 ? BUF_OOB : (uint32_t)s * KB + 16u * blk;
+        xs[u] = s < 0 ? BUF_OOB : (uint32_t)s * nb + blk;
+    }
+#pragma unroll
+    for (int i = 0; i < RT; i++) {
+        wo[i] = (uint32_t)(8 * i + r8) * KB + 16u * blk;
+        ws[i] = (uint32_t)(8 * i + r8) * nb + blk;
+    }
+    const int lines = (a.K + 255) / 256;
+    f32x4 acc[RT][TT];
+#pragma unroll
+    for (int i = 0; i < RT; i++)
+#pragma unroll
+        for (int u = 0; u < TT; u++) acc[i][u] = f32x4{0, 0, 0, 0};
+    for (int l0 = wave; l0 < lines; l0 += NW * B) {
+        v4i w[B][RT], x[B][TT];
+        uint32_t sw[B][RT], sx[B][TT];
+#pragma unroll
+        for (int b = 0; b < B; b++) {
+            const uint32_t l = (uint32_t)(l0 + NW * b);
+            const bool in = 8 * l + blk < nb;
+#pragma unroll
+            for (int i = 0; i < RT; i++) {
+                w[b][i] = buf_ld16<2>(rw, in ? wo[i] + 128u * l : BUF_OOB);
+                sw[b][i] = __builtin_amdgcn_raw_buffer_load_b8(rsw, (int)(in ? ws[i] + 8u * l : BUF_OOB), 0, 0);
+            }
+#pragma unroll
+            for (int u = 0; u < TT; u++) {
+                const bool ok = in && xo[u] != BUF_OOB;
+                x[b][u] = buf_ld16<0>(rx, ok ? xo[u] + 128u * l : BUF_OOB);
+                sx[b][u] = __builtin_amdgcn_raw_buffer_load_b8(rsx, (int)(ok ? xs[u] + 8u * l : BUF_OOB), 0, 0);
+            }
+        }
+#pragma unroll
+        for (int b = 0; b < B; b++)
+#pragma unroll
+            for (int i = 0; i < RT; i++)
+#pragma unroll
+                for (int u = 0; u < TT; u++) acc[i][u] = fp4_mfma16<0>(w[b][i], x[b][u], acc[i][u], sw[b][i], sx[b][u]);
+    }
+    /* element e of lane l: weight row 4 (g % 2) + e at half g / 2, token l % 8
+     * at half l / 8 % 2 */
+    if (half == g >> 1) {
+#pragma unroll
+        for (int i = 0; i < RT; i++)
+#pragma unroll
+            for (int u = 0; u < TT; u++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) sum[wave][half][i * TT + u][r8 * 8 + 4 * (g & 1) + e] = acc[i][u][e];
+    }
+    __syncthreads();
+    for (int o = threadIdx.x; o < TR * FR; o += 64 * NW) {
+        const int n = o % FR, i = o / FR;
+        if (i >= t.rows || n >= nf) continue;
+        float v = 0.0f;
+#pragma unroll
+        for (int w = 0; w < NW; w++)
+#pragma unroll
+            for (int h = 0; h < 2; h++) v += sum[w][h][(n / 8) * TT + i / 8][(i & 7) * 8 + (n & 7)];
+        if (GROUPED && fp4_source<GROUPED>(a, t, i) < 0) {
+            v = __builtin_nanf("");
+            if (n == 0) atomicOr(a.status, ST_BAD_EXPERT_ID);
+        }
+        fp4_store<OUT>(a.C, (size_t)(t.r0 + i) * a.N + n0 + n, v);
+    }
+}
+
+template <int RT, int TT, int NW, int B, bool GROUPED, int OUT>
+static hipError_t fp4_pair(const Fp4Args &a, Fp4Form form, hipStream_t st)
+{
+    const long groups = fp4_waves(form, a.M, a.N, GROUPED ? a.n_experts : 0) / NW;
+    hipLaunchKernelGGL((k_fp4_pair<RT, TT, NW, B, GROUPED, OUT>), dim3((unsigned)groups), dim3(64 * NW), 0, st, a);
+    return hipGetLastError();
+}
+
+/* --------------------------------------------------- K over the waves ---
+ * A workgroup takes 16 FA features by 16 TB rows, and its NW waves share out K in
+ * pieces of 512 values: operands go straight to registers, a whole piece's
+ * loads before its first product, and the sums meet in LDS, added in wave
+ * order. No wave waits for another before the end, so a product too small to
+ * fill the device costs one latency of its loads, not one a stage. */
+template <int FA, int TB, int NW, bool GROUPED, int OUT>
+__global__ __launch_bounds__(64 * NW) void k_fp4_split(Fp4Args a)
+{
+    constexpr int F = 16 * FA, TR = 16 * TB;
+    __shared__ float sum[NW][F * TR];
+    const int lane = threadIdx.x & 63, wave = wave_in_group(), r16 = lane & 15, g = lane >> 4;
+    const int nt = (a.N + F - 1) / F, tile = blockIdx.x / nt, n0 = (blockIdx.x - tile * nt) * F;
+    Fp4Bucket t;
+    if constexpr (GROUPED) {
+        t = bucket_tile<TR, uint8_t>(a, tile, lane, fp4_matrix(a));
+        if (t.rows <= 0) return;
+    } else {
+        t.w = a.W; t.s = a.Sw; t.e = 0; t.bad = false;
+        t.r0 = tile * TR;
+        t.rows = min(TR, a.M - t.r0);
+    }
+    const int nf = min(F, a.N - n0);
+    if (GROUPED && t.bad) {
+        fp4_bad<OUT>(a, t, n0, nf, 64 * NW);
+        return;
+    }
+    const uint32_t KB = (uint32_t)a.K / 2;
+    const int nb = a.K / 32;
+    const __amdgpu_buffer_rsrc_t rw = buf_rsrc(t.w + (size_t)n0 * KB, (uint32_t)nf * KB);
+    const size_t x0 = GROUPED ? 0 : (size_t)t.r0;
+    const __amdgpu_buffer_rsrc_t rx = buf_rsrc(a.Aq + x0 * KB, (GROUPED ? (uint32_t)a.n_a : (uint32_t)t.rows) * KB);
+    uint32_t wo[FA], xo[TB];
+    const uint8_t *ws[FA], *xs[TB];
+#pragma unroll
+    for (int i = 0; i < FA; i++) {
+        const int r = min(16 * i + r16, nf - 1);   /* rows past the last: the last again, not stored */
+        wo[i] = (uint32_t)r * KB + 16u * g;
+        ws[i] = t.s + (size_t)(n0 + r) * nb;
+    }
+#pragma unroll
+    for (int u = 0; u < TB; u++) {
+        const int s = fp4_source<GROUPED>(a, t, 16 * u + r16);
+        xo[u] = s < 0 ? BUF_OOB : (uint32_t)s * KB + 16u * g;
+        xs[u] = s < 0 ? nullptr : a.As + (x0 + s) * (size_t)nb;
+    }
+    f32x4 acc[FA][TB];
+#pragma unroll
+    for (int i = 0; i < FA; i++)
+#pragma unroll
+        for (int u = 0; u < TB; u++) acc[i][u] = f32x4{0, 0, 0, 0};
+    for (int p = wave; 16 * p < nb; p += NW) {
+        v4i w[4][FA], x[4][TB];
+        u32x4 sw[FA], sx[TB];
+#pragma unroll
+        for (int s = 0; s < 4; s++) {
+            const uint32_t at = 256u * p + 64u * s;
+            const bool in = 16 * p + 4 * s + g < nb;
+#pragma unroll
+            for (int i = 0; i < FA; i++) w[s][i] = buf_ld16<0>(rw, in ? wo[i] + at : BUF_OOB);
+#pragma unroll
+            for (int u = 0; u < TB; u++) x[s][u] = buf_ld16<0>(rx, in && xo[u] != BUF_OOB ? xo[u] + at : BUF_OOB);
+        }
+#pragma unroll
+        for (int i = 0; i < FA; i++) sw[i] = fp4_scales(ws[i], 16 * p, nb);
+#pragma unroll
+        for (int u = 0; u < TB; u++) sx[u] = xs[u] ? fp4_scales(xs[u], 16 * p, nb) : u32x4{0, 0, 0, 0};
+#pragma unroll
+        for (int s = 0; s < 4; s++)
+#pragma unroll
+            for (int i = 0; i < FA; i++)
+#pragma unroll
+                for (int u = 0; u < TB; u++)
+                    acc[i][u] = fp4_mfma16<0>(w[s][i], x[s][u], acc[i][u], sw[i][s] >> (8 * g), sx[u][s] >> (8 * g));
+    }
+#pragma unroll
+    for (int i = 0; i < FA; i++)
+#pragma unroll
+        for (int u = 0; u < TB; u++) *(f32x4 *)&sum[wave][(16 * u + r16) * F + 16 * i + 4 * g] = acc[i][u];
+    __syncthreads();
+    for (int o = threadIdx.x; o < TR * F; o += 64 * NW) {
+        const int n = o % F, i = o / F;
+        if (i >= t.rows || n >= nf) continue;
+        float v = 0.0f;
+#pragma unroll
+        for (int w = 0; w < NW; w++) v += sum[w][o];
+        if (GROUPED && fp4_source<GROUPED>(a, t, i) < 0) {
+            v = __builtin_nanf("");
+            if (n == 0) atomicOr(a.status, ST_BAD_EXPERT_ID);
+        }
+        fp4_store<OUT>(a.C, (size_t)(t.r0 + i) * a.N + n0 + n, v);
+    }
+}
+
+template <int FA, int TB, int NW, bool GROUPED, int OUT>
+static hipError_t fp4_split(const Fp4Args &a, Fp4Form form, hipStream_t st)
+{
+    const long groups = fp4_waves(form, a.M, a.N, GROUPED ? a.n_experts : 0) / NW;
+    hipLaunchKernelGGL((k_fp4_split<FA, TB, NW, GROUPED, OUT>), dim3((unsigned)groups), dim3(64 * NW), 0, st, a);
+    return hipGetLastError();
+}
+
+/* ------------------------------------------------------- many rows ------
+ * A workgroup takes F features by T rows, its WR x WT waves each F / WR by T / WT
+ * of them in 32 x 32 results. K goes in stages of 256 values, a staged row a
+ * 128-byte line: both operands by loads straight to LDS into a ring of NST
+ * stages (16-byte pieces XOR-swizzled by row), a wave reading the operands of
+ * the next 64 values while it multiplies these. The scales of two stages, 16
+ * bytes a row, go through a thread's registers (rows of scales have any
+ * alignment) into one of two LDS tables; a lane picks the four bytes of its
+ * block in each step with one permutation. One barrier a stage: after it every
+ * wave's loads of the next stage have landed and no wave still reads this one,
+ * so the stage NST ahead takes its place. The tile leaves through LDS as whole
+ * 16-byte pieces of rows. */
+template <int F, int T, int WR, int WT, int NST_> struct Fp4Tile {
+    static constexpr int NWAVE = WR * WT, NT = 64 * NWAVE, NST = NST_;
+    static constexpr int WI = F / WR / 32, U = T / WT / 32;
+    static constexpr int OFF_X = F * 128, STAGE = (F + T) * 128;
+    static constexpr int LW = F / 8 / NWAVE, LX = T / 8 / NWAVE, VM = LW + LX;
+    static constexpr int RING = NST * STAGE, TABLE = (F + T) * 16;
+    static constexpr int out_ld(int eb) { return F * eb + 16; }
+    /* tokens that leave together: all, or a row of waves after the other */
+    static constexpr int out_rows(int eb) { return T * out_ld(eb) <= 160 * 1024 ? T : T / WT; }
+    static constexpr int lds(int eb)
+    {
+        return RING + 2 * TABLE > out_rows(eb) * out_ld(eb) ? RING + 2 * TABLE : out_rows(eb) * out_ld(eb);
+    }
+    static_assert(LW * NWAVE * 8 == F && LX * NWAVE * 8 == T && F + T <= NT && (NST - 1) * VM < 64 &&
+                      lds(4) <= 160 * 1024 && WI >= 1 && U >= 1, "tile");
+};
+
+template <int F, int T, int WR, int WT, int NST, bool GROUPED, int OUT>
+__global__ __launch_bounds__((Fp4Tile<F, T, WR, WT, NST>::NT)) void k_fp4_tile(Fp4Args a)
+{
+    using C = Fp4Tile<F, T, WR, WT, NST>;
+    constexpr int U = C::U, WI = C::WI;
+    constexpr bool SHARED = GROUPED && F == 256;
+    extern __shared__ __align__(16) uint8_t lds[];
+    uint8_t *const table = lds + C::RING;
+    const int lane = threadIdx.x & 63, wave = wave_in_group();
+    const int rr = lane & 31, g = lane >> 5, wr = wave % WR, wt = wave / WR;
+    const int nt = (a.N + F - 1) / F, nb = a.K / 32;
+    Fp4Bucket t;
+    int n0;
+    if constexpr (GROUPED) {
+        int f = blockIdx.x % nt;
+        if constexpr (SHARED) t = bucket_tile<T, uint8_t>(a, blockIdx.x, lane, fp4_matrix(a), nt, &f);
+        else t = bucket_tile<T, uint8_t>(a, blockIdx.x / nt, lane, fp4_matrix(a));
+        n0 = f * F;
+        if (t.rows <= 0) return;
+    } else {
+        /* each XCD a contiguous run of tiles, eight row tiles by their feature
+         * tiles at a time */
+        const int mt = (a.M + T - 1) / T, total = mt * nt;
+        const int per = total / 8, rest = total % 8, x = blockIdx.x % 8, y = blockIdx.x / 8;
+        const int id = x * per + min(x, rest) + y;
+        const int grp = id / (8 * nt), gm = min(8, mt - 8 * grp), in = id - grp * 8 * nt;
+        t.w = a.W; t.s = a.Sw; t.e = 0; t.bad = false;
+        t.r0 = (8 * grp + in % gm) * T;
+        t.rows = min(T, a.M - t.r0);
+        n0 = in / gm * F;
+    }
+    const int nf = min(F, a.N - n0);
+    if (GROUPED && t.bad) {
+        fp4_bad<OUT>(a, t, n0, nf, C::NT);
+        return;
+    }
+    const uint32_t KB = (uint32_t)a.K / 2;
+    /* stages, whole pairs of them where they begin anywhere (rot) */
+    const int nst = GROUPED ? (a.K + 511) / 512 * 2 : (a.K + 255) / 256;
+    const __amdgpu_buffer_rsrc_t rw = buf_rsrc(t.w + (size_t)n0 * KB, (uint32_t)nf * KB);
+    const size_t x0 = GROUPED ? 0 : (size_t)t.r0;
+    const __amdgpu_buffer_rsrc_t rx = buf_rsrc(a.Aq + x0 * KB, (GROUPED ? (uint32_t)a.n_a : (uint32_t)t.rows) * KB);
+    auto swz = [](int r, int c) { return c ^ ((r >> 1) & 7); };
+    uint32_t wo[C::LW], xo[C::LX];
+    int xc[C::LX];                                 /* the lane's block of a stage */
+#pragma unroll
+    for (int i = 0; i < C::LW; i++) {
+        const int r = 8 * (C::LW * wave + i) + lane / 8;
+        wo[i] = (uint32_t)r * KB + 16u * (uint32_t)swz(r, lane & 7);
+    }
+#pragma unroll
+    for (int i = 0; i < C::LX; i++) {
+        const int r = 8 * (C::LX * wave + i) + lane / 8, s = fp4_source<GROUPED>(a, t, r);
+        xc[i] = swz(r, lane & 7);
+        xo[i] = s < 0 ? BUF_OOB : (uint32_t)s * KB + 16u * (uint32_t)xc[i];
+    }
+    /* the row whose scales this thread fetches; rows past the last weight row
+     * take the last one's, tokens that are not there zeros */
+    const uint8_t *srow = nullptr;
+    if ((int)threadIdx.x < F) {
+        srow = t.s + (size_t)(n0 + min((int)threadIdx.x, nf - 1)) * nb;
+    } else if ((int)threadIdx.x < F + T) {
+        const int s = fp4_source<GROUPED>(a, t, (int)threadIdx.x - F);
+        if (s >= 0) srow = a.As + (x0 + s) * (size_t)nb;
+    }
+    /* the stage this workgroup begins with: experts that run through K side by
+     * side would meet in the same memory channels */
+    const int rot = !GROUPED ? 0 : 2 * ((SHARED ? t.e * 4 + t.e / 8 : n0 / F * 2 + t.e) % (nst / 2));
+    auto block_of = [&](int st) { return st + rot < nst ? st + rot : st + rot - nst; };
+    auto fetch_scales = [&](int pair) -> u32x4 {   /* of stages 2 pair and 2 pair + 1 */
+        if (2 * pair >= nst || !srow) return u32x4{0, 0, 0, 0};
+        return fp4_scales(srow, 8 * block_of(2 * pair), nb);
+    };
+    auto put_scales = [&](int pair, const u32x4 &v) {
+        if ((int)threadIdx.x < F + T) *(u32x4 *)(table + (pair & 1) * C::TABLE + 16 * threadIdx.x) = v;
+    };
+    /* load i of a wave's share of stage st; past the end zeros, no traffic */
+    auto issue = [&](int st, int slot, int i) {
+        const int blk = block_of(min(st, nst - 1));
+        const uint32_t oob = st < nst ? 0u : BUF_OOB;
+        uint8_t *buf = lds + slot * C::STAGE;
+        if (i < C::LW) {
+            buf_dma16(rw, (wo[min(i, C::LW - 1)] + 128u * blk) | oob, 0, buf + 1024 * (C::LW * wave + i));
+        } else {
+            const int j = max(0, min(i - C::LW, C::LX - 1));
+            buf_dma16(rx, 8 * blk + xc[j] < nb && xo[j] != BUF_OOB ? (xo[j] + 128u * blk) | oob : BUF_OOB, 0,
+                      buf + C::OFF_X + 1024 * (C::LX * wave + j));
+        }
+    };
+    const u32x4 first = fetch_scales(0);
+    u32x4 held = fetch_scales(1);
+#pragma unroll
+    for (int s = 0; s < NST; s++)
+#pragma unroll
+        for (int i = 0; i < C::VM; i++) issue(s, s, i);
+    put_scales(0, first);
+
+    struct Op { v4i w[WI], x[U]; };
+    struct Sc { uint32_t w[WI], x[U]; };
+    auto read_w = [&](Op &o, const uint8_t *buf, int i, int s) {
+        const int r = 32 * (WI * wr + i) + rr;
+        o.w[i] = *(const v4i *)(buf + r * 128 + 16 * swz(r, 2 * s + g));
+    };
+    auto read_x = [&](Op &o, const uint8_t *buf, int u, int s) {
+        const int r = 32 * (U * wt + u) + rr;
+        o.x[u] = *(const v4i *)(buf + C::OFF_X + r * 128 + 16 * swz(r, 2 * s + g));
+    };
+    const uint32_t pick = g ? 0x07050301u : 0x06040200u;
+    /* the scales of stage st: byte s of a row's register is step s's */
+    auto read_scales = [&](Sc &o, int st) {
+        const uint8_t *p = table + (st / 2 & 1) * C::TABLE + 8 * (st & 1);
+#pragma unroll
+        for (int i = 0; i < WI; i++) {
+            const u32x2 v = *(const u32x2 *)(p + 16 * (32 * (WI * wr + i) + rr));
+            o.w[i] = __builtin_amdgcn_perm(v.y, v.x, pick);
+        }
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            const u32x2 v = *(const u32x2 *)(p + 16 * (F + 32 * (U * wt + u) + rr));
+            o.x[u] = __builtin_amdgcn_perm(v.y, v.x, pick);
+        }
+    };
+    f32x16 acc[WI][U];
+#pragma unroll
+    for (int i = 0; i < WI; i++)
+#pragma unroll
+        for (int u = 0; u < U; u++)
+#pragma unroll
+            for (int e = 0; e < 16; e++) acc[i][u][e] = 0.0f;
+    int slot = 0;
+    /* the products of `cur` (step S), the reads of `nxt` (step s of the stage in
+     * buf) and, with `load`, stage st's loads into slot `to`, spread among them */
+    auto step = [&](auto S, const Op &cur, const Sc &sc, Op &nxt, const uint8_t *buf, int s, bool load, int st, int to) {
+#pragma unroll
+        for (int q = 0; q < WI * U; q++) {
+            constexpr int N = WI * U, R = WI + U;
+            acc[q % WI][q / WI] = fp4_mfma32<decltype(S)::value>(cur.w[q % WI], cur.x[q / WI], acc[q % WI][q / WI], sc.w[q % WI], sc.x[q / WI]);
+            if (N >= 8 && q == 0) __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int j = 0; j < R; j++)
+                if (j * N / (R + 1) == q) {
+                    if (j < WI) read_w(nxt, buf, j, s);
+                    else read_x(nxt, buf, j - WI, s);
+                }
+            if (load) {
+#pragma unroll
+                for (int l = 0; l < C::VM; l++)
+                    if (l * N / C::VM == q) issue(st, to, l);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    };
+    wait_vm<(NST - 1) * C::VM>();
+    __builtin_amdgcn_s_waitcnt(0xC07F);
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    Op o0, o1;
+    Sc sc;
+#pragma unroll
+    for (int i = 0; i < WI; i++) read_w(o0, lds, i, 0);
+#pragma unroll
+    for (int u = 0; u < U; u++) read_x(o0, lds, u, 0);
+    read_scales(sc, 0);
+    for (int st = 0; st < nst; st++) {
+        const uint8_t *buf = lds + slot * C::STAGE;
+        step(IC<0>{}, o0, sc, o1, buf, 1, false, 0, 0);
+        step(IC<1>{}, o1, sc, o0, buf, 2, false, 0, 0);
+        step(IC<2>{}, o0, sc, o1, buf, 3, false, 0, 0);
+        if (st & 1) put_scales(st / 2 + 1, held);
+        __builtin_amdgcn_s_waitcnt(0xC07F);        /* this stage's operands are in registers */
+        wait_vm<(NST - 2) * C::VM>();              /* the wave's loads of the next have landed */
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+        if (st & 1) held = fetch_scales(st / 2 + 2);
+        const int free = slot;
+        slot = slot + 1 == NST ? 0 : slot + 1;
+        Sc sn;
+        read_scales(sn, st + 1);
+        step(IC<3>{}, o1, sc, o0, lds + slot * C::STAGE, 0, true, st + NST, free);
+        sc = sn;
+    }
+    /* the loads past the end, then the ring becomes the output tile */
+    __builtin_amdgcn_s_waitcnt(0xC07F);
+    wait_vm<0>();
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+
+    constexpr int EB = elem_bytes<OUT>(), LD = C::out_ld(EB), ROWS = C::out_rows(EB), PMAX = F * EB / 16;
+    const int pieces = nf * EB / 16;
+    const size_t ld = (size_t)a.N * EB;
+    const bool whole = (((uintptr_t)a.C | ld) & 15u) == 0;   /* n0 and nf are whole pieces then too */
+    typedef u32x4 piece __attribute__((aligned(2)));
+#pragma unroll
+    for (int m0 = 0; m0 < T; m0 += ROWS) {
+        if (ROWS == T || m0 == wt * ROWS) {
+#pragma unroll
+            for (int u = 0; u < U; u++) {
+                const int m = 32 * (U * wt + u) + rr;
+                const bool none = GROUPED && m < t.rows && fp4_source<GROUPED>(a, t, m) < 0;
+                if (none && wr == 0 && g == 0) atomicOr(a.status, ST_BAD_EXPERT_ID);
+#pragma unroll
+                for (int i = 0; i < WI; i++)
+#pragma unroll
+                    for (int q = 0; q < 4; q++) {
+                        uint8_t *o = lds + (m - m0) * LD + (32 * (WI * wr + i) + 8 * q + 4 * g) * EB;
+                        float v[4];
+#pragma unroll
+                        for (int e = 0; e < 4; e++) v[e] = none ? __builtin_nanf("") : acc[i][u][4 * q + e];
+                        if constexpr (OUT == DSV4_HIP_F32) {
+                            *(f32x4 *)o = f32x4{v[0], v[1], v[2], v[3]};
+                        } else {
+                            u32x2 p;
+                            p.x = narrow16<OUT>(v[0]) | (narrow16<OUT>(v[1]) << 16);
+                            p.y = narrow16<OUT>(v[2]) | (narrow16<OUT>(v[3]) << 16);
+                            *(u32x2 *)o = p;
+                        }
+                    }
+            }
+        }
+        __syncthreads();
+        uint8_t *out = (uint8_t *)a.C + ((size_t)(t.r0 + m0) * a.N + n0) * EB;
+        const int rows = min(ROWS, t.rows - m0);
+        for (int i = threadIdx.x; i < rows * PMAX; i += C::NT) {
+            const int m = i / PMAX, p = i % PMAX;
+            const uint8_t *src = lds + m * LD + 16 * p;
+            uint8_t *dst = out + m * ld + 16 * p;
+            if (p < pieces) {
+                if (whole) __builtin_nontemporal_store(*(const u32x4 *)src, (DSV4_GLOBAL u32x4 *)dst);
+                else *(DSV4_GLOBAL piece *)dst = *(const u32x4 *)src;
+            } else {
+                for (int b = 0; b < nf * EB - 16 * p; b += EB) {
+                    if constexpr (EB == 4) *(DSV4_GLOBAL float *)(dst + b) = *(const float *)(src + b);
+                    else *(DSV4_GLOBAL uint16_t *)(dst + b) = *(const uint16_t *)(src + b);
+                }
+            }
+        }
+        if (m0 + ROWS < T) __syncthreads();
+    }
+}
+
+template <int F, int T, int WR, int WT, int NST, bool GROUPED, int OUT>
+static hipError_t fp4_tile(const Fp4Args &a, Fp4Form form, hipStream_t st)
+{
+    using C = Fp4Tile<F, T, WR, WT, NST>;
+    constexpr int lds = C::lds(elem_bytes<OUT>());
+    static uint64_t done = 0;
+    const hipError_t e = allow_lds((const void *)k_fp4_tile<F, T, WR, WT, NST, GROUPED, OUT>, lds, done);
+    if (e != hipSuccess) return e;
+    const long groups = fp4_waves(form, a.M, a.N, GROUPED ? a.n_experts : 0) / C::NWAVE;
+    hipLaunchKernelGGL((k_fp4_tile<F, T, WR, WT, NST, GROUPED, OUT>), dim3((unsigned)groups), dim3(C::NT), lds, st, a);
+    return hipGetLastError();
+}
+
+template <bool GROUPED, int OUT>
+static hipError_t fp4_launch(const Fp4Args &a, hipStream_t st)
+{
+    const Fp4Form form = GROUPED ? fp4_grouped_form(a.M, a.N, a.K, a.n_experts) : fp4_form(a.M, a.N, a.K);
+    if (fp4_waves(form, a.M, a.N, GROUPED ? a.n_experts : 0) > FP4_MAX_WAVES) return hipErrorInvalidConfiguration;
+    switch (form) {
+    case FP4_PAIR:
+        if constexpr (GROUPED) return fp4_pair<4, 2, 4, 2, GROUPED, OUT>(a, form, st);
+        else return fp4_pair<1, 1, 8, 4, GROUPED, OUT>(a, form, st);
+    case FP4_SPLIT: return fp4_split<2, 2, 8, GROUPED, OUT>(a, form, st);
+    case FP4_64x64: return fp4_tile<64, 64, 2, 2, 3, GROUPED, OUT>(a, form, st);
+    case FP4_128x128: return fp4_tile<128, 128, 2, 2, 2, GROUPED, OUT>(a, form, st);
+    case FP4_256x128: return fp4_tile<256, 128, 4, 2, 3, GROUPED, OUT>(a, form, st);
+    default: return fp4_tile<256, 256, 4, 2, 2, GROUPED, OUT>(a, form, st);
+    }
+}
+
+hipError_t gemm_fp4_launch(const Fp4Args &a, int out_type, hipStream_t st)
+{
+    if (a.M <= 0 || a.N <= 0 || a.K <= 0 || a.K % 32) return hipErrorInvalidValue;
+    const bool grouped = a.table != nullptr;
+    switch (out_type) {
+    case DSV4_HIP_F32: return grouped ? fp4_launch<true, DSV4_HIP_F32>(a, st) : fp4_launch<false, DSV4_HIP_F32>(a, st);
+    case DSV4_HIP_BF16: return grouped ? fp4_launch<true, DSV4_HIP_BF16>(a, st) : fp4_launch<false, DSV4_HIP_BF16>(a, st);
+    case DSV4_HIP_F16: return grouped ? fp4_launch<true, DSV4_HIP_F16>(a, st) : fp4_launch<false, DSV4_HIP_F16>(a, st);
+    default: return hipErrorInvalidValue;
+    }
+}
+
+} // namespace dsv4

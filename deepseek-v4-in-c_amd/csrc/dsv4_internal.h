@@ -561,6 +561,61 @@ struct I8Args {
 };
 hipError_t gemm_i8_launch(const I8Args &a, int out_type, hipStream_t st);
 
+/* ------------------------------------------------ 4-bit products ----- */
+
+/* Rows to e2m1 codes and E8M0 bytes: a (and with SWIGLU u, a being the gate)
+ * rows of k elements, `ld` elements apart; Q [n][k / 2], S [n][k / 32]. COLUMNS:
+ * the columns of a instead, Q [k][n' / 2], S [k][n' / 32] with n' = n rounded
+ * up to 32. */
+enum Mxfp4Rows { MXFP4_ROWS, MXFP4_SWIGLU, MXFP4_COLUMNS };
+struct QuantMxfp4Args {
+    uint8_t *Q, *S;
+    const void *a, *u;
+    long ld;
+    int n, k;
+    float limit;
+};
+hipError_t quant_mxfp4_launch(const QuantMxfp4Args &a, int type, Mxfp4Rows rows, hipStream_t st);
+
+/* C [M][N]. One matrix: W [N][K / 2], Sw [N][K / 32], Aq [M][K / 2], As [M][K /
+ * 32]. Grouped (table set): row r of bucket e (ex_off[e] <= r < ex_off[e + 1])
+ * from row row_tok[r] (or r) of Aq [n_a][K / 2], n_a * K < 2^32. K a multiple of
+ * 32, at most 2^20, Aq and W 16-byte aligned, fp4_waves() at most
+ * FP4_MAX_WAVES. */
+struct Fp4Args {
+    const uint8_t *Aq, *As, *W, *Sw;
+    void *C;
+    int M, N, K;
+    const DSV4QMat *table;
+    const int *ex_off, *row_tok;
+    int n_experts, n_a;
+    unsigned *status;
+};
+hipError_t gemm_fp4_launch(const Fp4Args &a, int out_type, hipStream_t st);
+
+/* -------------------------------------------- router with groups ----- */
+
+struct RouteGroupsArgs {
+    DSV4HipRouter r;
+    int n;
+    const void *logits;
+    const float *bias;        /* or NULL */
+    int *idx;
+    float *w, *scores;        /* scores: or NULL */
+    unsigned *status;
+};
+struct RouteGroupsBwdArgs {
+    DSV4HipRouter r;
+    int n;
+    const void *logits;
+    const int *idx;
+    const float *dw, *dscores;   /* dscores: or NULL */
+    void *dlogits;
+    unsigned *status;
+};
+hipError_t route_groups_launch(const RouteGroupsArgs &a, int type, hipStream_t st);
+hipError_t route_groups_bwd_launch(const RouteGroupsBwdArgs &a, int type, hipStream_t st);
+
 /* ------------------------------------------------- expert order ------ */
 
 /* pairs up to which the sort and the copy are one launch */

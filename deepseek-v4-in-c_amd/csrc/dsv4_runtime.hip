@@ -2224,6 +2224,135 @@ int dsv4_hip_gemm_i8_grouped_dev(void *C, int out_type, const int8_t *Aq, const 
     return 0;
 }
 
+/* ------------------------------- 4-bit products, router with groups ---- */
+
+constexpr int FP4_KMAX = 1 << 20;                  /* a tile's rows within 31-bit byte offsets */
+
+static int fp4_checks(const char *what, const void *C, int out_type, const void *Aq, int K)
+{
+    if (!elem_type_ok(out_type)) return fail("%s: unknown out_type %d", what, out_type);
+    if (K < 32 || K % 32 || K > FP4_KMAX) return fail("%s: K must be a multiple of 32 up to %d (got %d)", what, FP4_KMAX, K);
+    if (!aligned16(Aq) || !elem_aligned(C, out_type))
+        return fail("%s: Aq must be 16-byte aligned, C to its elements", what);
+    return 0;
+}
+
+int dsv4_hip_gemm_mxfp4q_dev(void *C, int out_type, const uint8_t *Aq, const uint8_t *As, int M, const DSV4QMat *W,
+                             void *stream)
+{
+    std::lock_guard<std::mutex> lk(g.mu);
+    Range rg("dsv4_hip_gemm_mxfp4q_dev");
+    if (!W || (M && (!C || !Aq || !As || !W->w || !W->s))) return fail("gemm_mxfp4q_dev: NULL pointer");
+    if (M < 0) return fail("gemm_mxfp4q_dev: bad M %d", M);
+    if (W->wdt != DSV4_WFP4 || W->rows < 1 || W->blk_r != 1 || W->blk_c != 32)
+        return fail("gemm_mxfp4q_dev: W must be DSV4_WFP4 with 1 x 32 blocks (got wdt %d, %d rows, %d x %d)", W->wdt,
+                    W->rows, W->blk_r, W->blk_c);
+    if (fp4_checks("gemm_mxfp4q_dev", C, out_type, Aq, W->cols)) return -1;
+    if (!aligned16(W->w)) return fail("gemm_mxfp4q_dev: w must be 16-byte aligned");
+    if (M && fp4_waves(fp4_form(M, W->rows, W->cols), M, W->rows, 0) > FP4_MAX_WAVES)
+        return fail("gemm_mxfp4q_dev: %d x %d results are too many for one launch", M, W->rows);
+    if (usable()) return -1;
+    if (M == 0) return 0;
+    OnDevice on;
+    if (stream_check(on, stream, "gemm_mxfp4q_dev")) return -1;
+    dev_call();
+    Fp4Args a;
+    memset(&a, 0, sizeof a);
+    a.Aq = Aq; a.As = As; a.W = (const uint8_t *)W->w; a.Sw = (const uint8_t *)W->s; a.C = C;
+    a.M = M; a.N = W->rows; a.K = W->cols; a.status = g.st;
+    LAUNCH(gemm_fp4_launch(a, out_type, (hipStream_t)stream), "gemm_mxfp4q_dev");
+    return 0;
+}
+
+int dsv4_hip_gemm_mxfp4q_grouped_dev(void *C, int out_type, const uint8_t *Aq, const uint8_t *As, int n_a,
+                                     const int *row_tok, int n_rows, const int *ex_off, const DSV4QMat *table,
+                                     int n_experts, int N, int K, void *stream)
+{
+    std::lock_guard<std::mutex> lk(g.mu);
+    Range rg("dsv4_hip_gemm_mxfp4q_grouped_dev");
+    if (n_rows && (!C || !Aq || !As || !ex_off || !table)) return fail("gemm_mxfp4q_grouped_dev: NULL pointer");
+    if (n_rows < 0 || n_a < (n_rows > 0)) return fail("gemm_mxfp4q_grouped_dev: bad n_rows %d or n_a %d", n_rows, n_a);
+    if (n_experts < 1 || n_experts > 1024)
+        return fail("gemm_mxfp4q_grouped_dev: n_experts %d outside 1..1024", n_experts);
+    if (N < 1) return fail("gemm_mxfp4q_grouped_dev: bad N %d", N);
+    if (fp4_checks("gemm_mxfp4q_grouped_dev", C, out_type, Aq, K)) return -1;
+    if ((long)n_a * K > 0xFFFFFFFFL) return fail("gemm_mxfp4q_grouped_dev: n_a * K is 2^32 or more");
+    if (n_rows && fp4_waves(fp4_grouped_form(n_rows, N, K, n_experts), n_rows, N, n_experts) > FP4_MAX_WAVES)
+        return fail("gemm_mxfp4q_grouped_dev: %d x %d results are too many for one launch", n_rows, N);
+    if (((uintptr_t)ex_off & 3u) || ((uintptr_t)row_tok & 3u) || ((uintptr_t)table & 7u))
+        return fail("gemm_mxfp4q_grouped_dev: misaligned offsets, row_tok or table");
+    if (usable()) return -1;
+    if (n_rows == 0) return 0;
+    OnDevice on;
+    if (stream_check(on, stream, "gemm_mxfp4q_grouped_dev")) return -1;
+    dev_call();
+    Fp4Args a;
+    memset(&a, 0, sizeof a);
+    a.Aq = Aq; a.As = As; a.C = C; a.M = n_rows; a.N = N; a.K = K;
+    a.table = table; a.ex_off = ex_off; a.row_tok = row_tok; a.n_experts = n_experts; a.n_a = n_a;
+    a.status = g.st;
+    LAUNCH(gemm_fp4_launch(a, out_type, (hipStream_t)stream), "gemm_mxfp4q_grouped_dev");
+    return 0;
+}
+
+/* what both directions of the router ask of their arguments */
+static int router_checks(const char *what, const DSV4HipRouter *r, int type, int n)
+{
+    if (!r) return fail("%s: NULL router", what);
+    if (!elem_type_ok(type)) return fail("%s: unknown element type %d", what, type);
+    if (n < 0 || n >= 1 << 26) return fail("%s: n %d outside 0..2^26 - 1", what, n);
+    if (r->score < DSV4_HIP_SQRT_SOFTPLUS || r->score > DSV4_HIP_SIGMOID) return fail("%s: unknown score %d", what, r->score);
+    return route_checks(what, r->n_experts, r->topk, nullptr, 0);
+}
+
+int dsv4_hip_route_groups_dev(int *idx, float *w, float *scores, const void *logits, int type, int n,
+                              const float *bias, const DSV4HipRouter *r, void *stream)
+{
+    std::lock_guard<std::mutex> lk(g.mu);
+    Range rg("dsv4_hip_route_groups_dev");
+    if (router_checks("route_groups_dev", r, type, n)) return -1;
+    if (r->n_group < 1 || r->n_group > 64 || r->n_experts % r->n_group || r->topk_group < 1 ||
+        r->topk_group > r->n_group || r->group_top < 1 || r->group_top > 2 ||
+        r->topk > r->n_experts / r->n_group * r->topk_group)
+        return fail("route_groups_dev: %d experts, %d of %d groups by %d, topk %d do not fit", r->n_experts,
+                    r->topk_group, r->n_group, r->group_top, r->topk);
+    if (n && (!idx || !w || !logits)) return fail("route_groups_dev: NULL pointer");
+    if (((uintptr_t)idx & 3u) || ((uintptr_t)w & 3u) || ((uintptr_t)scores & 3u) || ((uintptr_t)bias & 3u) ||
+        !elem_aligned(logits, type))
+        return fail("route_groups_dev: misaligned array");
+    if (usable()) return -1;
+    if (n == 0) return 0;
+    OnDevice on;
+    if (stream_check(on, stream, "route_groups_dev")) return -1;
+    dev_call();
+    RouteGroupsArgs a;
+    a.r = *r; a.n = n; a.logits = logits; a.bias = bias; a.idx = idx; a.w = w; a.scores = scores; a.status = g.st;
+    LAUNCH(route_groups_launch(a, type, (hipStream_t)stream), "route_groups_dev");
+    return 0;
+}
+
+int dsv4_hip_route_groups_bwd_dev(void *dlogits, const float *dw, const float *dscores, const void *logits, int type,
+                                  const int *idx, int n, const DSV4HipRouter *r, void *stream)
+{
+    std::lock_guard<std::mutex> lk(g.mu);
+    Range rg("dsv4_hip_route_groups_bwd_dev");
+    if (router_checks("route_groups_bwd_dev", r, type, n)) return -1;
+    if (n && (!dlogits || !dw || !logits || !idx)) return fail("route_groups_bwd_dev: NULL pointer");
+    if (((uintptr_t)idx & 3u) || ((uintptr_t)dw & 3u) || ((uintptr_t)dscores & 3u) || !elem_aligned(logits, type) ||
+        !elem_aligned(dlogits, type))
+        return fail("route_groups_bwd_dev: misaligned array");
+    if (usable()) return -1;
+    if (n == 0) return 0;
+    OnDevice on;
+    if (stream_check(on, stream, "route_groups_bwd_dev")) return -1;
+    dev_call();
+    RouteGroupsBwdArgs a;
+    a.r = *r; a.n = n; a.logits = logits; a.idx = idx; a.dw = dw; a.dscores = dscores; a.dlogits = dlogits;
+    a.status = g.st;
+    LAUNCH(route_groups_bwd_launch(a, type, (hipStream_t)stream), "route_groups_bwd_dev");
+    return 0;
+}
+
 /* shared checks of the expert-order calls */
 static int order_checks(int type, int n, int topk, int hidden, std::initializer_list<const void *> elems,
                         std::initializer_list<const void *> words, const char *what)
@@ -2423,6 +2552,53 @@ int dsv4_hip_swiglu_quant_i8_dev(int8_t *Q, float *S, const void *g_, const void
     std::lock_guard<std::mutex> lk(g.mu);
     Range rg("dsv4_hip_swiglu_quant_i8_dev");
     return quant_i8(Q, S, g_, u, true, type, ld, n, k, limit, stream, "swiglu_quant_i8_dev");
+}
+
+static int quant_mxfp4(uint8_t *Q, uint8_t *S, const void *x, const void *u, Mxfp4Rows rows, int type, int64_t ld,
+                       int n, int k, float limit, void *stream, const char *what)
+{
+    const bool cols = rows == MXFP4_COLUMNS;
+    if (n && (!Q || !S || !x || (rows == MXFP4_SWIGLU && !u))) return fail("%s: NULL pointer", what);
+    if (!elem_type_ok(type)) return fail("%s: unknown element type %d", what, type);
+    if (n < 0 || k < (cols ? 0 : 32) || k > 1 << 24 || ld < k || ld > (1LL << 40) || (cols && n >= 1 << 24) ||
+        (!cols && (k % 32 || ld * elem_bytes_of(type) % 16)))
+        return fail(cols ? "%s: need 0 <= n < 2^24, k up to 2^24 and ld >= k (got %d, %d, %lld)"
+                         : "%s: need n >= 0, k a multiple of 32 up to 2^24 and ld >= k of whole 16-byte steps (got %d, %d, %lld)",
+                    what, n, k, (long long)ld);
+    if ((cols ? (long)(n + 31) / 32 * 32 : (long)n) * k >= 1L << 35)
+        return fail("%s: %d x %d elements are too many for one launch", what, n, k);
+    if (cols ? !aligned16(Q) || !elem_aligned(x, type) : !aligned16(x) || !aligned16(u) || ((uintptr_t)Q & 3u) != 0)
+        return fail(cols ? "%s: need Q 16-byte aligned and a to its elements" : "%s: need rows 16- and Q 4-byte aligned", what);
+    if (usable()) return -1;
+    if (n == 0 || k == 0) return 0;
+    OnDevice on;
+    if (stream_check(on, stream, what)) return -1;
+    QuantMxfp4Args a;
+    a.Q = Q; a.S = S; a.a = x; a.u = u; a.ld = (long)ld; a.n = n; a.k = k; a.limit = limit;
+    LAUNCH(quant_mxfp4_launch(a, type, rows, (hipStream_t)stream), what);
+    return 0;
+}
+
+int dsv4_hip_quant_mxfp4_dev(uint8_t *Q, uint8_t *S, const void *a, int type, int64_t ld, int n, int k, void *stream)
+{
+    std::lock_guard<std::mutex> lk(g.mu);
+    Range rg("dsv4_hip_quant_mxfp4_dev");
+    return quant_mxfp4(Q, S, a, nullptr, MXFP4_ROWS, type, ld, n, k, 0.0f, stream, "quant_mxfp4_dev");
+}
+
+int dsv4_hip_swiglu_quant_mxfp4_dev(uint8_t *Q, uint8_t *S, const void *g_, const void *u, int type, int64_t ld, int n,
+                                    int k, float limit, void *stream)
+{
+    std::lock_guard<std::mutex> lk(g.mu);
+    Range rg("dsv4_hip_swiglu_quant_mxfp4_dev");
+    return quant_mxfp4(Q, S, g_, u, MXFP4_SWIGLU, type, ld, n, k, limit, stream, "swiglu_quant_mxfp4_dev");
+}
+
+int dsv4_hip_quant_mxfp4_t_dev(uint8_t *Q, uint8_t *S, const void *a, int type, int64_t ld, int n, int k, void *stream)
+{
+    std::lock_guard<std::mutex> lk(g.mu);
+    Range rg("dsv4_hip_quant_mxfp4_t_dev");
+    return quant_mxfp4(Q, S, a, nullptr, MXFP4_COLUMNS, type, ld, n, k, 0.0f, stream, "quant_mxfp4_t_dev");
 }
 
 int dsv4_hip_synth_normal_dev(float *out, size_t n, uint64_t seed, float sigma,

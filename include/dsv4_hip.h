@@ -397,6 +397,78 @@ int  dsv4_hip_gemm_i8_grouped_dev(void *C, int out_type, const int8_t *Aq, const
                                   const int *row_tok, int n_rows, const int *ex_off,
                                   const DSV4QMat *table, int n_experts, int N, int K, void *stream);
 
+/* ------------------------------------------- 4-bit products ---------------
+ * No counterpart in the reference, whose activations stay fp32: both operands
+ * as microscaled 4-bit rows, e2m1 codes (low nibble the even element) with one
+ * E8M0 byte for 32 elements along the sum (dsv4_hip_quant_mxfp4_dev and its kin
+ * write them; W is the framework's FP4 format, DSV4_WFP4 with 1 x 32 blocks).
+ *   C[m][n] = sum_k a[m][k] * w[n][k],  a = e2m1(Aq) * 2^(As - 127), w alike
+ * Aq [M][cols / 2], As [M][cols / 32], W a HOST descriptor holding device
+ * pointers, C [M][W->rows] of out_type. Accumulated in fp32 on the block-scaled
+ * MFMA, rounded once more for a 16-bit out_type (values beyond fp16 become
+ * infinite). A scale byte of 255 is NaN and makes the results that it enters
+ * NaN. cols a multiple of 32 up to 2^20; M and W->rows any that cover less than
+ * 2^23 tiles of 128 x 128 results (more is refused, nothing enqueued); Aq and w
+ * 16-byte aligned, scales anywhere. The order of the sum depends on the sizes
+ * alone: the same call gives the same bits. With dsv4_hip_quant_mxfp4_t_dev's
+ * columns the same call gives a projection's gradients, dX = dY W and dW = dY^T
+ * X. No workspace; streams as above. 0 enqueued (M = 0: nothing), -1 otherwise. */
+int  dsv4_hip_gemm_mxfp4q_dev(void *C, int out_type, const uint8_t *Aq, const uint8_t *As, int M,
+                              const DSV4QMat *W, void *stream);
+
+/* The same for rows in expert order: row r of bucket e (ex_off[e] <= r <
+ * ex_off[e + 1]) is row row_tok[r] of Aq [n_a][K / 2] (row_tok NULL: row r)
+ * times expert e's matrix. C [n_rows][N]; rows from ex_off[n_experts] on stay
+ * as they are. `table` is a DEVICE array of n_experts descriptors (DSV4_WFP4,
+ * [N x K], 1 x 32 blocks, device pointers, w 16-byte aligned); one of another
+ * kind raises status bit 1 and its rows become NaN. A row_tok outside [0, n_a)
+ * raises bit 0 and its row becomes NaN. n_experts <= 1024; n_a * K < 2^32; else
+ * as above, with up to one more row of tiles for each expert. */
+int  dsv4_hip_gemm_mxfp4q_grouped_dev(void *C, int out_type, const uint8_t *Aq, const uint8_t *As, int n_a,
+                                      const int *row_tok, int n_rows, const int *ex_off,
+                                      const DSV4QMat *table, int n_experts, int N, int K, void *stream);
+
+/* --------------------------------------- router with groups ---------------
+ * No counterpart in the reference, whose one router is dsv4_route above: other
+ * scores, groups of experts, gradients. For each of n tokens, with x its
+ * logits [n_experts] of `type`:
+ *   s = sqrt(softplus(x)) (as dsv4_hip_route_dev, bit for bit), softmax(x) or
+ *       1 / (1 + e^-x), the latter two in fp64, rounded once to fp32
+ *   c = s + bias (fp32; bias [n_experts] or NULL)
+ *   groups: n_group of n_experts / n_group neighbours each; a group is worth the
+ *       sum of its group_top (1 or 2) largest c, and the topk_group groups that
+ *       are worth most stay (n_group 1: no groups), the lower one of equals
+ *   idx [topk]: the largest c of the groups that stay, descending, the lower id
+ *       of equals
+ *   w [topk] = scale * s[idx] / (renorm: sum of s[idx], else 1), sums in fp64,
+ *       one rounding; 0 where that sum is 0
+ * scores [n][n_experts] receives s (may be NULL). An expert whose logit is -inf,
+ * or whose c is NaN or -inf, is not there: it is never chosen, and when fewer
+ * than topk are left the last ids are -1 with weight 0 (what dsv4_hip_moe_permute_dev
+ * takes for a pair without an expert). A token with a logit of NaN or +inf
+ * raises status bit 0: its ids are -1, its weights and scores NaN.
+ * n_experts <= 1024, topk <= 16 and at most the experts of topk_group groups,
+ * n_group <= 64 and a divisor of n_experts, n < 2^26. No workspace; streams as
+ * above. */
+enum { DSV4_HIP_SQRT_SOFTPLUS = 0, DSV4_HIP_SOFTMAX = 1, DSV4_HIP_SIGMOID = 2 };
+typedef struct {
+    int   score;                        /* DSV4_HIP_SQRT_SOFTPLUS, ...          */
+    int   n_experts, topk;
+    int   n_group, topk_group, group_top;
+    int   renorm;
+    float scale;
+} DSV4HipRouter;
+int  dsv4_hip_route_groups_dev(int *idx, float *w, float *scores, const void *logits, int type, int n,
+                               const float *bias, const DSV4HipRouter *r, void *stream);
+
+/* Gradient of the logits, dlogits [n][n_experts] of `type`, from dw [n][topk]
+ * and (or NULL) dscores [n][n_experts], the gradients of w and scores, for the
+ * ids that the forward call chose; the choice itself has none. idx -1: its dw
+ * adds nothing; another id outside [0, n_experts) likewise, and raises status
+ * bit 0. In fp64, one rounding. n_group and what belongs to it are not read. */
+int  dsv4_hip_route_groups_bwd_dev(void *dlogits, const float *dw, const float *dscores, const void *logits,
+                                   int type, const int *idx, int n, const DSV4HipRouter *r, void *stream);
+
 /* --------------------------------------- tokens in expert order -----------
  * The steps of the reference's union path around its bucket products
  * (src/80_prefill/dsv4_prefill_union.c:30-66, dsv4_prefill_experts.c:47-76,

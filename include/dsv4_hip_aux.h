@@ -63,6 +63,30 @@ int dsv4_hip_quant_i8_dev(int8_t *Q, float *S, const void *a, int type, int64_t 
 int dsv4_hip_swiglu_quant_i8_dev(int8_t *Q, float *S, const void *g, const void *u, int type, int64_t ld,
                                  int n, int k, float limit, void *stream);
 
+/* n rows of k elements of `type`, `ld` elements apart -> e2m1 codes Q[n][k / 2]
+ * (low nibble the even element) and E8M0 bytes S[n][k / 32]: 2^e least with
+ * 6 * 2^e >= blockmax (127 if all zero), codes the nearest values, ties to even,
+ * the rule of dsv4_hip_quant_fp4_mx_dev. A block with a value that is not finite
+ * gets byte 255 (NaN) and codes 0. Rows of the 4-bit products, or DSV4_WFP4
+ * weights. k a multiple of 32 up to 2^24, n * k < 2^35, the bytes of ld a multiple of 16, a 16-byte and Q
+ * 4-byte aligned; n = 0: nothing. No workspace. */
+int dsv4_hip_quant_mxfp4_dev(uint8_t *Q, uint8_t *S, const void *a, int type, int64_t ld, int n, int k,
+                             void *stream);
+
+/* The same for a = SwiGLU(g, u) as dsv4_hip_swiglu_quant_i8_dev takes it: codes
+ * and scales are those of the exact SwiGLU values (taken in fp64; a value beyond
+ * 6 * 2^127 saturates). */
+int dsv4_hip_swiglu_quant_mxfp4_dev(uint8_t *Q, uint8_t *S, const void *g, const void *u, int type, int64_t ld,
+                                    int n, int k, float limit, void *stream);
+
+/* The same for the columns of a, the operands of a backward pass: with n' = n
+ * rounded up to 32, Q[k][n' / 2] and S[k][n' / 32] hold a^T, zeros behind row n.
+ * k any number up to 2^24, n < 2^24, k * n' < 2^35, ld >= k, a aligned to its
+ * elements (rows of even length at an even pitch and 2-element alignment are the
+ * fast ones), Q 16-byte aligned. n or k 0: nothing. */
+int dsv4_hip_quant_mxfp4_t_dev(uint8_t *Q, uint8_t *S, const void *a, int type, int64_t ld, int n, int k,
+                               void *stream);
+
 /* The grouped MoE's permutation on its own (the first step of
  * dsv4_hip_moe_grouped_dev): the counting sort of the n * topk routing ids
  * idx[n][topk] by expert, as src/80_prefill/dsv4_prefill_union.c:30-51
