@@ -49,11 +49,33 @@ __device__ __forceinline__ auto fp4_matrix(const Fp4Args &a)
     };
 }
 
-/* 16 scale bytes of a row from block b on (nb blocks a row); blocks past the
- * row's end 0. Rows of scales have any alignment. */
+/* 16 scale bytes of a row from block b on (nb blocks a row, at least 16), zeros
+ * past its end: the row's last 16, shifted, so that nothing beyond the row is
+ * read and no branch parts the code around. Rows of scales have any alignment.
+ * Loaded here, shifted where they are used: the shift waits for the load. */
+__device__ __forceinline__ u32x4 fp4_scales_load(const uint8_t *row, int b, int nb)
+{
+    return *(const DSV4_GLOBAL u32x4_any *)(row + min(b, nb - 16));
+}
+__device__ __forceinline__ u32x4 fp4_scales_shift(const u32x4 &v, int b, int nb)
+{
+    const int gone = min(b - min(b, nb - 16), 16), q = gone / 4, r = gone % 4;
+    uint32_t t[5];
+#pragma unroll
+    for (int i = 0; i < 5; i++) {
+        t[i] = 0;
+#pragma unroll
+        for (int j = i; j < 4; j++) t[i] = j - i == q ? v[j] : t[i];
+    }
+    u32x4 o;
+#pragma unroll
+    for (int i = 0; i < 4; i++) o[i] = __builtin_amdgcn_alignbyte(t[i + 1], t[i], r);
+    return o;
+}
+/* the same for rows of any length */
 __device__ __forceinline__ u32x4 fp4_scales(const uint8_t *row, int b, int nb)
 {
-    if (b + 16 <= nb) return *(const DSV4_GLOBAL u32x4_any *)(row + b);
+    if (nb >= 16) return fp4_scales_shift(fp4_scales_load(row, b, nb), b, nb);
     u32x4 v = {0, 0, 0, 0};
     for (int i = 0; i < nb - b; i++) {
         const uint32_t s = gptr(row)[b + i] << (8 * (i & 3));
@@ -77,6 +99,19 @@ template <int B>
 __device__ __forceinline__ f32x16 fp4_mfma32(const v4i &w, const v4i &x, f32x16 c, uint32_t sw, uint32_t sx)
 {
     return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(fp4_operand(w), fp4_operand(x), c, 4, 4, B, (int)sw, B, (int)sx);
+}
+
+/* two results as 16-bit elements, rounded to nearest even */
+template <int OUT>
+__device__ __forceinline__ uint32_t fp4_pack(float a, float b)
+{
+    if constexpr (OUT == DSV4_HIP_BF16) {
+        typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+        return __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{a, b}, bf16x2));
+    } else {
+        typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+        return __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{a, b}, f16x2));
+    }
 }
 
 /* one result: element i of C */
@@ -345,7 +380,7 @@ template <int F, int T, int WR, int WT, int NST_> struct Fp4Tile {
     static constexpr int WI = F / WR / 32, U = T / WT / 32;
     static constexpr int OFF_X = F * 128, STAGE = (F + T) * 128;
     static constexpr int LW = F / 8 / NWAVE, LX = T / 8 / NWAVE, VM = LW + LX;
-    static constexpr int RING = NST * STAGE, TABLE = (F + T) * 16;
+    static constexpr int RING = NST * STAGE, TABLE = NT * 16;
     static constexpr int out_ld(int eb) { return F * eb + 16; }
     /* tokens that leave together: all, or a row of waves after the other */
     static constexpr int out_rows(int eb) { return T * out_ld(eb) <= 160 * 1024 ? T : T / WT; }
@@ -394,8 +429,9 @@ __global__ __launch_bounds__((Fp4Tile<F, T, WR, WT, NST>::NT)) void k_fp4_tile(F
         return;
     }
     const uint32_t KB = (uint32_t)a.K / 2;
-    /* stages, whole pairs of them where they begin anywhere (rot) */
-    const int nst = GROUPED ? (a.K + 511) / 512 * 2 : (a.K + 255) / 256;
+    /* stages, whole pairs of them: a way out between the two, or the last one
+     * after the loop, cost registers that the large tiles do not have */
+    const int nst = (a.K + 511) / 512 * 2;
     const __amdgpu_buffer_rsrc_t rw = buf_rsrc(t.w + (size_t)n0 * KB, (uint32_t)nf * KB);
     const size_t x0 = GROUPED ? 0 : (size_t)t.r0;
     const __amdgpu_buffer_rsrc_t rx = buf_rsrc(a.Aq + x0 * KB, (GROUPED ? (uint32_t)a.n_a : (uint32_t)t.rows) * KB);
@@ -413,12 +449,11 @@ __global__ __launch_bounds__((Fp4Tile<F, T, WR, WT, NST>::NT)) void k_fp4_tile(F
         xc[i] = swz(r, lane & 7);
         xo[i] = s < 0 ? BUF_OOB : (uint32_t)s * KB + 16u * (uint32_t)xc[i];
     }
-    /* the row whose scales this thread fetches; rows past the last weight row
-     * take the last one's, tokens that are not there zeros */
-    const uint8_t *srow = nullptr;
-    if ((int)threadIdx.x < F) {
-        srow = t.s + (size_t)(n0 + min((int)threadIdx.x, nf - 1)) * nb;
-    } else if ((int)threadIdx.x < F + T) {
+    /* the row whose scales this thread fetches. Rows past the last weight row take
+     * its, and so do tokens that are not there and threads without a row: what
+     * they give is not stored, or multiplies zeros */
+    const uint8_t *srow = t.s + (size_t)(n0 + min((int)threadIdx.x, nf - 1)) * nb;
+    if ((int)threadIdx.x >= F && (int)threadIdx.x < F + T) {
         const int s = fp4_source<GROUPED>(a, t, (int)threadIdx.x - F);
         if (s >= 0) srow = a.As + (x0 + s) * (size_t)nb;
     }
@@ -426,13 +461,13 @@ __global__ __launch_bounds__((Fp4Tile<F, T, WR, WT, NST>::NT)) void k_fp4_tile(F
      * side would meet in the same memory channels */
     const int rot = !GROUPED ? 0 : 2 * ((SHARED ? t.e * 4 + t.e / 8 : n0 / F * 2 + t.e) % (nst / 2));
     auto block_of = [&](int st) { return st + rot < nst ? st + rot : st + rot - nst; };
-    auto fetch_scales = [&](int pair) -> u32x4 {   /* of stages 2 pair and 2 pair + 1 */
-        if (2 * pair >= nst || !srow) return u32x4{0, 0, 0, 0};
-        return fp4_scales(srow, 8 * block_of(2 * pair), nb);
+    /* the scales of stages 2 pair and 2 pair + 1 */
+    auto block_of_pair = [&](int pair) { return 8 * (2 * pair < nst ? block_of(2 * pair) : nst + 1); };
+    const int nb16 = max(nb, 16);                  /* shorter rows have no second pair to fetch */
+    auto fetch_scales = [&](int pair) {            /* w: 16 bytes that are there */
+        return fp4_scales_load(nb < 16 ? t.w : srow, block_of_pair(pair), nb16);
     };
-    auto put_scales = [&](int pair, const u32x4 &v) {
-        if ((int)threadIdx.x < F + T) *(u32x4 *)(table + (pair & 1) * C::TABLE + 16 * threadIdx.x) = v;
-    };
+    auto put_scales = [&](int pair, const u32x4 &v) { *(u32x4 *)(table + (pair & 1) * C::TABLE + 16 * threadIdx.x) = v; };
     /* load i of a wave's share of stage st; past the end zeros, no traffic */
     auto issue = [&](int st, int slot, int i) {
         const int blk = block_of(min(st, nst - 1));
@@ -446,7 +481,7 @@ __global__ __launch_bounds__((Fp4Tile<F, T, WR, WT, NST>::NT)) void k_fp4_tile(F
                       buf + C::OFF_X + 1024 * (C::LX * wave + j));
         }
     };
-    const u32x4 first = fetch_scales(0);
+    const u32x4 first = fp4_scales(srow, block_of_pair(0), nb);
     u32x4 held = fetch_scales(1);
 #pragma unroll
     for (int s = 0; s < NST; s++)
@@ -520,23 +555,29 @@ __global__ __launch_bounds__((Fp4Tile<F, T, WR, WT, NST>::NT)) void k_fp4_tile(F
 #pragma unroll
     for (int u = 0; u < U; u++) read_x(o0, lds, u, 0);
     read_scales(sc, 0);
-    for (int st = 0; st < nst; st++) {
+    /* stage st, the first or second of its pair. Nothing here branches: the
+     * compiler would move products over the barrier into another block. */
+    auto stage = [&](auto SECOND, int st) {
         const uint8_t *buf = lds + slot * C::STAGE;
         step(IC<0>{}, o0, sc, o1, buf, 1, false, 0, 0);
         step(IC<1>{}, o1, sc, o0, buf, 2, false, 0, 0);
         step(IC<2>{}, o0, sc, o1, buf, 3, false, 0, 0);
-        if (st & 1) put_scales(st / 2 + 1, held);
+        if constexpr (decltype(SECOND)::value) put_scales(st / 2 + 1, fp4_scales_shift(held, block_of_pair(st / 2 + 1), nb16));
         __builtin_amdgcn_s_waitcnt(0xC07F);        /* this stage's operands are in registers */
         wait_vm<(NST - 2) * C::VM>();              /* the wave's loads of the next have landed */
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
-        if (st & 1) held = fetch_scales(st / 2 + 2);
+        if constexpr (decltype(SECOND)::value) held = fetch_scales(st / 2 + 2);
         const int free = slot;
         slot = slot + 1 == NST ? 0 : slot + 1;
         Sc sn;
         read_scales(sn, st + 1);
         step(IC<3>{}, o1, sc, o0, lds + slot * C::STAGE, 0, true, st + NST, free);
         sc = sn;
+    };
+    for (int st = 0; st < nst; st += 2) {
+        stage(IC<0>{}, st);
+        stage(IC<1>{}, st + 1);
     }
     /* the loads past the end, then the ring becomes the output tile */
     __builtin_amdgcn_s_waitcnt(0xC07F);
@@ -569,8 +610,8 @@ __global__ __launch_bounds__((Fp4Tile<F, T, WR, WT, NST>::NT)) void k_fp4_tile(F
                             *(f32x4 *)o = f32x4{v[0], v[1], v[2], v[3]};
                         } else {
                             u32x2 p;
-                            p.x = narrow16<OUT>(v[0]) | (narrow16<OUT>(v[1]) << 16);
-                            p.y = narrow16<OUT>(v[2]) | (narrow16<OUT>(v[3]) << 16);
+                            p.x = fp4_pack<OUT>(v[0], v[1]);
+                            p.y = fp4_pack<OUT>(v[2], v[3]);
                             *(u32x2 *)o = p;
                         }
                     }
