@@ -129,9 +129,11 @@ __device__ __forceinline__ Bucket<S> bucket_tile(const ARGS &a, int t, int lane,
 
 typedef __attribute__((address_space(3))) void lds_mem;
 
+/* CPOL 2: past the caches, for what is read once */
+template <int CPOL = 0>
 __device__ __forceinline__ void buf_dma16(__amdgpu_buffer_rsrc_t r, uint32_t voff, int soff, uint8_t *dst)
 {
-    __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_mem *)dst, 16, (int)voff, soff, 0, 0);
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_mem *)dst, 16, (int)voff, soff, 0, CPOL);
 }
 template <int N>
 __device__ __forceinline__ void wait_vm()

@@ -322,44 +322,93 @@ inline long i8_waves(I8Form form, long M, long N, long ne)
 
 /* ------------------------------------------------ 4-bit products -------- */
 
-/* Forms of the product of 4-bit rows. FP4_PAIR: weights as whole lines straight
- * to registers, one matrix in workgroups of 8 weight rows x 8 tokens, experts in
- * 32 x 16. FP4_SPLIT: 32 x 32 results a workgroup, K over its waves. The others
- * by their tiles, features x rows, through a ring in LDS. */
-enum Fp4Form { FP4_PAIR = 1, FP4_SPLIT, FP4_64x64, FP4_128x128, FP4_256x128, FP4_256x256 };
+/* Forms of the product of 4-bit rows: 16 x 16 results a workgroup with K over
+ * its waves (one matrix only), the others tiles of features x rows through a
+ * ring in LDS. */
+enum Fp4Form { FP4_SPLIT = 1, FP4_64x32, FP4_64x64, FP4_128x32, FP4_128x64, FP4_128x128, FP4_256x128, FP4_256x256 };
 struct Fp4Shape { int F, TR, waves; };
-inline Fp4Shape fp4_shape(Fp4Form form, bool grouped)
+inline Fp4Shape fp4_shape(Fp4Form form)
 {
     switch (form) {
-    case FP4_PAIR: return grouped ? Fp4Shape{32, 16, 4} : Fp4Shape{8, 8, 8};
-    case FP4_SPLIT: return {32, 32, 8};
+    case FP4_SPLIT: return {16, 16, 8};
+    case FP4_64x32: return {64, 32, 2};
     case FP4_64x64: return {64, 64, 4};
+    case FP4_128x32: return {128, 32, 4};
+    case FP4_128x64: return {128, 64, 4};
     case FP4_128x128: return {128, 128, 4};
     case FP4_256x128: return {256, 128, 8};
     default: return {256, 256, 8};
     }
 }
 
-inline Fp4Form fp4_form(int M, int N, int K)
+/* Cost of a form, in hundredths of a us: c1 and, at K = 4096, c0 once, and for a
+ * round of 256 workgroups fix + slope at K = 4096; the last round costs the share
+ * r of one and the rest by how full it is. Fitted to 1,255 times (176 shapes of 1
+ * to 4,096 rows, 300 to 32,768 features, K 256 to 8,192), of which the form that
+ * they choose costs 1 % more than the best, at most 23 % (2,048 x 32,768 x 1024:
+ * 256x256 74.6, 128x128 60.6). us, split / 64x32 / 64x64 / 128x64 / 128x128 /
+ * 256x128 / 256x256: 1 x 4096 x 4096 3.4 / 6.1 / 6.6 / 8.1 / 10 / 15 / 23, 128 rows
+ * - / 7.1 / 7.7 / 9.4 / 15 / 18 / 25, 512 rows - / 17.8 / 12.1 / 11.0 / 16 / 19 / 27,
+ * 2,048 rows - / 52 / 39 / 30 / 24.6 / 24.1 / 29, 4,096 rows - / 100 / 74 / 57 / 47 / 46 /
+ * 39.5; 333 x 1024 x 4096 - / 6.8 / 7.1 / 8.8 / 12 / 18 / 25; 2,048 x 4096 x 1024 - /
+ * 23 / 16 / 12 / 9.2 / 10.4 / 12.6. */
+struct Fp4Cost { Fp4Form form; int c1, c0, fix, slope, r; };
+constexpr Fp4Cost FP4_COSTS[] = {
+    {FP4_SPLIT, 195, 62, 36, 153, 71},      {FP4_64x32, 256, 172, 68, 238, 62},     {FP4_64x64, 233, 165, 100, 337, 63},
+    {FP4_128x64, 278, 182, 120, 534, 59},   {FP4_128x128, 282, 487, 159, 840, 42},  {FP4_256x128, 112, 56, 497, 1650, 71},
+    {FP4_256x256, 0, 0, 890, 2722, 65}};
+/* row tiles: whole ones, and with ne experts one for each that rows may hit */
+inline long fp4_row_tiles(Fp4Form form, long M, long ne)
 {
-    (void)K;
-    if (M <= 8 && N <= 1 << 20) return FP4_PAIR;
-    if (ceil_div(M, 64) * ceil_div(N, 64) < CUS) return FP4_SPLIT;
-    if (ceil_div(M, 128) * ceil_div(N, 128) < CUS) return FP4_64x64;
-    if (ceil_div(M, 256) * ceil_div(N, 128) < CUS) return FP4_128x128;
-    if (ceil_div(M, 256) * ceil_div(N, 256) < CUS) return FP4_256x128;
-    return FP4_256x256;
+    const long TR = fp4_shape(form).TR;
+    return ne ? M / TR + (M < ne ? M : ne) : ceil_div(M, TR);
 }
-
-/* Buckets of ne experts, M rows in all; the mean bucket decides. */
-inline Fp4Form fp4_grouped_form(int M, int N, int K, int ne)
+template <int NF>
+inline Fp4Form fp4_least(const Fp4Cost (&costs)[NF], long M, long N, long K, long ne)
 {
-    (void)N; (void)K;
+    const Fp4Form largest = costs[NF - 1].form;
+    if (ceil_div(M, 128) * ceil_div(N, 128) >= 1L << 20) return largest;      /* costs beyond 64 bits */
+    const long stages = 2 * ceil_div(K, 512);      /* of 256 values, in pairs */
+    Fp4Form best = largest;
+    long least = -1;
+    for (const Fp4Cost &c : costs) {
+        const long w = fp4_row_tiles(c.form, M, ne) * ceil_div(N, fp4_shape(c.form).F);
+        const long full = (w - 1) / CUS, last = w - full * CUS, round = c.fix + c.slope * stages / 16;
+        const long cost = c.c1 + c.c0 * stages / 16 + round * full + round * (c.r + (100 - c.r) * last / CUS) / 100;
+        if (least < 0 || cost < least) {
+            least = cost;
+            best = c.form;
+        }
+    }
+    return best;
+}
+inline Fp4Form fp4_form(int M, int N, int K) { return fp4_least(FP4_COSTS, M, N, K, 0); }
+
+/* Buckets of ne experts, M rows in all: the same sum over the tiles of the launch,
+ * fitted to 1,040 times with weights out of the caches (130 routings, even and
+ * Zipf, of 6 to 24,576 rows to 8 to 256 experts of 300 x 544 to 4096 x 4096), the
+ * chosen form 2 % above the best, at most 20 %. us, 64x32 / 128x32 / 128x64 /
+ * 256x128, experts 2048 x 4096 on 256: 6 rows 8.7 / 10.1 / 10.7 / 16.3, 384 rows 148
+ * / 143 / 149 / 168, 1,536 rows 196 / 183 / 189 / 191, 6,144 rows 277 / 213 / 210 /
+ * 199, 24,576 rows - / - / 360 / 236, Zipf - / - / 361 / 301; 8 of 4096 x 4096, 240
+ * rows 21 / 21 / 16.6 / 26, 3,072 rows - / - / 65 / 52; 64 of 512 x 1024, 384 rows 7.6
+ * / 7.3 / 7.6 / 9.9, 6,144 rows - / 14 / 11.7 / 11.0. */
+constexpr Fp4Cost FP4_BUCKET_COSTS[] = {{FP4_64x32, 337, 311, 93, 314, 0},
+                                        {FP4_128x32, 326, 432, 136, 575, 3},
+                                        {FP4_128x64, 400, 334, 148, 669, 0},
+                                        {FP4_256x128, 364, 806, 368, 1445, 16}};
+inline Fp4Form fp4_grouped_form(int M, int N, int K, int ne) { return fp4_least(FP4_BUCKET_COSTS, M, N, K, ne); }
+
+/* Whether the experts' weights go past the caches: rows few enough that an expert
+ * is read once, and more weights than the memory-side cache (256 MB) keeps for a
+ * next call beside other layers'. us, past the caches / through them: 384 rows on
+ * 256 experts 2048 x 4096 143 / 158, 1,536 rows 183 / 196, on 64 48.6 / 54.1; but
+ * 24,576 rows 251 / 236, and 300 rows on 8 of 4096 x 4096 called again and again 23
+ * / 17. */
+inline bool fp4_stream(int M, int N, int K, int ne)
+{
     const long hit = M < ne ? M : ne;
-    if (M <= 10 * hit) return FP4_PAIR;
-    if (M <= 24 * hit) return FP4_SPLIT;
-    if (M <= 48 * hit) return FP4_64x64;
-    return M <= 96 * hit ? FP4_128x128 : FP4_256x128;
+    return hit * N * (K / 2) >= 1L << 27 && M <= 64 * hit && fp4_grouped_form(M, N, K, ne) != FP4_256x128;
 }
 
 /* Waves of the launch that multiplies M rows by N features in a form: tiles
@@ -368,8 +417,8 @@ inline Fp4Form fp4_grouped_form(int M, int N, int K, int ne)
 constexpr long FP4_MAX_WAVES = (1L << 26) - 1;
 inline long fp4_waves(Fp4Form form, long M, long N, long ne)
 {
-    const Fp4Shape s = fp4_shape(form, ne != 0);
-    return (ne ? M / s.TR + (M < ne ? M : ne) : ceil_div(M, s.TR)) * ceil_div(N, s.F) * s.waves;
+    const Fp4Shape s = fp4_shape(form);
+    return fp4_row_tiles(form, M, ne) * ceil_div(N, s.F) * s.waves;
 }
 
 } // namespace dsv4

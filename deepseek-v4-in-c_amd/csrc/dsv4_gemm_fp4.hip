@@ -49,33 +49,11 @@ __device__ __forceinline__ auto fp4_matrix(const Fp4Args &a)
     };
 }
 
-/* 16 scale bytes of a row from block b on (nb blocks a row, at least 16), zeros
- * past its end: the row's last 16, shifted, so that nothing beyond the row is
- * read and no branch parts the code around. Rows of scales have any alignment.
- * Loaded here, shifted where they are used: the shift waits for the load. */
-__device__ __forceinline__ u32x4 fp4_scales_load(const uint8_t *row, int b, int nb)
-{
-    return *(const DSV4_GLOBAL u32x4_any *)(row + min(b, nb - 16));
-}
-__device__ __forceinline__ u32x4 fp4_scales_shift(const u32x4 &v, int b, int nb)
-{
-    const int gone = min(b - min(b, nb - 16), 16), q = gone / 4, r = gone % 4;
-    uint32_t t[5];
-#pragma unroll
-    for (int i = 0; i < 5; i++) {
-        t[i] = 0;
-#pragma unroll
-        for (int j = i; j < 4; j++) t[i] = j - i == q ? v[j] : t[i];
-    }
-    u32x4 o;
-#pragma unroll
-    for (int i = 0; i < 4; i++) o[i] = __builtin_amdgcn_alignbyte(t[i + 1], t[i], r);
-    return o;
-}
-/* the same for rows of any length */
+/* 16 scale bytes of a row from block b on (nb blocks a row); blocks past the
+ * row's end 0. Rows of scales have any alignment. */
 __device__ __forceinline__ u32x4 fp4_scales(const uint8_t *row, int b, int nb)
 {
-    if (nb >= 16) return fp4_scales_shift(fp4_scales_load(row, b, nb), b, nb);
+    if (b + 16 <= nb) return *(const DSV4_GLOBAL u32x4_any *)(row + b);
     u32x4 v = {0, 0, 0, 0};
     for (int i = 0; i < nb - b; i++) {
         const uint32_t s = gptr(row)[b + i] << (8 * (i & 3));
@@ -89,12 +67,11 @@ __device__ __forceinline__ v8i fp4_operand(const v4i &v)
 {
     return __builtin_shufflevector(v, v, 0, 1, 2, 3, -1, -1, -1, -1);
 }
-/* B: which byte of the scale registers */
-template <int B>
 __device__ __forceinline__ f32x4 fp4_mfma16(const v4i &w, const v4i &x, f32x4 c, uint32_t sw, uint32_t sx)
 {
-    return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(fp4_operand(w), fp4_operand(x), c, 4, 4, B, (int)sw, B, (int)sx);
+    return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(fp4_operand(w), fp4_operand(x), c, 4, 4, 0, (int)sw, 0, (int)sx);
 }
+/* B: which byte of the scale registers */
 template <int B>
 __device__ __forceinline__ f32x16 fp4_mfma32(const v4i &w, const v4i &x, f32x16 c, uint32_t sw, uint32_t sx)
 {
@@ -144,223 +121,51 @@ __device__ __forceinline__ int fp4_source(const Fp4Args &a, const Fp4Bucket &t, 
 
 } // namespace
 
-/* ------------------------------------------------------- few rows -------
- * Weights as whole 128-byte lines: an instruction takes 256 codes of 8 weight
- * rows, lane l (row l % 8) block 4 (l / 8 % 2) + l / 16 of the line's eight. Rows
- * 0 - 7 of the MFMA's A operand are then the 8 weight rows at the line's first
- * four blocks, rows 8 - 15 the same rows at its last four; the B operand holds 8
- * tokens the same way, and of the 16 x 16 result the two quadrants that multiply
- * equal blocks count. A workgroup takes 8 RT weight rows by 8 TT tokens, its
- * waves share out K in lines, B of them in flight, and add up in LDS, in wave
- * order. */
-template <int RT, int TT, int NW, int B, bool GROUPED, int OUT>
-__global__ __launch_bounds__(64 * NW) void k_fp4_pair(Fp4Args a)
-{
-    constexpr int TR = 8 * TT, FR = 8 * RT;
-    __shared__ float sum[NW][2][TT * RT][64];
-    const int lane = threadIdx.x & 63, wave = wave_in_group();
-    const int r8 = lane & 7, half = (lane >> 3) & 1, g = lane >> 4;
-    const int slabs = (a.N + FR - 1) / FR, tile = blockIdx.x / slabs, n0 = (blockIdx.x - tile * slabs) * FR;
-    Fp4Bucket t;
-    if constexpr (GROUPED) {
-        t = bucket_tile<TR, uint8_t>(a, tile, lane, fp4_matrix(a));
-        if (t.rows <= 0) return;
-    } else {
-        t.w = a.W; t.s = a.Sw; t.e = 0; t.bad = false;
-        t.r0 = tile * TR;
-        t.rows = min(TR, a.M - t.r0);
-    }
-    const int nf = min(FR, a.N - n0);
-    if (GROUPED && t.bad) {
-        fp4_bad<OUT>(a, t, n0, nf, 64 * NW);
-        return;
-    }
-    const uint32_t KB = (uint32_t)a.K / 2, nb = (uint32_t)a.K / 32;   /* a row's bytes, its scales */
-    const __amdgpu_buffer_rsrc_t rw = buf_rsrc(t.w + (size_t)n0 * KB, (uint32_t)nf * KB);
-    const __amdgpu_buffer_rsrc_t rsw = buf_rsrc(t.s + (size_t)n0 * nb, (uint32_t)nf * nb);
-    const size_t x0 = GROUPED ? 0 : (size_t)t.r0;
-    const uint32_t xr = GROUPED ? (uint32_t)a.n_a : (uint32_t)t.rows;
-    const __amdgpu_buffer_rsrc_t rx = buf_rsrc(a.Aq + x0 * KB, xr * KB), rsx = buf_rsrc(a.As + x0 * nb, xr * nb);
-    const uint32_t blk = 4u * half + g;
-    uint32_t xo[TT], xs[TT], wo[RT], ws[RT];
-#pragma unroll
-    for (int u = 0; u < TT; u++) {
-        const int s = fp4_source<GROUPED>(a, t, 8 * u + r8);
-        xo[u] = s < 0 ? BUF_OOB : (uint32_t)s * KB + 16u * blk;
-        xs[u] = s < 0 ? BUF_OOB : (uint32_t)s * nb + blk;
-    }
-#pragma unroll
-    for (int i = 0; i < RT; i++) {
-        wo[i] = (uint32_t)(8 * i + r8) * KB + 16u * blk;
-        ws[i] = (uint32_t)(8 * i + r8) * nb + blk;
-    }
-    const int lines = (a.K + 255) / 256;
-    f32x4 acc[RT][TT];
-#pragma unroll
-    for (int i = 0; i < RT; i++)
-#pragma unroll
-        for (int u = 0; u < TT; u++) acc[i][u] = f32x4{0, 0, 0, 0};
-    for (int l0 = wave; l0 < lines; l0 += NW * B) {
-        v4i w[B][RT], x[B][TT];
-        uint32_t sw[B][RT], sx[B][TT];
-#pragma unroll
-        for (int b = 0; b < B; b++) {
-            const uint32_t l = (uint32_t)(l0 + NW * b);
-            const bool in = 8 * l + blk < nb;
-#pragma unroll
-            for (int i = 0; i < RT; i++) {
-                w[b][i] = buf_ld16<2>(rw, in ? wo[i] + 128u * l : BUF_OOB);
-                sw[b][i] = __builtin_amdgcn_raw_buffer_load_b8(rsw, (int)(in ? ws[i] + 8u * l : BUF_OOB), 0, 0);
-            }
-#pragma unroll
-            for (int u = 0; u < TT; u++) {
-                const bool ok = in && xo[u] != BUF_OOB;
-                x[b][u] = buf_ld16<0>(rx, ok ? xo[u] + 128u * l : BUF_OOB);
-                sx[b][u] = __builtin_amdgcn_raw_buffer_load_b8(rsx, (int)(ok ? xs[u] + 8u * l : BUF_OOB), 0, 0);
-            }
-        }
-#pragma unroll
-        for (int b = 0; b < B; b++)
-#pragma unroll
-            for (int i = 0; i < RT; i++)
-#pragma unroll
-                for (int u = 0; u < TT; u++) acc[i][u] = fp4_mfma16<0>(w[b][i], x[b][u], acc[i][u], sw[b][i], sx[b][u]);
-    }
-    /* element e of lane l: weight row 4 (g % 2) + e at half g / 2, token l % 8
-     * at half l / 8 % 2 */
-    if (half == g >> 1) {
-#pragma unroll
-        for (int i = 0; i < RT; i++)
-#pragma unroll
-            for (int u = 0; u < TT; u++)
-#pragma unroll
-                for (int e = 0; e < 4; e++) sum[wave][half][i * TT + u][r8 * 8 + 4 * (g & 1) + e] = acc[i][u][e];
-    }
-    __syncthreads();
-    for (int o = threadIdx.x; o < TR * FR; o += 64 * NW) {
-        const int n = o % FR, i = o / FR;
-        if (i >= t.rows || n >= nf) continue;
-        float v = 0.0f;
-#pragma unroll
-        for (int w = 0; w < NW; w++)
-#pragma unroll
-            for (int h = 0; h < 2; h++) v += sum[w][h][(n / 8) * TT + i / 8][(i & 7) * 8 + (n & 7)];
-        if (GROUPED && fp4_source<GROUPED>(a, t, i) < 0) {
-            v = __builtin_nanf("");
-            if (n == 0) atomicOr(a.status, ST_BAD_EXPERT_ID);
-        }
-        fp4_store<OUT>(a.C, (size_t)(t.r0 + i) * a.N + n0 + n, v);
-    }
-}
-
-template <int RT, int TT, int NW, int B, bool GROUPED, int OUT>
-static hipError_t fp4_pair(const Fp4Args &a, Fp4Form form, hipStream_t st)
-{
-    const long groups = fp4_waves(form, a.M, a.N, GROUPED ? a.n_experts : 0) / NW;
-    hipLaunchKernelGGL((k_fp4_pair<RT, TT, NW, B, GROUPED, OUT>), dim3((unsigned)groups), dim3(64 * NW), 0, st, a);
-    return hipGetLastError();
-}
-
 /* --------------------------------------------------- K over the waves ---
- * A workgroup takes 16 FA features by 16 TB rows, and its NW waves share out K in
- * pieces of 512 values: operands go straight to registers, a whole piece's
- * loads before its first product, and the sums meet in LDS, added in wave
- * order. No wave waits for another before the end, so a product too small to
- * fill the device costs one latency of its loads, not one a stage. */
-template <int FA, int TB, int NW, bool GROUPED, int OUT>
-__global__ __launch_bounds__(64 * NW) void k_fp4_split(Fp4Args a)
+ * A workgroup takes 16 features by 16 rows of one matrix, and its eight waves
+ * share out K in pieces of 512 values: operands go straight to registers, a
+ * whole piece's loads before its first product, and the sums meet in LDS, added
+ * in wave order. No wave waits for another before the end, so a product too
+ * small to fill the device costs one latency of its loads, not one a stage.
+ * Bound: that latency (one token of 4096 x 4096 3.4 us, the weights alone 1.4 at
+ * 6.2 TB/s; 64 x 32 tiles 6.1); with many rows the loads, 64 bytes of a row each. */
+template <int OUT>
+__global__ __launch_bounds__(512) void k_fp4_split(Fp4Args a)
 {
-    constexpr int F = 16 * FA, TR = 16 * TB;
-    __shared__ float sum[NW][F * TR];
+    constexpr int NW = 8;
+    __shared__ float sum[NW][256];
     const int lane = threadIdx.x & 63, wave = wave_in_group(), r16 = lane & 15, g = lane >> 4;
-    const int nt = (a.N + F - 1) / F, tile = blockIdx.x / nt, n0 = (blockIdx.x - tile * nt) * F;
-    Fp4Bucket t;
-    if constexpr (GROUPED) {
-        t = bucket_tile<TR, uint8_t>(a, tile, lane, fp4_matrix(a));
-        if (t.rows <= 0) return;
-    } else {
-        t.w = a.W; t.s = a.Sw; t.e = 0; t.bad = false;
-        t.r0 = tile * TR;
-        t.rows = min(TR, a.M - t.r0);
-    }
-    const int nf = min(F, a.N - n0);
-    if (GROUPED && t.bad) {
-        fp4_bad<OUT>(a, t, n0, nf, 64 * NW);
-        return;
-    }
+    const int nt = (a.N + 15) / 16, tile = blockIdx.x / nt, n0 = (blockIdx.x - tile * nt) * 16;
+    const int r0 = tile * 16, rows = min(16, a.M - r0), nf = min(16, a.N - n0);
     const uint32_t KB = (uint32_t)a.K / 2;
     const int nb = a.K / 32;
-    const __amdgpu_buffer_rsrc_t rw = buf_rsrc(t.w + (size_t)n0 * KB, (uint32_t)nf * KB);
-    const size_t x0 = GROUPED ? 0 : (size_t)t.r0;
-    const __amdgpu_buffer_rsrc_t rx = buf_rsrc(a.Aq + x0 * KB, (GROUPED ? (uint32_t)a.n_a : (uint32_t)t.rows) * KB);
-    uint32_t wo[FA], xo[TB];
-    const uint8_t *ws[FA], *xs[TB];
-#pragma unroll
-    for (int i = 0; i < FA; i++) {
-        const int r = min(16 * i + r16, nf - 1);   /* rows past the last: the last again, not stored */
-        wo[i] = (uint32_t)r * KB + 16u * g;
-        ws[i] = t.s + (size_t)(n0 + r) * nb;
-    }
-#pragma unroll
-    for (int u = 0; u < TB; u++) {
-        const int s = fp4_source<GROUPED>(a, t, 16 * u + r16);
-        xo[u] = s < 0 ? BUF_OOB : (uint32_t)s * KB + 16u * g;
-        xs[u] = s < 0 ? nullptr : a.As + (x0 + s) * (size_t)nb;
-    }
-    f32x4 acc[FA][TB];
-#pragma unroll
-    for (int i = 0; i < FA; i++)
-#pragma unroll
-        for (int u = 0; u < TB; u++) acc[i][u] = f32x4{0, 0, 0, 0};
+    const __amdgpu_buffer_rsrc_t rw = buf_rsrc(a.W + (size_t)n0 * KB, (uint32_t)nf * KB);
+    const __amdgpu_buffer_rsrc_t rx = buf_rsrc(a.Aq + (size_t)r0 * KB, (uint32_t)rows * KB);
+    /* rows past the last: the last again, not stored */
+    const int wr = min(r16, nf - 1), xr = min(r16, rows - 1);
+    const uint8_t *ws = a.Sw + (size_t)(n0 + wr) * nb, *xs = a.As + (size_t)(r0 + xr) * nb;
+    f32x4 acc = {0, 0, 0, 0};
     for (int p = wave; 16 * p < nb; p += NW) {
-        v4i w[4][FA], x[4][TB];
-        u32x4 sw[FA], sx[TB];
+        v4i w[4], x[4];
 #pragma unroll
         for (int s = 0; s < 4; s++) {
-            const uint32_t at = 256u * p + 64u * s;
+            const uint32_t at = 256u * p + 64u * s + 16u * g;
             const bool in = 16 * p + 4 * s + g < nb;
-#pragma unroll
-            for (int i = 0; i < FA; i++) w[s][i] = buf_ld16<0>(rw, in ? wo[i] + at : BUF_OOB);
-#pragma unroll
-            for (int u = 0; u < TB; u++) x[s][u] = buf_ld16<0>(rx, in && xo[u] != BUF_OOB ? xo[u] + at : BUF_OOB);
+            w[s] = buf_ld16<0>(rw, in ? (uint32_t)wr * KB + at : BUF_OOB);
+            x[s] = buf_ld16<0>(rx, in ? (uint32_t)xr * KB + at : BUF_OOB);
         }
+        const u32x4 sw = fp4_scales(ws, 16 * p, nb), sx = fp4_scales(xs, 16 * p, nb);
 #pragma unroll
-        for (int i = 0; i < FA; i++) sw[i] = fp4_scales(ws[i], 16 * p, nb);
-#pragma unroll
-        for (int u = 0; u < TB; u++) sx[u] = xs[u] ? fp4_scales(xs[u], 16 * p, nb) : u32x4{0, 0, 0, 0};
-#pragma unroll
-        for (int s = 0; s < 4; s++)
-#pragma unroll
-            for (int i = 0; i < FA; i++)
-#pragma unroll
-                for (int u = 0; u < TB; u++)
-                    acc[i][u] = fp4_mfma16<0>(w[s][i], x[s][u], acc[i][u], sw[i][s] >> (8 * g), sx[u][s] >> (8 * g));
+        for (int s = 0; s < 4; s++) acc = fp4_mfma16(w[s], x[s], acc, sw[s] >> (8 * g), sx[s] >> (8 * g));
     }
-#pragma unroll
-    for (int i = 0; i < FA; i++)
-#pragma unroll
-        for (int u = 0; u < TB; u++) *(f32x4 *)&sum[wave][(16 * u + r16) * F + 16 * i + 4 * g] = acc[i][u];
+    *(f32x4 *)&sum[wave][r16 * 16 + 4 * g] = acc;
     __syncthreads();
-    for (int o = threadIdx.x; o < TR * F; o += 64 * NW) {
-        const int n = o % F, i = o / F;
-        if (i >= t.rows || n >= nf) continue;
-        float v = 0.0f;
+    const int o = threadIdx.x, n = o % 16, i = o / 16;
+    if (i >= rows || n >= nf) return;
+    float v = 0.0f;
 #pragma unroll
-        for (int w = 0; w < NW; w++) v += sum[w][o];
-        if (GROUPED && fp4_source<GROUPED>(a, t, i) < 0) {
-            v = __builtin_nanf("");
-            if (n == 0) atomicOr(a.status, ST_BAD_EXPERT_ID);
-        }
-        fp4_store<OUT>(a.C, (size_t)(t.r0 + i) * a.N + n0 + n, v);
-    }
-}
-
-template <int FA, int TB, int NW, bool GROUPED, int OUT>
-static hipError_t fp4_split(const Fp4Args &a, Fp4Form form, hipStream_t st)
-{
-    const long groups = fp4_waves(form, a.M, a.N, GROUPED ? a.n_experts : 0) / NW;
-    hipLaunchKernelGGL((k_fp4_split<FA, TB, NW, GROUPED, OUT>), dim3((unsigned)groups), dim3(64 * NW), 0, st, a);
-    return hipGetLastError();
+    for (int w = 0; w < NW; w++) v += sum[w][o];
+    fp4_store<OUT>(a.C, (size_t)(r0 + i) * a.N + n0 + n, v);
 }
 
 /* ------------------------------------------------------- many rows ------
@@ -378,12 +183,13 @@ static hipError_t fp4_split(const Fp4Args &a, Fp4Form form, hipStream_t st)
 template <int F, int T, int WR, int WT, int NST_> struct Fp4Tile {
     static constexpr int NWAVE = WR * WT, NT = 64 * NWAVE, NST = NST_;
     static constexpr int WI = F / WR / 32, U = T / WT / 32;
+    static constexpr bool DEEP = WI * U <= 2;          /* few products a step: latencies of LDS show */
     static constexpr int OFF_X = F * 128, STAGE = (F + T) * 128;
     static constexpr int LW = F / 8 / NWAVE, LX = T / 8 / NWAVE, VM = LW + LX;
     static constexpr int RING = NST * STAGE, TABLE = NT * 16;
     static constexpr int out_ld(int eb) { return F * eb + 16; }
-    /* tokens that leave together: all, or a row of waves after the other */
-    static constexpr int out_rows(int eb) { return T * out_ld(eb) <= 160 * 1024 ? T : T / WT; }
+    /* tokens that leave together */
+    static constexpr int out_rows(int eb) { return T * out_ld(eb) <= 160 * 1024 ? T : T / 2; }
     static constexpr int lds(int eb)
     {
         return RING + 2 * TABLE > out_rows(eb) * out_ld(eb) ? RING + 2 * TABLE : out_rows(eb) * out_ld(eb);
@@ -392,7 +198,7 @@ template <int F, int T, int WR, int WT, int NST_> struct Fp4Tile {
                       lds(4) <= 160 * 1024 && WI >= 1 && U >= 1, "tile");
 };
 
-template <int F, int T, int WR, int WT, int NST, bool GROUPED, int OUT>
+template <int F, int T, int WR, int WT, int NST, bool GROUPED, bool STREAM, int OUT>
 __global__ __launch_bounds__((Fp4Tile<F, T, WR, WT, NST>::NT)) void k_fp4_tile(Fp4Args a)
 {
     using C = Fp4Tile<F, T, WR, WT, NST>;
@@ -432,12 +238,12 @@ __global__ __launch_bounds__((Fp4Tile<F, T, WR, WT, NST>::NT)) void k_fp4_tile(F
     /* stages, whole pairs of them: a way out between the two, or the last one
      * after the loop, cost registers that the large tiles do not have */
     const int nst = (a.K + 511) / 512 * 2;
-    const __amdgpu_buffer_rsrc_t rw = buf_rsrc(t.w + (size_t)n0 * KB, (uint32_t)nf * KB);
     const size_t x0 = GROUPED ? 0 : (size_t)t.r0;
-    const __amdgpu_buffer_rsrc_t rx = buf_rsrc(a.Aq + x0 * KB, (GROUPED ? (uint32_t)a.n_a : (uint32_t)t.rows) * KB);
+    const uint8_t *const wb = t.w + (size_t)n0 * KB, *const xb = a.Aq + x0 * KB;
+    const uint32_t wlen = (uint32_t)nf * KB, xlen = (GROUPED ? (uint32_t)a.n_a : (uint32_t)t.rows) * KB;
     auto swz = [](int r, int c) { return c ^ ((r >> 1) & 7); };
-    uint32_t wo[C::LW], xo[C::LX];
-    int xc[C::LX];                                 /* the lane's block of a stage */
+    const int nreal = (a.K + 255) / 256;           /* stages with values */
+    uint32_t wo[C::LW], xo[C::LX], xl[C::LX];      /* xl: of the last of them, pieces past K out of range */
 #pragma unroll
     for (int i = 0; i < C::LW; i++) {
         const int r = 8 * (C::LW * wave + i) + lane / 8;
@@ -445,9 +251,9 @@ __global__ __launch_bounds__((Fp4Tile<F, T, WR, WT, NST>::NT)) void k_fp4_tile(F
     }
 #pragma unroll
     for (int i = 0; i < C::LX; i++) {
-        const int r = 8 * (C::LX * wave + i) + lane / 8, s = fp4_source<GROUPED>(a, t, r);
-        xc[i] = swz(r, lane & 7);
-        xo[i] = s < 0 ? BUF_OOB : (uint32_t)s * KB + 16u * (uint32_t)xc[i];
+        const int r = 8 * (C::LX * wave + i) + lane / 8, c = swz(r, lane & 7), s = fp4_source<GROUPED>(a, t, r);
+        xo[i] = s < 0 ? BUF_OOB : (uint32_t)s * KB + 16u * (uint32_t)c;
+        xl[i] = 8 * (nreal - 1) + c < nb ? xo[i] : BUF_OOB;
     }
     /* the row whose scales this thread fetches. Rows past the last weight row take
      * its, and so do tokens that are not there and threads without a row: what
@@ -457,31 +263,35 @@ __global__ __launch_bounds__((Fp4Tile<F, T, WR, WT, NST>::NT)) void k_fp4_tile(F
         const int s = fp4_source<GROUPED>(a, t, (int)threadIdx.x - F);
         if (s >= 0) srow = a.As + (x0 + s) * (size_t)nb;
     }
-    /* the stage this workgroup begins with: experts that run through K side by
-     * side would meet in the same memory channels */
-    const int rot = !GROUPED ? 0 : 2 * ((SHARED ? t.e * 4 + t.e / 8 : n0 / F * 2 + t.e) % (nst / 2));
-    auto block_of = [&](int st) { return st + rot < nst ? st + rot : st + rot - nst; };
-    /* the scales of stages 2 pair and 2 pair + 1 */
-    auto block_of_pair = [&](int pair) { return 8 * (2 * pair < nst ? block_of(2 * pair) : nst + 1); };
-    const int nb16 = max(nb, 16);                  /* shorter rows have no second pair to fetch */
-    auto fetch_scales = [&](int pair) {            /* w: 16 bytes that are there */
-        return fp4_scales_load(nb < 16 ? t.w : srow, block_of_pair(pair), nb16);
+    /* the scales of stages 2 pair and 2 pair + 1; of the last pair, which may end
+     * inside 16, from the start. No branch, and few instructions: in the loop a
+     * wave's own instructions are what small tiles wait for. */
+    const int last = nst / 2 - 1;
+    const u32x4 ends = fp4_scales(srow, 16 * last, nb);
+    auto fetch_scales = [&](int pair) -> u32x4 {   /* w: 16 bytes that are there */
+        return *(const DSV4_GLOBAL u32x4_any *)(nb < 16 ? t.w : srow + min(16 * pair, nb - 16));
     };
-    auto put_scales = [&](int pair, const u32x4 &v) { *(u32x4 *)(table + (pair & 1) * C::TABLE + 16 * threadIdx.x) = v; };
-    /* load i of a wave's share of stage st; past the end zeros, no traffic */
+    auto put_scales = [&](int pair, const u32x4 &v) {
+        u32x4 o;
+#pragma unroll
+        for (int j = 0; j < 4; j++) o[j] = pair == last ? ends[j] : v[j];
+        *(u32x4 *)(table + (pair & 1) * C::TABLE + 16 * threadIdx.x) = o;
+    };
+    /* load i of a wave's share of stage st; past the end zeros, no traffic (an
+     * empty buffer, and no scalar offset: the range check takes it off the size) */
     auto issue = [&](int st, int slot, int i) {
-        const int blk = block_of(min(st, nst - 1));
-        const uint32_t oob = st < nst ? 0u : BUF_OOB;
+        const bool in = st < nreal;
+        const int so = in ? 128 * st : 0;
         uint8_t *buf = lds + slot * C::STAGE;
         if (i < C::LW) {
-            buf_dma16(rw, (wo[min(i, C::LW - 1)] + 128u * blk) | oob, 0, buf + 1024 * (C::LW * wave + i));
+            buf_dma16<STREAM ? 2 : 0>(buf_rsrc(wb, in ? wlen : 0u), wo[min(i, C::LW - 1)], so, buf + 1024 * (C::LW * wave + i));
         } else {
             const int j = max(0, min(i - C::LW, C::LX - 1));
-            buf_dma16(rx, 8 * blk + xc[j] < nb && xo[j] != BUF_OOB ? (xo[j] + 128u * blk) | oob : BUF_OOB, 0,
+            buf_dma16<0>(buf_rsrc(xb, in ? xlen : 0u), st < nreal - 1 ? xo[j] : xl[j], so,
                       buf + C::OFF_X + 1024 * (C::LX * wave + j));
         }
     };
-    const u32x4 first = fp4_scales(srow, block_of_pair(0), nb);
+    const u32x4 first = fetch_scales(0);
     u32x4 held = fetch_scales(1);
 #pragma unroll
     for (int s = 0; s < NST; s++)
@@ -491,29 +301,17 @@ __global__ __launch_bounds__((Fp4Tile<F, T, WR, WT, NST>::NT)) void k_fp4_tile(F
 
     struct Op { v4i w[WI], x[U]; };
     struct Sc { uint32_t w[WI], x[U]; };
+    /* a wave's row groups are WT apart, so that a bucket's last few rows keep as
+     * many waves busy as they can */
     auto read_w = [&](Op &o, const uint8_t *buf, int i, int s) {
         const int r = 32 * (WI * wr + i) + rr;
         o.w[i] = *(const v4i *)(buf + r * 128 + 16 * swz(r, 2 * s + g));
     };
     auto read_x = [&](Op &o, const uint8_t *buf, int u, int s) {
-        const int r = 32 * (U * wt + u) + rr;
+        const int r = 32 * (WT * u + wt) + rr;
         o.x[u] = *(const v4i *)(buf + C::OFF_X + r * 128 + 16 * swz(r, 2 * s + g));
     };
     const uint32_t pick = g ? 0x07050301u : 0x06040200u;
-    /* the scales of stage st: byte s of a row's register is step s's */
-    auto read_scales = [&](Sc &o, int st) {
-        const uint8_t *p = table + (st / 2 & 1) * C::TABLE + 8 * (st & 1);
-#pragma unroll
-        for (int i = 0; i < WI; i++) {
-            const u32x2 v = *(const u32x2 *)(p + 16 * (32 * (WI * wr + i) + rr));
-            o.w[i] = __builtin_amdgcn_perm(v.y, v.x, pick);
-        }
-#pragma unroll
-        for (int u = 0; u < U; u++) {
-            const u32x2 v = *(const u32x2 *)(p + 16 * (F + 32 * (U * wt + u) + rr));
-            o.x[u] = __builtin_amdgcn_perm(v.y, v.x, pick);
-        }
-    };
     f32x16 acc[WI][U];
 #pragma unroll
     for (int i = 0; i < WI; i++)
@@ -522,62 +320,149 @@ __global__ __launch_bounds__((Fp4Tile<F, T, WR, WT, NST>::NT)) void k_fp4_tile(F
 #pragma unroll
             for (int e = 0; e < 16; e++) acc[i][u][e] = 0.0f;
     int slot = 0;
-    /* the products of `cur` (step S), the reads of `nxt` (step s of the stage in
-     * buf) and, with `load`, stage st's loads into slot `to`, spread among them */
-    auto step = [&](auto S, const Op &cur, const Sc &sc, Op &nxt, const uint8_t *buf, int s, bool load, int st, int to) {
-#pragma unroll
-        for (int q = 0; q < WI * U; q++) {
-            constexpr int N = WI * U, R = WI + U;
-            acc[q % WI][q / WI] = fp4_mfma32<decltype(S)::value>(cur.w[q % WI], cur.x[q / WI], acc[q % WI][q / WI], sc.w[q % WI], sc.x[q / WI]);
-            if (N >= 8 && q == 0) __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-            for (int j = 0; j < R; j++)
-                if (j * N / (R + 1) == q) {
-                    if (j < WI) read_w(nxt, buf, j, s);
-                    else read_x(nxt, buf, j - WI, s);
-                }
-            if (load) {
-#pragma unroll
-                for (int l = 0; l < C::VM; l++)
-                    if (l * N / C::VM == q) issue(st, to, l);
-            }
-            __builtin_amdgcn_sched_barrier(0);
-        }
-    };
     wait_vm<(NST - 1) * C::VM>();
     __builtin_amdgcn_s_waitcnt(0xC07F);
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
-    Op o0, o1;
-    Sc sc;
+    /* the whole sum of a wave with UA row groups that hold rows */
+    auto multiply = [&](auto ACTIVE) {
+        constexpr int UA = decltype(ACTIVE)::value, N = WI * UA, R = WI + UA;
+        /* the scales of stage st: byte s of a row's register is step s's */
+        auto read_scales = [&](Sc &o, int st) {
+            const uint8_t *p = table + (st / 2 & 1) * C::TABLE + 8 * (st & 1);
 #pragma unroll
-    for (int i = 0; i < WI; i++) read_w(o0, lds, i, 0);
+            for (int i = 0; i < WI; i++) {
+                const u32x2 v = *(const u32x2 *)(p + 16 * (32 * (WI * wr + i) + rr));
+                o.w[i] = __builtin_amdgcn_perm(v.y, v.x, pick);
+            }
 #pragma unroll
-    for (int u = 0; u < U; u++) read_x(o0, lds, u, 0);
-    read_scales(sc, 0);
-    /* stage st, the first or second of its pair. Nothing here branches: the
-     * compiler would move products over the barrier into another block. */
-    auto stage = [&](auto SECOND, int st) {
-        const uint8_t *buf = lds + slot * C::STAGE;
-        step(IC<0>{}, o0, sc, o1, buf, 1, false, 0, 0);
-        step(IC<1>{}, o1, sc, o0, buf, 2, false, 0, 0);
-        step(IC<2>{}, o0, sc, o1, buf, 3, false, 0, 0);
-        if constexpr (decltype(SECOND)::value) put_scales(st / 2 + 1, fp4_scales_shift(held, block_of_pair(st / 2 + 1), nb16));
-        __builtin_amdgcn_s_waitcnt(0xC07F);        /* this stage's operands are in registers */
-        wait_vm<(NST - 2) * C::VM>();              /* the wave's loads of the next have landed */
-        __builtin_amdgcn_s_barrier();
-        asm volatile("" ::: "memory");
-        if constexpr (decltype(SECOND)::value) held = fetch_scales(st / 2 + 2);
-        const int free = slot;
-        slot = slot + 1 == NST ? 0 : slot + 1;
-        Sc sn;
-        read_scales(sn, st + 1);
-        step(IC<3>{}, o1, sc, o0, lds + slot * C::STAGE, 0, true, st + NST, free);
-        sc = sn;
+            for (int u = 0; u < UA; u++) {
+                const u32x2 v = *(const u32x2 *)(p + 16 * (F + 32 * (WT * u + wt) + rr));
+                o.x[u] = __builtin_amdgcn_perm(v.y, v.x, pick);
+            }
+        };
+        /* the products of `cur` (step S), the reads of `nxt` (step s of the stage
+         * in buf) and, with `load`, stage st's loads into slot `to`, spread among
+         * them */
+        auto step = [&](auto S, const Op &cur, const Sc &sc, Op &nxt, const uint8_t *buf, int s, bool load, int st, int to) {
+            if constexpr (UA == 0) {
+                if (load) {
+#pragma unroll
+                    for (int l = 0; l < C::VM; l++) issue(st, to, l);
+                }
+            }
+#pragma unroll
+            for (int q = 0; q < N; q++) {
+                const int i = q % WI, u = q / WI;
+                acc[i][u] = fp4_mfma32<decltype(S)::value>(cur.w[i], cur.x[u], acc[i][u], sc.w[i], sc.x[u]);
+                if (N >= 8 && q == 0) __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int j = 0; j < R; j++)
+                    if (j * N / (R + 1) == q) {
+                        if (j < WI) read_w(nxt, buf, j, s);
+                        else read_x(nxt, buf, j - WI, s);
+                    }
+                if (load) {
+#pragma unroll
+                    for (int l = 0; l < C::VM; l++)
+                        if (l * N / C::VM == q) issue(st, to, l);
+                }
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        };
+        /* stage st, the first or second of its pair. Nothing here branches: the
+         * compiler would move products over the barrier into another block. */
+        auto meet = [&](auto SECOND, int st) {
+            if constexpr (decltype(SECOND)::value)
+                put_scales(st / 2 + 1, held);
+            __builtin_amdgcn_s_waitcnt(0xC07F);    /* this stage's operands are in registers */
+            wait_vm<(NST - 2) * C::VM>();          /* the wave's loads of the next have landed */
+            __builtin_amdgcn_s_barrier();
+            asm volatile("" ::: "memory");
+            if constexpr (decltype(SECOND)::value) held = fetch_scales(st / 2 + 2);
+        };
+        if constexpr (C::DEEP) {
+            /* the operands of a whole stage ahead */
+            struct Ops { Op s[4]; } o0, o1;
+            Sc c0, c1;
+            auto read = [&](Ops &o, const uint8_t *buf, int k) {   /* the k-th of 4 R */
+                if (k % R < WI) read_w(o.s[k / R], buf, k % R, k / R);
+                else read_x(o.s[k / R], buf, k % R - WI, k / R);
+            };
+            auto stage = [&](auto SECOND, int st, const Ops &cur, const Sc &sc, Ops &nxt, Sc &sn) {
+                meet(SECOND, st);
+                const int free = slot;
+                slot = slot + 1 == NST ? 0 : slot + 1;
+                const uint8_t *buf = lds + slot * C::STAGE;
+                if constexpr (UA == 0) {
+#pragma unroll
+                    for (int l = 0; l < C::VM; l++) issue(st + NST, free, l);
+                } else {
+                    read_scales(sn, st + 1);
+#pragma unroll
+                    for (int q = 0; q < 4 * N; q++) {
+                        const int s = q / N, i = q % N % WI, u = q % N / WI;
+                        acc[i][u] = s == 0   ? fp4_mfma32<0>(cur.s[s].w[i], cur.s[s].x[u], acc[i][u], sc.w[i], sc.x[u])
+                                    : s == 1 ? fp4_mfma32<1>(cur.s[s].w[i], cur.s[s].x[u], acc[i][u], sc.w[i], sc.x[u])
+                                    : s == 2 ? fp4_mfma32<2>(cur.s[s].w[i], cur.s[s].x[u], acc[i][u], sc.w[i], sc.x[u])
+                                             : fp4_mfma32<3>(cur.s[s].w[i], cur.s[s].x[u], acc[i][u], sc.w[i], sc.x[u]);
+#pragma unroll
+                        for (int k = 0; k < 4 * R; k++)
+                            if (k / (R / N + 1) == q || (q == 4 * N - 1 && k / (R / N + 1) > q)) read(nxt, buf, k);
+#pragma unroll
+                        for (int l = 0; l < C::VM; l++)
+                            if (l * 4 * N / C::VM == q) issue(st + NST, free, l);
+                        __builtin_amdgcn_sched_barrier(0);
+                    }
+                }
+            };
+            if constexpr (UA > 0) {
+#pragma unroll
+                for (int k = 0; k < 4 * R; k++) read(o0, lds, k);
+                read_scales(c0, 0);
+            }
+            for (int st = 0; st < nst; st += 2) {
+                stage(IC<0>{}, st, o0, c0, o1, c1);
+                stage(IC<1>{}, st + 1, o1, c1, o0, c0);
+            }
+        } else {
+            /* those of the next 64 values */
+            Op o0, o1;
+            Sc sc;
+            if constexpr (UA > 0) {
+#pragma unroll
+                for (int i = 0; i < WI; i++) read_w(o0, lds, i, 0);
+#pragma unroll
+                for (int u = 0; u < UA; u++) read_x(o0, lds, u, 0);
+                read_scales(sc, 0);
+            }
+            auto stage = [&](auto SECOND, int st) {
+                const uint8_t *buf = lds + slot * C::STAGE;
+                step(IC<0>{}, o0, sc, o1, buf, 1, false, 0, 0);
+                step(IC<1>{}, o1, sc, o0, buf, 2, false, 0, 0);
+                step(IC<2>{}, o0, sc, o1, buf, 3, false, 0, 0);
+                meet(SECOND, st);
+                const int free = slot;
+                slot = slot + 1 == NST ? 0 : slot + 1;
+                Sc sn;
+                if constexpr (UA > 0) read_scales(sn, st + 1);
+                step(IC<3>{}, o1, sc, o0, lds + slot * C::STAGE, 0, true, st + NST, free);
+                sc = sn;
+            };
+            for (int st = 0; st < nst; st += 2) {
+                stage(IC<0>{}, st);
+                stage(IC<1>{}, st + 1);
+            }
+        }
     };
-    for (int st = 0; st < nst; st += 2) {
-        stage(IC<0>{}, st);
-        stage(IC<1>{}, st + 1);
+    if constexpr (GROUPED && U <= 2) {
+        /* row groups of the wave that begin before the bucket's end */
+        const int ua = (t.rows - 32 * wt + 32 * WT - 1) / (32 * WT);
+        if (ua >= U) multiply(IC<U>{});
+        else if (U == 2 && ua == 1) multiply(IC<U / 2>{});
+        else multiply(IC<0>{});
+    } else {
+        multiply(IC<U>{});
     }
     /* the loads past the end, then the ring becomes the output tile */
     __builtin_amdgcn_s_waitcnt(0xC07F);
@@ -592,30 +477,28 @@ __global__ __launch_bounds__((Fp4Tile<F, T, WR, WT, NST>::NT)) void k_fp4_tile(F
     typedef u32x4 piece __attribute__((aligned(2)));
 #pragma unroll
     for (int m0 = 0; m0 < T; m0 += ROWS) {
-        if (ROWS == T || m0 == wt * ROWS) {
 #pragma unroll
-            for (int u = 0; u < U; u++) {
-                const int m = 32 * (U * wt + u) + rr;
-                const bool none = GROUPED && m < t.rows && fp4_source<GROUPED>(a, t, m) < 0;
-                if (none && wr == 0 && g == 0) atomicOr(a.status, ST_BAD_EXPERT_ID);
+        for (int u = m0 / (32 * WT); u < (m0 + ROWS) / (32 * WT); u++) {
+            const int m = 32 * (WT * u + wt) + rr;
+            const bool none = GROUPED && m < t.rows && fp4_source<GROUPED>(a, t, m) < 0;
+            if (none && wr == 0 && g == 0) atomicOr(a.status, ST_BAD_EXPERT_ID);
 #pragma unroll
-                for (int i = 0; i < WI; i++)
+            for (int i = 0; i < WI; i++)
 #pragma unroll
-                    for (int q = 0; q < 4; q++) {
-                        uint8_t *o = lds + (m - m0) * LD + (32 * (WI * wr + i) + 8 * q + 4 * g) * EB;
-                        float v[4];
+                for (int q = 0; q < 4; q++) {
+                    uint8_t *o = lds + (m - m0) * LD + (32 * (WI * wr + i) + 8 * q + 4 * g) * EB;
+                    float v[4];
 #pragma unroll
-                        for (int e = 0; e < 4; e++) v[e] = none ? __builtin_nanf("") : acc[i][u][4 * q + e];
-                        if constexpr (OUT == DSV4_HIP_F32) {
-                            *(f32x4 *)o = f32x4{v[0], v[1], v[2], v[3]};
-                        } else {
-                            u32x2 p;
-                            p.x = fp4_pack<OUT>(v[0], v[1]);
-                            p.y = fp4_pack<OUT>(v[2], v[3]);
-                            *(u32x2 *)o = p;
-                        }
+                    for (int e = 0; e < 4; e++) v[e] = none ? __builtin_nanf("") : acc[i][u][4 * q + e];
+                    if constexpr (OUT == DSV4_HIP_F32) {
+                        *(f32x4 *)o = f32x4{v[0], v[1], v[2], v[3]};
+                    } else {
+                        u32x2 p;
+                        p.x = fp4_pack<OUT>(v[0], v[1]);
+                        p.y = fp4_pack<OUT>(v[2], v[3]);
+                        *(u32x2 *)o = p;
                     }
-            }
+                }
         }
         __syncthreads();
         uint8_t *out = (uint8_t *)a.C + ((size_t)(t.r0 + m0) * a.N + n0) * EB;
@@ -638,44 +521,67 @@ __global__ __launch_bounds__((Fp4Tile<F, T, WR, WT, NST>::NT)) void k_fp4_tile(F
     }
 }
 
-template <int F, int T, int WR, int WT, int NST, bool GROUPED, int OUT>
-static hipError_t fp4_tile(const Fp4Args &a, Fp4Form form, hipStream_t st)
+template <int F, int T, int WR, int WT, int NST, bool GROUPED, bool STREAM, int OUT>
+static hipError_t fp4_tile(const Fp4Args &a, unsigned groups, hipStream_t st)
 {
     using C = Fp4Tile<F, T, WR, WT, NST>;
     constexpr int lds = C::lds(elem_bytes<OUT>());
     static uint64_t done = 0;
-    const hipError_t e = allow_lds((const void *)k_fp4_tile<F, T, WR, WT, NST, GROUPED, OUT>, lds, done);
+    const hipError_t e = allow_lds((const void *)k_fp4_tile<F, T, WR, WT, NST, GROUPED, STREAM, OUT>, lds, done);
     if (e != hipSuccess) return e;
-    const long groups = fp4_waves(form, a.M, a.N, GROUPED ? a.n_experts : 0) / C::NWAVE;
-    hipLaunchKernelGGL((k_fp4_tile<F, T, WR, WT, NST, GROUPED, OUT>), dim3((unsigned)groups), dim3(C::NT), lds, st, a);
+    hipLaunchKernelGGL((k_fp4_tile<F, T, WR, WT, NST, GROUPED, STREAM, OUT>), dim3(groups), dim3(C::NT), lds, st, a);
     return hipGetLastError();
 }
 
-template <bool GROUPED, int OUT>
+template <int OUT>
+static hipError_t fp4_one(const Fp4Args &a, hipStream_t st)
+{
+    const Fp4Form form = fp4_form(a.M, a.N, a.K);
+    const long waves = fp4_waves(form, a.M, a.N, 0);
+    if (waves > FP4_MAX_WAVES) return hipErrorInvalidConfiguration;
+    const unsigned groups = (unsigned)(waves / fp4_shape(form).waves);
+    switch (form) {
+    case FP4_SPLIT:
+        hipLaunchKernelGGL(k_fp4_split<OUT>, dim3(groups), dim3(512), 0, st, a);
+        return hipGetLastError();
+    case FP4_64x32: return fp4_tile<64, 32, 2, 1, 4, false, false, OUT>(a, groups, st);
+    case FP4_64x64: return fp4_tile<64, 64, 2, 2, 3, false, false, OUT>(a, groups, st);
+    case FP4_128x64: return fp4_tile<128, 64, 2, 2, 3, false, false, OUT>(a, groups, st);
+    case FP4_128x128: return fp4_tile<128, 128, 2, 2, 2, false, false, OUT>(a, groups, st);
+    case FP4_256x128: return fp4_tile<256, 128, 4, 2, 3, false, false, OUT>(a, groups, st);
+    default: return fp4_tile<256, 256, 4, 2, 2, false, false, OUT>(a, groups, st);
+    }
+}
+
+template <bool STREAM, int OUT>
+static hipError_t fp4_grouped(const Fp4Args &a, hipStream_t st)
+{
+    const Fp4Form form = fp4_grouped_form(a.M, a.N, a.K, a.n_experts);
+    const long waves = fp4_waves(form, a.M, a.N, a.n_experts);
+    if (waves > FP4_MAX_WAVES) return hipErrorInvalidConfiguration;
+    const unsigned groups = (unsigned)(waves / fp4_shape(form).waves);
+    switch (form) {
+    case FP4_64x32: return fp4_tile<64, 32, 2, 1, 4, true, STREAM, OUT>(a, groups, st);
+    case FP4_128x32: return fp4_tile<128, 32, 4, 1, 3, true, STREAM, OUT>(a, groups, st);
+    case FP4_128x64: return fp4_tile<128, 64, 2, 2, 3, true, STREAM, OUT>(a, groups, st);
+    default: return fp4_tile<256, 128, 4, 2, 3, true, false, OUT>(a, groups, st);
+    }
+}
+
+template <int OUT>
 static hipError_t fp4_launch(const Fp4Args &a, hipStream_t st)
 {
-    const Fp4Form form = GROUPED ? fp4_grouped_form(a.M, a.N, a.K, a.n_experts) : fp4_form(a.M, a.N, a.K);
-    if (fp4_waves(form, a.M, a.N, GROUPED ? a.n_experts : 0) > FP4_MAX_WAVES) return hipErrorInvalidConfiguration;
-    switch (form) {
-    case FP4_PAIR:
-        if constexpr (GROUPED) return fp4_pair<4, 2, 4, 2, GROUPED, OUT>(a, form, st);
-        else return fp4_pair<1, 1, 8, 4, GROUPED, OUT>(a, form, st);
-    case FP4_SPLIT: return fp4_split<2, 2, 8, GROUPED, OUT>(a, form, st);
-    case FP4_64x64: return fp4_tile<64, 64, 2, 2, 3, GROUPED, OUT>(a, form, st);
-    case FP4_128x128: return fp4_tile<128, 128, 2, 2, 2, GROUPED, OUT>(a, form, st);
-    case FP4_256x128: return fp4_tile<256, 128, 4, 2, 3, GROUPED, OUT>(a, form, st);
-    default: return fp4_tile<256, 256, 4, 2, 2, GROUPED, OUT>(a, form, st);
-    }
+    if (!a.table) return fp4_one<OUT>(a, st);
+    return fp4_stream(a.M, a.N, a.K, a.n_experts) ? fp4_grouped<true, OUT>(a, st) : fp4_grouped<false, OUT>(a, st);
 }
 
 hipError_t gemm_fp4_launch(const Fp4Args &a, int out_type, hipStream_t st)
 {
     if (a.M <= 0 || a.N <= 0 || a.K <= 0 || a.K % 32) return hipErrorInvalidValue;
-    const bool grouped = a.table != nullptr;
     switch (out_type) {
-    case DSV4_HIP_F32: return grouped ? fp4_launch<true, DSV4_HIP_F32>(a, st) : fp4_launch<false, DSV4_HIP_F32>(a, st);
-    case DSV4_HIP_BF16: return grouped ? fp4_launch<true, DSV4_HIP_BF16>(a, st) : fp4_launch<false, DSV4_HIP_BF16>(a, st);
-    case DSV4_HIP_F16: return grouped ? fp4_launch<true, DSV4_HIP_F16>(a, st) : fp4_launch<false, DSV4_HIP_F16>(a, st);
+    case DSV4_HIP_F32: return fp4_launch<DSV4_HIP_F32>(a, st);
+    case DSV4_HIP_BF16: return fp4_launch<DSV4_HIP_BF16>(a, st);
+    case DSV4_HIP_F16: return fp4_launch<DSV4_HIP_F16>(a, st);
     default: return hipErrorInvalidValue;
     }
 }

@@ -278,7 +278,9 @@ def product(lib, pkg, a, w, out=torch.float32, off=0):
 SHAPES = [(1, 1, 32), (1, 77, 4128), (3, 130, 96), (8, 4096, 544), (5, 1000, 256), (9, 33, 32), (17, 100, 4096),
           (32, 64, 512), (45, 257, 672), (100, 300, 1056), (200, 1500, 288), (333, 1024, 4096), (700, 1001, 160),
           (130, 8200, 224), (300, 8192, 512), (900, 3333, 320), (1100, 4104, 96), (700, 6000, 1184), (2048, 2048, 768),
-          (1300, 6001, 160), (2100, 8200, 288), (4100, 4097, 64), (2048, 8192, 1280), (4097, 4352, 32)]
+          (1300, 6001, 160), (2100, 8200, 288), (4100, 4097, 64), (2048, 8192, 1280), (4097, 4352, 32), (70, 15000, 544),
+          (40, 20001, 1120), (333, 2111, 2080), (500, 4111, 2080), (1001, 4099, 1056), (2803, 4100, 2080), (1999, 4097, 4128),
+          (1, 20000, 4128)]
 
 
 @pytest.mark.parametrize("M,N,K", SHAPES)
@@ -395,7 +397,9 @@ def grouped(lib, pkg, counts, N, K, n_a, seed, out=torch.float32, row_tok=True, 
     r = 0
     for e, n in enumerate(counts):
         if n:
-            want[r:r + n] = va[tok[r:r + n].long()] @ values(w[0][e], w[1][e]).t().contiguous()
+            vw = values(w[0][e], w[1][e]).t().contiguous()
+            want[r:r + n] = va[tok[r:r + n].long()] @ vw
+            assert K <= 5000 or float((va[tok[r:r + n].long()].abs() @ vw.abs()).max()) < 2 ** 20
         r += n
     return c, want
 
@@ -403,7 +407,11 @@ def grouped(lib, pkg, counts, N, K, n_a, seed, out=torch.float32, row_tok=True, 
 GROUPS = [([1], 1, 32), ([0, 0, 3, 0], 40, 96), ([1] * 40, 64, 544), ([5, 0, 9, 1, 12, 0, 3] * 3, 100, 288),
           ([20, 0, 31, 18, 2, 40], 77, 1056), ([64, 10, 0, 30, 33, 48], 130, 352), ([100, 0, 60, 130, 1, 90], 333, 608),
           ([300, 0, 3, 129, 128, 127, 500], 300, 416), ([0, 700, 0, 0, 20], 520, 96), ([2500, 3, 0, 300], 1000, 160),
-          ([1, 0, 1200, 0, 60, 200, 1100] * 2, 300, 288), ([1] * 300 + [0] * 700 + [4] * 24, 33, 64)]
+          ([1, 0, 1200, 0, 60, 200, 1100] * 2, 300, 288), ([1] * 300 + [0] * 700 + [4] * 24, 33, 64),
+          ([33, 64, 65, 0, 1, 31, 32, 96] * 4, 1000, 1056), ([257, 128, 129, 1, 0, 127, 31, 65] * 4, 1030, 544)]
+# weights that go past the caches: 128 MB and more of them, few rows an expert
+STREAMS = [([1, 0, 2, 1, 0, 0, 3] * 9, 2051, 4128), ([5, 0, 9, 1, 12, 0, 3] * 9, 2051, 4128),
+           ([60, 33, 64, 0, 1, 20, 50, 31], 8200, 8224)]
 
 
 @pytest.mark.parametrize("counts,N,K", GROUPS)
@@ -411,6 +419,14 @@ def test_experts(lib, pkg, counts, N, K):
     lib.status()
     c, want = grouped(lib, pkg, counts, N, K, 211, len(counts) + N)
     assert torch.equal(c.double(), want) and lib.status() == 0
+
+
+@pytest.mark.parametrize("out", TYPES)
+@pytest.mark.parametrize("counts,N,K", STREAMS)
+def test_experts_past_the_caches(lib, pkg, counts, N, K, out):
+    """K beyond 5,000: the sums of magnitudes, which bound every partial sum, are below 2^20"""
+    c, want = grouped(lib, pkg, counts, N, K, 211, len(counts) + N, out)
+    assert torch.equal(c, want.to(out))
 
 
 @pytest.mark.parametrize("out", [torch.bfloat16, torch.float16])

@@ -18,9 +18,10 @@ extern "C" {
 int c_form(int M, int N, int K) { return fp4_form(M, N, K); }
 int c_grouped(int M, int N, int K, int ne) { return fp4_grouped_form(M, N, K, ne); }
 long c_waves(int form, long M, long N, long ne) { return fp4_waves((Fp4Form)form, M, N, ne); }
-int c_shape(int form, int grouped, int what)
+int c_stream(int M, int N, int K, int ne) { return fp4_stream(M, N, K, ne); }
+int c_shape(int form, int what)
 {
-    const Fp4Shape s = fp4_shape((Fp4Form)form, grouped);
+    const Fp4Shape s = fp4_shape((Fp4Form)form);
     return what == 0 ? s.F : what == 1 ? s.TR : s.waves;
 }
 int c_last() { return FP4_256x256; }
@@ -42,18 +43,22 @@ def rules(tmp_path_factory):
 
 def test_gpu_tests_reach_every_form(rules):
     """each with rows, features and K that end inside a tile"""
-    every = set(range(1, rules.c_last() + 1))
+    every = {rules.c_form(M, N, K) for N in (100, 1024, 4096, 32768) for K in (256, 1024, 4096)
+             for M in (1, 8, 30, 100, 333, 700, 1500, 2803, 4096, 8192)}
     ragged = set()
     for M, N, K in test_gpu_mxfp4.SHAPES:
         f = rules.c_form(M, N, K)
-        if M % rules.c_shape(f, 0, 1) and N % rules.c_shape(f, 0, 0) and K % 256:
+        if M % rules.c_shape(f, 1) and N % rules.c_shape(f, 0) and K % 256:
             ragged.add(f)
-    assert {rules.c_form(*s) for s in test_gpu_mxfp4.SHAPES} == ragged == every
+    assert {rules.c_form(*s) for s in test_gpu_mxfp4.SHAPES} == ragged == every and len(every) == 7
 
 
 def test_gpu_tests_reach_every_form_of_the_experts_product(rules):
-    forms = {rules.c_grouped(sum(c) + 5, N, K, len(c)) for c, N, K in test_gpu_mxfp4.GROUPS}
-    assert forms == {rules.c_grouped(M, N, K, E) for E in (1, 8, 256) for N in (64, 2048, 4096) for K in (512, 4096)
+    """and each with weights that go past the caches"""
+    def of(M, N, K, E):
+        return rules.c_grouped(M, N, K, E), rules.c_stream(M, N, K, E)
+    forms = {of(sum(c) + 5, N, K, len(c)) for c, N, K in test_gpu_mxfp4.GROUPS + test_gpu_mxfp4.STREAMS}
+    assert forms == {of(M, N, K, E) for E in (1, 8, 64, 256) for N in (64, 512, 2048, 4096) for K in (512, 1024, 4096)
                      for M in range(1, 300 * E, 1 + E // 2)}
 
 
@@ -62,7 +67,7 @@ def test_waves_of_a_launch(rules, ne):
     """A tile for every F features and TR rows, one more row tile for each expert;
     rows and features of 2^31 - 1 do not wrap."""
     for form in range(1, rules.c_last() + 1):
-        F, TR, waves = (rules.c_shape(form, int(ne > 0), i) for i in range(3))
+        F, TR, waves = (rules.c_shape(form, i) for i in range(3))
         for M, N in ((1, 1), (TR, F), (TR + 1, F + 1), (1000, 777), ((1 << 31) - 1, (1 << 31) - 1)):
             rows = M // TR + min(M, ne) if ne else -(-M // TR)
             assert rules.c_waves(form, M, N, ne) == rows * -(-N // F) * waves
@@ -71,7 +76,7 @@ def test_waves_of_a_launch(rules, ne):
 @pytest.mark.parametrize("counts", [[0, 0, 5], [1] * 300, [127, 129, 0, 31, 33], [2000], [257, 255, 1, 1]])
 def test_waves_hold_every_bucket(rules, counts):
     for form in range(1, rules.c_last() + 1):
-        F, TR, waves = (rules.c_shape(form, 1, i) for i in range(3))
+        F, TR, waves = (rules.c_shape(form, i) for i in range(3))
         tiles = sum(-(-c // TR) for c in counts)
         assert rules.c_waves(form, sum(counts), 100, len(counts)) >= tiles * -(-100 // F) * waves
 
