@@ -98,7 +98,10 @@ __device__ __forceinline__ uint32_t mxfp4_code64(double v)
 } // namespace
 
 /* Four lanes hold a block, eight elements each; a thread takes NU units, 256
- * apart. */
+ * apart. us, NU 1 / 2 / 4: 4,206 rows of 2,048 bf16 5.3 / 4.8 / 5.2, SwiGLU 10.7 /
+ * 11.6 / 13.7; 24,576 rows 23.1 / 20.9 / 21.0, SwiGLU 43.9 / 44.3 / 44.0. Bound: HBM
+ * (24,576 rows 6.1 TB/s, SwiGLU 5.2), the vector unit for SwiGLU of fewer rows
+ * (4,206: 3.6 TB/s), latency for a few. */
 template <int TYPE, bool SWIGLU, int NU>
 __global__ __launch_bounds__(256) void k_quant_mxfp4(QuantMxfp4Args a)
 {
@@ -202,85 +205,80 @@ __global__ __launch_bounds__(256) void k_quant_mxfp4(QuantMxfp4Args a)
     }
 }
 
-/* Columns: a wave takes 32 rows of 128 columns, two a lane, so that a block lies
- * in one lane; eight waves take eight blocks of the same columns and meet in
- * LDS, from which 128-byte pieces of a's columns leave. */
+/* Columns: a wave takes 32 rows of 64 columns, one a lane, so that a block lies in
+ * one lane; eight waves take as many blocks of the same columns and meet in LDS,
+ * from which 128-byte pieces of a's columns leave. Every load is made, from an
+ * element that is there, and what lies behind the last row is zeroed afterwards:
+ * loads under conditions waited for each other. Bound: the rows' latency, then
+ * HBM (1,024 rows of 4,096 bf16 3.3 us, 2,803 6.7, 24,576 of 2,048 28 us, 4.6 TB/s;
+ * under conditions 9.9 and 11.6; two columns a lane 4.0, 7.4 and 27, four waves
+ * 3.3, 6.7 and 29). */
 template <int TYPE>
 __global__ __launch_bounds__(512) void k_quant_mxfp4_t(QuantMxfp4Args a)
 {
-    constexpr int NC = 128, NB = 8, EB = elem_bytes<TYPE>(), LD = NB * 16 + 16;
+    constexpr int NC = 64, NB = 8, EB = elem_bytes<TYPE>(), LD = NB * 16 + 16;
     __shared__ __align__(16) uint8_t codes[NC * LD];
     __shared__ __align__(8) uint8_t bytes[NC][NB];
     const int lane = threadIdx.x & 63, wave = wave_in_group();
     const uint32_t ct = ((uint32_t)a.k + NC - 1) / NC;
     const int c0 = (int)(blockIdx.x % ct) * NC, b0 = (int)(blockIdx.x / ct) * NB, nb = (a.n + 31) / 32;
-    const int c = c0 + 2 * lane, r0 = (b0 + wave) * 32;
-    /* two elements, at any alignment of one */
-    typedef uint32_t Pair __attribute__((ext_vector_type(EB / 2)));
-    typedef Pair PairAt __attribute__((aligned(EB)));
-    Pair raw[32];
-    const uint8_t *src = (const uint8_t *)a.a + ((size_t)r0 * (size_t)a.ld + c) * EB;
+    const int r0 = (b0 + wave) * 32, rows = max(a.n - r0, 0);
+    const uint8_t *src =
+        (const uint8_t *)a.a + ((size_t)min(r0, a.n - 1) * (size_t)a.ld + min(c0 + lane, a.k - 1)) * EB;
+    const size_t step = (size_t)a.ld * EB;
+    uint32_t raw[32];
 #pragma unroll
     for (int i = 0; i < 32; i++) {
-        raw[i] = Pair(0u);
-        if (r0 + i < a.n) {
-            const DSV4_GLOBAL uint8_t *p = (const DSV4_GLOBAL uint8_t *)(src + (size_t)i * (size_t)a.ld * EB);
-            if (c + 1 < a.k) raw[i] = *(const DSV4_GLOBAL PairAt *)p;
-            else if (c < a.k) {
-                if constexpr (EB == 4) raw[i][0] = *(const DSV4_GLOBAL uint32_t *)p;
-                else raw[i][0] = *(const DSV4_GLOBAL uint16_t *)p;
-            }
-        }
+        const uint8_t *p = src + (size_t)min(i, max(rows - 1, 0)) * step;
+        if constexpr (EB == 4) raw[i] = *gptr((const uint32_t *)p);
+        else raw[i] = *gptr((const uint16_t *)p);
     }
+    if (rows < 32) {
 #pragma unroll
-    for (int h = 0; h < 2; h++) {
-        auto elem = [&](int i) -> float {
-            if constexpr (EB == 4) return __uint_as_float(raw[i][h]);
-            else return widen16<TYPE>(h ? raw[i][0] >> 16 : raw[i][0] & 0xFFFFu);
-        };
-        uint32_t m = 0;
-#pragma unroll
-        for (int i = 0; i < 32; i++) m = max(m, __float_as_uint(elem(i)) & 0x7FFFFFFFu);
-        const uint32_t byte = mxfp4_byte(m);
-        const float inv = mxfp4_inverse(byte);
-        u32x4 q;
-#pragma unroll
-        for (int d = 0; d < 4; d++) {
-            float v[MU];
-#pragma unroll
-            for (int e = 0; e < MU; e++) v[e] = __fmul_rn(elem(8 * d + e), inv);
-            q[d] = byte == 255u ? 0u : mxfp4_codes(v);
-        }
-        *(u32x4 *)(codes + (2 * lane + h) * LD + 16 * wave) = q;
-        bytes[2 * lane + h][wave] = (uint8_t)byte;
+        for (int i = 0; i < 32; i++) raw[i] = i < rows ? raw[i] : 0u;
     }
+    auto elem = [&](int i) -> float {
+        if constexpr (EB == 4) return __uint_as_float(raw[i]);
+        else return widen16<TYPE>(raw[i]);
+    };
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < 32; i++) m = max(m, __float_as_uint(elem(i)) & 0x7FFFFFFFu);
+    const uint32_t byte = mxfp4_byte(m);
+    const float inv = mxfp4_inverse(byte);
+    u32x4 q;
+#pragma unroll
+    for (int d = 0; d < 4; d++) {
+        float v[MU];
+#pragma unroll
+        for (int e = 0; e < MU; e++) v[e] = __fmul_rn(elem(8 * d + e), inv);
+        q[d] = byte == 255u ? 0u : mxfp4_codes(v);
+    }
+    *(u32x4 *)(codes + lane * LD + 16 * wave) = q;
+    bytes[lane][wave] = (uint8_t)byte;
     __syncthreads();
-    const int have = min(NB, nb - b0);
-    for (int i = threadIdx.x; i < NC * NB; i += 512) {
-        const int col = i / NB, b = i % NB;
-        if (c0 + col >= a.k || b >= have) continue;
-        const size_t at = (size_t)(c0 + col) * nb + b0 + b;
-        *(DSV4_GLOBAL u32x4 *)(a.Q + 16 * at) = *(const u32x4 *)(codes + col * LD + 16 * b);
-        ((DSV4_GLOBAL uint8_t *)a.S)[at] = bytes[col][b];
-    }
+    const int col = threadIdx.x / NB, b = threadIdx.x % NB;
+    if (c0 + col >= a.k || b0 + b >= nb) return;
+    const size_t at = (size_t)(c0 + col) * nb + b0 + b;
+    *(DSV4_GLOBAL u32x4 *)(a.Q + 16 * at) = *(const u32x4 *)(codes + col * LD + 16 * b);
+    ((DSV4_GLOBAL uint8_t *)a.S)[at] = bytes[col][b];
 }
 
 template <int TYPE>
 static hipError_t quant_mxfp4_t(const QuantMxfp4Args &a, Mxfp4Rows rows, hipStream_t st)
 {
     if (rows == MXFP4_COLUMNS) {
-        const size_t groups = (((size_t)a.n + 255) / 256) * (((size_t)a.k + 127) / 128);
+        const size_t groups = (((size_t)a.n + 255) / 256) * (((size_t)a.k + 63) / 64);
         if (groups >= 1u << 23) return hipErrorInvalidConfiguration;
         hipLaunchKernelGGL(k_quant_mxfp4_t<TYPE>, dim3((unsigned)groups), dim3(512), 0, st, a);
         return hipGetLastError();
     }
-    constexpr int NU = 4;
-    const size_t units = (size_t)a.n * (a.k / MU), groups = (units + 256 * NU - 1) / (256 * NU);
+    const size_t units = (size_t)a.n * (a.k / MU);
     if (units >> 32) return hipErrorInvalidConfiguration;
     if (rows == MXFP4_SWIGLU)
-        hipLaunchKernelGGL((k_quant_mxfp4<TYPE, true, NU>), dim3((unsigned)groups), dim3(256), 0, st, a);
+        hipLaunchKernelGGL((k_quant_mxfp4<TYPE, true, 1>), dim3((unsigned)((units + 255) / 256)), dim3(256), 0, st, a);
     else
-        hipLaunchKernelGGL((k_quant_mxfp4<TYPE, false, NU>), dim3((unsigned)groups), dim3(256), 0, st, a);
+        hipLaunchKernelGGL((k_quant_mxfp4<TYPE, false, 2>), dim3((unsigned)((units + 511) / 512)), dim3(256), 0, st, a);
     return hipGetLastError();
 }
 

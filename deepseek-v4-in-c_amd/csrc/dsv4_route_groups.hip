@@ -11,12 +11,13 @@
  *   sqrt(x) there)
  * Scores are fp64 rounded once to fp32 (sqrt(softplus) the router's own bits,
  * dsv4_route_math.h); the choice compares fp32 sums, so it depends on no order
- * and on no exp's last bit.
+ * and, but for a score within 2^-20 of a step of a rounding border, on no exp's
+ * last bit.
  *
- * A wave takes a token, lane l the NJ experts from l NJ on, so the lowest id of
- * equals is the lowest lane's first. A choice is one key an expert, its fp32
- * bits in an order of unsigned numbers, 0 for an expert that is not there; a pick
- * is a wave maximum and a ballot.
+ * A token is held by L lanes, 16 (four tokens a wave) or 64, lane l the experts 4
+ * l + 4 L q + i, i < 4, q < NQ: rows are read in whole lines. A choice is one key
+ * an expert, its fp32 bits in an order of unsigned numbers, 0 for an expert that
+ * is not there. A pick is a maximum over the lanes and the least id among equals.
  */
 #include "dsv4_elem.h"
 #include "dsv4_gate_route.h"
@@ -25,298 +26,489 @@ namespace dsv4 {
 
 namespace {
 
-/* the lane's NJ logits of a token's row; past the last expert -inf */
-template <int TYPE, int NJ>
-__device__ __forceinline__ void load_logits(const void *logits, size_t token, int ne, int e0, float (&x)[NJ])
+constexpr float NO_EXPERT = -__builtin_inff();     /* the logit of one that is not there */
+
+/* four consecutive elements of a row from e on, at any alignment of one; past
+ * the row's end NO_EXPERT */
+template <int TYPE>
+__device__ __forceinline__ void load4(const void *row, int e, int ne, float (&x)[4])
 {
     constexpr int EB = elem_bytes<TYPE>();
-    const uint8_t *row = (const uint8_t *)logits + (token * ne + e0) * EB;
-    typedef float F32 __attribute__((ext_vector_type(NJ), aligned(4)));
-    typedef uint16_t F16 __attribute__((ext_vector_type(NJ), aligned(2)));
-    if (e0 + NJ <= ne) {
+    typedef uint32_t W4 __attribute__((ext_vector_type(4), aligned(4)));
+    typedef uint16_t H4 __attribute__((ext_vector_type(4), aligned(2)));
+    const uint8_t *p = (const uint8_t *)row + (size_t)e * EB;
+    if (e + 4 <= ne) {
         if constexpr (EB == 4) {
-            const F32 v = *(const DSV4_GLOBAL F32 *)row;
+            const W4 v = *(const DSV4_GLOBAL W4 *)p;
 #pragma unroll
-            for (int j = 0; j < NJ; j++) x[j] = v[j];
+            for (int i = 0; i < 4; i++) x[i] = __uint_as_float(v[i]);
         } else {
-            const F16 v = *(const DSV4_GLOBAL F16 *)row;
+            const H4 v = *(const DSV4_GLOBAL H4 *)p;
 #pragma unroll
-            for (int j = 0; j < NJ; j++) x[j] = widen16<TYPE>(v[j]);
+            for (int i = 0; i < 4; i++) x[i] = widen16<TYPE>(v[i]);
         }
     } else {
 #pragma unroll
-        for (int j = 0; j < NJ; j++) {
-            x[j] = -__builtin_inff();
-            if (e0 + j < ne) {
-                if constexpr (EB == 4) x[j] = ((const DSV4_GLOBAL float *)row)[j];
-                else x[j] = widen16<TYPE>(((const DSV4_GLOBAL uint16_t *)row)[j]);
+        for (int i = 0; i < 4; i++) {
+            x[i] = NO_EXPERT;
+            if (e + i < ne) {
+                if constexpr (EB == 4) x[i] = gptr((const float *)p)[i];
+                else x[i] = widen16<TYPE>(gptr((const uint16_t *)p)[i]);
             }
         }
     }
 }
-
-__device__ __forceinline__ double wave_sum_f64(double v)
+template <int TYPE>
+__device__ __forceinline__ void store4(void *row, int e, int ne, const float (&x)[4])
 {
+    constexpr int EB = elem_bytes<TYPE>();
+    typedef uint32_t W4 __attribute__((ext_vector_type(4), aligned(4)));
+    typedef uint16_t H4 __attribute__((ext_vector_type(4), aligned(2)));
+    uint8_t *p = (uint8_t *)row + (size_t)e * EB;
+    if (e + 4 <= ne) {
+        if constexpr (EB == 4) {
+            W4 v;
 #pragma unroll
-    for (int d = 1; d < 64; d <<= 1) v += __shfl_xor(v, d, 64);
+            for (int i = 0; i < 4; i++) v[i] = __float_as_uint(x[i]);
+            *(DSV4_GLOBAL W4 *)p = v;
+        } else {
+            H4 v;
+#pragma unroll
+            for (int i = 0; i < 4; i++) v[i] = (uint16_t)narrow16<TYPE>(x[i]);
+            *(DSV4_GLOBAL H4 *)p = v;
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            if (e + i >= ne) break;
+            if constexpr (EB == 4) ((DSV4_GLOBAL float *)p)[i] = x[i];
+            else ((DSV4_GLOBAL uint16_t *)p)[i] = (uint16_t)narrow16<TYPE>(x[i]);
+        }
+    }
+}
+template <int TYPE>
+__device__ __forceinline__ float load1(const void *row, int e)
+{
+    if constexpr (TYPE == DSV4_HIP_F32) return gptr((const float *)row)[e];
+    else return widen16<TYPE>(gptr((const uint16_t *)row)[e]);
+}
+template <int TYPE>
+__device__ __forceinline__ void store1(void *row, int e, float v)
+{
+    if constexpr (TYPE == DSV4_HIP_F32) ((DSV4_GLOBAL float *)row)[e] = v;
+    else ((DSV4_GLOBAL uint16_t *)row)[e] = (uint16_t)narrow16<TYPE>(v);
+}
+
+/* Over the L lanes of a token, to all of them, in an order of its own. */
+template <int L, class OP>
+__device__ __forceinline__ uint32_t over_lanes(uint32_t v, OP op)
+{
+    v = op(v, dpp_u32<DPP_QUAD_1032>(v, v));
+    v = op(v, dpp_u32<DPP_QUAD_2301>(v, v));
+    v = op(v, dpp_u32<DPP_ROW_HALF_MIRROR>(v, v));
+    v = op(v, dpp_u32<DPP_ROW_MIRROR>(v, v));
+    if constexpr (L == 64) {
+        v = op(v, dpp_u32<DPP_ROW_BCAST15, 0xA>(v, v));
+        v = op(v, dpp_u32<DPP_ROW_BCAST31, 0xC>(v, v));
+        v = (uint32_t)__builtin_amdgcn_readlane((int)v, 63);
+    }
     return v;
 }
-__device__ __forceinline__ float wave_max_f32(float v)
+template <int L>
+__device__ __forceinline__ double sum_lanes(double v)
 {
 #pragma unroll
-    for (int d = 1; d < 64; d <<= 1) v = fmaxf(v, __shfl_xor(v, d, 64));
+    for (int d = 1; d < L; d <<= 1) v += __shfl_xor(v, d, 64);
     return v;
 }
+template <int L>
+__device__ __forceinline__ bool any_lane(bool b, int lane)
+{
+    const uint64_t m = __builtin_amdgcn_ballot_w64(b);
+    return L == 64 ? m != 0 : (m >> (lane & 48) & 0xFFFFu) != 0;
+}
 
-/* order-preserving bits of a choice; 0: not there. A choice is never -0: a
- * score is not, and +0 plus a bias of -0 is +0. */
-__device__ __forceinline__ uint32_t choice_key(float c)
+/* order-preserving bits of a number that is not NaN; larger for larger ones. -0
+ * does not occur: a score is none, and +0 plus a bias of -0 is +0. */
+__device__ __forceinline__ uint32_t order_of(float c)
 {
     const uint32_t u = __float_as_uint(c);
-    return !(c > -__builtin_inff()) ? 0u : (u & 0x80000000u) ? ~u : (u | 0x80000000u);
+    return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
 }
-__device__ __forceinline__ float key_choice(uint32_t k) { return __uint_as_float((k & 0x80000000u) ? k ^ 0x80000000u : ~k); }
+__device__ __forceinline__ float of_order(uint32_t k) { return __uint_as_float((k & 0x80000000u) ? k ^ 0x80000000u : ~k); }
 
-/* softmax's largest logit and sum over a token's experts */
-struct Norm { float top; double inv; };
-template <int NJ>
-__device__ __forceinline__ Norm softmax_norm(const float (&x)[NJ], double (&p)[NJ])
+/* e^x in fp64 for |x| <= 708 (beyond: clamped): x = k ln 2 + r, |r| <= 0.347, and
+ * r's Taylor series to r^12, cut at 0.347^13 / 13! = 2^-52 of it. */
+__device__ __forceinline__ double exp64(double x)
 {
-    Norm o;
-    float top = x[0];
+    x = fmin(fmax(x, -708.0), 708.0);
+    const double k = rint(x * 1.4426950408889634);
+    const double r = fma(k, -2.3190468138462996e-17, fma(k, -0.6931471805599453, x));
+    double p = 1.0 / 479001600;
+    p = fma(p, r, 1.0 / 39916800);
+    p = fma(p, r, 1.0 / 3628800);
+    p = fma(p, r, 1.0 / 362880);
+    p = fma(p, r, 1.0 / 40320);
+    p = fma(p, r, 1.0 / 5040);
+    p = fma(p, r, 1.0 / 720);
+    p = fma(p, r, 1.0 / 120);
+    p = fma(p, r, 1.0 / 24);
+    p = fma(p, r, 1.0 / 6);
+    p = fma(p, r, 0.5);
+    p = fma(p, r, 1.0);
+    p = fma(p, r, 1.0);
+    return __builtin_amdgcn_ldexp(p, (int)k);
+}
+/* 1 / v for normal v whose reciprocal is normal: two Newton steps */
+__device__ __forceinline__ double rcp64(double v)
+{
+    double y = __builtin_amdgcn_rcp(v);
+    y = fma(fma(-v, y, 1.0), y, y);
+    return fma(fma(-v, y, 1.0), y, y);
+}
+__device__ __forceinline__ double sigmoid64(float x) { return rcp64(1.0 + exp64(-(double)x)); }
+__device__ __forceinline__ double softplus64(float x) { return x > 20.0f ? (double)x : log1p(exp((double)x)); }
+
+/* softmax over a token's L x 4 NQ logits: e^(x - top), top and 1 / sum; an expert
+ * that is not there adds nothing, a token without experts has inv 0 */
+struct Norm { float top; double inv; };
+template <int L, int NQ>
+__device__ __forceinline__ Norm softmax_norm(const float (&x)[NQ][4], double (&p)[NQ][4])
+{
+    uint32_t top = 0;
 #pragma unroll
-    for (int j = 1; j < NJ; j++) top = fmaxf(top, x[j]);
-    o.top = wave_max_f32(top);
+    for (int q = 0; q < NQ; q++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) top = max32(top, order_of(x[q][i]));
+    Norm o;
+    o.top = of_order(over_lanes<L>(top, max32));
     double sum = 0.0;
 #pragma unroll
-    for (int j = 0; j < NJ; j++) {
-        p[j] = x[j] > -__builtin_inff() ? exp((double)x[j] - (double)o.top) : 0.0;
-        sum += p[j];
-    }
-    sum = wave_sum_f64(sum);
+    for (int q = 0; q < NQ; q++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            p[q][i] = x[q][i] > NO_EXPERT ? exp64((double)x[q][i] - (double)o.top) : 0.0;
+            sum += p[q][i];
+        }
+    sum = sum_lanes<L>(sum);
     o.inv = sum > 0.0 ? 1.0 / sum : 0.0;
     return o;
 }
 
-__device__ __forceinline__ double sigmoid64(float x) { return 1.0 / (1.0 + exp(-(double)x)); }
+/* one score as the forward call gives it */
+template <int SCORE>
+__device__ __forceinline__ float score32(float x, const Norm &m)
+{
+    if constexpr (SCORE == DSV4_HIP_SOFTMAX) return x > NO_EXPERT ? (float)(exp64((double)x - (double)m.top) * m.inv) : 0.0f;
+    else if constexpr (SCORE == DSV4_HIP_SIGMOID) return (float)sigmoid64(x);
+    else return route_orig(x);
+}
 
 } // namespace
 
-template <int TYPE, int SCORE, int NJ>
+template <int TYPE, int SCORE, int L, int NQ>
 __global__ __launch_bounds__(256) void k_route_groups(RouteGroupsArgs a)
 {
-    const int lane = threadIdx.x & 63, ne = a.r.n_experts, topk = a.r.topk, e0 = lane * NJ;
-    const long t = (long)blockIdx.x * 4 + wave_in_group();
-    if (t >= a.n) return;
-    float x[NJ], s[NJ];
-    load_logits<TYPE, NJ>(a.logits, (size_t)t, ne, e0, x);
+    constexpr int TPW = 64 / L;                    /* tokens of a wave */
+    const int lane = threadIdx.x & 63, l = lane % L, ne = a.r.n_experts, topk = a.r.topk;
+    const long t0 = ((long)blockIdx.x * 4 + wave_in_group()) * TPW, t = t0 + lane / L;
+    if (t0 >= a.n) return;
+    const bool there = t < a.n;                    /* tokens past the last: the last again, not stored */
+    const size_t tok = (size_t)min(t, (long)a.n - 1);
+    const void *row = (const uint8_t *)a.logits + tok * ne * elem_bytes<TYPE>();
+    auto id_of = [&](int q, int i) { return 4 * l + 4 * L * q + i; };
+    float x[NQ][4];
+#pragma unroll
+    for (int q = 0; q < NQ; q++) load4<TYPE>(row, id_of(q, 0), ne, x[q]);
+    float b[NQ][4];
+#pragma unroll
+    for (int q = 0; q < NQ; q++) {
+        if (a.bias) load4<DSV4_HIP_F32>(a.bias, id_of(q, 0), ne, b[q]);
+        else
+#pragma unroll
+            for (int i = 0; i < 4; i++) b[q][i] = 0.0f;
+    }
     bool bad = false;
 #pragma unroll
-    for (int j = 0; j < NJ; j++) bad |= !(x[j] < __builtin_inff());
-    const bool refused = __builtin_amdgcn_ballot_w64(bad) != 0;
-    if constexpr (SCORE == DSV4_HIP_SOFTMAX) {
-        double p[NJ];
-        const Norm m = softmax_norm<NJ>(x, p);
+    for (int q = 0; q < NQ; q++)
 #pragma unroll
-        for (int j = 0; j < NJ; j++) s[j] = (float)(p[j] * m.inv);
-    } else {
+        for (int i = 0; i < 4; i++) bad |= !(x[q][i] < __builtin_inff());
+    const bool refused = any_lane<L>(bad, lane);
+    uint32_t key[NQ][4];
+    Norm m = {0.0f, 0.0};
+    {
+        float s[NQ][4];
+        if constexpr (SCORE == DSV4_HIP_SOFTMAX) {
+            double p[NQ][4];
+            m = softmax_norm<L, NQ>(x, p);
 #pragma unroll
-        for (int j = 0; j < NJ; j++) s[j] = SCORE == DSV4_HIP_SIGMOID ? (float)sigmoid64(x[j]) : route_orig(x[j]);
-    }
-    if (a.scores) {
-        float *o = a.scores + (size_t)t * ne + e0;
+            for (int q = 0; q < NQ; q++)
 #pragma unroll
-        for (int j = 0; j < NJ; j++)
-            if (e0 + j < ne) o[j] = refused ? __builtin_nanf("") : s[j];
-    }
-    uint32_t key[NJ];
+                for (int i = 0; i < 4; i++) s[q][i] = (float)(p[q][i] * m.inv);
+        } else {
 #pragma unroll
-    for (int j = 0; j < NJ; j++) {
-        const float c = a.bias && e0 + j < ne ? s[j] + a.bias[e0 + j] : s[j];
-        key[j] = x[j] > -__builtin_inff() && !refused ? choice_key(c) : 0u;
+            for (int q = 0; q < NQ; q++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) s[q][i] = score32<SCORE>(x[q][i], m);
+        }
+#pragma unroll
+        for (int q = 0; q < NQ; q++) {
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const float c = __fadd_rn(s[q][i], b[q][i]);
+                key[q][i] = x[q][i] > NO_EXPERT && c > NO_EXPERT && !refused ? order_of(c) : 0u;
+                if (refused) s[q][i] = __builtin_nanf("");
+            }
+            if (a.scores && there && id_of(q, 0) < ne) store4<DSV4_HIP_F32>(a.scores + tok * ne, id_of(q, 0), ne, s[q]);
+        }
     }
     if (a.r.topk_group < a.r.n_group) {
-        /* the group's two largest by the lanes that hold it, met in LDS */
-        __shared__ uint32_t keys[4][64 * NJ];
-        uint32_t *k = keys[wave_in_group()];
+        /* Keys through LDS, a group's beside each other and groups 4 words further
+         * apart, so that lanes with a group each read from different banks. */
+        constexpr int E = 4 * L * NQ, G = 64;
+        __shared__ uint32_t keys[4][TPW][E + 4 * G];
+        uint32_t *const k = keys[wave_in_group()][lane / L];
+        const int ng = a.r.n_group, per = ne / ng;
+        const uint32_t mul = ((1u << 22) + per - 1) / per;     /* e / per = e mul >> 22 for e < 1024 */
 #pragma unroll
-        for (int j = 0; j < NJ; j++) k[e0 + j] = key[j];
+        for (int q = 0; q < NQ; q++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const int e = id_of(q, i);
+                if (e < ne) k[e + 4 * (e * mul >> 22)] = key[q][i];
+            }
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");
         __builtin_amdgcn_wave_barrier();
-        const int G = a.r.n_group, per = ne / G;
-        uint32_t a1 = 0, a2 = 0;
-        if (lane < G)
-            for (int i = 0; i < per; i++) {
-                const uint32_t v = k[lane * per + i];
-                a2 = max(a2, min(a1, v));
-                a1 = max(a1, v);
-            }
-        float worth = a1 ? key_choice(a1) : -__builtin_inff();
-        if (a.r.group_top == 2 && a2) worth += key_choice(a2);
-        /* kept: fewer than topk_group groups are worth more, or as much and lower */
-        int before = 0;
-        for (int i = 0; i < G; i++) {
-            const float w = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(worth), i));
-            before += w > worth || (w == worth && i < lane);
-        }
-        const uint64_t kept = __builtin_amdgcn_ballot_w64(lane < G && before < a.r.topk_group);
+        /* worth of groups l, l + L, ..: in the order of unsigned numbers */
+        uint32_t worth[G / L];
 #pragma unroll
-        for (int j = 0; j < NJ; j++) {
-            const int grp = min((e0 + j) / per, 63);
-            key[j] = kept >> grp & 1 ? key[j] : 0u;
+        for (int h = 0; h < G / L; h++) {
+            const int grp = l + L * h;
+            uint32_t a1 = 0, a2 = 0;
+            if (grp < ng) {
+                const uint32_t *p = k + grp * (per + 4);
+                int i = 0;
+                if (per % 4 == 0)
+                    for (; i < per; i += 4) {
+                        const u32x4 v = *(const u32x4 *)(p + i);
+#pragma unroll
+                        for (int j = 0; j < 4; j++) {
+                            a2 = max32(a2, min32(a1, v[j]));
+                            a1 = max32(a1, v[j]);
+                        }
+                    }
+                for (; i < per; i++) {
+                    a2 = max32(a2, min32(a1, p[i]));
+                    a1 = max32(a1, p[i]);
+                }
+            }
+            float w = of_order(a1);
+            if (a.r.group_top == 2 && a2) w = __fadd_rn(w, of_order(a2));
+            worth[h] = a1 ? order_of(w == 0.0f ? 0.0f : w) : 0u;
         }
+        /* kept: fewer than topk_group groups are worth more, or as much and lower */
+        int before[G / L];
+#pragma unroll
+        for (int h = 0; h < G / L; h++) before[h] = 0;
+#pragma unroll
+        for (int h = 0; h < G / L; h++)
+            for (int i = 0; i < L && L * h + i < ng; i++) {
+                const uint32_t w = (uint32_t)__shfl((int)worth[h], i, L);
+#pragma unroll
+                for (int o = 0; o < G / L; o++)
+                    before[o] += w > worth[o] || (w == worth[o] && L * h + i < l + L * o);
+            }
+        uint64_t kept = 0;
+#pragma unroll
+        for (int h = 0; h < G / L; h++) {
+            const uint64_t m64 = __builtin_amdgcn_ballot_w64(l + L * h < ng && before[h] < a.r.topk_group);
+            if constexpr (L == 64) kept = m64;
+            else kept |= (m64 >> (lane & 48) & 0xFFFFu) << (16 * h);
+        }
+#pragma unroll
+        for (int q = 0; q < NQ; q++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const uint32_t grp = min32((uint32_t)id_of(q, i) * mul >> 22, 63u);
+                key[q][i] = kept >> grp & 1 ? key[q][i] : 0u;
+            }
     }
     int pick = -1;
-    float got = 0.0f;
 #pragma clang loop unroll(disable)
     for (int k = 0; k < topk; k++) {
-        uint32_t mine = key[0];
+        uint32_t best = 0;
 #pragma unroll
-        for (int j = 1; j < NJ; j++) mine = max(mine, key[j]);
-        const uint32_t best = wave_max_u32(mine);
-        if (!best) break;
-        const int owner = __builtin_ctzll(__builtin_amdgcn_ballot_w64(mine == best));
-        int at = 0;
-        float sv = s[0];
+        for (int q = 0; q < NQ; q++)
 #pragma unroll
-        for (int j = NJ - 1; j >= 0; j--) {
-            at = key[j] == best ? j : at;
-            sv = key[j] == best ? s[j] : sv;
-        }
-        const int p = owner * NJ + __builtin_amdgcn_readlane(at, owner);
-        const float v = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(sv), owner));
-        if (lane == k) {
-            pick = p;
-            got = v;
-        }
+            for (int i = 0; i < 4; i++) best = max32(best, key[q][i]);
+        best = over_lanes<L>(best, max32);
+        uint32_t id = 0xFFFFFFFFu;
 #pragma unroll
-        for (int j = 0; j < NJ; j++) key[j] = lane == owner && at == j ? 0u : key[j];
+        for (int q = NQ - 1; q >= 0; q--)
+#pragma unroll
+            for (int i = 3; i >= 0; i--) id = key[q][i] == best ? (uint32_t)id_of(q, i) : id;
+        id = best ? over_lanes<L>(id, min32) : 0xFFFFFFFFu;
+        if (l == k) pick = (int)id;
+#pragma unroll
+        for (int q = 0; q < NQ; q++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) key[q][i] = (uint32_t)id_of(q, i) == id ? 0u : key[q][i];
     }
-    double sum = 1.0;
-    if (a.r.renorm) {
-        sum = 0.0;
-#pragma clang loop unroll(disable)
-        for (int k = 0; k < topk; k++) sum += (double)__int_as_float(__builtin_amdgcn_readlane(__float_as_int(got), k));
-    }
-    if (lane < topk) {
+    /* lane k's pick again, from its logit: the same bits */
+    const float got = pick >= 0 ? score32<SCORE>(load1<TYPE>(row, pick), m) : 0.0f;
+    const double sum = a.r.renorm ? sum_lanes<16>((double)got) : 1.0;
+    if (l < topk && there) {
         const double w = sum != 0.0 ? (double)got * (double)a.r.scale / sum : 0.0;
-        a.idx[(size_t)t * topk + lane] = pick;
-        a.w[(size_t)t * topk + lane] = refused ? __builtin_nanf("") : (float)w;
+        a.idx[tok * topk + l] = pick;
+        a.w[tok * topk + l] = refused ? __builtin_nanf("") : (float)w;
     }
-    if (refused && lane == 0) atomicOr(a.status, ST_BAD_EXPERT_ID);
+    if (refused && l == 0 && there) atomicOr(a.status, ST_BAD_EXPERT_ID);
 }
 
-template <int TYPE, int SCORE, int NJ>
+/* Gradients that come from dscores (or none), expert by expert; then, when those
+ * stores have arrived, the chosen experts', whole, from lane k < topk. Without
+ * dscores only softmax without renorm reads the row: elsewhere what is not chosen
+ * has gradient 0. */
+template <int TYPE, int SCORE, int L, int NQ>
 __global__ __launch_bounds__(256) void k_route_groups_bwd(RouteGroupsBwdArgs a)
 {
-    const int lane = threadIdx.x & 63, ne = a.r.n_experts, topk = a.r.topk, e0 = lane * NJ;
-    const long t = (long)blockIdx.x * 4 + wave_in_group();
-    if (t >= a.n) return;
-    float x[NJ];
-    double s[NJ], g[NJ];
-    load_logits<TYPE, NJ>(a.logits, (size_t)t, ne, e0, x);
-    /* the chosen ones, lane k the k-th */
+    constexpr int TPW = 64 / L;
+    const int lane = threadIdx.x & 63, l = lane % L, ne = a.r.n_experts, topk = a.r.topk;
+    const long t0 = ((long)blockIdx.x * 4 + wave_in_group()) * TPW, t = t0 + lane / L;
+    if (t0 >= a.n) return;
+    const bool there = t < a.n;
+    const size_t tok = (size_t)min(t, (long)a.n - 1);
+    const void *row = (const uint8_t *)a.logits + tok * ne * elem_bytes<TYPE>();
+    void *const out = (uint8_t *)a.dlogits + tok * ne * elem_bytes<TYPE>();
+    auto id_of = [&](int q) { return 4 * l + 4 * L * q; };
+    const bool dense = a.dscores || SCORE == DSV4_HIP_SOFTMAX;
+    /* lane k's expert */
     int id = -1;
     double dw = 0.0;
-    if (lane < topk) {
-        id = a.idx[(size_t)t * topk + lane];
+    if (l < topk) {
+        id = a.idx[tok * topk + l];
         if ((unsigned)id >= (unsigned)ne) {
-            if (id != -1) atomicOr(a.status, ST_BAD_EXPERT_ID);
+            if (id != -1 && there) atomicOr(a.status, ST_BAD_EXPERT_ID);
             id = -1;
         } else {
-            dw = (double)a.dw[(size_t)t * topk + lane] * (double)a.r.scale;
+            dw = (double)a.dw[tok * topk + l] * (double)a.r.scale;
+        }
+    }
+    const float xk = id >= 0 ? load1<TYPE>(row, id) : 0.0f;
+    const double gk = id >= 0 && a.dscores ? (double)gptr(a.dscores)[tok * ne + id] : 0.0;
+    float x[NQ][4];
+    float g[NQ][4];
+#pragma unroll
+    for (int q = 0; q < NQ; q++) {
+        if (dense) load4<TYPE>(row, id_of(q), ne, x[q]);
+        if (a.dscores) load4<DSV4_HIP_F32>(a.dscores + tok * ne, id_of(q), ne, g[q]);
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            if (!dense) x[q][i] = NO_EXPERT;
+            if (!a.dscores || id_of(q) + i >= ne) g[q][i] = 0.0f;
         }
     }
     Norm m = {0.0f, 0.0};
-    if constexpr (SCORE == DSV4_HIP_SOFTMAX) {
-        m = softmax_norm<NJ>(x, s);
-#pragma unroll
-        for (int j = 0; j < NJ; j++) s[j] *= m.inv;
-    }
-    auto softplus = [](float v) { return v > 20.0f ? (double)v : log1p(exp((double)v)); };
-    double mine = 0.0;                             /* the score of id */
-    if (id >= 0) {
-        float v;
-        if constexpr (TYPE == DSV4_HIP_F32) v = ((const float *)a.logits)[(size_t)t * ne + id];
-        else v = widen16<TYPE>(((const uint16_t *)a.logits)[(size_t)t * ne + id]);
-        if constexpr (SCORE == DSV4_HIP_SOFTMAX) mine = v > -__builtin_inff() ? exp((double)v - (double)m.top) * m.inv : 0.0;
-        else if constexpr (SCORE == DSV4_HIP_SIGMOID) mine = sigmoid64(v);
-        else mine = sqrt(softplus(v));
-    }
+    double s[NQ][4];
+    if constexpr (SCORE == DSV4_HIP_SOFTMAX) m = softmax_norm<L, NQ>(x, s);
+    /* a score, and its own derivative (softmax: the score) */
+    auto score = [&](float v) -> double {
+        if constexpr (SCORE == DSV4_HIP_SOFTMAX) return v > NO_EXPERT ? exp64((double)v - (double)m.top) * m.inv : 0.0;
+        else if constexpr (SCORE == DSV4_HIP_SIGMOID) return sigmoid64(v);
+        else return sqrt(softplus64(v));
+    };
+    auto slope = [&](float v, double sv) -> double {
+        if constexpr (SCORE == DSV4_HIP_SOFTMAX) return sv;
+        else if constexpr (SCORE == DSV4_HIP_SIGMOID) return v > NO_EXPERT ? sv * (1.0 - sv) : 0.0;
+        else return sv == 0.0 ? 0.0 : (v > 20.0f ? 1.0 : sigmoid64(v)) / (2.0 * sv);
+    };
+    const double sk = id >= 0 ? score(xk) : 0.0;
     double ds = dw;
     if (a.r.renorm) {
-        const double P = wave_sum_f64(mine), dot = wave_sum_f64(mine * dw);
+        const double P = sum_lanes<16>(sk), dot = sum_lanes<16>(sk * dw);
         /* the forward call's weights are constant 0 where its fp32 scores are */
-        const bool none = __builtin_amdgcn_ballot_w64((float)mine != 0.0f) == 0;
+        const bool none = !any_lane<L>((float)sk != 0.0f, lane);
         ds = none ? 0.0 : (dw - dot / P) / P;
     }
-#pragma unroll
-    for (int j = 0; j < NJ; j++) g[j] = a.dscores && e0 + j < ne ? (double)a.dscores[(size_t)t * ne + e0 + j] : 0.0;
+    /* the same expert twice: its gradient holds both */
+    double mine = id >= 0 ? gk : 0.0;
 #pragma clang loop unroll(disable)
     for (int k = 0; k < topk; k++) {
-        const int e = __builtin_amdgcn_readlane(id, k);
-        const long long b = __double_as_longlong(ds);
-        const double d = __longlong_as_double(((long long)__builtin_amdgcn_readlane((int)(b >> 32), k) << 32) |
-                                              (uint32_t)__builtin_amdgcn_readlane((int)b, k));
-#pragma unroll
-        for (int j = 0; j < NJ; j++) g[j] += e0 + j == e ? d : 0.0;
+        const int e = __shfl(id, k, L);
+        const double d = __shfl(ds, k, L);
+        if (e == id) mine += d;
     }
-    double all = 0.0;
+    double all = 0.0;                              /* softmax: sum_e s_e g_e */
     if constexpr (SCORE == DSV4_HIP_SOFTMAX) {
+        if (a.dscores) {
 #pragma unroll
-        for (int j = 0; j < NJ; j++) all += s[j] * g[j];
-        all = wave_sum_f64(all);
-    }
+            for (int q = 0; q < NQ; q++)
 #pragma unroll
-    for (int j = 0; j < NJ; j++) {
-        if (e0 + j >= ne) continue;
-        double d;
-        if constexpr (SCORE == DSV4_HIP_SOFTMAX) {
-            d = s[j] * (g[j] - all);
-        } else if constexpr (SCORE == DSV4_HIP_SIGMOID) {
-            const double v = sigmoid64(x[j]);
-            d = v * (1.0 - v) * g[j];
-        } else {
-            const double v = sqrt(softplus(x[j]));
-            d = v == 0.0 ? 0.0 : (x[j] > 20.0f ? 1.0 : sigmoid64(x[j])) / (2.0 * v) * g[j];
+                for (int i = 0; i < 4; i++) all += s[q][i] * m.inv * (double)g[q][i];
         }
-        const size_t at = (size_t)t * ne + e0 + j;
-        if constexpr (TYPE == DSV4_HIP_F32) ((float *)a.dlogits)[at] = (float)d;
-        else ((uint16_t *)a.dlogits)[at] = (uint16_t)narrow16<TYPE>((float)d);
+        all = sum_lanes<L>(all + (id >= 0 ? sk * ds : 0.0));
     }
+#pragma unroll
+    for (int q = 0; q < NQ; q++) {
+        float o[4];
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            if constexpr (SCORE == DSV4_HIP_SOFTMAX) {
+                o[i] = (float)(s[q][i] * m.inv * ((double)g[q][i] - all));
+            } else {
+                o[i] = 0.0f;
+                if (a.dscores) {
+                    const double v = score(x[q][i]);
+                    o[i] = (float)(slope(x[q][i], v) * (double)g[q][i]);
+                }
+            }
+        }
+        if (there && id_of(q) < ne) store4<TYPE>(out, id_of(q), ne, o);
+    }
+    __builtin_amdgcn_s_waitcnt(0x0F70);            /* vmcnt(0) */
+    asm volatile("" ::: "memory");
+    if (id >= 0 && there) store1<TYPE>(out, id, (float)(slope(xk, sk) * (mine - all)));
 }
 
 namespace {
 
-template <int TYPE, int SCORE, int NJ>
+template <int TYPE, int SCORE, int L, int NQ>
 hipError_t launch(const RouteGroupsArgs &a, hipStream_t st)
 {
-    hipLaunchKernelGGL((k_route_groups<TYPE, SCORE, NJ>), dim3((unsigned)((a.n + 3) / 4)), dim3(256), 0, st, a);
+    constexpr int tokens = 4 * (64 / L);
+    hipLaunchKernelGGL((k_route_groups<TYPE, SCORE, L, NQ>), dim3((unsigned)((a.n + tokens - 1) / tokens)), dim3(256), 0, st, a);
     return hipGetLastError();
 }
-template <int TYPE, int SCORE, int NJ>
+template <int TYPE, int SCORE, int L, int NQ>
 hipError_t launch(const RouteGroupsBwdArgs &a, hipStream_t st)
 {
-    hipLaunchKernelGGL((k_route_groups_bwd<TYPE, SCORE, NJ>), dim3((unsigned)((a.n + 3) / 4)), dim3(256), 0, st, a);
+    constexpr int tokens = 4 * (64 / L);
+    hipLaunchKernelGGL((k_route_groups_bwd<TYPE, SCORE, L, NQ>), dim3((unsigned)((a.n + tokens - 1) / tokens)), dim3(256), 0, st,
+                       a);
     return hipGetLastError();
 }
+/* Tokens from which four share a wave: fewer leave lanes of the device idle. */
+constexpr int ROUTE_SHARED_TOKENS = 2048;
 template <int TYPE, int SCORE, class ARGS>
-hipError_t launch_nj(const ARGS &a, hipStream_t st)
+hipError_t launch_size(const ARGS &a, hipStream_t st)
 {
-    const int nj = (a.r.n_experts + 63) / 64;
-    if (nj <= 1) return launch<TYPE, SCORE, 1>(a, st);
-    if (nj <= 2) return launch<TYPE, SCORE, 2>(a, st);
-    if (nj <= 4) return launch<TYPE, SCORE, 4>(a, st);
-    if (nj <= 8) return launch<TYPE, SCORE, 8>(a, st);
-    return launch<TYPE, SCORE, RT_MAXJ>(a, st);
+    const int ne = a.r.n_experts;
+    if (ne <= 256 && a.n >= ROUTE_SHARED_TOKENS) {
+        if (ne <= 64) return launch<TYPE, SCORE, 16, 1>(a, st);
+        if (ne <= 128) return launch<TYPE, SCORE, 16, 2>(a, st);
+        return launch<TYPE, SCORE, 16, 4>(a, st);
+    }
+    if (ne <= 256) return launch<TYPE, SCORE, 64, 1>(a, st);
+    if (ne <= 512) return launch<TYPE, SCORE, 64, 2>(a, st);
+    return launch<TYPE, SCORE, 64, 4>(a, st);
 }
 template <int TYPE, class ARGS>
 hipError_t launch_score(const ARGS &a, hipStream_t st)
 {
     switch (a.r.score) {
-    case DSV4_HIP_SQRT_SOFTPLUS: return launch_nj<TYPE, DSV4_HIP_SQRT_SOFTPLUS>(a, st);
-    case DSV4_HIP_SOFTMAX: return launch_nj<TYPE, DSV4_HIP_SOFTMAX>(a, st);
-    case DSV4_HIP_SIGMOID: return launch_nj<TYPE, DSV4_HIP_SIGMOID>(a, st);
+    case DSV4_HIP_SQRT_SOFTPLUS: return launch_size<TYPE, DSV4_HIP_SQRT_SOFTPLUS>(a, st);
+    case DSV4_HIP_SOFTMAX: return launch_size<TYPE, DSV4_HIP_SOFTMAX>(a, st);
+    case DSV4_HIP_SIGMOID: return launch_size<TYPE, DSV4_HIP_SIGMOID>(a, st);
     default: return hipErrorInvalidValue;
     }
 }
