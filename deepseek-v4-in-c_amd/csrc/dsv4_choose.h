@@ -324,8 +324,11 @@ inline long i8_waves(I8Form form, long M, long N, long ne)
 
 /* Forms of the product of 4-bit rows: 16 x 16 results a workgroup with K over
  * its waves (one matrix only), the others tiles of features x rows through a
- * ring in LDS. */
-enum Fp4Form { FP4_SPLIT = 1, FP4_64x32, FP4_64x64, FP4_128x32, FP4_128x64, FP4_128x128, FP4_256x128, FP4_256x256 };
+ * ring in LDS; _W8: by eight waves, one workgroup a CU rather than two of four
+ * waves. */
+enum Fp4Form {
+    FP4_SPLIT = 1, FP4_64x32, FP4_64x64, FP4_128x32, FP4_128x64, FP4_128x128, FP4_128x128_W8, FP4_256x128, FP4_256x256
+};
 struct Fp4Shape { int F, TR, waves; };
 inline Fp4Shape fp4_shape(Fp4Form form)
 {
@@ -336,6 +339,7 @@ inline Fp4Shape fp4_shape(Fp4Form form)
     case FP4_128x32: return {128, 32, 4};
     case FP4_128x64: return {128, 64, 4};
     case FP4_128x128: return {128, 128, 4};
+    case FP4_128x128_W8: return {128, 128, 8};
     case FP4_256x128: return {256, 128, 8};
     default: return {256, 256, 8};
     }
@@ -351,12 +355,14 @@ inline Fp4Shape fp4_shape(Fp4Form form)
  * - / 7.1 / 7.7 / 9.4 / 15 / 18 / 25, 512 rows - / 17.8 / 12.1 / 11.0 / 16 / 19 / 27,
  * 2,048 rows - / 52 / 39 / 30 / 24.6 / 24.1 / 29, 4,096 rows - / 100 / 74 / 57 / 47 / 46 /
  * 39.5; 333 x 1024 x 4096 - / 6.8 / 7.1 / 8.8 / 12 / 18 / 25; 2,048 x 4096 x 1024 - /
- * 23 / 16 / 12 / 9.2 / 10.4 / 12.6. */
+ * 23 / 16 / 12 / 9.2 / 10.4 / 12.6. 128x128_W8 after another 12 shapes, of 128x64 /
+ * 128x128 / it / 256x128: 2,803 x 1024 x 4096 17.4 / 17.4 / 13.9 / 19.6, 1,024 x 4096 x
+ * 4096 17.4 / 18.3 / 15.6 / 20.1, 2,048 x 4096 x 4096 35 / 25.7 / 29 / 25.2. */
 struct Fp4Cost { Fp4Form form; int c1, c0, fix, slope, r; };
 constexpr Fp4Cost FP4_COSTS[] = {
     {FP4_SPLIT, 195, 62, 36, 153, 71},      {FP4_64x32, 256, 172, 68, 238, 62},     {FP4_64x64, 233, 165, 100, 337, 63},
-    {FP4_128x64, 278, 182, 120, 534, 59},   {FP4_128x128, 282, 487, 159, 840, 42},  {FP4_256x128, 112, 56, 497, 1650, 71},
-    {FP4_256x256, 0, 0, 890, 2722, 65}};
+    {FP4_128x64, 278, 182, 120, 534, 59},   {FP4_128x128, 282, 487, 159, 840, 42},  {FP4_128x128_W8, 78, 107, 283, 1087, 62},
+    {FP4_256x128, 112, 56, 497, 1650, 71},  {FP4_256x256, 0, 0, 890, 2722, 65}};
 /* row tiles: whole ones, and with ne experts one for each that rows may hit */
 inline long fp4_row_tiles(Fp4Form form, long M, long ne)
 {
@@ -391,8 +397,8 @@ inline Fp4Form fp4_form(int M, int N, int K) { return fp4_least(FP4_COSTS, M, N,
  * 256x128, experts 2048 x 4096 on 256: 6 rows 8.7 / 10.1 / 10.7 / 16.3, 384 rows 148
  * / 143 / 149 / 168, 1,536 rows 196 / 183 / 189 / 191, 6,144 rows 277 / 213 / 210 /
  * 199, 24,576 rows - / - / 360 / 236, Zipf - / - / 361 / 301; 8 of 4096 x 4096, 240
- * rows 21 / 21 / 16.6 / 26, 3,072 rows - / - / 65 / 52; 64 of 512 x 1024, 384 rows 7.6
- * / 7.3 / 7.6 / 9.9, 6,144 rows - / 14 / 11.7 / 11.0. */
+ * rows 21 / 21 / 16.6 / 26; 64 of 512 x 1024, 384 rows 7.6 / 7.3 / 7.6 / 9.9, 6,144
+ * rows - / 14 / 11.7 / 11.0. */
 constexpr Fp4Cost FP4_BUCKET_COSTS[] = {{FP4_64x32, 337, 311, 93, 314, 0},
                                         {FP4_128x32, 326, 432, 136, 575, 3},
                                         {FP4_128x64, 400, 334, 148, 669, 0},

@@ -548,6 +548,7 @@ static hipError_t fp4_one(const Fp4Args &a, hipStream_t st)
     case FP4_64x64: return fp4_tile<64, 64, 2, 2, 3, false, false, OUT>(a, groups, st);
     case FP4_128x64: return fp4_tile<128, 64, 2, 2, 3, false, false, OUT>(a, groups, st);
     case FP4_128x128: return fp4_tile<128, 128, 2, 2, 2, false, false, OUT>(a, groups, st);
+    case FP4_128x128_W8: return fp4_tile<128, 128, 4, 2, 3, false, false, OUT>(a, groups, st);
     case FP4_256x128: return fp4_tile<256, 128, 4, 2, 3, false, false, OUT>(a, groups, st);
     default: return fp4_tile<256, 256, 4, 2, 2, false, false, OUT>(a, groups, st);
     }

@@ -26,6 +26,8 @@ namespace dsv4 {
 
 namespace {
 
+template <int N> struct IC { static constexpr int value = N; };
+
 constexpr float NO_EXPERT = -__builtin_inff();     /* the logit of one that is not there */
 
 /* four consecutive elements of a row from e on, at any alignment of one; past
@@ -137,36 +139,40 @@ __device__ __forceinline__ uint32_t order_of(float c)
 }
 __device__ __forceinline__ float of_order(uint32_t k) { return __uint_as_float((k & 0x80000000u) ? k ^ 0x80000000u : ~k); }
 
-/* e^x in fp64 for |x| <= 708 (beyond: clamped): x = k ln 2 + r, |r| <= 0.347, and
- * r's Taylor series to r^12, cut at 0.347^13 / 13! = 2^-52 of it. */
+/* e^x in fp64 for |x| <= 700: x = k ln 2 + r with k the nearest integer, read from
+ * the low bits of a sum with 1.5 x 2^52, and e^r by the polynomial of degree 10
+ * that is nearest to it on |r| <= 0.3466 in the Chebyshev sense (relatively within
+ * 2^-52; fitted in 50 digits), k added to the exponent: 15 instructions. */
 __device__ __forceinline__ double exp64(double x)
 {
-    x = fmin(fmax(x, -708.0), 708.0);
-    const double k = rint(x * 1.4426950408889634);
+    const double magic = 6755399441055744.0, s = fma(x, 1.4426950408889634, magic), k = s - magic;
     const double r = fma(k, -2.3190468138462996e-17, fma(k, -0.6931471805599453, x));
-    double p = 1.0 / 479001600;
-    p = fma(p, r, 1.0 / 39916800);
-    p = fma(p, r, 1.0 / 3628800);
-    p = fma(p, r, 1.0 / 362880);
-    p = fma(p, r, 1.0 / 40320);
-    p = fma(p, r, 1.0 / 5040);
-    p = fma(p, r, 1.0 / 720);
-    p = fma(p, r, 1.0 / 120);
-    p = fma(p, r, 1.0 / 24);
-    p = fma(p, r, 1.0 / 6);
-    p = fma(p, r, 0.5);
+    double p = 2.762637106569635607642e-7;
+    p = fma(p, r, 2.764019739169484046713e-6);
+    p = fma(p, r, 2.480150431378554016571e-5);
+    p = fma(p, r, 1.984117023057028666426e-4);
+    p = fma(p, r, 1.388888893251477935536e-3);
+    p = fma(p, r, 8.333333385699211726935e-3);
+    p = fma(p, r, 4.166666666657306773181e-2);
+    p = fma(p, r, 0.1666666666655431458301);
+    p = fma(p, r, 0.5000000000000005622546);
+    p = fma(p, r, 1.000000000000006749096);
     p = fma(p, r, 1.0);
-    p = fma(p, r, 1.0);
-    return __builtin_amdgcn_ldexp(p, (int)k);
+    return __longlong_as_double(__double_as_longlong(p) + (long long)((uint64_t)__double_as_longlong(s) << 52));
 }
-/* 1 / v for normal v whose reciprocal is normal: two Newton steps */
+/* 1 / v for normal v whose reciprocal is normal: the instruction's 24 bits to 53
+ * in one step of third order */
 __device__ __forceinline__ double rcp64(double v)
 {
-    double y = __builtin_amdgcn_rcp(v);
-    y = fma(fma(-v, y, 1.0), y, y);
-    return fma(fma(-v, y, 1.0), y, y);
+    const double y = __builtin_amdgcn_rcp(v), e = fma(-v, y, 1.0);
+    return fma(fma(e, e, e), y, y);
 }
-__device__ __forceinline__ double sigmoid64(float x) { return rcp64(1.0 + exp64(-(double)x)); }
+/* beyond 700 the score is 0 or 1 in fp32, and in fp64 next to it */
+__device__ __forceinline__ double sigmoid64(float x)
+{
+    return rcp64(1.0 + exp64((double)__builtin_amdgcn_fmed3f(-x, -700.0f, 700.0f)));
+}
+__device__ __forceinline__ double exp_below(float x, float top) { return exp64(fmax((double)x - (double)top, -700.0)); }
 __device__ __forceinline__ double softplus64(float x) { return x > 20.0f ? (double)x : log1p(exp((double)x)); }
 
 /* softmax over a token's L x 4 NQ logits: e^(x - top), top and 1 / sum; an expert
@@ -187,7 +193,7 @@ __device__ __forceinline__ Norm softmax_norm(const float (&x)[NQ][4], double (&p
     for (int q = 0; q < NQ; q++)
 #pragma unroll
         for (int i = 0; i < 4; i++) {
-            p[q][i] = x[q][i] > NO_EXPERT ? exp64((double)x[q][i] - (double)o.top) : 0.0;
+            p[q][i] = x[q][i] > NO_EXPERT ? exp_below(x[q][i], o.top) : 0.0;
             sum += p[q][i];
         }
     sum = sum_lanes<L>(sum);
@@ -199,7 +205,7 @@ __device__ __forceinline__ Norm softmax_norm(const float (&x)[NQ][4], double (&p
 template <int SCORE>
 __device__ __forceinline__ float score32(float x, const Norm &m)
 {
-    if constexpr (SCORE == DSV4_HIP_SOFTMAX) return x > NO_EXPERT ? (float)(exp64((double)x - (double)m.top) * m.inv) : 0.0f;
+    if constexpr (SCORE == DSV4_HIP_SOFTMAX) return x > NO_EXPERT ? (float)(exp_below(x, m.top) * m.inv) : 0.0f;
     else if constexpr (SCORE == DSV4_HIP_SIGMOID) return (float)sigmoid64(x);
     else return route_orig(x);
 }
@@ -266,30 +272,31 @@ __global__ __launch_bounds__(256) void k_route_groups(RouteGroupsArgs a)
         /* Keys through LDS, a group's beside each other and groups 4 words further
          * apart, so that lanes with a group each read from different banks. */
         constexpr int E = 4 * L * NQ, G = 64;
-        __shared__ uint32_t keys[4][TPW][E + 4 * G];
+        __shared__ __align__(16) uint32_t keys[4][TPW][E + 4 * G];
         uint32_t *const k = keys[wave_in_group()][lane / L];
         const int ng = a.r.n_group, per = ne / ng;
         const uint32_t mul = ((1u << 22) + per - 1) / per;     /* e / per = e mul >> 22 for e < 1024 */
+        const bool quads = per % 4 == 0;           /* four neighbours share a group */
 #pragma unroll
-        for (int q = 0; q < NQ; q++)
+        for (int q = 0; q < NQ; q++) {
+            const int e = id_of(q, 0);
+            if (quads) {
+                if (e < ne) *(u32x4 *)(k + e + 4 * (e * mul >> 22)) = u32x4{key[q][0], key[q][1], key[q][2], key[q][3]};
+            } else {
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const int e = id_of(q, i);
-                if (e < ne) k[e + 4 * (e * mul >> 22)] = key[q][i];
+                for (int i = 0; i < 4; i++)
+                    if (e + i < ne) k[e + i + 4 * ((e + i) * mul >> 22)] = key[q][i];
             }
+        }
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");
         __builtin_amdgcn_wave_barrier();
-        /* worth of groups l, l + L, ..: in the order of unsigned numbers */
-        uint32_t worth[G / L];
-#pragma unroll
-        for (int h = 0; h < G / L; h++) {
-            const int grp = l + L * h;
+        /* what group grp is worth, in the order of unsigned numbers */
+        auto worth_of = [&](int grp) -> uint32_t {
             uint32_t a1 = 0, a2 = 0;
             if (grp < ng) {
                 const uint32_t *p = k + grp * (per + 4);
-                int i = 0;
-                if (per % 4 == 0)
-                    for (; i < per; i += 4) {
+                if (quads)
+                    for (int i = 0; i < per; i += 4) {
                         const u32x4 v = *(const u32x4 *)(p + i);
 #pragma unroll
                         for (int j = 0; j < 4; j++) {
@@ -297,41 +304,54 @@ __global__ __launch_bounds__(256) void k_route_groups(RouteGroupsArgs a)
                             a1 = max32(a1, v[j]);
                         }
                     }
-                for (; i < per; i++) {
-                    a2 = max32(a2, min32(a1, p[i]));
-                    a1 = max32(a1, p[i]);
-                }
+                else
+                    for (int i = 0; i < per; i++) {
+                        a2 = max32(a2, min32(a1, p[i]));
+                        a1 = max32(a1, p[i]);
+                    }
             }
             float w = of_order(a1);
             if (a.r.group_top == 2 && a2) w = __fadd_rn(w, of_order(a2));
-            worth[h] = a1 ? order_of(w == 0.0f ? 0.0f : w) : 0u;
-        }
-        /* kept: fewer than topk_group groups are worth more, or as much and lower */
-        int before[G / L];
-#pragma unroll
-        for (int h = 0; h < G / L; h++) before[h] = 0;
-#pragma unroll
-        for (int h = 0; h < G / L; h++)
-            for (int i = 0; i < L && L * h + i < ng; i++) {
-                const uint32_t w = (uint32_t)__shfl((int)worth[h], i, L);
-#pragma unroll
-                for (int o = 0; o < G / L; o++)
-                    before[o] += w > worth[o] || (w == worth[o] && L * h + i < l + L * o);
-            }
+            return a1 ? order_of(w == 0.0f ? 0.0f : w) : 0u;
+        };
+        /* kept: fewer than topk_group groups are worth more, or as much and lower.
+         * H groups a lane: l, l + L, .. */
         uint64_t kept = 0;
+        auto keep = [&](auto HS) {
+            constexpr int H = decltype(HS)::value;
+            uint32_t worth[H];
+            int before[H];
 #pragma unroll
-        for (int h = 0; h < G / L; h++) {
-            const uint64_t m64 = __builtin_amdgcn_ballot_w64(l + L * h < ng && before[h] < a.r.topk_group);
-            if constexpr (L == 64) kept = m64;
-            else kept |= (m64 >> (lane & 48) & 0xFFFFu) << (16 * h);
-        }
+            for (int h = 0; h < H; h++) {
+                worth[h] = worth_of(l + L * h);
+                before[h] = 0;
+            }
 #pragma unroll
-        for (int q = 0; q < NQ; q++)
+            for (int h = 0; h < H; h++)
+                for (int i = 0; i < L && L * h + i < ng; i++) {
+                    const uint32_t w = (uint32_t)__shfl((int)worth[h], i, L);
+#pragma unroll
+                    for (int o = 0; o < H; o++) before[o] += w > worth[o] || (w == worth[o] && L * h + i < l + L * o);
+                }
+#pragma unroll
+            for (int h = 0; h < H; h++) {
+                const uint64_t m64 = __builtin_amdgcn_ballot_w64(l + L * h < ng && before[h] < a.r.topk_group);
+                if constexpr (L == 64) kept = m64;
+                else kept |= (m64 >> (lane & 48) & 0xFFFFu) << (16 * h);
+            }
+        };
+        if (ng <= L) keep(IC<1>{});
+        else keep(IC<G / L>{});
+#pragma unroll
+        for (int q = 0; q < NQ; q++) {
+            const uint32_t e = (uint32_t)id_of(q, 0);
+            const bool in0 = kept >> min32(e * mul >> 22, 63u) & 1;
 #pragma unroll
             for (int i = 0; i < 4; i++) {
-                const uint32_t grp = min32((uint32_t)id_of(q, i) * mul >> 22, 63u);
-                key[q][i] = kept >> grp & 1 ? key[q][i] : 0u;
+                const bool in = quads ? in0 : kept >> min32((e + i) * mul >> 22, 63u) & 1;
+                key[q][i] = in ? key[q][i] : 0u;
             }
+        }
     }
     int pick = -1;
 #pragma clang loop unroll(disable)
@@ -413,7 +433,7 @@ __global__ __launch_bounds__(256) void k_route_groups_bwd(RouteGroupsBwdArgs a)
     if constexpr (SCORE == DSV4_HIP_SOFTMAX) m = softmax_norm<L, NQ>(x, s);
     /* a score, and its own derivative (softmax: the score) */
     auto score = [&](float v) -> double {
-        if constexpr (SCORE == DSV4_HIP_SOFTMAX) return v > NO_EXPERT ? exp64((double)v - (double)m.top) * m.inv : 0.0;
+        if constexpr (SCORE == DSV4_HIP_SOFTMAX) return v > NO_EXPERT ? exp_below(v, m.top) * m.inv : 0.0;
         else if constexpr (SCORE == DSV4_HIP_SIGMOID) return sigmoid64(v);
         else return sqrt(softplus64(v));
     };
@@ -487,13 +507,17 @@ hipError_t launch(const RouteGroupsBwdArgs &a, hipStream_t st)
                        a);
     return hipGetLastError();
 }
-/* Tokens from which four share a wave: fewer leave lanes of the device idle. */
-constexpr int ROUTE_SHARED_TOKENS = 2048;
+/* Tokens from which four share a wave: fewer leave lanes of the device idle. us, a
+ * wave each / shared, 256 experts: sigmoid, 8 groups, top 8 2,048 tokens 7.0 / 8.8,
+ * 4,096 9.4 / 9.3, 16,384 25 / 19; softmax, top 6 4,096 6.9 / 7.9, 8,192 10.4 / 9.0;
+ * backward 8,192 9.0 / 9.3, 16,384 16.3 / 15.4; sqrt(softplus), whose table is a
+ * latency an expert, 8,192 15.7 / 18.8, 16,384 27 / 27. */
+constexpr int shared_from(int score) { return score == DSV4_HIP_SQRT_SOFTPLUS ? 16384 : 6144; }
 template <int TYPE, int SCORE, class ARGS>
 hipError_t launch_size(const ARGS &a, hipStream_t st)
 {
     const int ne = a.r.n_experts;
-    if (ne <= 256 && a.n >= ROUTE_SHARED_TOKENS) {
+    if (ne <= 256 && a.n >= shared_from(SCORE)) {
         if (ne <= 64) return launch<TYPE, SCORE, 16, 1>(a, st);
         if (ne <= 128) return launch<TYPE, SCORE, 16, 2>(a, st);
         return launch<TYPE, SCORE, 16, 4>(a, st);

@@ -173,6 +173,20 @@ def test_rows_with_a_pitch(lib, dtype):
         check_rows(quant(lib, x, ld=ld, k=k, form="columns"), columns(x))
 
 
+def test_rows_past_4_gib(lib):
+    """The last rows, and columns, of more than 4 GiB as by themselves."""
+    x = torch.empty((1 << 21) + 3, 1056, dtype=torch.bfloat16, device=DEV).normal_(generator=gen(1))
+    q, s = quant(lib, x)
+    check_rows((q[-5:], s[-5:]), x[-5:].double())
+    u = x.flip(0)
+    q, s = quant(lib, x, form="swiglu", u=u)
+    check_rows((q[-5:], s[-5:]), swiglu64(x[-5:], u[-5:], 10.0))
+    del u
+    x = x.view(-1)[:40037 * 55000].view(40037, 55000)
+    q, s = quant(lib, x, form="columns")
+    check_rows((q[-3:], s[-3:]), columns(x[:, -3:]))
+
+
 def swiglu64(g, u, limit):
     g, u = g.double(), u.double()
     lim = float(np.float32(limit))
@@ -336,6 +350,17 @@ def test_scales_of_the_ends(lib, pkg):
     a[1].fill_(254)
     got = product(lib, pkg, a, w)
     assert (torch.isinf(got) | torch.isnan(got) | (got == 0)).all()
+
+
+@pytest.mark.parametrize("M,N,K", [(70001, 16390, 32), (3, 70003, 1 << 17), (40, 70003, 1 << 17), (70003, 9, 1 << 17)])
+def test_matrices_past_4_gib(lib, pkg, M, N, K):
+    """Results, weights and tokens beyond 4 GiB: the last of them, and a call's guards."""
+    a, w = operand(M, K, 1, wide=True), operand(N, K, 2, wide=True)
+    got = product(lib, pkg, a, w)
+    m, n = min(M, 40), min(N, 40)
+    va, vw = values(a[0][-m:], a[1][-m:]), values(w[0][-n:], w[1][-n:])
+    want, most = va @ vw.t().contiguous(), va.abs() @ vw.abs().t().contiguous()
+    assert ((got[-m:, -n:].double() - want).abs() <= (K / 32 + 16) * 2 * U * most).all()
 
 
 def test_wide_rows(lib, pkg):

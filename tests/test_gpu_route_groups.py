@@ -125,6 +125,59 @@ def test_routing(lib, pkg, kind, dtype, n, E, topk, G, kept, top):
         check(lib, pkg.Router(kind, E, topk, G, kept, top, renorm, 2.5), x, b)
 
 
+# tokens that share a wave: from 6,144 on, 16,384 for sqrt(softplus), of up to 256 experts
+MANY = [(6147, 60, 4, 5, 2, 2), (6145, 128, 6, 8, 3, 1), (6149, 256, 8, 8, 4, 2), (6146, 160, 16, 32, 9, 2),
+        (6144, 250, 5, 1, 1, 1), (6150, 64, 8, 64, 20, 1), (6151, 3, 2, 1, 1, 1)]
+
+
+def with_masks(x):
+    """in every fourth token some experts, in some all but one, in some all are not there"""
+    x[1::4][torch.rand(x[1::4].shape, device=DEV, generator=gen(7)) < 0.7] = -INF
+    x[5::64, 1:] = -INF
+    x[7::64] = -INF
+    x[9::64] = torch.finfo(x.dtype).min
+    return x
+
+
+@pytest.mark.parametrize("kind", [SQRT, SOFTMAX, SIGMOID])
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n,E,topk,G,kept,top", MANY)
+def test_routing_many(lib, pkg, kind, dtype, n, E, topk, G, kept, top):
+    n += (16384 - 6144) * (kind == SQRT)
+    x = with_masks((1.5 * torch.randn(n, E, device=DEV, generator=gen(n + E))).to(dtype))
+    bias = 0.1 * torch.randn(E, device=DEV, generator=gen(3))
+    lib.status()
+    check(lib, pkg.Router(kind, E, topk, G, kept, top, 1, 2.5), x, bias)
+    assert lib.status() == 0
+
+
+@pytest.mark.parametrize("kind", [SOFTMAX, SIGMOID])
+def test_ties_of_many(lib, pkg, kind):
+    x = torch.randint(-1, 2, (6200, 256), device=DEV, generator=gen(1)).float()
+    check(lib, pkg.Router(kind, 256, 8, 8, 3, 2, 1, 1.0), x)
+    x = torch.randint(17, 40, (6200, 96), device=DEV, generator=gen(2)).float()
+    check(lib, pkg.Router(kind, 96, 8, 6, 2, 1, 0, 1.0), x)
+
+
+@pytest.mark.parametrize("kind", [SQRT, SOFTMAX, SIGMOID])
+def test_refused_among_many(lib, pkg, kind):
+    """The same bits for a token in a small call and among many; refusals stay with their tokens."""
+    n = 16390 if kind == SQRT else 6150
+    x = torch.randn(n, 200, device=DEV, generator=gen(1))
+    x[3, 199], x[n - 1, 0], x[n - 2, 77] = float("nan"), INF, float("nan")
+    r = pkg.Router(kind, 200, 5, 10, 3, 2, 1, 1.0)
+    lib.status()
+    many = route(lib, r, x)
+    assert lib.status() == 1
+    few = route(lib, r, x[-50:].contiguous())
+    lib.status()
+    for a, b in zip(many, few):
+        assert torch.equal(a[-50:].contiguous().view(torch.int32), b.contiguous().view(torch.int32))
+    for t in (3, n - 1, n - 2):
+        assert (many[0][t] == -1).all() and torch.isnan(many[1][t]).all() and torch.isnan(many[2][t]).all()
+    assert (many[0][[0, 1, 2, 4, 5, n - 3]] >= 0).all()
+
+
 @pytest.mark.parametrize("kind", [SOFTMAX, SIGMOID])
 def test_ties_go_to_the_lower_id(lib, pkg, kind):
     """Few distinct logits: experts and groups of equal worth; sigmoids that round to 1."""
@@ -237,6 +290,58 @@ def test_gradients(lib, pkg, kind, dtype, n, E, topk, G, kept, top):
             want = want_grad(r, x, idx, dw, ds)
             got = backward(lib, r, x, idx, dw, ds).double()
             assert ((got - want).abs() <= 1.001 * HALF[dtype] * want.abs() + 1e-12 * 20 + TINY[dtype]).all()
+
+
+@pytest.mark.parametrize("kind", [SQRT, SOFTMAX, SIGMOID])
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n,E,topk,G,kept,top", MANY)
+def test_gradients_of_many(lib, pkg, kind, dtype, n, E, topk, G, kept, top):
+    n += (16384 - 6144) * (kind == SQRT)
+    x = (1.5 * torch.randn(n, E, device=DEV, generator=gen(n + E))).to(dtype)
+    dw = torch.randn(n, topk, device=DEV, generator=gen(2))
+    ds = torch.randn(n, E, device=DEV, generator=gen(5))
+    for renorm, d in ((0, ds), (1, None), (1, ds), (0, None)):
+        r = pkg.Router(kind, E, topk, G, kept, top, renorm, 2.5)
+        idx, _, _ = route(lib, r, x)
+        want = want_grad(r, x, idx, dw, d)
+        got = backward(lib, r, x, idx, dw, d).double()
+        assert ((got - want).abs() <= 1.001 * HALF[dtype] * want.abs() + 1e-12 * 20 + TINY[dtype]).all()
+
+
+def test_gradients_of_masked_tokens(lib, pkg):
+    """Tokens without experts have gradient 0, masked experts too; a token's gradient is the
+    same among few and many. Softmax adds up its 96 terms, of at most 30, in fp64 in
+    another order there: 2 x 96 x 2^-53 x 30 < 1e-12, and the rounding to fp32 may then
+    fall to the other side, 2^-23 of the value."""
+    for kind in (SQRT, SOFTMAX, SIGMOID):
+        x = with_masks(torch.randn(16390, 96, device=DEV, generator=gen(3)))
+        dw, ds = (torch.randn(16390, k, device=DEV, generator=gen(4)) for k in (6, 96))
+        r = pkg.Router(kind, 96, 6, 8, 3, 2, 1, 2.5)
+        idx, _, _ = route(lib, r, x)
+        for d in (None, ds):
+            got = backward(lib, r, x, idx, dw, d)
+            assert torch.isfinite(got).all() and (got[x == -INF] == 0).all()
+            t = slice(16390 - 77, 16390)
+            few = backward(lib, r, x[t].contiguous(), idx[t].contiguous(), dw[t].contiguous(), d[t].contiguous() if d is not None else None)
+            if kind == SOFTMAX:
+                assert ((got[t].double() - few.double()).abs() <= 1e-12 + 2 * U * few.abs()).all()
+            else:
+                assert torch.equal(got[t], few)
+
+
+def test_tokens_past_4_gib(lib, pkg):
+    """The last tokens of 4.4 GB of logits as by themselves, both ways."""
+    n, E = (1 << 22) + 3, 260
+    x = torch.empty(n, E, device=DEV)
+    x.normal_(generator=gen(1))
+    r = pkg.Router(SIGMOID, E, 4, 4, 2, 2, 1, 1.0)
+    big, few = route(lib, r, x), route(lib, r, x[-9:].contiguous())
+    for a, b in zip(big, few):
+        assert torch.equal(a[-9:], b)
+    dw = torch.randn(n, 4, device=DEV, generator=gen(2))
+    a = backward(lib, r, x, big[0].contiguous(), dw, big[2].contiguous())
+    b = backward(lib, r, x[-9:].contiguous(), few[0].contiguous(), dw[-9:].contiguous(), few[2].contiguous())
+    assert torch.equal(a[-9:], b)
 
 
 @pytest.mark.parametrize("kind", [SQRT, SOFTMAX, SIGMOID])
