@@ -130,6 +130,124 @@ __device__ __forceinline__ bool any_lane(bool b, int lane)
     return L == 64 ? m != 0 : (m >> (lane & 48) & 0xFFFFu) != 0;
 }
 
+/* An expert's place as one positive fp64 number, key bits above those of 1023 - id
+ * (below 2^62: neither infinite nor NaN): the maximum of two is one instruction
+ * and settles ties. Key 0: below every other, no expert. */
+__device__ __forceinline__ double place_of(uint32_t key, int id)
+{
+    return __longlong_as_double((long long)((uint64_t)key << 30 | (uint32_t)(1023 - id)));
+}
+__device__ __forceinline__ int expert_of(double place)
+{
+    const uint64_t u = (uint64_t)__double_as_longlong(place);
+    return u >> 30 ? 1023 - (int)(u & 1023) : -1;
+}
+template <int CTRL, int ROWS = 0xF>
+__device__ __forceinline__ double dpp_f64(double v)
+{
+    const uint64_t u = (uint64_t)__double_as_longlong(v);
+    const uint32_t lo = (uint32_t)u, hi = (uint32_t)(u >> 32);
+    return __longlong_as_double((long long)((uint64_t)dpp_u32<CTRL, ROWS>(hi, hi) << 32 | dpp_u32<CTRL, ROWS>(lo, lo)));
+}
+template <int L>
+__device__ __forceinline__ double max_lanes(double v)
+{
+    v = fmax(v, dpp_f64<DPP_QUAD_1032>(v));
+    v = fmax(v, dpp_f64<DPP_QUAD_2301>(v));
+    v = fmax(v, dpp_f64<DPP_ROW_HALF_MIRROR>(v));
+    v = fmax(v, dpp_f64<DPP_ROW_MIRROR>(v));
+    if constexpr (L == 64) {
+        v = fmax(v, dpp_f64<DPP_ROW_BCAST15, 0xA>(v));
+        v = fmax(v, dpp_f64<DPP_ROW_BCAST31, 0xC>(v));
+        const uint64_t u = (uint64_t)__double_as_longlong(v);
+        const uint32_t lo = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)u, 63);
+        const uint32_t hi = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(u >> 32), 63);
+        v = __longlong_as_double((long long)((uint64_t)hi << 32 | lo));
+    }
+    return v;
+}
+
+/* The l-th largest (l < 8) of the 4 NQ numbers in each of a token's 16 lanes. A lane
+ * sorts its own, then sorted lists of eight meet: the eight largest of two are the
+ * larger of a[i] and b[7 - i], which rise and then fall, so three rounds of
+ * exchanges sort them. 16 numbers a lane: some 300 instructions, eight picks one
+ * after the other 500. With 64 lanes and fewer numbers in each the picks are the
+ * shorter (us, lists / picks: 1 token of 256 experts in groups, top 8, 4.5 / 4.7, but
+ * 4,096 9.9 / 9.4, with softmax and top 6 7.7 / 7.0). */
+__device__ __forceinline__ void exchange(double &a, double &b)
+{
+    const double hi = fmax(a, b);
+    b = fmin(a, b);
+    a = hi;
+}
+struct Eight { double v[8]; };
+__device__ __forceinline__ void sort_bitonic(Eight &a)
+{
+#pragma unroll
+    for (int d = 4; d; d >>= 1)
+#pragma unroll
+        for (int i = 0; i < 8; i++)
+            if (!(i & d)) exchange(a.v[i], a.v[i + d]);
+}
+__device__ __forceinline__ void sort_any(Eight &a)          /* merges of odd and even places */
+{
+    constexpr int from[19] = {0, 2, 4, 6, 0, 1, 4, 5, 1, 5, 0, 1, 2, 3, 2, 3, 1, 3, 5};
+    constexpr int to[19] = {1, 3, 5, 7, 2, 3, 6, 7, 2, 6, 4, 5, 6, 7, 4, 5, 2, 4, 6};
+#pragma unroll
+    for (int i = 0; i < 19; i++) exchange(a.v[from[i]], a.v[to[i]]);
+}
+/* the eight largest of two sorted lists, sorted */
+__device__ __forceinline__ void join(Eight &a, const Eight &b)
+{
+#pragma unroll
+    for (int i = 0; i < 8; i++) a.v[i] = fmax(a.v[i], b.v[7 - i]);
+    sort_bitonic(a);
+}
+template <int CTRL>
+__device__ __forceinline__ void join_lanes(Eight &a)
+{
+    Eight b;
+#pragma unroll
+    for (int i = 0; i < 8; i++) b.v[i] = dpp_f64<CTRL>(a.v[i]);
+    join(a, b);
+}
+template <int NQ>
+__device__ __forceinline__ double largest_of_lanes(const double (&v)[4 * NQ], int l)
+{
+    Eight a;
+    if constexpr (NQ == 1) {
+#pragma unroll
+        for (int i = 0; i < 4; i++) a.v[i] = v[i];
+        exchange(a.v[0], a.v[1]);
+        exchange(a.v[2], a.v[3]);
+        exchange(a.v[0], a.v[2]);
+        exchange(a.v[1], a.v[3]);
+        exchange(a.v[1], a.v[2]);
+#pragma unroll
+        for (int i = 0; i < 4; i++) a.v[7 - i] = dpp_f64<DPP_QUAD_1032>(a.v[i]);
+        sort_bitonic(a);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; i++) a.v[i] = v[i];
+        sort_any(a);
+        if constexpr (NQ == 4) {
+            Eight b;
+#pragma unroll
+            for (int i = 0; i < 8; i++) b.v[i] = v[8 + i];
+            sort_any(b);
+            join(a, b);
+        }
+        join_lanes<DPP_QUAD_1032>(a);
+    }
+    join_lanes<DPP_QUAD_2301>(a);
+    join_lanes<DPP_ROW_HALF_MIRROR>(a);
+    join_lanes<DPP_ROW_MIRROR>(a);
+    double o = a.v[0];
+#pragma unroll
+    for (int i = 1; i < 8; i++) o = l == i ? a.v[i] : o;
+    return o;
+}
+
 /* order-preserving bits of a number that is not NaN; larger for larger ones. -0
  * does not occur: a score is none, and +0 plus a bias of -0 is +0. */
 __device__ __forceinline__ uint32_t order_of(float c)
@@ -353,27 +471,27 @@ __global__ __launch_bounds__(256) void k_route_groups(RouteGroupsArgs a)
             }
         }
     }
-    int pick = -1;
+    double place[4 * NQ];
+#pragma unroll
+    for (int q = 0; q < NQ; q++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) place[4 * q + i] = place_of(key[q][i], id_of(q, i));
+    double mine = 0.0;
+    if (L == 16 && topk <= 8) {
+        mine = largest_of_lanes<NQ>(place, l);
+    } else {
 #pragma clang loop unroll(disable)
-    for (int k = 0; k < topk; k++) {
-        uint32_t best = 0;
+        for (int k = 0; k < topk; k++) {
+            double best = place[0];
 #pragma unroll
-        for (int q = 0; q < NQ; q++)
+            for (int j = 1; j < 4 * NQ; j++) best = fmax(best, place[j]);
+            best = max_lanes<L>(best);
+            mine = l == k ? best : mine;
 #pragma unroll
-            for (int i = 0; i < 4; i++) best = max32(best, key[q][i]);
-        best = over_lanes<L>(best, max32);
-        uint32_t id = 0xFFFFFFFFu;
-#pragma unroll
-        for (int q = NQ - 1; q >= 0; q--)
-#pragma unroll
-            for (int i = 3; i >= 0; i--) id = key[q][i] == best ? (uint32_t)id_of(q, i) : id;
-        id = best ? over_lanes<L>(id, min32) : 0xFFFFFFFFu;
-        if (l == k) pick = (int)id;
-#pragma unroll
-        for (int q = 0; q < NQ; q++)
-#pragma unroll
-            for (int i = 0; i < 4; i++) key[q][i] = (uint32_t)id_of(q, i) == id ? 0u : key[q][i];
+            for (int j = 0; j < 4 * NQ; j++) place[j] = place[j] == best ? 0.0 : place[j];
+        }
     }
+    const int pick = l < topk ? expert_of(mine) : -1;
     /* lane k's pick again, from its logit: the same bits */
     const float got = pick >= 0 ? score32<SCORE>(load1<TYPE>(row, pick), m) : 0.0f;
     const double sum = a.r.renorm ? sum_lanes<16>((double)got) : 1.0;
@@ -508,16 +626,18 @@ hipError_t launch(const RouteGroupsBwdArgs &a, hipStream_t st)
     return hipGetLastError();
 }
 /* Tokens from which four share a wave: fewer leave lanes of the device idle. us, a
- * wave each / shared, 256 experts: sigmoid, 8 groups, top 8 2,048 tokens 7.0 / 8.8,
- * 4,096 9.4 / 9.3, 16,384 25 / 19; softmax, top 6 4,096 6.9 / 7.9, 8,192 10.4 / 9.0;
- * backward 8,192 9.0 / 9.3, 16,384 16.3 / 15.4; sqrt(softplus), whose table is a
- * latency an expert, 8,192 15.7 / 18.8, 16,384 27 / 27. */
-constexpr int shared_from(int score) { return score == DSV4_HIP_SQRT_SOFTPLUS ? 16384 : 6144; }
+ * wave each / shared, 256 experts: sigmoid, 8 groups, top 8 2,048 tokens 6.8 / 7.2,
+ * 3,000 7.8 / 7.3, 16,384 26 / 16.4; softmax, top 6 3,000 6.1 / 6.9, 4,096 7.0 / 6.8,
+ * 16,384 19 / 12.3; sqrt(softplus), whose table is a latency an expert, 8,192 16.1 /
+ * 18.0, 12,288 22.4 / 22.4, 16,384 28 / 27; backward with scores' gradients 6,000 7.5 /
+ * 8.4, 8,192 9.1 / 9.3, 16,384 16.3 / 15.4, without 6,000 6.1 / 4.6. */
+int shared_from(const RouteGroupsArgs &a) { return a.r.score == DSV4_HIP_SQRT_SOFTPLUS ? 12288 : 3500; }
+int shared_from(const RouteGroupsBwdArgs &a) { return a.dscores ? 8192 : 4096; }
 template <int TYPE, int SCORE, class ARGS>
 hipError_t launch_size(const ARGS &a, hipStream_t st)
 {
     const int ne = a.r.n_experts;
-    if (ne <= 256 && a.n >= shared_from(SCORE)) {
+    if (ne <= 256 && a.n >= shared_from(a)) {
         if (ne <= 64) return launch<TYPE, SCORE, 16, 1>(a, st);
         if (ne <= 128) return launch<TYPE, SCORE, 16, 2>(a, st);
         return launch<TYPE, SCORE, 16, 4>(a, st);
