@@ -2300,7 +2300,7 @@ static int router_checks(const char *what, const DSV4HipRouter *r, int type, int
 {
     if (!r) return fail("%s: NULL router", what);
     if (!elem_type_ok(type)) return fail("%s: unknown element type %d", what, type);
-    if (n < 0 || n >= 1 << 26) return fail("%s: n %d outside 0..2^26 - 1", what, n);
+    if (n < 0 || n > (1 << 26) - 4) return fail("%s: n %d outside 0..2^26 - 4", what, n);   /* a launch: 2^32 threads */
     if (r->score < DSV4_HIP_SQRT_SOFTPLUS || r->score > DSV4_HIP_SIGMOID) return fail("%s: unknown score %d", what, r->score);
     return route_checks(what, r->n_experts, r->topk, nullptr, 0);
 }
@@ -2565,7 +2565,7 @@ static int quant_mxfp4(uint8_t *Q, uint8_t *S, const void *x, const void *u, Mxf
         return fail(cols ? "%s: need 0 <= n < 2^24, k up to 2^24 and ld >= k (got %d, %d, %lld)"
                          : "%s: need n >= 0, k a multiple of 32 up to 2^24 and ld >= k of whole 16-byte steps (got %d, %d, %lld)",
                     what, n, k, (long long)ld);
-    if ((cols ? (long)(n + 31) / 32 * 32 : (long)n) * k >= 1L << 35)
+    if ((cols ? (long)(n + 31) / 32 * 32 : (long)n) * k > (1L << 35) - 4096)                /* likewise */
         return fail("%s: %d x %d elements are too many for one launch", what, n, k);
     if (cols ? !aligned16(Q) || !elem_aligned(x, type) : !aligned16(x) || !aligned16(u) || ((uintptr_t)Q & 3u) != 0)
         return fail(cols ? "%s: need Q 16-byte aligned and a to its elements" : "%s: need rows 16- and Q 4-byte aligned", what);

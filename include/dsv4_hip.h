@@ -448,8 +448,8 @@ int  dsv4_hip_gemm_mxfp4q_grouped_dev(void *C, int out_type, const uint8_t *Aq, 
  * takes for a pair without an expert). A token with a logit of NaN or +inf
  * raises status bit 0: its ids are -1, its weights and scores NaN.
  * n_experts <= 1024, topk <= 16 and at most the experts of topk_group groups,
- * n_group <= 64 and a divisor of n_experts, n < 2^26. No workspace; streams as
- * above. */
+ * n_group <= 64 and a divisor of n_experts, n <= 2^26 - 4. The arrays do not
+ * overlap. No workspace; streams as above. */
 enum { DSV4_HIP_SQRT_SOFTPLUS = 0, DSV4_HIP_SOFTMAX = 1, DSV4_HIP_SIGMOID = 2 };
 typedef struct {
     int   score;                        /* DSV4_HIP_SQRT_SOFTPLUS, ...          */
@@ -465,7 +465,8 @@ int  dsv4_hip_route_groups_dev(int *idx, float *w, float *scores, const void *lo
  * and (or NULL) dscores [n][n_experts], the gradients of w and scores, for the
  * ids that the forward call chose; the choice itself has none. idx -1: its dw
  * adds nothing; another id outside [0, n_experts) likewise, and raises status
- * bit 0. In fp64, one rounding. n_group and what belongs to it are not read. */
+ * bit 0. In fp64, one rounding. n_group and what belongs to it are not read.
+ * dlogits may be logits, or dscores if they are of one type. */
 int  dsv4_hip_route_groups_bwd_dev(void *dlogits, const float *dw, const float *dscores, const void *logits,
                                    int type, const int *idx, int n, const DSV4HipRouter *r, void *stream);
 

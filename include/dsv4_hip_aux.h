@@ -68,8 +68,8 @@ int dsv4_hip_swiglu_quant_i8_dev(int8_t *Q, float *S, const void *g, const void 
  * 6 * 2^e >= blockmax (127 if all zero), codes the nearest values, ties to even,
  * the rule of dsv4_hip_quant_fp4_mx_dev. A block with a value that is not finite
  * gets byte 255 (NaN) and codes 0. Rows of the 4-bit products, or DSV4_WFP4
- * weights. k a multiple of 32 up to 2^24, n * k < 2^35, the bytes of ld a multiple of 16, a 16-byte and Q
- * 4-byte aligned; n = 0: nothing. No workspace. */
+ * weights. k a multiple of 32 up to 2^24, n * k <= 2^35 - 4096, the bytes of ld a
+ * multiple of 16, a 16-byte and Q 4-byte aligned; n = 0: nothing. No workspace. */
 int dsv4_hip_quant_mxfp4_dev(uint8_t *Q, uint8_t *S, const void *a, int type, int64_t ld, int n, int k,
                              void *stream);
 
@@ -81,7 +81,7 @@ int dsv4_hip_swiglu_quant_mxfp4_dev(uint8_t *Q, uint8_t *S, const void *g, const
 
 /* The same for the columns of a, the operands of a backward pass: with n' = n
  * rounded up to 32, Q[k][n' / 2] and S[k][n' / 32] hold a^T, zeros behind row n.
- * k any number up to 2^24, n < 2^24, k * n' < 2^35, ld >= k, a aligned to its
+ * k any number up to 2^24, n < 2^24, k * n' <= 2^35 - 4096, ld >= k, a aligned to its
  * elements (rows of even length at an even pitch and 2-element alignment are the
  * fast ones), Q 16-byte aligned. n or k 0: nothing. */
 int dsv4_hip_quant_mxfp4_t_dev(uint8_t *Q, uint8_t *S, const void *a, int type, int64_t ld, int n, int k,

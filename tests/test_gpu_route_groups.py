@@ -407,3 +407,37 @@ def test_no_tokens(lib, pkg):
     r = pkg.Router(SIGMOID, 8, 2, 1, 1, 1, 1, 1.0)
     lib.route_groups_dev(None, None, None, None, 0, 0, None, r)
     lib.route_groups_bwd_dev(None, None, None, None, 0, None, 0, r)
+
+
+@pytest.mark.parametrize("kind", [SQRT, SOFTMAX, SIGMOID])
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n", [5, 8203, 16391])
+def test_gradients_in_place(lib, pkg, kind, dtype, n):
+    """Over the logits, and over the scores' gradients, the bits of a call of its own."""
+    x = with_masks((1.5 * torch.randn(n, 70, device=DEV, generator=gen(n))).to(dtype))
+    dw, ds = (torch.randn(n, k, device=DEV, generator=gen(k)) for k in (6, 70))
+    r = pkg.Router(kind, 70, 6, 7, 4, 2, 1, 2.5)
+    idx, _, _ = route(lib, r, x)
+    want = backward(lib, r, x, idx, dw, ds)
+    y = x.clone()
+    lib.route_groups_bwd_dev(y.data_ptr(), dw.data_ptr(), ds.data_ptr(), y.data_ptr(), CODE[dtype], idx.data_ptr(), n, r)
+    assert torch.equal(y, want)
+    if dtype == torch.float32:
+        lib.route_groups_bwd_dev(ds.data_ptr(), dw.data_ptr(), ds.data_ptr(), x.data_ptr(), 0, idx.data_ptr(), n, r)
+        assert torch.equal(ds, want)
+
+
+@pytest.mark.parametrize("E", [3, 300])
+def test_most_tokens(lib, pkg, E):
+    """2^26 - 4 tokens, a wave's worth for three experts, past four waves a workgroup for 300."""
+    n = (1 << 26) - 4
+    x = torch.empty(n, E, dtype=torch.bfloat16, device=DEV).normal_(generator=gen(E))
+    r = pkg.Router(SIGMOID, E, 1, 1, 1, 1, 0, 1.0)
+    idx, w, _ = route(lib, r, x, scores=False)
+    few, w2, _ = route(lib, r, x[-9:].contiguous(), scores=False)
+    assert torch.equal(idx[-9:], few) and torch.equal(w[-9:], w2)
+    assert (idx[:: 1 << 20] >= 0).all()
+    dw = torch.ones(n, 1, device=DEV)
+    dx = backward(lib, r, x, idx.contiguous(), dw)
+    assert torch.equal(dx[-9:], backward(lib, r, x[-9:].contiguous(), few.contiguous(), dw[-9:].contiguous()))
+    assert lib.status() == 0

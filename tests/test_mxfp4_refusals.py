@@ -91,9 +91,9 @@ BAD += [("grouped", k, v) for k, v in [("C", None), ("ex_off", None), ("table", 
                                        ("N", 0), ("K", 16), ("K", 80), ("K", (1 << 20) + 32), ("n_a", 0), ("out", -2),
                                        ("Aq", P + 1), ("table", P + 4), ("row_tok", P + 2), ("n_a", 1 << 26)]]
 BAD += [("route", k, v) for k, v in [("idx", None), ("w", None), ("logits", None), ("r", None), ("type", 5), ("idx", P + 2),
-                                     ("scores", P + 1), ("bias", P + 2), ("logits", P + 2), ("n", 1 << 26)]]
+                                     ("scores", P + 1), ("bias", P + 2), ("logits", P + 2), ("n", (1 << 26) - 3)]]
 BAD += [("route_bwd", k, v) for k, v in [("dlogits", None), ("dw", None), ("logits", None), ("idx", None), ("r", None),
-                                         ("type", 9), ("dscores", P + 1), ("dlogits", P + 1), ("n", 1 << 26)]]
+                                         ("type", 9), ("dscores", P + 1), ("dlogits", P + 1), ("n", (1 << 26) - 3)]]
 
 
 @pytest.mark.parametrize("name,arg,value", BAD)
@@ -142,6 +142,7 @@ def test_more_than_a_launch_takes_is_refused(calls, m, n):
 
 
 @pytest.mark.parametrize("name,n,k", [("rows", (1 << 31) - 1, 64), ("rows", 1 << 11, 1 << 24), ("swiglu", 1 << 29, 64),
+                                      ("swiglu", (1 << 30) - 127, 32),
                                       ("columns", 1 << 20, 1 << 15), ("columns", (1 << 24) - 1, 1 << 12)])
 def test_more_elements_than_a_launch_takes_are_refused(calls, name, n, k):
     rc, why = calls[0](name, n=n, k=k, ld=k)
