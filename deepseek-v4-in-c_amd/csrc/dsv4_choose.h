@@ -322,18 +322,21 @@ inline long i8_waves(I8Form form, long M, long N, long ne)
 
 /* ------------------------------------------------ 4-bit products -------- */
 
-/* Forms of the product of 4-bit rows: 16 x 16 results a workgroup with K over
- * its waves (one matrix only), the others tiles of features x rows through a
- * ring in LDS; _W8: by eight waves, one workgroup a CU rather than two of four
- * waves. */
+/* Forms of the product of 4-bit rows: 16 x 16 results a workgroup with K over its
+ * eight waves, 32 x 32 with the stages of K over its four waves (TEAM), both for one
+ * matrix only, and tiles of features x rows whose waves share every stage
+ * through a ring in LDS; _W8: by eight waves, one workgroup a CU rather than two
+ * of four waves. 64x32 and 128x32: buckets only. */
 enum Fp4Form {
-    FP4_SPLIT = 1, FP4_64x32, FP4_64x64, FP4_128x32, FP4_128x64, FP4_128x128, FP4_128x128_W8, FP4_256x128, FP4_256x256
+    FP4_SPLIT = 1, FP4_TEAM, FP4_64x32, FP4_64x64, FP4_128x32, FP4_128x64, FP4_128x128,
+    FP4_128x128_W8, FP4_256x128, FP4_256x256
 };
 struct Fp4Shape { int F, TR, waves; };
 inline Fp4Shape fp4_shape(Fp4Form form)
 {
     switch (form) {
     case FP4_SPLIT: return {16, 16, 8};
+    case FP4_TEAM: return {32, 32, 4};
     case FP4_64x32: return {64, 32, 2};
     case FP4_64x64: return {64, 64, 4};
     case FP4_128x32: return {128, 32, 4};
@@ -347,22 +350,28 @@ inline Fp4Shape fp4_shape(Fp4Form form)
 
 /* Cost of a form, in hundredths of a us: c1 and, at K = 4096, c0 once, and for a
  * round of 256 workgroups fix + slope at K = 4096; the last round costs the share
- * r of one and the rest by how full it is. Fitted to 1,255 times (176 shapes of 1
- * to 4,096 rows, 300 to 32,768 features, K 256 to 8,192), of which the form that
- * they choose costs 1 % more than the best, at most 23 % (2,048 x 32,768 x 1024:
- * 256x256 74.6, 128x128 60.6). us, split / 64x32 / 64x64 / 128x64 / 128x128 /
- * 256x128 / 256x256: 1 x 4096 x 4096 3.4 / 6.1 / 6.6 / 8.1 / 10 / 15 / 23, 128 rows
- * - / 7.1 / 7.7 / 9.4 / 15 / 18 / 25, 512 rows - / 17.8 / 12.1 / 11.0 / 16 / 19 / 27,
- * 2,048 rows - / 52 / 39 / 30 / 24.6 / 24.1 / 29, 4,096 rows - / 100 / 74 / 57 / 47 / 46 /
- * 39.5; 333 x 1024 x 4096 - / 6.8 / 7.1 / 8.8 / 12 / 18 / 25; 2,048 x 4096 x 1024 - /
- * 23 / 16 / 12 / 9.2 / 10.4 / 12.6. 128x128_W8 after another 12 shapes, of 128x64 /
- * 128x128 / it / 256x128: 2,803 x 1024 x 4096 17.4 / 17.4 / 13.9 / 19.6, 1,024 x 4096 x
- * 4096 17.4 / 18.3 / 15.6 / 20.1, 2,048 x 4096 x 4096 35 / 25.7 / 29 / 25.2. */
+ * r of one and the rest by how full it is. Fitted to 2,300 times of 336 shapes (1 to
+ * 4,096 rows, 300 to 32,768 features, K 256 to 16,384), in which the form that they
+ * choose costs 0.8 % more than the best, in ten more than 10 % (1,024 x 4096 x 2048:
+ * 128x128_W8 13.3 us, 128x128 10.2; at other times of one card 9.7 and 10.3). us, split /
+ * team / 64x64 / 128x64 / 128x128 / _W8 / 256x128 / 256x256 (64x32 before the team: 64 x
+ * 4096 x 4096 6.5, 333 x 1024 x 1024 3.9):
+ *   1 x 4096 x 4096      3.3 / 3.9 / 6.6 / 8.1 / 10 / 11 / 15 / 23
+ *   64 rows              11 / 4.5 / 7.1 / 9.0
+ *   128 rows             - / 6.3 / 7.6 / 9.3
+ *   256 rows             - / 10.6 / 8.3 / 9.6
+ *   512 rows             - / - / 11.6 / 10.6 / 16 / 12.5 / 18 / 26
+ *   2,048 rows           - / - / 39 / 30 / 25.5 / 29.6 / 24.9 / 31
+ *   4,096 rows           - / - / - / 57 / 47 / - / 46 / 39.5
+ *   333 x 1024 x 4096    - / 6.0 / 7.0 / 8.7
+ *   333 x 1024 x 1024    - / 3.2 / 4.1 / 5.0
+ *   2,803 x 1024 x 4096  - / - / - / 16.6 / 15.9 / 13.1 / 18.8 / 26.5
+ *   2,048 x 4096 x 1024  - / - / - / 12.3 / 9.2 to 16.7 / 11.9 / 10.8 / 12.5 */
 struct Fp4Cost { Fp4Form form; int c1, c0, fix, slope, r; };
 constexpr Fp4Cost FP4_COSTS[] = {
-    {FP4_SPLIT, 195, 62, 36, 153, 71},      {FP4_64x32, 256, 172, 68, 238, 62},     {FP4_64x64, 233, 165, 100, 337, 63},
-    {FP4_128x64, 278, 182, 120, 534, 59},   {FP4_128x128, 282, 487, 159, 840, 42},  {FP4_128x128_W8, 78, 107, 283, 1087, 62},
-    {FP4_256x128, 112, 56, 497, 1650, 71},  {FP4_256x256, 0, 0, 890, 2722, 65}};
+    {FP4_SPLIT, 172, 57, 27, 158, 80},    {FP4_TEAM, 215, 57, 16, 184, 62},        {FP4_64x64, 211, 108, 111, 408, 68},
+    {FP4_128x64, 211, 79, 136, 655, 54},  {FP4_128x128, 354, 511, 137, 812, 16},   {FP4_128x128_W8, 63, 19, 320, 1077, 70},
+    {FP4_256x128, 75, 45, 626, 1595, 80}, {FP4_256x256, 9, 19, 872, 2427, 59}};
 /* row tiles: whole ones, and with ne experts one for each that rows may hit */
 inline long fp4_row_tiles(Fp4Form form, long M, long ne)
 {

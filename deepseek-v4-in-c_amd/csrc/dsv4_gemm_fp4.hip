@@ -49,18 +49,32 @@ __device__ __forceinline__ auto fp4_matrix(const Fp4Args &a)
     };
 }
 
-/* 16 scale bytes of a row from block b on (nb blocks a row); blocks past the
- * row's end 0. Rows of scales have any alignment. */
-__device__ __forceinline__ u32x4 fp4_scales(const uint8_t *row, int b, int nb)
+/* W scale bytes of a row from block b on (nb blocks a row), W = 8 or 16; blocks past
+ * the row's end 0. Rows of scales have any alignment. The last bytes come with those
+ * before them, shifted: a byte a time they waited for each other (1 row of 2048 x
+ * 2816 3.8 us, 3.1 so). */
+template <int W> struct Fp4Scales;
+template <> struct Fp4Scales<8> { typedef u32x2 type; typedef uint64_t bits; };
+template <> struct Fp4Scales<16> { typedef u32x4 type; typedef unsigned __int128 bits; };
+template <int W>
+__device__ __forceinline__ typename Fp4Scales<W>::type fp4_scales(const uint8_t *row, int b, int nb)
 {
-    if (b + 16 <= nb) return *(const DSV4_GLOBAL u32x4_any *)(row + b);
-    u32x4 v = {0, 0, 0, 0};
-    for (int i = 0; i < nb - b; i++) {
-        const uint32_t s = gptr(row)[b + i] << (8 * (i & 3));
-#pragma unroll
-        for (int j = 0; j < 4; j++) v[j] |= i / 4 == j ? s : 0u;
+    using T = typename Fp4Scales<W>::type;
+    using B = typename Fp4Scales<W>::bits;
+    typedef T at_any __attribute__((aligned(1)));
+    if (b + W <= nb) return *(const DSV4_GLOBAL at_any *)(row + b);
+    if (b >= nb) return T(0);
+    if (nb >= W) {
+        const T v = *(const DSV4_GLOBAL at_any *)(row + nb - W);
+        return __builtin_bit_cast(T, __builtin_bit_cast(B, v) >> (8 * (b + W - nb)));
     }
-    return v;
+    uint32_t v[W];
+#pragma unroll
+    for (int i = 0; i < W; i++) v[i] = gptr(row)[min(b + i, nb - 1)];
+    T o(0);
+#pragma unroll
+    for (int i = 0; i < W; i++) o[i / 4] |= b + i < nb ? v[i] << (8 * (i & 3)) : 0u;
+    return o;
 }
 
 __device__ __forceinline__ v8i fp4_operand(const v4i &v)
@@ -154,7 +168,7 @@ __global__ __launch_bounds__(512) void k_fp4_split(Fp4Args a)
             w[s] = buf_ld16<0>(rw, in ? (uint32_t)wr * KB + at : BUF_OOB);
             x[s] = buf_ld16<0>(rx, in ? (uint32_t)xr * KB + at : BUF_OOB);
         }
-        const u32x4 sw = fp4_scales(ws, 16 * p, nb), sx = fp4_scales(xs, 16 * p, nb);
+        const u32x4 sw = fp4_scales<16>(ws, 16 * p, nb), sx = fp4_scales<16>(xs, 16 * p, nb);
 #pragma unroll
         for (int s = 0; s < 4; s++) acc = fp4_mfma16(w[s], x[s], acc, sw[s] >> (8 * g), sx[s] >> (8 * g));
     }
@@ -166,6 +180,113 @@ __global__ __launch_bounds__(512) void k_fp4_split(Fp4Args a)
 #pragma unroll
     for (int w = 0; w < NW; w++) v += sum[w][o];
     fp4_store<OUT>(a.C, (size_t)(r0 + i) * a.N + n0 + n, v);
+}
+
+/* ------------------------------------------- stages over the waves -----
+ * A workgroup takes 32 features by 32 rows of one matrix, and its four waves
+ * share out the stages of 256 values, each with a stage's place of its own in
+ * LDS and all of the tile's results in registers: no wave waits for another
+ * before the sums meet in LDS, added in wave order. A stage's loads are asked for
+ * when the one before is in registers; other workgroups, five to a CU, hide their
+ * latency better than a second place does (64 x 4096 x 4096 4.5 us with either, 128 x
+ * 4096 x 1024 4.5 against 3.2; eight waves 4.4 and 4.3; 64 rows a tile 5.9 and 3.6).
+ * Bound: latency of launch, a few stages and the sums, then a CU's loads
+ * (128 KB of operands a 32 x 32 tile at K = 4096). */
+template <int OUT>
+__global__ __launch_bounds__(256) void k_fp4_team(Fp4Args a)
+{
+    constexpr int NW = 4, F = 32, T = 32, LW = F / 8, LX = T / 8, LD = F + 4, STAGE = (F + T) * 128;
+    static_assert(T * LD * 4 <= STAGE, "the sums take the stage's place");
+    __shared__ __align__(16) uint8_t lds[NW * STAGE];
+    const int lane = threadIdx.x & 63, wave = wave_in_group(), rr = lane & 31, g = lane >> 5;
+    const int mt = (a.M + T - 1) / T, nt = (a.N + F - 1) / F, total = mt * nt, nb = a.K / 32;
+    /* each XCD a contiguous run of tiles, row tiles first: it reads a weight once */
+    const int per = total / 8, rest = total % 8, x = blockIdx.x % 8, y = blockIdx.x / 8;
+    const int id = x * per + min(x, rest) + y, n0 = id / mt * F, r0 = id % mt * T;
+    const int rows = min(T, a.M - r0), nf = min(F, a.N - n0);
+    const uint32_t KB = (uint32_t)a.K / 2;
+    const int nreal = (a.K + 255) / 256;
+    const __amdgpu_buffer_rsrc_t rw = buf_rsrc(a.W + (size_t)n0 * KB, (uint32_t)nf * KB);
+    const __amdgpu_buffer_rsrc_t rx = buf_rsrc(a.Aq + (size_t)r0 * KB, (uint32_t)rows * KB);
+    uint8_t *const buf = lds + wave * STAGE;
+    auto swz = [](int r, int c) { return c ^ ((r >> 1) & 7); };
+    uint32_t wo[LW], xo[LX], xl[LX];               /* xl: of the last stage, pieces past K out of range */
+#pragma unroll
+    for (int i = 0; i < LW; i++) {
+        const int r = 8 * i + lane / 8;
+        wo[i] = r < nf ? (uint32_t)r * KB + 16u * (uint32_t)swz(r, lane & 7) : BUF_OOB;
+    }
+#pragma unroll
+    for (int i = 0; i < LX; i++) {
+        const int r = 8 * i + lane / 8, c = swz(r, lane & 7);
+        xo[i] = r < rows ? (uint32_t)r * KB + 16u * (uint32_t)c : BUF_OOB;
+        xl[i] = 8 * (nreal - 1) + c < nb ? xo[i] : BUF_OOB;
+    }
+    /* rows past the last: the last one's scales, not stored */
+    const uint8_t *const ws = a.Sw + (size_t)(n0 + min(rr, nf - 1)) * nb;
+    const uint8_t *const xs = a.As + (size_t)(r0 + min(rr, rows - 1)) * nb;
+    u32x2 bw, bx;                                  /* the eight scale bytes of a stage */
+    auto ask = [&](int st) {
+        bw = fp4_scales<8>(ws, 8 * st, nb);
+        bx = fp4_scales<8>(xs, 8 * st, nb);
+#pragma unroll
+        for (int i = 0; i < LW; i++) buf_dma16<0>(rw, wo[i] + 128u * (uint32_t)st, 0, buf + 1024 * i);
+#pragma unroll
+        for (int i = 0; i < LX; i++)
+            buf_dma16<0>(rx, (st < nreal - 1 ? xo[i] : xl[i]) + 128u * (uint32_t)st, 0, buf + 128 * F + 1024 * i);
+    };
+    const uint32_t pick = g ? 0x07050301u : 0x06040200u;
+    f32x16 acc;
+#pragma unroll
+    for (int e = 0; e < 16; e++) acc[e] = 0.0f;
+    if (wave < nreal) ask(wave);
+    for (int st = wave; st < nreal; st += NW) {
+        wait_vm<0>();
+        asm volatile("" ::: "memory");
+        v4i w[4], v[4];
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            w[k] = *(const v4i *)(buf + rr * 128 + 16 * swz(rr, 2 * k + g));
+            v[k] = *(const v4i *)(buf + 128 * (F + rr) + 16 * swz(rr, 2 * k + g));
+        }
+        const uint32_t sw = __builtin_amdgcn_perm(bw.y, bw.x, pick);
+        const uint32_t sx = __builtin_amdgcn_perm(bx.y, bx.x, pick);
+        __builtin_amdgcn_s_waitcnt(0xC07F);        /* the operands are in registers: the place is free */
+        asm volatile("" ::: "memory");
+        if (st + NW < nreal) ask(st + NW);
+        acc = fp4_mfma32<0>(w[0], v[0], acc, sw, sx);
+        acc = fp4_mfma32<1>(w[1], v[1], acc, sw, sx);
+        acc = fp4_mfma32<2>(w[2], v[2], acc, sw, sx);
+        acc = fp4_mfma32<3>(w[3], v[3], acc, sw, sx);
+    }
+#pragma unroll
+    for (int q = 0; q < 4; q++) {
+        f32x4 o;
+#pragma unroll
+        for (int e = 0; e < 4; e++) o[e] = acc[4 * q + e];
+        *(f32x4 *)(buf + 4 * (rr * LD + 8 * q + 4 * g)) = o;
+    }
+    __syncthreads();
+    static_assert(T * F == 4 * 64 * NW, "four results a thread");
+    const int m = threadIdx.x / (F / 4), n = threadIdx.x % (F / 4) * 4;
+    if (m >= rows || n >= nf) return;
+    f32x4 v = {0, 0, 0, 0};
+#pragma unroll
+    for (int k = 0; k < NW; k++) {
+        const f32x4 t = *(const f32x4 *)(lds + k * STAGE + 4 * (m * LD + n));
+#pragma unroll
+        for (int e = 0; e < 4; e++) v[e] += t[e];
+    }
+    const size_t at = (size_t)(r0 + m) * a.N + n0 + n;
+    if (n + 4 > nf) {
+        for (int e = 0; e < nf - n; e++) fp4_store<OUT>(a.C, at + e, v[e]);
+    } else if constexpr (OUT == DSV4_HIP_F32) {
+        typedef f32x4 any __attribute__((aligned(4)));
+        *(DSV4_GLOBAL any *)((float *)a.C + at) = v;
+    } else {
+        typedef u32x2 any __attribute__((aligned(2)));
+        *(DSV4_GLOBAL any *)((uint16_t *)a.C + at) = u32x2{fp4_pack<OUT>(v[0], v[1]), fp4_pack<OUT>(v[2], v[3])};
+    }
 }
 
 /* ------------------------------------------------------- many rows ------
@@ -274,7 +395,7 @@ __global__ __launch_bounds__((Fp4Tile<F, T, WR, WT, NST>::NT)) void k_fp4_tile(F
      * inside 16, from the start. No branch, and few instructions: in the loop a
      * wave's own instructions are what small tiles wait for. */
     const int last = nst / 2 - 1;
-    const u32x4 ends = fp4_scales(srow, 16 * last, nb);
+    const u32x4 ends = fp4_scales<16>(srow, 16 * last, nb);
     auto fetch_scales = [&](int pair) -> u32x4 {   /* w: 16 bytes that are there */
         return *(const DSV4_GLOBAL u32x4_any *)(nb < 16 ? t.w : srow + min(16 * pair, nb - 16));
     };
@@ -551,7 +672,9 @@ static hipError_t fp4_one(const Fp4Args &a, hipStream_t st)
     case FP4_SPLIT:
         hipLaunchKernelGGL(k_fp4_split<OUT>, dim3(groups), dim3(512), 0, st, a);
         return hipGetLastError();
-    case FP4_64x32: return fp4_tile<64, 32, 2, 1, 4, false, false, OUT>(a, groups, st);
+    case FP4_TEAM:
+        hipLaunchKernelGGL(k_fp4_team<OUT>, dim3(groups), dim3(256), 0, st, a);
+        return hipGetLastError();
     case FP4_64x64: return fp4_tile<64, 64, 2, 2, 3, false, false, OUT>(a, groups, st);
     case FP4_128x64: return fp4_tile<128, 64, 2, 2, 3, false, false, OUT>(a, groups, st);
     case FP4_128x128: return fp4_tile<128, 128, 2, 2, 2, false, false, OUT>(a, groups, st);

@@ -294,7 +294,7 @@ SHAPES = [(1, 1, 32), (1, 77, 4128), (3, 130, 96), (8, 4096, 544), (5, 1000, 256
           (130, 8200, 224), (300, 8192, 512), (900, 3333, 320), (1100, 4104, 96), (700, 6000, 1184), (2048, 2048, 768),
           (1300, 6001, 160), (2100, 8200, 288), (4100, 4097, 64), (2048, 8192, 1280), (4097, 4352, 32), (70, 15000, 544),
           (40, 20001, 1120), (333, 2111, 2080), (500, 4111, 2080), (1001, 4099, 1056), (2803, 4100, 2080), (1999, 4097, 4128),
-          (1, 20000, 4128)]
+          (1, 20000, 4128), (1990, 3416, 3040), (2044, 3357, 1632), (333, 2111, 160), (70, 999, 2720), (64, 4100, 4128)]
 
 
 @pytest.mark.parametrize("M,N,K", SHAPES)
