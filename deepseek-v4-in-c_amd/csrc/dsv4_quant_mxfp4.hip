@@ -98,10 +98,12 @@ __device__ __forceinline__ uint32_t mxfp4_code64(double v)
 } // namespace
 
 /* Four lanes hold a block, eight elements each; a thread takes NU units, 256
- * apart. us, NU 1 / 2 / 4: 4,206 rows of 2,048 bf16 5.3 / 4.8 / 5.2, SwiGLU 10.7 /
- * 11.6 / 13.7; 24,576 rows 23.1 / 20.9 / 21.0, SwiGLU 43.9 / 44.3 / 44.0. Bound: HBM
- * (24,576 rows 6.1 TB/s, SwiGLU 5.2), the vector unit for SwiGLU of fewer rows
- * (4,206: 3.6 TB/s), latency for a few. */
+ * apart: two of 16-bit elements where the device is full, else one. us, NU 1 / 2 / 4:
+ * 1,024 rows of 4,096 bf16 2.7 / 3.3 / 3.6, 1,600 4.1 / 3.9 / 4.6; 4,206 of 2,048 5.3 /
+ * 4.8 / 5.2, SwiGLU 10.7 / 11.6 / 13.7; 24,576 rows 23.1 / 20.9 / 21.0, SwiGLU 43.9 /
+ * 44.3 / 44.0; fp32 333 rows of 4,096 2.7 / 2.9 / 3.4, 8,192 rows 27.8 / 28.1 / 28.8.
+ * Bound: HBM (24,576 rows 6.1 TB/s, SwiGLU 5.2), the vector unit for SwiGLU of fewer
+ * rows (4,206: 3.6 TB/s), latency for a few. */
 template <int TYPE, bool SWIGLU, int NU>
 __global__ __launch_bounds__(256) void k_quant_mxfp4(QuantMxfp4Args a)
 {
@@ -277,8 +279,10 @@ static hipError_t quant_mxfp4_t(const QuantMxfp4Args &a, Mxfp4Rows rows, hipStre
     if (units >> 32) return hipErrorInvalidConfiguration;
     if (rows == MXFP4_SWIGLU)
         hipLaunchKernelGGL((k_quant_mxfp4<TYPE, true, 1>), dim3((unsigned)((units + 255) / 256)), dim3(256), 0, st, a);
-    else
+    else if (TYPE != DSV4_HIP_F32 && units > 5u << 17)
         hipLaunchKernelGGL((k_quant_mxfp4<TYPE, false, 2>), dim3((unsigned)((units + 511) / 512)), dim3(256), 0, st, a);
+    else
+        hipLaunchKernelGGL((k_quant_mxfp4<TYPE, false, 1>), dim3((unsigned)((units + 255) / 256)), dim3(256), 0, st, a);
     return hipGetLastError();
 }
 

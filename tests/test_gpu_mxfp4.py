@@ -79,7 +79,7 @@ def columns(v):
 
 # ------------------------------------------------------------------- rows ----
 
-SIZES = [(1, 32), (1, 4096), (3, 96), (33, 1024), (7, 2080), (2, 20000 // 32 * 32), (1030, 512)]
+SIZES = [(1, 32), (1, 4096), (3, 96), (33, 1024), (7, 2080), (2, 20000 // 32 * 32), (1030, 512), (1303, 4128)]
 
 
 @pytest.mark.parametrize("dtype", TYPES)
