@@ -328,8 +328,8 @@ inline long i8_waves(I8Form form, long M, long N, long ne)
  * through a ring in LDS; _W8: by eight waves, one workgroup a CU rather than two
  * of four waves. 64x32 and 128x32: buckets only. */
 enum Fp4Form {
-    FP4_SPLIT = 1, FP4_TEAM, FP4_64x32, FP4_64x64, FP4_128x32, FP4_128x64, FP4_128x128,
-    FP4_128x128_W8, FP4_256x128, FP4_256x256
+    FP4_SPLIT = 1, FP4_TEAM, FP4_64x32, FP4_64x64, FP4_128x32, FP4_128x64, FP4_128x96, FP4_128x128,
+    FP4_128x128_W8, FP4_256x128, FP4_256x192, FP4_256x256
 };
 struct Fp4Shape { int F, TR, waves; };
 inline Fp4Shape fp4_shape(Fp4Form form)
@@ -341,37 +341,40 @@ inline Fp4Shape fp4_shape(Fp4Form form)
     case FP4_64x64: return {64, 64, 4};
     case FP4_128x32: return {128, 32, 4};
     case FP4_128x64: return {128, 64, 4};
+    case FP4_128x96: return {128, 96, 4};
     case FP4_128x128: return {128, 128, 4};
     case FP4_128x128_W8: return {128, 128, 8};
     case FP4_256x128: return {256, 128, 8};
+    case FP4_256x192: return {256, 192, 8};
     default: return {256, 256, 8};
     }
 }
 
 /* Cost of a form, in hundredths of a us: c1 and, at K = 4096, c0 once, and for a
  * round of 256 workgroups fix + slope at K = 4096; the last round costs the share
- * r of one and the rest by how full it is. Fitted to 2,300 times of 336 shapes (1 to
+ * r of one and the rest by how full it is. Fitted to 3,000 times of 368 shapes (1 to
  * 4,096 rows, 300 to 32,768 features, K 256 to 16,384), in which the form that they
- * choose costs 0.8 % more than the best, in ten more than 10 % (1,024 x 4096 x 2048:
- * 128x128_W8 13.3 us, 128x128 10.2; at other times of one card 9.7 and 10.3). us, split /
- * team / 64x64 / 128x64 / 128x128 / _W8 / 256x128 / 256x256 (64x32 before the team: 64 x
- * 4096 x 4096 6.5, 333 x 1024 x 1024 3.9):
- *   1 x 4096 x 4096      3.3 / 3.9 / 6.6 / 8.1 / 10 / 11 / 15 / 23
- *   64 rows              11 / 4.5 / 7.1 / 9.0
- *   128 rows             - / 6.3 / 7.6 / 9.3
- *   256 rows             - / 10.6 / 8.3 / 9.6
- *   512 rows             - / - / 11.6 / 10.6 / 16 / 12.5 / 18 / 26
- *   2,048 rows           - / - / 39 / 30 / 25.5 / 29.6 / 24.9 / 31
- *   4,096 rows           - / - / - / 57 / 47 / - / 46 / 39.5
- *   333 x 1024 x 4096    - / 6.0 / 7.0 / 8.7
- *   333 x 1024 x 1024    - / 3.2 / 4.1 / 5.0
- *   2,803 x 1024 x 4096  - / - / - / 16.6 / 15.9 / 13.1 / 18.8 / 26.5
- *   2,048 x 4096 x 1024  - / - / - / 12.3 / 9.2 to 16.7 / 11.9 / 10.8 / 12.5 */
+ * choose costs 0.3 % more than the best, at most 13 % (16 x 512 x 8192: split 6.3 us, team
+ * 5.6). us, split / team / 64x64 / 128x64 / 128x96 / 128x128 / _W8 / 256x128 / 256x192 /
+ * 256x256 (64x32 before the team: 64 x 4096 x 4096 6.5, 333 x 1024 x 1024 3.9):
+ *   1 x 4096 x 4096      3.3 / 3.9 / 6.6 / 8.1 / ..
+ *   64 rows              11 / 4.5 / 7.1 / 9.0 / ..
+ *   128 rows             - / 6.3 / 7.6 / 9.3 / ..
+ *   256 rows             - / 10.6 / 8.3 / 9.6 / ..
+ *   768 rows             - / - / 19 / 15.5 / 11.9 / 16.0 / 12.7 / 18 / 23 / 26
+ *   1,536 rows           - / - / - / 24.5 / 22.8 / 22.5 / 25 / 20.2 / 23.7 / 27
+ *   2,803 rows           - / - / - / 44 / 45 / 36.3 / 40 / 40 / 29.6 / 31.1
+ *   4,096 rows           - / - / - / 57 / 62 / 45.7 / 51 / 44 / 51 / 38.3
+ *   333 x 1024 x 4096    - / 6.0 / 7.0 / 8.7 / ..
+ *   333 x 1024 x 1024    - / 3.2 / 4.1 / 5.0 / ..
+ *   2,803 x 1024 x 4096  - / - / - / 16.2 / 12.0 / 15.9 / 12.8 / 18.5 / 23 / 26
+ *   2,803 x 4096 x 1024  - / - / - / 17.3 / 20 / 14.3 / 17.1 / 16.8 / 12.3 / 13.6 */
 struct Fp4Cost { Fp4Form form; int c1, c0, fix, slope, r; };
 constexpr Fp4Cost FP4_COSTS[] = {
-    {FP4_SPLIT, 172, 57, 27, 158, 80},    {FP4_TEAM, 215, 57, 16, 184, 62},        {FP4_64x64, 211, 108, 111, 408, 68},
-    {FP4_128x64, 211, 79, 136, 655, 54},  {FP4_128x128, 354, 511, 137, 812, 16},   {FP4_128x128_W8, 63, 19, 320, 1077, 70},
-    {FP4_256x128, 75, 45, 626, 1595, 80}, {FP4_256x256, 9, 19, 872, 2427, 59}};
+    {FP4_SPLIT, 178, 43, 29, 175, 84},     {FP4_TEAM, 214, 69, 13, 185, 60},      {FP4_64x64, 212, 146, 129, 391, 46},
+    {FP4_128x64, 195, 36, 138, 622, 82},   {FP4_128x96, 207, 14, 187, 838, 65},   {FP4_128x128, 328, 319, 128, 775, 65},
+    {FP4_128x128_W8, 130, 0, 315, 841, 94}, {FP4_256x128, 35, 66, 670, 1604, 59}, {FP4_256x192, 42, 13, 577, 1917, 89},
+    {FP4_256x256, 30, 6, 1119, 2002, 77}};
 /* row tiles: whole ones, and with ne experts one for each that rows may hit */
 inline long fp4_row_tiles(Fp4Form form, long M, long ne)
 {
@@ -400,18 +403,19 @@ inline Fp4Form fp4_least(const Fp4Cost (&costs)[NF], long M, long N, long K, lon
 inline Fp4Form fp4_form(int M, int N, int K) { return fp4_least(FP4_COSTS, M, N, K, 0); }
 
 /* Buckets of ne experts, M rows in all: the same sum over the tiles of the launch,
- * fitted to 1,040 times with weights out of the caches (130 routings, even and
+ * fitted to 1,820 times with weights out of the caches (227 routings, even and
  * Zipf, of 6 to 24,576 rows to 8 to 256 experts of 300 x 544 to 4096 x 4096), the
- * chosen form 2 % above the best, at most 20 %. us, 64x32 / 128x32 / 128x64 /
+ * chosen form 0.9 % above the best, at most 16 %. us, 64x32 / 128x32 / 128x64 /
  * 256x128, experts 2048 x 4096 on 256: 6 rows 8.7 / 10.1 / 10.7 / 16.3, 384 rows 148
  * / 143 / 149 / 168, 1,536 rows 196 / 183 / 189 / 191, 6,144 rows 277 / 213 / 210 /
- * 199, 24,576 rows - / - / 360 / 236, Zipf - / - / 361 / 301; 8 of 4096 x 4096, 240
- * rows 21 / 21 / 16.6 / 26; 64 of 512 x 1024, 384 rows 7.6 / 7.3 / 7.6 / 9.9, 6,144
- * rows - / 14 / 11.7 / 11.0. */
-constexpr Fp4Cost FP4_BUCKET_COSTS[] = {{FP4_64x32, 337, 311, 93, 314, 0},
-                                        {FP4_128x32, 326, 432, 136, 575, 3},
-                                        {FP4_128x64, 400, 334, 148, 669, 0},
-                                        {FP4_256x128, 364, 806, 368, 1445, 16}};
+ * 199, 24,576 rows - / - / 360 / 236, Zipf - / - / 361 / 319 (by 256 rows 299); 8 of 4096
+ * x 4096, 240 rows 21 / 21 / 16.6 / 26; 64 of 512 x 1024, 384 rows 7.6 / 7.3 / 7.6 / 9.9,
+ * 6,144 rows - / 14 / 11.7 / 11.0. */
+constexpr Fp4Cost FP4_BUCKET_COSTS[] = {{FP4_64x32, 392, 211, 67, 358, 2},
+                                        {FP4_128x32, 364, 429, 117, 643, 0},
+                                        {FP4_128x64, 358, 459, 157, 654, 8},
+                                        {FP4_256x128, 226, 974, 497, 1411, 22},
+                                        {FP4_256x256, 524, 1882, 527, 1551, 0}};
 inline Fp4Form fp4_grouped_form(int M, int N, int K, int ne) { return fp4_least(FP4_BUCKET_COSTS, M, N, K, ne); }
 
 /* Whether the experts' weights go past the caches: rows few enough that an expert
@@ -423,7 +427,7 @@ inline Fp4Form fp4_grouped_form(int M, int N, int K, int ne) { return fp4_least(
 inline bool fp4_stream(int M, int N, int K, int ne)
 {
     const long hit = M < ne ? M : ne;
-    return hit * N * (K / 2) >= 1L << 27 && M <= 64 * hit && fp4_grouped_form(M, N, K, ne) != FP4_256x128;
+    return hit * N * (K / 2) >= 1L << 27 && M <= 64 * hit && fp4_grouped_form(M, N, K, ne) < FP4_256x128;
 }
 
 /* Waves of the launch that multiplies M rows by N features in a form: tiles

@@ -302,12 +302,13 @@ __global__ __launch_bounds__(256) void k_fp4_team(Fp4Args a)
  * so the stage NST ahead takes its place. The tile leaves through LDS as whole
  * 16-byte pieces of rows.
  * Bound, 256 x 256: the matrix instructions at the clock that power allows (4096^3
- * 39.4 us, 3.5 PFLOP/s; of it 9 us first loads and the way out, as one workgroup
+ * 37.5 us, 3.7 PFLOP/s; of it 9 us first loads and the way out, as one workgroup
  * has the CU). 128 x 128: a CU's loads, 32 KB a stage in 0.52 us (63 GB/s, alone
- * they reach 80): 2,803 x 1024 x 4096 13.7 us, 5 of them launch, first loads and the
- * way out. Buckets: the weights' stream (7 tokens, top 6 of 256 experts 2048 x 4096
- * 35 us, 5.0 TB/s; 4,096 tokens, Zipf, 311 us, 4.0 TB/s, and there a tile's products,
- * 1.17 us a stage with one workgroup a CU). */
+ * they reach 80): 2,803 x 1024 x 4096 13 us, in 128 x 96 tiles, which fill more of the
+ * CUs, 12, 5 of them launch, first loads and the way out. Buckets: the weights'
+ * stream (7 tokens, top 6 of 256 experts 2048 x 4096 35 us, 5.0 TB/s), with many rows
+ * the time between a tile's last load and the next one's first (4,096 tokens, Zipf,
+ * 300 us; without products 294, stores 276, tokens 276). */
 template <int F, int T, int WR, int WT, int NST_> struct Fp4Tile {
     static constexpr int NWAVE = WR * WT, NT = 64 * NWAVE, NST = NST_;
     static constexpr int WI = F / WR / 32, U = T / WT / 32;
@@ -316,8 +317,13 @@ template <int F, int T, int WR, int WT, int NST_> struct Fp4Tile {
     static constexpr int LW = F / 8 / NWAVE, LX = T / 8 / NWAVE, VM = LW + LX;
     static constexpr int RING = NST * STAGE, TABLE = NT * 16;
     static constexpr int out_ld(int eb) { return F * eb + 16; }
-    /* tokens that leave together */
-    static constexpr int out_rows(int eb) { return T * out_ld(eb) <= 160 * 1024 ? T : T / 2; }
+    /* tokens that leave together, whole row groups of every wave */
+    static constexpr int out_rows(int eb)
+    {
+        int parts = 1;
+        while (T / parts * out_ld(eb) > 160 * 1024 || T % (32 * WT * parts)) parts++;
+        return T / parts;
+    }
     static constexpr int lds(int eb)
     {
         return RING + 2 * TABLE > out_rows(eb) * out_ld(eb) ? RING + 2 * TABLE : out_rows(eb) * out_ld(eb);
@@ -327,36 +333,15 @@ template <int F, int T, int WR, int WT, int NST_> struct Fp4Tile {
 };
 
 template <int F, int T, int WR, int WT, int NST, bool GROUPED, bool STREAM, int OUT>
-__global__ __launch_bounds__((Fp4Tile<F, T, WR, WT, NST>::NT)) void k_fp4_tile(Fp4Args a)
+__device__ __forceinline__ void fp4_tile_sum(const Fp4Args &a, const Fp4Bucket &t, int n0)
 {
     using C = Fp4Tile<F, T, WR, WT, NST>;
     constexpr int U = C::U, WI = C::WI;
-    constexpr bool SHARED = GROUPED && F == 256;
     extern __shared__ __align__(16) uint8_t lds[];
     uint8_t *const table = lds + C::RING;
     const int lane = threadIdx.x & 63, wave = wave_in_group();
     const int rr = lane & 31, g = lane >> 5, wr = wave % WR, wt = wave / WR;
-    const int nt = (a.N + F - 1) / F, nb = a.K / 32;
-    Fp4Bucket t;
-    int n0;
-    if constexpr (GROUPED) {
-        int f = blockIdx.x % nt;
-        if constexpr (SHARED) t = bucket_tile<T, uint8_t>(a, blockIdx.x, lane, fp4_matrix(a), nt, &f);
-        else t = bucket_tile<T, uint8_t>(a, blockIdx.x / nt, lane, fp4_matrix(a));
-        n0 = f * F;
-        if (t.rows <= 0) return;
-    } else {
-        /* each XCD a contiguous run of tiles, eight row tiles by their feature
-         * tiles at a time */
-        const int mt = (a.M + T - 1) / T, total = mt * nt;
-        const int per = total / 8, rest = total % 8, x = blockIdx.x % 8, y = blockIdx.x / 8;
-        const int id = x * per + min(x, rest) + y;
-        const int grp = id / (8 * nt), gm = min(8, mt - 8 * grp), in = id - grp * 8 * nt;
-        t.w = a.W; t.s = a.Sw; t.e = 0; t.bad = false;
-        t.r0 = (8 * grp + in % gm) * T;
-        t.rows = min(T, a.M - t.r0);
-        n0 = in / gm * F;
-    }
+    const int nb = a.K / 32;
     const int nf = min(F, a.N - n0);
     if (GROUPED && t.bad) {
         fp4_bad<OUT>(a, t, n0, nf, C::NT);
@@ -376,6 +361,18 @@ __global__ __launch_bounds__((Fp4Tile<F, T, WR, WT, NST>::NT)) void k_fp4_tile(F
     for (int i = 0; i < C::LW; i++) {
         const int r = 8 * (C::LW * wave + i) + lane / 8;
         wo[i] = (uint32_t)r * KB + 16u * (uint32_t)swz(r, lane & 7);
+    }
+    /* the weights of the ring's first stages before the tokens are looked up
+     * (24,576 rows on 256 experts 2 %; where a tile is short it costs more: 42 rows 5 %) */
+    constexpr bool AHEAD = GROUPED && F == 256;
+    if constexpr (AHEAD) {
+#pragma unroll
+        for (int s = 0; s < NST; s++)
+#pragma unroll
+            for (int i = 0; i < C::LW; i++)
+                buf_dma16<STREAM ? 2 : 0>(buf_rsrc(wb, s < nreal ? wlen : 0u), wo[i], s < nreal ? 128 * s : 0,
+                                          lds + s * C::STAGE + 1024 * (C::LW * wave + i));
+        asm volatile("" ::: "memory");
     }
 #pragma unroll
     for (int i = 0; i < C::LX; i++) {
@@ -424,7 +421,7 @@ __global__ __launch_bounds__((Fp4Tile<F, T, WR, WT, NST>::NT)) void k_fp4_tile(F
 #pragma unroll
     for (int s = 0; s < NST; s++)
 #pragma unroll
-        for (int i = 0; i < C::VM; i++) issue(s, s, i);
+        for (int i = AHEAD ? C::LW : 0; i < C::VM; i++) issue(s, s, i);
     put_scales(0, first);
 
     struct Op { v4i w[WI], x[U]; };
@@ -448,7 +445,7 @@ __global__ __launch_bounds__((Fp4Tile<F, T, WR, WT, NST>::NT)) void k_fp4_tile(F
 #pragma unroll
             for (int e = 0; e < 16; e++) acc[i][u][e] = 0.0f;
     int slot = 0;
-    wait_vm<(NST - 1) * C::VM>();
+    wait_vm<(NST - 1) * (AHEAD ? C::LX : C::VM)>();
     __builtin_amdgcn_s_waitcnt(0xC07F);
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
@@ -650,6 +647,48 @@ __global__ __launch_bounds__((Fp4Tile<F, T, WR, WT, NST>::NT)) void k_fp4_tile(F
 }
 
 template <int F, int T, int WR, int WT, int NST, bool GROUPED, bool STREAM, int OUT>
+__global__ __launch_bounds__((Fp4Tile<F, T, WR, WT, NST>::NT)) void k_fp4_tile(Fp4Args a)
+{
+    const int nt = (a.N + F - 1) / F;
+    Fp4Bucket t;
+    int n0;
+    if constexpr (GROUPED) {
+        int f = blockIdx.x % nt;
+        if constexpr (F == 256) t = bucket_tile<T, uint8_t>(a, blockIdx.x, threadIdx.x & 63, fp4_matrix(a), nt, &f);
+        else t = bucket_tile<T, uint8_t>(a, blockIdx.x / nt, threadIdx.x & 63, fp4_matrix(a));
+        n0 = f * F;
+        if (t.rows <= 0) return;
+    } else {
+        /* each XCD a contiguous run of tiles, eight row tiles by their feature
+         * tiles at a time */
+        const int mt = (a.M + T - 1) / T, total = mt * nt;
+        const int per = total / 8, rest = total % 8, x = blockIdx.x % 8, y = blockIdx.x / 8;
+        const int id = x * per + min(x, rest) + y;
+        const int grp = id / (8 * nt), gm = min(8, mt - 8 * grp), in = id - grp * 8 * nt;
+        t.w = a.W; t.s = a.Sw; t.e = 0; t.bad = false;
+        t.r0 = (8 * grp + in % gm) * T;
+        t.rows = min(T, a.M - t.r0);
+        n0 = in / gm * F;
+    }
+    fp4_tile_sum<F, T, WR, WT, NST, GROUPED, STREAM, OUT>(a, t, n0);
+}
+
+/* Buckets of many rows: 256 features by the 256 rows of a bucket's whole tiles, a
+ * last tile of up to 128 rows in the smaller form with its deeper ring: a weight is
+ * read once for 256 rows (24,576 rows, Zipf, on 256 experts 2048 x 4096 319 us by 128
+ * rows, 300 so). */
+template <int OUT>
+__global__ __launch_bounds__(512) void k_fp4_buckets(Fp4Args a)
+{
+    const int nt = (a.N + 255) / 256;
+    int f = 0;
+    const Fp4Bucket t = bucket_tile<256, uint8_t>(a, blockIdx.x, threadIdx.x & 63, fp4_matrix(a), nt, &f);
+    if (t.rows <= 0) return;
+    if (t.rows > 128) fp4_tile_sum<256, 256, 4, 2, 2, true, false, OUT>(a, t, 256 * f);
+    else fp4_tile_sum<256, 128, 4, 2, 3, true, false, OUT>(a, t, 256 * f);
+}
+
+template <int F, int T, int WR, int WT, int NST, bool GROUPED, bool STREAM, int OUT>
 static hipError_t fp4_tile(const Fp4Args &a, unsigned groups, hipStream_t st)
 {
     using C = Fp4Tile<F, T, WR, WT, NST>;
@@ -658,6 +697,18 @@ static hipError_t fp4_tile(const Fp4Args &a, unsigned groups, hipStream_t st)
     const hipError_t e = allow_lds((const void *)k_fp4_tile<F, T, WR, WT, NST, GROUPED, STREAM, OUT>, lds, done);
     if (e != hipSuccess) return e;
     hipLaunchKernelGGL((k_fp4_tile<F, T, WR, WT, NST, GROUPED, STREAM, OUT>), dim3(groups), dim3(C::NT), lds, st, a);
+    return hipGetLastError();
+}
+
+template <int OUT>
+static hipError_t fp4_buckets(const Fp4Args &a, unsigned groups, hipStream_t st)
+{
+    constexpr int small = Fp4Tile<256, 128, 4, 2, 3>::lds(elem_bytes<OUT>()), large = Fp4Tile<256, 256, 4, 2, 2>::lds(elem_bytes<OUT>());
+    constexpr int lds = small > large ? small : large;
+    static uint64_t done = 0;
+    const hipError_t e = allow_lds((const void *)k_fp4_buckets<OUT>, lds, done);
+    if (e != hipSuccess) return e;
+    hipLaunchKernelGGL(k_fp4_buckets<OUT>, dim3(groups), dim3(512), lds, st, a);
     return hipGetLastError();
 }
 
@@ -677,9 +728,11 @@ static hipError_t fp4_one(const Fp4Args &a, hipStream_t st)
         return hipGetLastError();
     case FP4_64x64: return fp4_tile<64, 64, 2, 2, 3, false, false, OUT>(a, groups, st);
     case FP4_128x64: return fp4_tile<128, 64, 2, 2, 3, false, false, OUT>(a, groups, st);
+    case FP4_128x96: return fp4_tile<128, 96, 4, 1, 3, false, false, OUT>(a, groups, st);
     case FP4_128x128: return fp4_tile<128, 128, 2, 2, 2, false, false, OUT>(a, groups, st);
     case FP4_128x128_W8: return fp4_tile<128, 128, 4, 2, 3, false, false, OUT>(a, groups, st);
     case FP4_256x128: return fp4_tile<256, 128, 4, 2, 3, false, false, OUT>(a, groups, st);
+    case FP4_256x192: return fp4_tile<256, 192, 4, 2, 2, false, false, OUT>(a, groups, st);
     default: return fp4_tile<256, 256, 4, 2, 2, false, false, OUT>(a, groups, st);
     }
 }
@@ -695,7 +748,8 @@ static hipError_t fp4_grouped(const Fp4Args &a, hipStream_t st)
     case FP4_64x32: return fp4_tile<64, 32, 2, 1, 4, true, STREAM, OUT>(a, groups, st);
     case FP4_128x32: return fp4_tile<128, 32, 4, 1, 3, true, STREAM, OUT>(a, groups, st);
     case FP4_128x64: return fp4_tile<128, 64, 2, 2, 3, true, STREAM, OUT>(a, groups, st);
-    default: return fp4_tile<256, 128, 4, 2, 3, true, false, OUT>(a, groups, st);
+    case FP4_256x128: return fp4_tile<256, 128, 4, 2, 3, true, false, OUT>(a, groups, st);
+    default: return fp4_buckets<OUT>(a, groups, st);
     }
 }
 

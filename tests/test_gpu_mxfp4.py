@@ -294,7 +294,8 @@ SHAPES = [(1, 1, 32), (1, 77, 4128), (3, 130, 96), (8, 4096, 544), (5, 1000, 256
           (130, 8200, 224), (300, 8192, 512), (900, 3333, 320), (1100, 4104, 96), (700, 6000, 1184), (2048, 2048, 768),
           (1300, 6001, 160), (2100, 8200, 288), (4100, 4097, 64), (2048, 8192, 1280), (4097, 4352, 32), (70, 15000, 544),
           (40, 20001, 1120), (333, 2111, 2080), (500, 4111, 2080), (1001, 4099, 1056), (2803, 4100, 2080), (1999, 4097, 4128),
-          (1, 20000, 4128), (1990, 3416, 3040), (2044, 3357, 1632), (333, 2111, 160), (70, 999, 2720), (64, 4100, 4128)]
+          (1, 20000, 4128), (1990, 3416, 3040), (2044, 3357, 1632), (333, 2111, 160), (70, 999, 2720), (64, 4100, 4128),
+          (3658, 3624, 800), (312, 2659, 1216), (1609, 1153, 160), (431, 6829, 160)]
 
 
 @pytest.mark.parametrize("M,N,K", SHAPES)
@@ -433,7 +434,8 @@ GROUPS = [([1], 1, 32), ([0, 0, 3, 0], 40, 96), ([1] * 40, 64, 544), ([5, 0, 9, 
           ([20, 0, 31, 18, 2, 40], 77, 1056), ([64, 10, 0, 30, 33, 48], 130, 352), ([100, 0, 60, 130, 1, 90], 333, 608),
           ([300, 0, 3, 129, 128, 127, 500], 300, 416), ([0, 700, 0, 0, 20], 520, 96), ([2500, 3, 0, 300], 1000, 160),
           ([1, 0, 1200, 0, 60, 200, 1100] * 2, 300, 288), ([1] * 300 + [0] * 700 + [4] * 24, 33, 64),
-          ([33, 64, 65, 0, 1, 31, 32, 96] * 4, 1000, 1056), ([257, 128, 129, 1, 0, 127, 31, 65] * 4, 1030, 544)]
+          ([33, 64, 65, 0, 1, 31, 32, 96] * 4, 1000, 1056), ([257, 128, 129, 1, 0, 127, 31, 65] * 4, 1030, 544),
+          ([700, 0, 128, 129, 256, 257, 1, 1500, 900], 4111, 288), ([2000, 31, 255, 0, 1900, 65], 2100, 1120)]
 # weights that go past the caches: 128 MB and more of them, few rows an expert
 STREAMS = [([1, 0, 2, 1, 0, 0, 3] * 9, 2051, 4128), ([5, 0, 9, 1, 12, 0, 3] * 9, 2051, 4128),
            ([60, 33, 64, 0, 1, 20, 50, 31], 8200, 8224)]

@@ -50,7 +50,7 @@ def test_gpu_tests_reach_every_form(rules):
         f = rules.c_form(M, N, K)
         if M % rules.c_shape(f, 1) and N % rules.c_shape(f, 0) and K % 256:
             ragged.add(f)
-    assert {rules.c_form(*s) for s in test_gpu_mxfp4.SHAPES} == ragged == every and len(every) == 8
+    assert {rules.c_form(*s) for s in test_gpu_mxfp4.SHAPES} == ragged == every and len(every) == 10
 
 
 def test_gpu_tests_reach_every_form_of_the_experts_product(rules):
