@@ -445,7 +445,9 @@ __device__ __forceinline__ void fp4_tile_sum(const Fp4Args &a, const Fp4Bucket &
 #pragma unroll
             for (int e = 0; e < 16; e++) acc[i][u][e] = 0.0f;
     int slot = 0;
-    wait_vm<(NST - 1) * (AHEAD ? C::LX : C::VM)>();
+    /* AHEAD: the first stages' tokens come last, all but the last stage's are waited
+     * for here, as the waits of the loop count whole stages */
+    wait_vm<AHEAD ? C::LX : (NST - 1) * C::VM>();
     __builtin_amdgcn_s_waitcnt(0xC07F);
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
