@@ -307,8 +307,8 @@ __global__ __launch_bounds__(256) void k_fp4_team(Fp4Args a)
  * they reach 80): 2,803 x 1024 x 4096 13 us, in 128 x 96 tiles, which fill more of the
  * CUs, 12, 5 of them launch, first loads and the way out. Buckets: the weights'
  * stream (7 tokens, top 6 of 256 experts 2048 x 4096 35 us, 5.0 TB/s), with many rows
- * the time between a tile's last load and the next one's first (4,096 tokens, Zipf,
- * 300 us; without products 294, stores 276, tokens 276). */
+ * beside it the tokens and the results (4,096 tokens, Zipf, 300 us, 4.2 TB/s; without
+ * products 294, without either of the two 276). */
 template <int F, int T, int WR, int WT, int NST_> struct Fp4Tile {
     static constexpr int NWAVE = WR * WT, NT = 64 * NWAVE, NST = NST_;
     static constexpr int WI = F / WR / 32, U = T / WT / 32;
