@@ -331,7 +331,11 @@ __device__ __forceinline__ float score32(float x, const Norm &m)
 {
     if constexpr (SCORE == DSV4_HIP_SOFTMAX) return x > NO_EXPERT ? (float)(exp_below(x, m.top) * m.inv) : 0.0f;
     else if constexpr (SCORE == DSV4_HIP_SIGMOID) return (float)sigmoid64(x);
-    else return route_orig(x);
+    else {
+        bool rare = false;
+        const float s = dsv4_route::route_orig_most(x, rare);
+        return rare ? route_orig(x) : s;
+    }
 }
 
 } // namespace
@@ -375,11 +379,26 @@ __global__ __launch_bounds__(256) void k_route_groups(RouteGroupsArgs a)
             for (int q = 0; q < NQ; q++)
 #pragma unroll
                 for (int i = 0; i < 4; i++) s[q][i] = (float)(p[q][i] * m.inv);
-        } else {
+        } else if constexpr (SCORE == DSV4_HIP_SIGMOID) {
 #pragma unroll
             for (int q = 0; q < NQ; q++)
 #pragma unroll
                 for (int i = 0; i < 4; i++) s[q][i] = score32<SCORE>(x[q][i], m);
+        } else {
+            /* all without a branch, so that the table's loads overlap (1 token of 256
+             * experts 4.6 us, with branches 6.1; 16,384 21, 27); again where that does
+             * not serve */
+            bool rare = false;
+#pragma unroll
+            for (int q = 0; q < NQ; q++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) s[q][i] = dsv4_route::route_orig_most(x[q][i], rare);
+            if (rare) {
+#pragma unroll
+                for (int q = 0; q < NQ; q++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++) s[q][i] = route_orig(x[q][i]);
+            }
         }
 #pragma unroll
         for (int q = 0; q < NQ; q++) {
@@ -634,10 +653,10 @@ hipError_t launch(const RouteGroupsBwdArgs &a, hipStream_t st)
 /* Tokens from which four share a wave: fewer leave lanes of the device idle. us, a
  * wave each / shared, 256 experts: sigmoid, 8 groups, top 8 2,048 tokens 6.8 / 7.2,
  * 3,000 7.8 / 7.3, 16,384 26 / 16.4; softmax, top 6 3,000 6.1 / 6.9, 4,096 7.0 / 6.8,
- * 16,384 19 / 12.3; sqrt(softplus), whose table is a latency an expert, 8,192 16.1 /
- * 18.0, 12,288 22.4 / 22.4, 16,384 28 / 27; backward with scores' gradients 6,000 7.5 /
+ * 16,384 19 / 12.3; sqrt(softplus), top 6 4,096 8.9 / 10.4, 8,192 14.0 / 12.6, 16,384 -
+ * / 21; backward with scores' gradients 6,000 7.5 /
  * 8.4, 8,192 9.1 / 9.3, 16,384 16.3 / 15.4, without 6,000 6.1 / 4.6. */
-int shared_from(const RouteGroupsArgs &a) { return a.r.score == DSV4_HIP_SQRT_SOFTPLUS ? 12288 : 3500; }
+int shared_from(const RouteGroupsArgs &a) { return a.r.score == DSV4_HIP_SQRT_SOFTPLUS ? 6144 : 3500; }
 int shared_from(const RouteGroupsBwdArgs &a) { return a.dscores ? 8192 : 4096; }
 template <int TYPE, int SCORE, class ARGS>
 hipError_t launch_size(const ARGS &a, hipStream_t st)

@@ -184,6 +184,46 @@ DSV4_HD float route_orig(float x)
     return (float)sqrt((double)sp);
 }
 
+/* The same bits without a branch, for x of -20 and more and below expf's underflow;
+ * between them `rare` is set and the result is none. The steps are those above with
+ * k = 0 and c = 0 for a small e^x, which add exact zeros; sqrtf is correctly rounded
+ * on the GPU too. */
+DSV4_HD float route_orig_most(float x, bool &rare)
+{
+    DSV4_UNFUSED
+    const float ln2_hi = 6.9313812256e-01f, ln2_lo = 9.0580006145e-06f;
+    const float Lp1 = 6.6666668653e-01f, Lp2 = 4.0000000596e-01f, Lp3 = 2.8571429849e-01f,
+                Lp4 = 2.2222198546e-01f, Lp5 = 1.8183572590e-01f, Lp6 = 1.5313838422e-01f,
+                Lp7 = 1.4798198640e-01f;
+    const double N = 32.0, shift = 0x1.8p+52, inv_ln2_n = 0x1.71547652b82fep+0 * N;
+    const bool under = x < -0x1.9fe368p6f;
+    const double xd = (double)(x > 20.0f ? 20.0f : x < -20.0f ? -20.0f : x);
+    double kd = fma(inv_ln2_n, xd, shift);
+    const uint64_t ki = dbits(kd);
+    kd -= shift;
+    const double r = fma(inv_ln2_n, xd, -kd), r2 = r * r;
+    const double p = dof(kExp2Tab[ki % 32] + (ki << (52 - 5)));
+    const double z2 = fma(0x1.c6af84b912394p-5 / N / N / N, r, 0x1.ebfce50fac4f3p-3 / N / N);
+    const float e = (float)(fma(z2, r2, fma(0x1.62e42ff0c52d6p-1 / N, r, 1.0)) * p);
+    const bool small = fbits(e) < 0x3ed413d7u;
+    const float u = 1.0f + e;
+    const uint32_t hu = fbits(u) & 0x007fffffu;
+    const int32_t k0 = (int32_t)(fbits(u) >> 23) - 127;
+    const bool low = hu < 0x3504f7u;
+    const float cu = (k0 > 0 ? 1.0f - (u - e) : e - (u - 1.0f)) / u;
+    rare |= x < -20.0f && !under;
+    const bool tiny = !small && (low ? hu : (0x00800000u - hu) >> 2) == 0u;     /* |f| < 2^-20 */
+    const float f = small ? e : fof(hu | (low ? 0x3f800000u : 0x3f000000u)) - 1.0f;
+    const float k = small ? 0.0f : (float)(k0 + (low ? 0 : 1)), c = k == 0.0f ? 0.0f : cu;
+    const float hfsq = 0.5f * f * f;
+    const float s = f / (2.0f + f);
+    const float z = s * s;
+    const float R = z * (Lp1 + z * (Lp2 + z * (Lp3 + z * (Lp4 + z * (Lp5 + z * (Lp6 + z * Lp7))))));
+    const float kc = k * ln2_lo + c, a = tiny ? hfsq * (1.0f - 0.66666666666666666f * f) - kc : hfsq - (s * (hfsq + R) + kc);
+    const float l = tiny && f == 0.0f ? k * ln2_hi + kc : k * ln2_hi - (a - f);
+    return under ? 0.0f : sqrtf(x > 20.0f ? x : l);
+}
+
 } // namespace dsv4_route
 
 #endif /* DSV4_ROUTE_MATH_H */
