@@ -297,7 +297,37 @@ __device__ __forceinline__ double sigmoid64(float x)
     return rcp64(1.0 + exp64((double)__builtin_amdgcn_fmed3f(-x, -700.0f, 700.0f)));
 }
 __device__ __forceinline__ double exp_below(float x, float top) { return exp64(fmax((double)x - (double)top, -700.0)); }
-__device__ __forceinline__ double softplus64(float x) { return x > 20.0f ? (double)x : log1p(exp((double)x)); }
+/* sqrt(softplus(x)) and its derivative sigmoid(x) / (2 sqrt(softplus(x))) in fp64,
+ * relatively within 2^-44; 1 / (2 sqrt(x)) above 20; 0 for an expert that is not
+ * there. With 1 + e^x = 2^k (1 + f), 1 + f in [sqrt(1/2), sqrt(2)) (f = e^x itself
+ * where k is 0, so that a small one keeps its bits), the logarithm is k ln 2 + 2 t (1 +
+ * t^2 / 3 + .. + t^14 / 15), t = f / (2 + f), |t| < 0.172; the square root and the division
+ * are one reciprocal root, the instruction's bits and a step of third order. */
+struct Root { double s, d; };
+__device__ __forceinline__ Root sqrt_softplus64(float x)
+{
+    const double e = exp64((double)__builtin_amdgcn_fmed3f(x, -700.0f, 20.0f)), u = 1.0 + e;
+    const uint64_t bits = (uint64_t)__double_as_longlong(u);
+    const int k = ((int)(bits >> 32) - 0x3FE6A09E) >> 20;
+    const double m = __longlong_as_double((long long)(bits - ((uint64_t)(uint32_t)k << 52)));
+    const double f = k == 0 ? e : m - 1.0, t = f * rcp64(2.0 + f), w = t * t;
+    double p = 2.0 / 15;
+    p = fma(p, w, 2.0 / 13);
+    p = fma(p, w, 2.0 / 11);
+    p = fma(p, w, 2.0 / 9);
+    p = fma(p, w, 2.0 / 7);
+    p = fma(p, w, 2.0 / 5);
+    p = fma(p, w, 2.0 / 3);
+    p = fma((double)k, 0.6931471805599453, fma(t * w, p, t + t));
+    p = x > 20.0f ? fmin((double)x, 1e300) : p;
+    double y = __builtin_amdgcn_rsq(p);
+    const double h = fma(-p * y, y, 1.0);
+    y = fma(y * h, fma(h, 0.375, 0.5), y);
+    const double d = (x > 20.0f ? 0.5 : 0.5 * e * rcp64(u)) * y;
+    Root o = {p * y, d};
+    if (!(x > NO_EXPERT)) o.s = o.d = x < 0.0f ? 0.0 : (double)x;      /* -inf; NaN stays */
+    return o;
+}
 
 /* softmax over a token's L x 4 NQ logits: e^(x - top), top and 1 / sum; an expert
  * that is not there adds nothing, a token without experts has inv 0 */
@@ -578,12 +608,12 @@ __global__ __launch_bounds__(256) void k_route_groups_bwd(RouteGroupsBwdArgs a)
     auto score = [&](float v) -> double {
         if constexpr (SCORE == DSV4_HIP_SOFTMAX) return v > NO_EXPERT ? exp_below(v, m.top) * m.inv : 0.0;
         else if constexpr (SCORE == DSV4_HIP_SIGMOID) return sigmoid64(v);
-        else return sqrt(softplus64(v));
+        else return sqrt_softplus64(v).s;
     };
     auto slope = [&](float v, double sv) -> double {
         if constexpr (SCORE == DSV4_HIP_SOFTMAX) return sv;
         else if constexpr (SCORE == DSV4_HIP_SIGMOID) return v > NO_EXPERT ? sv * (1.0 - sv) : 0.0;
-        else return sv == 0.0 ? 0.0 : (v > 20.0f ? 1.0 : sigmoid64(v)) / (2.0 * sv);
+        else return sqrt_softplus64(v).d;
     };
     const double sk = id >= 0 ? score(xk) : 0.0;
     double ds = dw;
