@@ -368,6 +368,14 @@ __device__ __forceinline__ float score32(float x, const Norm &m)
     }
 }
 
+/* whether score32 of x, with s its score in fp64, is 0 */
+template <int SCORE>
+__device__ __forceinline__ bool zero_score(float x, double s)
+{
+    if constexpr (SCORE == DSV4_HIP_SQRT_SOFTPLUS) return dsv4_route::route_orig_zero(x);
+    else return (float)s == 0.0f;
+}
+
 } // namespace
 
 template <int TYPE, int SCORE, int L, int NQ>
@@ -620,7 +628,7 @@ __global__ __launch_bounds__(256) void k_route_groups_bwd(RouteGroupsBwdArgs a)
     if (a.r.renorm) {
         const double P = sum_lanes<16>(sk), dot = sum_lanes<16>(sk * dw);
         /* the forward call's weights are constant 0 where its fp32 scores are */
-        const bool none = !any_lane<L>((float)sk != 0.0f, lane);
+        const bool none = !any_lane<L>(id >= 0 && !zero_score<SCORE>(xk, sk), lane);
         ds = none ? 0.0 : (dw - dot / P) / P;
     }
     /* the same expert twice: its gradient holds both */

@@ -184,6 +184,11 @@ DSV4_HD float route_orig(float x)
     return (float)sqrt((double)sp);
 }
 
+/* Whether route_orig(x) is 0: where expf underflows, as log1pf and sqrtf of a
+ * positive number are positive. sqrt(softplus(x)) itself is a positive float down to
+ * -207. */
+DSV4_HD bool route_orig_zero(float x) { return x < -0x1.9fe368p6f; }
+
 /* The same bits without a branch, for x of -20 and more and below expf's underflow;
  * between them `rare` is set and the result is none. The steps are those above with
  * k = 0 and c = 0 for a small e^x, which add exact zeros; sqrtf is correctly rounded

@@ -463,7 +463,8 @@ int  dsv4_hip_route_groups_dev(int *idx, float *w, float *scores, const void *lo
 
 /* Gradient of the logits, dlogits [n][n_experts] of `type`, from dw [n][topk]
  * and (or NULL) dscores [n][n_experts], the gradients of w and scores, for the
- * ids that the forward call chose; the choice itself has none. idx -1: its dw
+ * ids that the forward call chose; the choice itself has none, and neither have
+ * renormalised weights that are 0 because every chosen score is. idx -1: its dw
  * adds nothing; another id outside [0, n_experts) likewise, and raises status
  * bit 0. In fp64, one rounding. n_group and what belongs to it are not read.
  * dlogits may be logits, or dscores if they are of one type. */

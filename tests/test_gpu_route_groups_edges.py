@@ -1,0 +1,49 @@
+# SPDX-License-Identifier: Apache-2.0
+"""The router with groups at its edges on the GPU: weights that are constant.
+
+Bounds as in test_gpu_route_groups.py: what is exactly 0 is compared with 0, a
+gradient is an fp64 value with one rounding to the logits' type, and an absolute
+part of 2e-11 for what cancels."""
+import pytest
+import torch
+
+from test_gpu_route_groups import DEV, HALF, SIGMOID, SOFTMAX, SQRT, TINY, TYPES, backward, gen, route, want_grad
+
+pytestmark = pytest.mark.gpu
+
+INF = float("inf")
+
+
+@pytest.mark.parametrize("kind", [SQRT, SOFTMAX, SIGMOID])
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n,E", [(6, 4), (40, 700), (4103, 200)])
+def test_constant_weights_have_no_gradient(lib, pkg, kind, dtype, n, E):
+    """Where every chosen score is 0 the weights are 0 whatever the logits: exactly no gradient.
+    sqrt(softplus) of fp32 is 0 from -104 down, its exact value e^(x / 2) only from -207 down."""
+    x = -104.0 - 100.0 * torch.rand(n, E, device=DEV, generator=gen(n + E))
+    x[0] = torch.arange(E, device=DEV) - (119.0 + E)
+    x[2, 1:] = -INF
+    x[3] = -INF
+    x[4] = torch.linspace(-300.0, -1000.0, E, device=DEV)
+    x[5::2] += 110.0                               # scores that are not 0
+    x = x.to(dtype)
+    dw = torch.randn(n, 3, device=DEV, generator=gen(2))
+    r = pkg.Router(kind, E, 3, 1, 1, 1, 1, 2.5)
+    lib.status()
+    idx, w, _ = route(lib, r, x)
+    got = backward(lib, r, x, idx, dw)
+    assert lib.status() == 0
+    none = (w == 0).all(1)
+    # softmax: a token's largest score is 1 / (experts near it) or more, so only one without experts has none
+    zeros = torch.ones(n, dtype=torch.bool, device=DEV)
+    zeros[5::2] = False
+    if kind == SOFTMAX:
+        zeros[:] = False
+        zeros[3] = True
+    assert torch.equal(none, zeros)
+    assert (got[none] == 0).all()
+    want = want_grad(r, x[~none], idx[~none], dw[~none], None)
+    # an id of -1 in a row of -inf differentiates to NaN beside it
+    want = torch.where(x[~none] > -INF, want, 0.0)
+    assert ((got[~none].double() - want).abs() <= 1.001 * HALF[dtype] * want.abs() + 1e-12 * 20 + TINY[dtype]).all()
+    assert (got[~none] != 0).any()
