@@ -609,6 +609,25 @@ __global__ __launch_bounds__(256) void k_route_groups_bwd(RouteGroupsBwdArgs a)
             if (!a.dscores || id_of(q) + i >= ne) g[q][i] = 0.0f;
         }
     }
+    /* a token that the forward call refuses has ids of -1: without its logits and its
+     * scores' gradients it counts as one without experts */
+    if (dense) {
+        float top = NO_EXPERT;                     /* NaN if one is */
+#pragma unroll
+        for (int q = 0; q < NQ; q++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) top = __builtin_elementwise_maximum(top, x[q][i]);
+        if (any_lane<L>(!(top < __builtin_inff()), lane)) {
+            if (l == 0 && there) atomicOr(a.status, ST_BAD_EXPERT_ID);
+#pragma unroll
+            for (int q = 0; q < NQ; q++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    x[q][i] = NO_EXPERT;
+                    g[q][i] = 0.0f;
+                }
+        }
+    }
     Norm m = {0.0f, 0.0};
     double s[NQ][4];
     if constexpr (SCORE == DSV4_HIP_SOFTMAX) m = softmax_norm<L, NQ>(x, s);

@@ -466,8 +466,11 @@ int  dsv4_hip_route_groups_dev(int *idx, float *w, float *scores, const void *lo
  * ids that the forward call chose; the choice itself has none, and neither have
  * renormalised weights that are 0 because every chosen score is. idx -1: its dw
  * adds nothing; another id outside [0, n_experts) likewise, and raises status
- * bit 0. In fp64, one rounding. n_group and what belongs to it are not read.
- * dlogits may be logits, or dscores if they are of one type. */
+ * bit 0. A token that the forward call refuses (a logit of NaN or +inf, its ids
+ * -1) has gradient 0 whatever dw and dscores hold; with dscores or softmax,
+ * which read all its logits, it raises bit 0 again. In fp64, one rounding.
+ * n_group and what belongs to it are not read. dlogits may be logits, or dscores
+ * if they are of one type. */
 int  dsv4_hip_route_groups_bwd_dev(void *dlogits, const float *dw, const float *dscores, const void *logits,
                                    int type, const int *idx, int n, const DSV4HipRouter *r, void *stream);
 

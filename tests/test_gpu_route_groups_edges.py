@@ -1,5 +1,6 @@
 # SPDX-License-Identifier: Apache-2.0
-"""The router with groups at its edges on the GPU: weights that are constant.
+"""The router with groups at its edges on the GPU: weights that are constant, tokens
+that are refused.
 
 Bounds as in test_gpu_route_groups.py: what is exactly 0 is compared with 0, a
 gradient is an fp64 value with one rounding to the logits' type, and an absolute
@@ -47,3 +48,35 @@ def test_constant_weights_have_no_gradient(lib, pkg, kind, dtype, n, E):
     want = torch.where(x[~none] > -INF, want, 0.0)
     assert ((got[~none].double() - want).abs() <= 1.001 * HALF[dtype] * want.abs() + 1e-12 * 20 + TINY[dtype]).all()
     assert (got[~none] != 0).any()
+
+
+@pytest.mark.parametrize("kind", [SQRT, SOFTMAX, SIGMOID])
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("renorm", [0, 1])
+@pytest.mark.parametrize("n,E", [(9, 70), (8205, 200), (21, 600)])
+def test_refused_tokens_have_no_gradient(lib, pkg, kind, dtype, renorm, n, E):
+    """A logit of NaN or +inf: ids of -1, gradient 0 whatever comes back for the weights and scores,
+    the other tokens' bits those of a batch without it."""
+    good = torch.randn(n, E, device=DEV, generator=gen(n + E)).to(dtype)
+    bad = torch.tensor([2, 5, n - 1, n - 2], device=DEV)
+    x = good.clone()
+    x[2, E - 1], x[5, 0], x[n - 1], x[n - 2, 7] = float("nan"), INF, float("nan"), INF
+    x[2, 3], x[5, 1:4] = INF, -INF
+    others = torch.ones(n, dtype=torch.bool, device=DEV)
+    others[bad] = False
+    r = pkg.Router(kind, E, 4, 5, 3, 2, renorm, 2.5)
+    idx, _, _ = route(lib, r, x)
+    i2, _, _ = route(lib, r, good)
+    dw, ds = (torch.randn(n, k, device=DEV, generator=gen(k)) for k in (4, E))
+    dw[5], ds[2], ds[n - 1] = float("nan"), float("nan"), INF
+    dw2, ds2 = dw.clone(), ds.clone()
+    dw2[bad], ds2[bad] = 0.0, 0.0
+    assert lib.status() == 1
+    for d, d2 in ((None, None), (ds, ds2)):
+        want = backward(lib, r, good, i2, dw2, d2)
+        assert lib.status() == 0
+        got = backward(lib, r, x, idx, dw, d)
+        # without scores' gradients only softmax reads a token whose ids are -1
+        assert lib.status() == (1 if d is not None or kind == SOFTMAX else 0)
+        assert (got[bad] == 0).all() and torch.equal(got[others], want[others])
+        assert (got[others] != 0).any()
