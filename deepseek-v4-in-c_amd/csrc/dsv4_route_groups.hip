@@ -607,6 +607,7 @@ __global__ __launch_bounds__(256) void k_route_groups_bwd(RouteGroupsBwdArgs a)
         for (int i = 0; i < 4; i++) {
             if (!dense) x[q][i] = NO_EXPERT;
             if (!a.dscores || id_of(q) + i >= ne) g[q][i] = 0.0f;
+            if (SCORE == DSV4_HIP_SOFTMAX && !(x[q][i] > NO_EXPERT)) g[q][i] = 0.0f;   /* before it enters a sum */
         }
     }
     /* a token that the forward call refuses has ids of -1: without its logits and its
@@ -639,7 +640,7 @@ __global__ __launch_bounds__(256) void k_route_groups_bwd(RouteGroupsBwdArgs a)
     };
     auto slope = [&](float v, double sv) -> double {
         if constexpr (SCORE == DSV4_HIP_SOFTMAX) return sv;
-        else if constexpr (SCORE == DSV4_HIP_SIGMOID) return v > NO_EXPERT ? sv * (1.0 - sv) : 0.0;
+        else if constexpr (SCORE == DSV4_HIP_SIGMOID) return sv * (1.0 - sv);
         else return sqrt_softplus64(v).d;
     };
     const double sk = id >= 0 ? score(xk) : 0.0;
@@ -679,7 +680,7 @@ __global__ __launch_bounds__(256) void k_route_groups_bwd(RouteGroupsBwdArgs a)
                 o[i] = 0.0f;
                 if (a.dscores) {
                     const double v = score(x[q][i]);
-                    o[i] = (float)(slope(x[q][i], v) * (double)g[q][i]);
+                    o[i] = x[q][i] > NO_EXPERT ? (float)(slope(x[q][i], v) * (double)g[q][i]) : 0.0f;
                 }
             }
         }

@@ -468,7 +468,8 @@ int  dsv4_hip_route_groups_dev(int *idx, float *w, float *scores, const void *lo
  * adds nothing; another id outside [0, n_experts) likewise, and raises status
  * bit 0. A token that the forward call refuses (a logit of NaN or +inf, its ids
  * -1) has gradient 0 whatever dw and dscores hold; with dscores or softmax,
- * which read all its logits, it raises bit 0 again. In fp64, one rounding.
+ * which read all its logits, it raises bit 0 again. An expert whose logit is -inf
+ * has gradient 0 whatever dscores holds for it. In fp64, one rounding.
  * n_group and what belongs to it are not read. dlogits may be logits, or dscores
  * if they are of one type. */
 int  dsv4_hip_route_groups_bwd_dev(void *dlogits, const float *dw, const float *dscores, const void *logits,

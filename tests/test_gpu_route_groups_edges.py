@@ -1,6 +1,6 @@
 # SPDX-License-Identifier: Apache-2.0
 """The router with groups at its edges on the GPU: weights that are constant, tokens
-that are refused.
+that are refused, experts that are not there.
 
 Bounds as in test_gpu_route_groups.py: what is exactly 0 is compared with 0, a
 gradient is an fp64 value with one rounding to the logits' type, and an absolute
@@ -80,3 +80,24 @@ def test_refused_tokens_have_no_gradient(lib, pkg, kind, dtype, renorm, n, E):
         assert lib.status() == (1 if d is not None or kind == SOFTMAX else 0)
         assert (got[bad] == 0).all() and torch.equal(got[others], want[others])
         assert (got[others] != 0).any()
+
+
+@pytest.mark.parametrize("kind", [SQRT, SOFTMAX, SIGMOID])
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n,E", [(9, 70), (8205, 200), (21, 600)])
+def test_experts_that_are_not_there_take_no_gradient(lib, pkg, kind, dtype, n, E):
+    """What a loss sends to the score of an expert whose logit is -inf (1 / 0 of a logarithm, NaN)
+    goes nowhere: gradient 0 for it, for the others the bits of a call with 0 there."""
+    x = torch.randn(n, E, device=DEV, generator=gen(n + E)).to(dtype)
+    x[torch.rand(n, E, device=DEV, generator=gen(7)) < 0.3] = -INF
+    x[4] = -INF
+    gone = x == -INF
+    r = pkg.Router(kind, E, 4, 1, 1, 1, 1, 2.5)
+    idx, _, _ = route(lib, r, x)
+    dw, ds = (torch.randn(n, k, device=DEV, generator=gen(k)) for k in (4, E))
+    ds[gone] = 0.0
+    want = backward(lib, r, x, idx, dw, ds)
+    for v in (INF, -INF, float("nan")):
+        got = backward(lib, r, x, idx, dw, torch.where(gone, v, ds))
+        assert (got[gone] == 0).all() and torch.equal(got, want)
+    assert lib.status() == 0 and (want != 0).any()
