@@ -1,6 +1,7 @@
 # SPDX-License-Identifier: Apache-2.0
 """The router with groups at its edges on the GPU: weights that are constant, tokens
-that are refused, experts that are not there.
+that are refused, experts that are not there, the token counts from which four
+tokens share a wave.
 
 Bounds as in test_gpu_route_groups.py: what is exactly 0 is compared with 0, a
 gradient is an fp64 value with one rounding to the logits' type, and an absolute
@@ -8,7 +9,8 @@ part of 2e-11 for what cancels."""
 import pytest
 import torch
 
-from test_gpu_route_groups import DEV, HALF, SIGMOID, SOFTMAX, SQRT, TINY, TYPES, backward, gen, route, want_grad
+from test_gpu_route_groups import (DEV, HALF, SIGMOID, SOFTMAX, SQRT, TINY, TYPES, U, backward, check, gen, route, want_grad,
+                                   with_masks)
 
 pytestmark = pytest.mark.gpu
 
@@ -101,3 +103,47 @@ def test_experts_that_are_not_there_take_no_gradient(lib, pkg, kind, dtype, n, E
         got = backward(lib, r, x, idx, dw, torch.where(gone, v, ds))
         assert (got[gone] == 0).all() and torch.equal(got, want)
     assert lib.status() == 0 and (want != 0).any()
+
+
+# Tokens share a wave, with up to 256 experts, from 3,500 forward, 6,144 with sqrt(softplus); backward from
+# 4,096, 8,192 with scores' gradients. Experts: each number of quads a lane.
+@pytest.mark.parametrize("kind,n", [(SOFTMAX, 3500), (SIGMOID, 3500), (SQRT, 6144)])
+@pytest.mark.parametrize("E,topk,G,kept", [(60, 4, 5, 2), (128, 6, 8, 3), (250, 8, 10, 4)])
+def test_one_token_less_than_share_a_wave(lib, pkg, kind, n, E, topk, G, kept):
+    """Both sides by the definition, and alike. Softmax adds up in another order: fp64 sums of 250
+    terms, 2^-44 of them, so a score may round to the other side, a step of 2^-23, and a weight,
+    a quotient of two sums of scores, to three of them."""
+    x = with_masks(1.5 * torch.randn(n, E, device=DEV, generator=gen(n + E)))
+    bias = 0.1 * torch.randn(E, device=DEV, generator=gen(3))
+    r = pkg.Router(kind, E, topk, G, kept, 2, 1, 2.5)
+    lib.status()
+    check(lib, r, x, bias)
+    check(lib, r, x[:-1], bias)
+    more, less = route(lib, r, x, bias), route(lib, r, x[:-1], bias)
+    assert lib.status() == 0 and torch.equal(more[0][:-1], less[0])
+    for a, b, steps in ((more[1][:-1], less[1], 3), (more[2][:-1], less[2], 1)):
+        if kind == SOFTMAX:
+            assert ((a - b).abs() <= steps * 2 * U * b + 2.0 ** -149).all()
+        else:
+            assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("kind", [SQRT, SOFTMAX, SIGMOID])
+@pytest.mark.parametrize("scores,n", [(False, 4096), (True, 8192)])
+@pytest.mark.parametrize("E,topk", [(60, 4), (128, 6), (250, 8)])
+def test_gradients_of_one_token_less_than_share_a_wave(lib, pkg, kind, scores, n, E, topk):
+    """As above; softmax: 1e-12 of what adds up, and the rounding to fp32 may fall to the other side."""
+    x = 1.5 * torch.randn(n, E, device=DEV, generator=gen(n + E))
+    dw = torch.randn(n, topk, device=DEV, generator=gen(2))
+    ds = torch.randn(n, E, device=DEV, generator=gen(5)) if scores else None
+    for renorm in (0, 1):
+        r = pkg.Router(kind, E, topk, 1, 1, 1, renorm, 2.5)
+        idx, _, _ = route(lib, r, x)
+        more = backward(lib, r, x, idx, dw, ds)
+        less = backward(lib, r, x[:-1], idx[:-1], dw[:-1], ds[:-1] if scores else None)
+        want = want_grad(r, x, idx, dw, ds)
+        assert ((more.double() - want).abs() <= 1.001 * HALF[torch.float32] * want.abs() + 1e-12 * 20 + 2.0 ** -149).all()
+        if kind == SOFTMAX:
+            assert ((more[:-1].double() - less.double()).abs() <= 1e-12 * 20 + 2 * U * less.abs()).all()
+        else:
+            assert torch.equal(more[:-1], less)
