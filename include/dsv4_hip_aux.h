@@ -82,8 +82,7 @@ int dsv4_hip_swiglu_quant_mxfp4_dev(uint8_t *Q, uint8_t *S, const void *g, const
 /* The same for the columns of a, the operands of a backward pass: with n' = n
  * rounded up to 32, Q[k][n' / 2] and S[k][n' / 32] hold a^T, zeros behind row n.
  * k any number up to 2^24, n < 2^24, k * n' <= 2^35 - 4096, ld >= k, a aligned to its
- * elements (rows of even length at an even pitch and 2-element alignment are the
- * fast ones), Q 16-byte aligned. n or k 0: nothing. */
+ * elements, Q 16-byte aligned. n or k 0: nothing. */
 int dsv4_hip_quant_mxfp4_t_dev(uint8_t *Q, uint8_t *S, const void *a, int type, int64_t ld, int n, int k,
                                void *stream);
 
