@@ -355,7 +355,9 @@ inline Fp4Shape fp4_shape(Fp4Form form)
  * r of one and the rest by how full it is. Fitted to 3,000 times of 368 shapes (1 to
  * 4,096 rows, 300 to 32,768 features, K 256 to 16,384), in which the form that they
  * choose costs 0.3 % more than the best, at most 13 % (16 x 512 x 8192: split 6.3 us, team
- * 5.6). us, split / team / 64x64 / 128x64 / 128x96 / 128x128 / _W8 / 256x128 / 256x192 /
+ * 5.6), three sets of operands in turn, so weights from the caches. From HBM one to 16
+ * rows of 1024 x 4096 and 4096 x 4096 cost 0.2 to 0.7 us more in the same forms, of 32768 x
+ * 4096 14.8 rather than 12.2: 4.8 TB/s, what a copy reaches. us, split / team / 64x64 / 128x64 / 128x96 / 128x128 / _W8 / 256x128 / 256x192 /
  * 256x256 (64x32 before the team: 64 x 4096 x 4096 6.5, 333 x 1024 x 1024 3.9):
  *   1 x 4096 x 4096      3.3 / 3.9 / 6.6 / 8.1 / ..
  *   64 rows              11 / 4.5 / 7.1 / 9.0 / ..

@@ -141,8 +141,8 @@ __device__ __forceinline__ int fp4_source(const Fp4Args &a, const Fp4Bucket &t, 
  * whole piece's loads before its first product, and the sums meet in LDS, added
  * in wave order. No wave waits for another before the end, so a product too
  * small to fill the device costs one latency of its loads, not one a stage.
- * Bound: that latency (one token of 4096 x 4096 3.4 us, the weights alone 1.4 at
- * 6.2 TB/s; 64 x 32 tiles 6.1); with many rows the loads, 64 bytes of a row each. */
+ * Bound: that latency (one token of 4096 x 4096 3.4 us, with weights from HBM 4.1, the
+ * weights alone 1.4 at 6.2 TB/s; 64 x 32 tiles 6.1); with many rows the loads, 64 bytes of a row each. */
 template <int OUT>
 __global__ __launch_bounds__(512) void k_fp4_split(Fp4Args a)
 {
@@ -187,8 +187,8 @@ __global__ __launch_bounds__(512) void k_fp4_split(Fp4Args a)
  * share out the stages of 256 values, each with a stage's place of its own in
  * LDS and all of the tile's results in registers: no wave waits for another
  * before the sums meet in LDS, added in wave order. A stage's loads are asked for
- * when the one before is in registers; other workgroups, five to a CU, hide their
- * latency better than a second place does (64 x 4096 x 4096 4.5 us with either, 128 x
+ * when the one before is in registers; other workgroups, four to a CU (103 registers;
+ * LDS has room for five), hide their latency better than a second place does (64 x 4096 x 4096 4.5 us with either, 128 x
  * 4096 x 1024 4.5 against 3.2; eight waves 4.4 and 4.3; 64 rows a tile 5.9 and 3.6).
  * Bound: latency of launch, a few stages and the sums, then a CU's loads
  * (128 KB of operands a 32 x 32 tile at K = 4096). */
@@ -302,8 +302,8 @@ __global__ __launch_bounds__(256) void k_fp4_team(Fp4Args a)
  * so the stage NST ahead takes its place. The tile leaves through LDS as whole
  * 16-byte pieces of rows.
  * Bound, 256 x 256: the matrix instructions at the clock that power allows (4096^3
- * 37.5 us, 3.7 PFLOP/s; of it 9 us first loads and the way out, as one workgroup
- * has the CU). 128 x 128: a CU's loads, 32 KB a stage in 0.52 us (63 GB/s, alone
+ * 36.5 to 39.4 us from card to card, 3.5 to 3.8 PFLOP/s; of it 9 us first loads and the
+ * way out, as one workgroup has the CU). 128 x 128: a CU's loads, 32 KB a stage in 0.52 us (63 GB/s, alone
  * they reach 80): 2,803 x 1024 x 4096 13 us, in 128 x 96 tiles, which fill more of the
  * CUs, 12, 5 of them launch, first loads and the way out. Buckets: the weights'
  * stream (7 tokens, top 6 of 256 experts 2048 x 4096 35 us, 5.0 TB/s), with many rows

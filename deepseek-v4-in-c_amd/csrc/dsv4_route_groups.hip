@@ -22,8 +22,10 @@
  * Bound: few tokens by the chain of loads, scores, groups and picks (1 token of 256
  * experts in 8 groups, top 6, 4.6 us, 3.9 without groups and top 1); many by the vector
  * unit, 50 instructions a score and 300 for eight picks of four tokens (16,384 tokens,
- * 8 groups, top 8, with scores 16.4 us for 33.5 MB; HBM alone 7); backward by HBM (50
- * MB in 15 us).
+ * 8 groups, top 8, with scores 16.4 us for 33.5 MB, which HBM alone moves in 7). Backward
+ * of 16,384 tokens: four waves a SIMD, all there at once, so loads, 4,700 vector
+ * instructions a SIMD and stores follow each other with little overlap (sigmoid 15.2 us
+ * for 50 MB, 3.3 TB/s, softmax 16, sqrt(softplus) 23.5 for its logarithms).
  */
 #include "dsv4_elem.h"
 #include "dsv4_gate_route.h"
@@ -711,9 +713,10 @@ hipError_t launch(const RouteGroupsBwdArgs &a, hipStream_t st)
 /* Tokens from which four share a wave: fewer leave lanes of the device idle. us, a
  * wave each / shared, 256 experts: sigmoid, 8 groups, top 8 2,048 tokens 6.8 / 7.2,
  * 3,000 7.8 / 7.3, 16,384 26 / 16.4; softmax, top 6 3,000 6.1 / 6.9, 4,096 7.0 / 6.8,
- * 16,384 19 / 12.3; sqrt(softplus), top 6 4,096 8.9 / 10.4, 8,192 14.0 / 12.6, 16,384 -
- * / 21; backward with scores' gradients 6,000 7.5 /
- * 8.4, 8,192 9.1 / 9.3, 16,384 16.3 / 15.4, without 6,000 6.1 / 4.6. */
+ * 16,384 19 / 12.3; sqrt(softplus), top 6 4,096 8.9 / 10.4, 8,192 14.0 / 12.6, 16,384 25
+ * / 21; backward with scores' gradients 6,000 7.5 / 8.4, 8,192 9.3 / 9.3, 16,384 16.6 /
+ * 15.4, softmax 18.6 / 16.4, sqrt(softplus) 26 / 23.5, without 6,000 6.1 / 4.6. Fewer
+ * experts go by the same counts. */
 int shared_from(const RouteGroupsArgs &a) { return a.r.score == DSV4_HIP_SQRT_SOFTPLUS ? 6144 : 3500; }
 int shared_from(const RouteGroupsBwdArgs &a) { return a.dscores ? 8192 : 4096; }
 template <int TYPE, int SCORE, class ARGS>
